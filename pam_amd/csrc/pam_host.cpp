@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/pam_hip.h"
+#include "../../include/pam_hip_block.h"
 #include "../../include/pam_hip_extra.h"
 
 // what this module was built on (pam_amd/build.py reads it from the file's bytes)
@@ -486,6 +487,8 @@ struct UnaryNode : torch::autograd::Function<UnaryNode> {
     }
 };
 
+#include "pam_host_block.h"
+
 // ---------------------------------------------------------------- optimizer
 
 // The parameters from `start` on that one launch can update: those with a gradient and moments that are contiguous fp32
@@ -570,5 +573,12 @@ PYBIND11_MODULE(_pam_host, module)
     module.def("mul", [](const Tensor& A, const Tensor& B, double offset, bool a, bool b) { return PairNode<false>::apply(A, B, offset, a, b); }, unlocked);
     module.def("div", [](const Tensor& A, const Tensor& B, double offset, bool a, bool b) { return PairNode<true>::apply(A, B, offset, a, b); }, unlocked);
     module.def("unary", [](const Tensor& x, int64_t op, double number, double offset, bool a, bool e) { return UnaryNode::apply(x, op, number, offset, a, e); }, unlocked);
+    module.def("layer", &call_layer, unlocked);
+    module.def("rotary", [](const Tensor& q, const std::optional<Tensor>& k, const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& positions,
+                            const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight, bool interleaved, double eps, double offset,
+                            bool a, bool b, bool e) {
+        return RotaryNode::apply(q, k, cos, sin, positions, q_weight, k_weight, interleaved, eps, offset, a, b, e);
+    }, unlocked);
+    module.def("clip", &clip, unlocked);
     module.def("adam_collect", &adam_collect);
 }

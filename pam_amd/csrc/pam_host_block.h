@@ -1,0 +1,270 @@
+// The host path of the decoder block's operators (include/pam_hip_block.h): nodes and calls for pam_host.cpp, which includes
+// this file inside its namespace, behind the helpers it uses.
+
+// ---------------------------------------------------------------- products with an activation, gated layers
+
+// (rows contiguous, or copied so)
+Tensor rows_contiguous(const Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+
+struct Layer { Tensor y, z; };
+
+// act(X W^T + bias) + residual, or with `gated` act(g) (*) u of W's two halves; want_z: what the activation is applied to, too
+Layer layer(bool gated, const Tensor& X, const Tensor& W, const Tensor& bias, int activation, const Tensor& residual, bool want_z, double offset)
+{
+    const char* const name = gated ? "gated_linear" : "linear_act";
+    check_tensor(X); check_tensor(W);
+    if (bias.defined()) check_tensor(bias);
+    if (residual.defined()) check_tensor(residual);
+    TORCH_CHECK_VALUE(X.dim() == 2 && W.dim() == 2 && X.size(1) == W.size(1), name, ": shapes ", shape(X), " and ", shape(W), " do not multiply");
+    const int64_t m = X.size(0), k = X.size(1), rows = W.size(0), n = gated ? rows / 2 : rows;
+    TORCH_CHECK_VALUE(!gated || rows % 2 == 0, name, ": the weight has the gate's rows and as many others, got ", rows);
+    TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.numel() == rows), name, ": bias must have one value per row of the weight");
+    TORCH_CHECK_VALUE(!residual.defined() || (residual.dim() == 2 && residual.size(0) == m && residual.size(1) == n), name, ": the residual must have the shape of the result");
+    for (const Tensor* t : {&W, &bias, &residual})
+        TORCH_CHECK_VALUE(!t->defined() || t->device() == X.device(), name, ": tensors are on different devices");
+    const OnDevice on(X);
+    Layer out;
+    out.y = new_floats({m, n}, X);
+    if (want_z) out.z = new_floats({m, rows}, X);
+    if (out.y.numel() == 0) return out;
+    const Tensor b = bias.defined() ? bias.contiguous() : bias, res = residual.defined() ? rows_contiguous(residual) : residual;
+    const size_t bytes = gated ? pam_hip_gated_linear_workspace_bytes(m, n, k) : pam_hip_linear_act_workspace_bytes(m, n, k);
+    Tensor ws;
+    if (bytes) ws = gemm_workspace(X, on.stream, bytes);
+    if (gated)
+        check_call(pam_hip_gated_linear_fwd(data(X), X.stride(0), X.stride(1), data(W), W.stride(0), W.stride(1), data_or_null(b), activation,
+                                            data_or_null(out.z), data(out.y), m, n, k, (float)offset, data_or_null(ws), bytes, on.stream), "gated_linear_fwd");
+    else
+        check_call(pam_hip_linear_act_fwd(data(X), X.stride(0), X.stride(1), data(W), W.stride(0), W.stride(1), data_or_null(b), activation,
+                                          data_or_null(res), res.defined() ? res.stride(0) : 0, data_or_null(out.z), data(out.y), m, n, k, (float)offset,
+                                          data_or_null(ws), bytes, on.stream), "linear_act_fwd");
+    return out;
+}
+
+struct LayerNode : torch::autograd::Function<LayerNode> {
+    static Tensor forward(AutogradContext* ctx, bool gated, const Tensor& X_in, const Tensor& W, const std::optional<Tensor>& bias, int64_t activation,
+                          const std::optional<Tensor>& residual, bool train, double offset, bool a, bool b, bool e)
+    {
+        TORCH_CHECK_VALUE(X_in.dim() == 2, gated ? "gated_linear" : "linear_act", ": expected rows of values");
+        const Tensor X = row_major(X_in, 2);
+        const bool keep_z = train && (gated || activation != PAM_HIP_ACT_NONE);
+        const Layer out = layer(gated, X, W, bias.value_or(Tensor()), (int)activation, residual.value_or(Tensor()), keep_z, offset);
+        ctx->saved_data["gated"] = gated; ctx->saved_data["activation"] = activation; ctx->saved_data["offset"] = offset;
+        ctx->saved_data["bias"] = bias.has_value(); ctx->saved_data["residual"] = residual.has_value(); ctx->saved_data["rows"] = W.size(0);
+        Approx{a, b, e}.save(ctx);
+        if (train) ctx->save_for_backward({X, W, out.z});
+        return out.y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        const Approx f = Approx::saved(ctx);
+        const bool gated = ctx->saved_data["gated"].toBool(), has_bias = ctx->saved_data["bias"].toBool(), has_residual = ctx->saved_data["residual"].toBool();
+        const int activation = (int)ctx->saved_data["activation"].toInt();
+        const double offset = ctx->saved_data["offset"].toDouble();
+        const int64_t rows = ctx->saved_data["rows"].toInt();
+        const char* const name = gated ? "gated_linear_bwd" : "linear_act_bwd";
+        const Tensor dy = grads[0];
+        check_tensor(dy);
+        const int64_t m = dy.size(0);
+        // (edges are counted over the tensors that are there)
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = has_bias && ctx->needs_input_grad(2);
+        Tensor dX, dW, db;
+        {
+            const at::AutoGradMode no_graph(false);
+            Tensor dz = row_major(dy, 2);
+            if ((gated || activation != PAM_HIP_ACT_NONE) && (want_x || want_w || want_b)) {
+                const Tensor z = whole(saved[2], dy, {m, rows}, name), d = dy.contiguous();
+                const OnDevice on(dy);
+                dz = new_floats({m, rows}, dy);
+                const float off = (float)offset;
+                if (gated) check_call(pam_hip_gated_bwd(data(z), data(d), data(dz), m, rows / 2, activation, off, f.a, f.b, f.e, on.stream), "gated_bwd");
+                else check_call(pam_hip_act_bwd(data(z), data(d), data(dz), d.numel(), activation, off, f.a, f.b, f.e, on.stream), "act_bwd");
+            }
+            const Tensor X = row_major(saved[0], 2), Wt = row_major(saved[1].t(), 2);
+            TORCH_CHECK_VALUE(X.size(0) == m && Wt.size(1) == rows, name, ": a saved tensor has not the shape that it was saved with");
+            const ProductGrads g = product_grads(X, Wt, dz, 2, f, offset, want_x, want_w);
+            dX = g.dA;
+            if (g.dB.defined()) dW = g.dB.t();
+            if (want_b) db = sum_rows(dz);
+        }
+        return {Tensor(), dX, dW, db, Tensor(), has_residual ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+bool wants_graph(std::initializer_list<const Tensor*> tensors)
+{
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : tensors)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+Tensor call_layer(bool gated, const Tensor& X, const Tensor& W, const std::optional<Tensor>& bias, int64_t activation, const std::optional<Tensor>& residual,
+                  double offset, bool a, bool b, bool e)
+{
+    const Tensor none;
+    if (!wants_graph({&X, &W, bias ? &*bias : &none, residual ? &*residual : &none}))
+        return layer(gated, row_major(X, 2), W, bias.value_or(none), (int)activation, residual.value_or(none), false, offset).y;
+    return LayerNode::apply(gated, X, W, bias, activation, residual, true, offset, a, b, e);
+}
+
+// ---------------------------------------------------------------- rotation of queries and keys
+
+struct Rotation {
+    Tensor cos, sin, positions;
+    int64_t batch, tokens, dim, rotated;
+    bool interleaved;
+    float eps, offset;
+};
+
+Tensor heads_contiguous(const Tensor& t) { return t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+
+// [batch][tokens][heads][dim]: the entry of a tensor in the call's table
+pam_hip_heads heads_of(const Tensor& x, const Tensor& weight, const Tensor& y)
+{
+    pam_hip_heads h{};
+    h.x = data(x); h.x_sb = x.stride(0); h.x_st = x.stride(1); h.x_sh = x.stride(2);
+    h.weight = data_or_null(weight); h.y = data(y); h.heads = x.size(2);
+    return h;
+}
+
+Rotation rotation(const variable_list& x, const variable_list& weights, const Tensor& cos, const Tensor& sin, const Tensor& positions, bool interleaved, double eps, double offset)
+{
+    const char* const name = "rotary";
+    Rotation r;
+    r.batch = x[0].dim() == 4 ? x[0].size(0) : 0; r.tokens = x[0].dim() == 4 ? x[0].size(1) : 0; r.dim = x[0].dim() == 4 ? x[0].size(3) : 0;
+    for (size_t i = 0; i < x.size(); ++i) {
+        check_tensor(x[i]);
+        TORCH_CHECK_VALUE(x[i].dim() == 4 && x[i].size(0) == r.batch && x[i].size(1) == r.tokens && x[i].size(3) == r.dim && x[i].device() == x[0].device(),
+                          name, ": queries and keys are [batch, tokens, heads, dim] on one device, got ", shape(x[0]), " and ", shape(x[i]));
+        if (!weights[i].defined()) continue;
+        check_tensor(weights[i]);
+        TORCH_CHECK_VALUE(weights[i].dim() == 1 && weights[i].numel() == r.dim && weights[i].device() == x[0].device(), name, ": a norm's weight has one value per value of a head");
+    }
+    check_tensor(cos); check_tensor(sin);
+    TORCH_CHECK_VALUE(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.device() == x[0].device() && sin.device() == x[0].device(),
+                      name, ": cos and sin are two tables of one shape on the tensors' device");
+    TORCH_CHECK_VALUE(2 * cos.size(1) <= r.dim, name, ": the tables rotate ", 2 * cos.size(1), " values of a head that has ", r.dim);
+    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), "rotary: the tables have no gradient");
+    r.cos = cos.contiguous(); r.sin = sin.contiguous();
+    r.rotated = 2 * cos.size(1);
+    if (positions.defined()) {
+        TORCH_CHECK_TYPE(positions.scalar_type() == at::kLong, name, ": positions are int64");
+        TORCH_CHECK_VALUE(positions.device() == x[0].device() && (positions.dim() == 1 || positions.dim() == 2) && positions.size(-1) == r.tokens
+                              && (positions.dim() == 1 || positions.size(0) == r.batch),
+                          name, ": positions are [tokens] or [batch, tokens] on the tensors' device, got ", shape(positions));
+        r.positions = positions;
+    } else {
+        TORCH_CHECK_VALUE(r.tokens <= cos.size(0), name, ": ", r.tokens, " tokens and tables of ", cos.size(0), " positions");
+    }
+    r.interleaved = interleaved; r.eps = (float)eps; r.offset = (float)offset;
+    return r;
+}
+
+struct RotationArgs { const long long* positions; int64_t sb, st; };
+RotationArgs positions_of(const Rotation& r)
+{
+    if (!r.positions.defined()) return {nullptr, 0, 0};
+    return {reinterpret_cast<const long long*>(r.positions.data_ptr<int64_t>()), r.positions.dim() == 2 ? r.positions.stride(0) : 0, r.positions.stride(-1)};
+}
+
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
+                                 const std::optional<Tensor>& positions, const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight,
+                                 bool interleaved, double eps, double offset, bool a, bool b, bool e)
+    {
+        variable_list x{q}, w{q_weight.value_or(Tensor())};
+        if (k) { x.push_back(*k); w.push_back(k_weight.value_or(Tensor())); }
+        const Rotation r = rotation(x, w, cos, sin, positions.value_or(Tensor()), interleaved, eps, offset);
+        const OnDevice on(q);
+        variable_list y;
+        std::vector<pam_hip_heads> parts;
+        for (size_t i = 0; i < x.size(); ++i) {
+            x[i] = heads_contiguous(x[i]);
+            if (w[i].defined()) w[i] = w[i].contiguous();
+            y.push_back(new_floats(x[i].sizes(), x[i]));
+            parts.push_back(heads_of(x[i], w[i], y[i]));
+        }
+        const RotationArgs at = positions_of(r);
+        check_call(pam_hip_rotary_fwd(parts.data(), (int)parts.size(), data(r.cos), data(r.sin), r.cos.size(0), at.positions, at.sb, at.st, r.batch, r.tokens,
+                                      r.dim, r.rotated, r.interleaved, r.eps, r.offset, on.stream), "rotary_fwd");
+        ctx->saved_data["count"] = (int64_t)x.size(); ctx->saved_data["positions"] = positions.has_value();
+        ctx->saved_data["wq"] = q_weight.has_value(); ctx->saved_data["wk"] = k_weight.has_value();
+        ctx->saved_data["interleaved"] = interleaved; ctx->saved_data["eps"] = eps; ctx->saved_data["offset"] = offset;
+        for (size_t i = 0; i < x.size(); ++i) ctx->saved_data[i ? "k" : "q"] = x[i].sizes();
+        Approx{a, b, e}.save(ctx);
+        x.resize(2); w.resize(2);
+        ctx->save_for_backward({x[0], x[1], w[0], w[1], r.cos, r.sin, r.positions});
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        const Approx f = Approx::saved(ctx);
+        const size_t count = (size_t)ctx->saved_data["count"].toInt();
+        const at::AutoGradMode no_graph(false);
+        variable_list x, w, dx, dw, dy;
+        // (edges are counted over the tensors that are there: q, k, cos, sin, positions, the weights)
+        size_t edge = count + 2 + (ctx->saved_data["positions"].toBool() ? 1 : 0);
+        bool want_w[2] = {false, false};
+        if (ctx->saved_data["wq"].toBool()) want_w[0] = ctx->needs_input_grad(edge++);
+        if (ctx->saved_data["wk"].toBool()) want_w[1] = ctx->needs_input_grad(edge++);
+        const OnDevice on(grads[0]);
+        std::vector<pam_hip_heads> parts;
+        for (size_t i = 0; i < count; ++i) {
+            check_tensor(grads[i]);
+            const std::vector<int64_t> sizes = ctx->saved_data[i ? "k" : "q"].toIntVector();
+            check_tensor(saved[i]);
+            TORCH_CHECK_VALUE(saved[i].sizes() == at::IntArrayRef(sizes) && saved[i].device() == grads[i].device() && grads[i].sizes() == at::IntArrayRef(sizes),
+                              "rotary_bwd: a saved tensor has not the shape or the device that it was saved with");
+            x.push_back(heads_contiguous(saved[i])); dy.push_back(heads_contiguous(grads[i]));
+            w.push_back(saved[2 + i].defined() ? whole(saved[2 + i], grads[i], {sizes[3]}, "rotary_bwd") : Tensor());
+            dx.push_back(new_floats(sizes, grads[i]));
+            dw.push_back(want_w[i] ? new_floats({sizes[3]}, grads[i]) : Tensor());
+            pam_hip_heads h = heads_of(x[i], w[i], dx[i]);
+            h.dy = data(dy[i]); h.dy_sb = dy[i].stride(0); h.dy_st = dy[i].stride(1); h.dy_sh = dy[i].stride(2);
+            h.dweight = data_or_null(dw[i]);
+            parts.push_back(h);
+        }
+        const Rotation r = rotation(x, w, saved[4], saved[5], saved[6], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["offset"].toDouble());
+        const RotationArgs at = positions_of(r);
+        const size_t bytes = pam_hip_rotary_bwd_workspace_bytes(parts.data(), (int)count, r.batch, r.tokens, r.dim);
+        const Tensor ws = bytes ? new_floats({(int64_t)((bytes + 3) / 4)}, grads[0]) : Tensor();
+        check_call(pam_hip_rotary_bwd(parts.data(), (int)count, data(r.cos), data(r.sin), r.cos.size(0), at.positions, at.sb, at.st, r.batch, r.tokens, r.dim,
+                                      r.rotated, r.interleaved, r.eps, r.offset, f.a, f.b, f.e, data_or_null(ws), bytes, on.stream), "rotary_bwd");
+        dx.resize(2); dw.resize(2);
+        return {dx[0], dx[1], Tensor(), Tensor(), Tensor(), dw[0], dw[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ---------------------------------------------------------------- clipping
+
+// The norm of all tensors; with `outs`, the clipped values there (a tensor may be its own output).  Each tensor's memory is
+// without gaps or overlaps, and an output has its tensor's strides.
+Tensor clip(const variable_list& ins, const variable_list& outs, double max_norm, double eps, double offset)
+{
+    TORCH_CHECK_VALUE(!ins.empty(), "clip_grads: no tensors");
+    TORCH_CHECK_VALUE(outs.empty() || outs.size() == ins.size(), "clip_grads: as many outputs as tensors");
+    std::vector<pam_hip_clip_tensor> table;
+    table.reserve(ins.size());
+    for (size_t i = 0; i < ins.size(); ++i) {
+        check_tensor(ins[i]);
+        TORCH_CHECK_VALUE(ins[i].device() == ins[0].device(), "clip_grads: tensors are on different devices");
+        TORCH_CHECK_VALUE(ins[i].is_non_overlapping_and_dense(), "clip_grads: a tensor's memory has gaps or overlaps");
+        if (!outs.empty()) {
+            check_tensor(outs[i]);
+            TORCH_CHECK_VALUE(outs[i].sizes() == ins[i].sizes() && outs[i].device() == ins[i].device() && outs[i].is_non_overlapping_and_dense()
+                                  && (ins[i].strides() == outs[i].strides() || (ins[i].is_contiguous() && outs[i].is_contiguous())),
+                              "clip_grads: an output has its tensor's shape, strides and device");
+        }
+        const size_t n = (size_t)ins[i].numel();
+        if (n) table.push_back({data(ins[i]), outs.empty() ? nullptr : data(outs[i]), n});
+    }
+    const OnDevice on(ins[0]);
+    const Tensor norm = new_floats({}, ins[0]);
+    const size_t bytes = pam_hip_clip_workspace_bytes(table.data(), (long)table.size());
+    const Tensor ws = new_floats({(int64_t)(bytes / 4)}, ins[0]);
+    check_call(pam_hip_clip_many(table.data(), (long)table.size(), (float)max_norm, (float)eps, data(norm), (float)offset, data(ws), bytes, on.stream), "clip_many");
+    return norm;
+}

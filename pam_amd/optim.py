@@ -17,7 +17,7 @@ import yaml
 from . import _abi
 from .factories import get_function_dict
 
-__all__ = ["Adam", "multiply_grads"]
+__all__ = ["Adam", "multiply_grads", "grad_norm", "clip_grads", "clip_grad_norm_"]
 
 
 def _pam_table_offset(cfg):
@@ -153,3 +153,61 @@ def multiply_grads(params, c, op_dict):
             p.grad.data.mul_(cc)
         else:
             op_dict["mul"](p.grad.data, cc)
+
+
+# ---------------------------------------------------------------- the global norm, clipping
+
+_CLIP_EPS = 1e-6
+
+
+def _dense(tensors):
+    """The tensors, copies in the place of those whose memory has gaps or overlaps."""
+    return [t if t.is_contiguous() or (t.layout is torch.strided and torch.ops.aten.is_non_overlapping_and_dense(t)) else t.contiguous() for t in tensors]
+
+
+def grad_norm(grads, *, offset=None):
+    """pow(sum of g (*) g over all tensors, 0.5), a tensor of no dimensions: the global norm of many fp32 GPU tensors."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    with torch.no_grad():
+        return _abi.host().clip(_dense(grads), [], math.inf, _CLIP_EPS, 1.0 if offset is None else float(offset))
+
+
+def clip_grads(grads, max_norm, *, out=None, offset=None):
+    """Scales the tensors so that their global norm is at most max_norm: g (*) min(1, max_norm (/) (norm + 1e-6)), one pass for
+    the norm and one for the products.  out: a list of tensors of the same shapes that takes the results; None: in place.
+    Returns the norm before, on the GPU (the host does not wait).  A norm that is not finite makes the gradients NaN, as an
+    ordinary clip does; a max_norm of infinity leaves them as they are."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    out = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grads: the bound is not negative, got {max_norm}")
+    if len(out) != len(grads):
+        raise ValueError("clip_grads: as many outputs as tensors")
+    with torch.no_grad():
+        ins, outs = _dense(grads), _dense(out)
+        ins = [g.contiguous() if g.stride() != o.stride() else g for g, o in zip(ins, outs)]
+        outs = [o if o.stride() == g.stride() or o.is_contiguous() else torch.empty_like(g) for g, o in zip(ins, outs)]
+        norm = _abi.host().clip(ins, outs, max_norm, _CLIP_EPS, 1.0 if offset is None else float(offset))
+        for target, result in zip(out, outs):
+            if target is not result:
+                target.copy_(result)
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, *, offset=None):
+    """torch.nn.utils.clip_grad_norm_ with PAM products, quotient and root: clips the parameters' gradients in place and returns
+    their norm before.  Only the 2-norm.  error_if_nonfinite: the host waits for the norm, and gradients that a norm that is not finite
+    would spoil stay as they are."""
+    if float(norm_type) != 2.0:
+        raise ValueError(f"clip_grad_norm_: only the 2-norm, got {norm_type}")
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    if any(g.is_sparse for g in grads):
+        raise RuntimeError("clip_grad_norm_ does not support sparse gradients")
+    if error_if_nonfinite and not bool(grad_norm(grads, offset=offset).isfinite()):
+        raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
+    return clip_grads(grads, max_norm, offset=offset)
