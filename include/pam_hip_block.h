@@ -59,7 +59,7 @@ typedef struct {
 int pam_hip_rotary_fwd(const pam_hip_heads *parts, int count, const float *cos, const float *sin, long table_rows,
                        const long long *positions, long positions_sb, long positions_st, long batch, long tokens, long dim,
                        long rotated, int interleaved, float eps, float offset, void *stream);
-size_t pam_hip_rotary_bwd_workspace_bytes(const pam_hip_heads *parts, int count, long batch, long tokens, long dim);
+size_t pam_hip_rotary_bwd_workspace_bytes(const pam_hip_heads *parts, int count, long batch, long tokens, long dim, long rotated);
 int pam_hip_rotary_bwd(const pam_hip_heads *parts, int count, const float *cos, const float *sin, long table_rows,
                        const long long *positions, long positions_sb, long positions_st, long batch, long tokens, long dim,
                        long rotated, int interleaved, float eps, float offset, int approx_a, int approx_b, int approx_exp,

@@ -574,11 +574,7 @@ PYBIND11_MODULE(_pam_host, module)
     module.def("div", [](const Tensor& A, const Tensor& B, double offset, bool a, bool b) { return PairNode<true>::apply(A, B, offset, a, b); }, unlocked);
     module.def("unary", [](const Tensor& x, int64_t op, double number, double offset, bool a, bool e) { return UnaryNode::apply(x, op, number, offset, a, e); }, unlocked);
     module.def("layer", &call_layer, unlocked);
-    module.def("rotary", [](const Tensor& q, const std::optional<Tensor>& k, const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& positions,
-                            const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight, bool interleaved, double eps, double offset,
-                            bool a, bool b, bool e) {
-        return RotaryNode::apply(q, k, cos, sin, positions, q_weight, k_weight, interleaved, eps, offset, a, b, e);
-    }, unlocked);
+    module.def("rotary", &call_rotary, unlocked);
     module.def("clip", &clip, unlocked);
     module.def("adam_collect", &adam_collect);
 }

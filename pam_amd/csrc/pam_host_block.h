@@ -169,6 +169,24 @@ RotationArgs positions_of(const Rotation& r)
     return {reinterpret_cast<const long long*>(r.positions.data_ptr<int64_t>()), r.positions.dim() == 2 ? r.positions.stride(0) : 0, r.positions.stride(-1)};
 }
 
+// The rotation of the tensors x, made contiguous along a head (and so left in x), by the weights w, made contiguous.
+variable_list rotate(variable_list& x, variable_list& w, const Rotation& r)
+{
+    const OnDevice on(x[0]);
+    variable_list y;
+    pam_hip_heads parts[2];
+    for (size_t i = 0; i < x.size(); ++i) {
+        x[i] = heads_contiguous(x[i]);
+        if (w[i].defined()) w[i] = w[i].contiguous();
+        y.push_back(new_floats(x[i].sizes(), x[i]));
+        parts[i] = heads_of(x[i], w[i], y[i]);
+    }
+    const RotationArgs at = positions_of(r);
+    check_call(pam_hip_rotary_fwd(parts, (int)x.size(), data(r.cos), data(r.sin), r.cos.size(0), at.positions, at.sb, at.st, r.batch, r.tokens, r.dim, r.rotated,
+                                  r.interleaved, r.eps, r.offset, on.stream), "rotary_fwd");
+    return y;
+}
+
 struct RotaryNode : torch::autograd::Function<RotaryNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
                                  const std::optional<Tensor>& positions, const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight,
@@ -177,18 +195,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
         variable_list x{q}, w{q_weight.value_or(Tensor())};
         if (k) { x.push_back(*k); w.push_back(k_weight.value_or(Tensor())); }
         const Rotation r = rotation(x, w, cos, sin, positions.value_or(Tensor()), interleaved, eps, offset);
-        const OnDevice on(q);
-        variable_list y;
-        std::vector<pam_hip_heads> parts;
-        for (size_t i = 0; i < x.size(); ++i) {
-            x[i] = heads_contiguous(x[i]);
-            if (w[i].defined()) w[i] = w[i].contiguous();
-            y.push_back(new_floats(x[i].sizes(), x[i]));
-            parts.push_back(heads_of(x[i], w[i], y[i]));
-        }
-        const RotationArgs at = positions_of(r);
-        check_call(pam_hip_rotary_fwd(parts.data(), (int)parts.size(), data(r.cos), data(r.sin), r.cos.size(0), at.positions, at.sb, at.st, r.batch, r.tokens,
-                                      r.dim, r.rotated, r.interleaved, r.eps, r.offset, on.stream), "rotary_fwd");
+        const variable_list y = rotate(x, w, r);
         ctx->saved_data["count"] = (int64_t)x.size(); ctx->saved_data["positions"] = positions.has_value();
         ctx->saved_data["wq"] = q_weight.has_value(); ctx->saved_data["wk"] = k_weight.has_value();
         ctx->saved_data["interleaved"] = interleaved; ctx->saved_data["eps"] = eps; ctx->saved_data["offset"] = offset;
@@ -229,7 +236,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
         }
         const Rotation r = rotation(x, w, saved[4], saved[5], saved[6], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["offset"].toDouble());
         const RotationArgs at = positions_of(r);
-        const size_t bytes = pam_hip_rotary_bwd_workspace_bytes(parts.data(), (int)count, r.batch, r.tokens, r.dim);
+        const size_t bytes = pam_hip_rotary_bwd_workspace_bytes(parts.data(), (int)count, r.batch, r.tokens, r.dim, r.rotated);
         const Tensor ws = bytes ? new_floats({(int64_t)((bytes + 3) / 4)}, grads[0]) : Tensor();
         check_call(pam_hip_rotary_bwd(parts.data(), (int)count, data(r.cos), data(r.sin), r.cos.size(0), at.positions, at.sb, at.st, r.batch, r.tokens, r.dim,
                                       r.rotated, r.interleaved, r.eps, r.offset, f.a, f.b, f.e, data_or_null(ws), bytes, on.stream), "rotary_bwd");
@@ -237,6 +244,17 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
         return {dx[0], dx[1], Tensor(), Tensor(), Tensor(), dw[0], dw[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
+
+variable_list call_rotary(const Tensor& q, const std::optional<Tensor>& k, const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& positions,
+                          const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight, bool interleaved, double eps, double offset, bool a, bool b, bool e)
+{
+    const Tensor none;
+    if (wants_graph({&q, k ? &*k : &none, &cos, &sin, q_weight ? &*q_weight : &none, k_weight ? &*k_weight : &none}))
+        return RotaryNode::apply(q, k, cos, sin, positions, q_weight, k_weight, interleaved, eps, offset, a, b, e);
+    variable_list x{q}, w{q_weight.value_or(none)};
+    if (k) { x.push_back(*k); w.push_back(k_weight.value_or(none)); }
+    return rotate(x, w, rotation(x, w, cos, sin, positions.value_or(none), interleaved, eps, offset));
+}
 
 // ---------------------------------------------------------------- clipping
 

@@ -1,6 +1,18 @@
 // The rotation of queries' and keys' heads by their positions, after an optional norm of each head, and its gradient.
+//
+// Bound by memory: 8 bytes a value forward, 12 backward.  4 x 4096 tokens of 16 + 4 heads of 128, normed: forward 65 us (5.2 TB/s, what a
+// large copy reaches), forward and gradients with both weights' 182 us (160 at that rate).  A head is taken by a group of 2 ... 64 lanes, one unit each: four
+// pairs of a rotated part (two 128-bit loads, `rotated / 2` apart or side by side) or four values of the rest, so that a
+// pair's two values meet in one lane and the only exchange is the norm's sum over the group.  cos and sin are read per head; the heads of a
+// token follow each other, so that all but the first find them in the cache next to the compute unit.  A work-group stays with
+// one of the two tensors.  The backward pass runs as many work-groups as are resident, each over a share of the heads, and keeps
+// the weight's gradient of its columns in registers; one row of sums per work-group is left to the column sums (one term per value
+// written and read back instead made the pass a third longer in bytes).
+// The chain of primitives is computed as one integer addition each (Raw), behind tests that what goes in is of ordinary size; a
+// wavefront that meets a zero, an infinity or an extreme exponent computes its heads by the checked functions, with the same results.
+// Heads that do not come in fours, or of more than 64 units, take a wavefront each by the checked functions; so does a group's lanes
+// an exact gradient.
 #include <algorithm>
-#include <climits>
 
 #include "../../include/pam_hip_extra.h"
 #include "pam_activation.h"
@@ -11,131 +23,514 @@ using namespace pamdev;
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 
+struct PartArgs {
+    const float* x; long x_sb, x_st, x_sh;
+    const float* dy; long dy_sb, dy_st, dy_sh;
+    const float* weight;
+    float* y;
+    float* sums;                                  // backward: [work-groups of the part][dim] of the weight's gradient, or null
+    uint32_t rows, heads;                         // heads of all tokens (at most 2^30), of one
+    int groups;                                   // work-groups of the part
+};
 struct RotaryArgs {
-    pam_hip_heads part[2];
-    float* terms[2];                              // backward: per-head terms of the weights' gradients, [rows of the part][dim]
+    PartArgs part[2];
     const float* cos; const float* sin; long table_rows;
     const long long* positions; long p_sb, p_st;
-    long tokens, rows;
-    int heads, dim, half, interleaved;            // heads: of both parts
+    uint32_t tokens;
+    int dim, half, interleaved, lanes;            // lanes: of a group
     float eps, off; bool has_off;
     ApproxFlags flags;
 };
 
-// A head: its values, its outputs, the rows of the tables.
+// The primitives as single integer additions: with signs and exponents in place a (*) b is bits(a) + bits(b) - bias, a (/) b is
+// bits(a) - bits(b) + bias, and an offset is one more constant in either.  That holds while operands and results are normal numbers, which the
+// callers make sure of by windows on what goes in: exponents of [first, last) per kind of value, chosen so that no result of
+// the chain leaves the normal range, whatever the values in them.
+struct Raw {
+    uint32_t mul_add, div_add;
+    __device__ __forceinline__ explicit Raw(float off) : mul_add(f2u(off) - 2u * kBias), div_add(f2u(off)) {}
+    __device__ __forceinline__ float mul(float a, float b) const { return u2f(f2u(a) + f2u(b) + mul_add); }
+    __device__ __forceinline__ float div(float a, float b) const { return u2f(f2u(a) - f2u(b) + div_add); }
+};
+template <int FIRST, int LAST>                    // magnitudes 2^FIRST <= |v| < 2^LAST: one shift-add and a max per value
+struct Window {
+    uint32_t most = 0;
+    __device__ __forceinline__ void see(float v) { most = max(most, (f2u(v) << 1) - ((uint32_t)(FIRST + 127) << 24)); }
+    __device__ __forceinline__ void see(const v4f& v) { see(v[0]); see(v[1]); see(v[2]); see(v[3]); }
+    __device__ __forceinline__ bool held() const { return most < ((uint32_t)(LAST - FIRST) << 24); }
+};
+// With x in 2^[-20, 20), its root in 2^[-14, 21), w in 2^[-10, 10), dz in 2^[-44, 20): x / root in 2^[-42, 35), x / root / root in
+// 2^[-64, 50), dz w in 2^[-55, 31), their product in 2^[-120, 82); the offset, between 3/4 and 3/2, is in at most five factors of it.  Heads
+// without a norm: x or dy in 2^[-60, 60), times a table's value.
+typedef Window<-20, 20> WindowX;
+typedef Window<-14, 21> WindowRoot;
+typedef Window<-10, 10> WindowW;
+typedef Window<-44, 20> WindowGrad;
+typedef Window<-40, 4> WindowTable;
+typedef Window<-60, 60> WindowPlain;
+typedef Window<-80, 60> WindowSquare;             // the gradient for x (*) x: times x it is in 2^[-101, 81)
+typedef Window<-50, 50> WindowRootGrad;           // between it and the root's there are the root, v in 2^[-28, 42) and the count
+typedef Window<-24, 8> WindowLog;                 // log2 v: not zero
+
+// A head: its values, the rows of the tables.
 struct Head {
-    int part; long row;                           // which tensor, which of its heads
-    const float* x; const float* dy; const float* weight;
-    float* y;
+    const float* x; const float* dy; float* y;
     const float* cos; const float* sin;           // null: no such position
 };
-__device__ __forceinline__ Head find_head(const RotaryArgs& a, long row)
+__device__ __forceinline__ Head find_head(const RotaryArgs& a, const PartArgs& p, uint32_t row)
 {
     Head h;
-    const long token = row / a.heads, b = token / a.tokens, t = token - b * a.tokens;
-    long at = row - token * a.heads;
-    h.part = at >= a.part[0].heads ? 1 : 0;
-    const pam_hip_heads& p = a.part[h.part];
-    if (h.part) at -= a.part[0].heads;
-    h.row = token * p.heads + at;
-    h.x = p.x + b * p.x_sb + t * p.x_st + at * p.x_sh;
-    h.dy = p.dy ? p.dy + b * p.dy_sb + t * p.dy_st + at * p.dy_sh : nullptr;
-    h.weight = p.weight;
-    h.y = p.y + h.row * a.dim;
-    const long long pos = a.positions ? a.positions[b * a.p_sb + t * a.p_st] : t;
+    const uint32_t token = row / p.heads, at = row - token * p.heads, b = token / a.tokens, t = token - b * a.tokens;
+    h.x = p.x + (long)b * p.x_sb + (long)t * p.x_st + (long)at * p.x_sh;
+    h.dy = p.dy ? p.dy + (long)b * p.dy_sb + (long)t * p.dy_st + (long)at * p.dy_sh : nullptr;
+    h.y = p.y + (long)row * a.dim;
+    const long long pos = a.positions ? a.positions[(long)b * a.p_sb + (long)t * a.p_st] : (long long)t;
     const bool there = pos >= 0 && pos < a.table_rows;
     h.cos = there ? a.cos + pos * a.half : nullptr;
     h.sin = there ? a.sin + pos * a.half : nullptr;
     return h;
 }
 
-__device__ __forceinline__ float wave_sum(float v)
+__device__ __forceinline__ float group_sum(float v, int lanes)
 {
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
+    for (int s = lanes / 2; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
     return v;
 }
 
-// mean(x (*) x) + eps and its root, over the wavefront
+// mean(x (*) x) + eps and its root, from the sum
 struct Root { float sum, variance, root; };
-__device__ __forceinline__ Root head_root(const RotaryArgs& a, const float* x, int lane)
+__device__ __forceinline__ Root root_of(const RotaryArgs& a, float sum)
 {
-    float sum = 0.0f;
-    for (int i = lane; i < a.dim; i += 64) sum += pam_mul_off(x[i], x[i], a.off, a.has_off);
     Root r;
-    r.sum = wave_sum(sum);
-    r.variance = pad_div_off(r.sum, (float)a.dim, a.off, a.has_off) + a.eps;
+    r.sum = sum;
+    r.variance = pad_div_off(sum, (float)a.dim, a.off, a.has_off) + a.eps;
     r.root = pow_half(r.variance, a.off, a.has_off);
     return r;
 }
-__device__ __forceinline__ float normed(const RotaryArgs& a, float x, float root) { return pad_div_off(x, root, a.off, a.has_off); }
-
-__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a)
+// The gradient for every x (*) x from that of the root: pow(v, 0.5) = 2^(log2(v) (*) 0.5), zero where v is zero; then the mean's quotient.
+__device__ __forceinline__ float square_grad(const RotaryArgs& a, const ApproxFlags& f, const Root& r, float droot)
 {
-    const long row = (long)blockIdx.x * kWaves + threadIdx.x / 64;
-    const int lane = threadIdx.x % 64;
-    if (row >= a.rows) return;
-    const Head h = find_head(a, row);
-    const float root = h.weight ? head_root(a, h.x, lane).root : 1.0f;
-    auto value = [&](int i) { return h.weight ? pam_mul_off(normed(a, h.x[i], root), h.weight[i], a.off, a.has_off) : h.x[i]; };
-    for (int p = lane; p < a.half; p += 64) {
-        const int i = a.interleaved ? 2 * p : p, j = a.interleaved ? 2 * p + 1 : p + a.half;
-        const float z1 = value(i), z2 = value(j);
-        const float c = h.cos ? h.cos[p] : u2f(kQNaN), s = h.sin ? h.sin[p] : u2f(kQNaN);
-        h.y[i] = pam_mul_off(z1, c, a.off, a.has_off) - pam_mul_off(z2, s, a.off, a.has_off);
-        h.y[j] = pam_mul_off(z2, c, a.off, a.has_off) + pam_mul_off(z1, s, a.off, a.has_off);
-    }
-    for (int i = 2 * a.half + lane; i < a.dim; i += 64) h.y[i] = value(i);
-}
-
-// The gradient: dz from dy by the rotation's products, then through weight, quotient, root, mean and square.
-__global__ __launch_bounds__(kThreads) void rotary_bwd_kernel(RotaryArgs a)
-{
-    const long row = (long)blockIdx.x * kWaves + threadIdx.x / 64;
-    const int lane = threadIdx.x % 64;
-    if (row >= a.rows) return;
-    const Head h = find_head(a, row);
-    const float off = a.off;
-    const bool has_off = a.has_off, norm = h.weight != nullptr;
-    const ApproxFlags f = a.flags;
-    const Root r = norm ? head_root(a, h.x, lane) : Root{0.0f, 0.0f, 1.0f};
-    float* terms = a.terms[h.part] ? a.terms[h.part] + h.row * a.dim : nullptr;
-    auto n_of = [&](int i) { return normed(a, h.x[i], r.root); };
-    auto z_of = [&](int i) { return norm ? pam_mul_off(n_of(i), h.weight[i], off, has_off) : h.x[i]; };
-    // calls to(i, dz of value i) for the lane's values
-    auto walk = [&](auto to) {
-        for (int p = lane; p < a.half; p += 64) {
-            const int i = a.interleaved ? 2 * p : p, j = a.interleaved ? 2 * p + 1 : p + a.half;
-            const float z1 = z_of(i), z2 = z_of(j), d1 = h.dy[i], d2 = h.dy[j];
-            const float c = h.cos ? h.cos[p] : u2f(kQNaN), s = h.sin ? h.sin[p] : u2f(kQNaN);
-            to(i, mul_grad(z1, c, d1, f.a, off, has_off) + mul_grad(z1, s, d2, f.a, off, has_off));
-            to(j, mul_grad(z2, c, d2, f.a, off, has_off) + mul_grad(z2, s, -d1, f.a, off, has_off));
-        }
-        for (int i = 2 * a.half + lane; i < a.dim; i += 64) to(i, h.dy[i]);
-    };
-    if (!norm) {
-        walk([&](int i, float dz) { h.y[i] = dz; });
-        return;
-    }
-    float droot = 0.0f;
-    walk([&](int i, float dz) {
-        const float n = n_of(i);
-        if (terms) terms[i] = mul_grad(h.weight[i], n, dz, f.b, off, has_off);
-        droot += div_grad_b(h.x[i], r.root, mul_grad(n, h.weight[i], dz, f.a, off, has_off), f.b, off, has_off);
-    });
-    droot = wave_sum(droot);
-    // pow(v, 0.5) = 2^(log2(v) (*) 0.5), zero where v is zero; then the mean's quotient
+    const float off = a.off; const bool has_off = a.has_off;
     const float l = log2_entry(r.variance, off, has_off), t = pam_mul_off(l, 0.5f, off, has_off);
     const float dt = exp2_grad(t, exp2_entry(t, off, has_off), r.variance == 0.0f ? 0.0f : droot, f.e, off, has_off);
     const float dl = mul_grad(l, 0.5f, dt, f.a, off, has_off);
     const float dv = f.e ? pad_div_off(pad_div_off(dl, r.variance, off, has_off), kActLn2, off, has_off) : log2_entry_bwd(r.variance, dl, off, has_off);
-    const float dsquare = div_grad_a(r.sum, (float)a.dim, dv, f.a, off, has_off);
-    walk([&](int i, float dz) {
-        const float x = h.x[i], n = n_of(i);
-        const float through = div_grad_a(x, r.root, mul_grad(n, h.weight[i], dz, f.a, off, has_off), f.a, off, has_off);
-        h.y[i] = through + (mul_grad(x, x, dsquare, f.a, off, has_off) + mul_grad(x, x, dsquare, f.b, off, has_off));
-    });
+    return div_grad_a(r.sum, (float)a.dim, dv, f.a, off, has_off);
+}
+
+// ---------------------------------------------------------------- value by value, by the checked functions
+
+// A head's output, or its gradient with any slopes, computed by `lanes` lanes with a pair or a value at a time.
+__device__ __forceinline__ Root head_root(const RotaryArgs& a, const float* x, int lane, int lanes)
+{
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int i = lane; i < a.dim; i += lanes) sum += pam_mul_off(x[i], x[i], a.off, a.has_off);
+    return root_of(a, group_sum(sum, lanes));
+}
+
+__device__ __forceinline__ void forward_by_value(const RotaryArgs& a, const float* weight, const Head& h, int lane, int lanes, bool store)
+{
+    const float root = weight ? head_root(a, h.x, lane, lanes).root : 1.0f;
+    if (!store) return;
+    auto value = [&](int i) { return weight ? pam_mul_off(pad_div_off(h.x[i], root, a.off, a.has_off), weight[i], a.off, a.has_off) : h.x[i]; };
+#pragma unroll 1
+    for (int q = lane; q < a.half; q += lanes) {
+        const int i = a.interleaved ? 2 * q : q, j = a.interleaved ? 2 * q + 1 : q + a.half;
+        const float z1 = value(i), z2 = value(j);
+        const float c = h.cos ? h.cos[q] : u2f(kQNaN), s = h.sin ? h.sin[q] : u2f(kQNaN);
+        h.y[i] = pam_mul_off(z1, c, a.off, a.has_off) - pam_mul_off(z2, s, a.off, a.has_off);
+        h.y[j] = pam_mul_off(z2, c, a.off, a.has_off) + pam_mul_off(z1, s, a.off, a.has_off);
+    }
+#pragma unroll 1
+    for (int i = 2 * a.half + lane; i < a.dim; i += lanes) h.y[i] = value(i);
+}
+
+// term(i, t): the weight's gradient gets t at value i from this head.  APPROXIMATE: all slopes are.
+template <bool APPROXIMATE, class Term>
+__device__ __forceinline__ void backward_by_value(const RotaryArgs& a, const float* weight, const Head& h, int lane, int lanes, bool store, Term term)
+{
+    const float off = a.off;
+    const bool has_off = a.has_off, norm = weight != nullptr;
+    const ApproxFlags f = APPROXIMATE ? ApproxFlags{true, true, true} : a.flags;
+    const Root r = norm ? head_root(a, h.x, lane, lanes) : Root{0.0f, 0.0f, 1.0f};
+    float droot = 0.0f, dsquare = 0.0f;
+    // first the weight's gradient and the root's, then x's (one loop over both, so that the code is there once)
+#pragma unroll 1
+    for (int round = norm ? 0 : 1; round < 2; ++round) {
+        auto take = [&](int i, float x, float n, float dz) {
+            const float dn = norm ? mul_grad(n, weight[i], dz, f.a, off, has_off) : dz;
+            if (round == 0) {
+                if (store) term(i, mul_grad(weight[i], n, dz, f.b, off, has_off));
+                droot += div_grad_b(x, r.root, dn, f.b, off, has_off);
+            } else if (store) {
+                h.y[i] = norm ? div_grad_a(x, r.root, dn, f.a, off, has_off) + (mul_grad(x, x, dsquare, f.a, off, has_off) + mul_grad(x, x, dsquare, f.b, off, has_off)) : dn;
+            }
+        };
+#pragma unroll 1
+        for (int q = lane; q < a.half; q += lanes) {
+            const int i = a.interleaved ? 2 * q : q, j = a.interleaved ? 2 * q + 1 : q + a.half;
+            const float x1 = h.x[i], x2 = h.x[j], d1 = h.dy[i], d2 = h.dy[j];
+            const float n1 = norm ? pad_div_off(x1, r.root, off, has_off) : x1, n2 = norm ? pad_div_off(x2, r.root, off, has_off) : x2;
+            const float z1 = norm ? pam_mul_off(n1, weight[i], off, has_off) : x1, z2 = norm ? pam_mul_off(n2, weight[j], off, has_off) : x2;
+            const float c = h.cos ? h.cos[q] : u2f(kQNaN), s = h.sin ? h.sin[q] : u2f(kQNaN);
+            take(i, x1, n1, mul_grad(z1, c, d1, f.a, off, has_off) + mul_grad(z1, s, d2, f.a, off, has_off));
+            take(j, x2, n2, mul_grad(z2, c, d2, f.a, off, has_off) + mul_grad(z2, s, -d1, f.a, off, has_off));
+        }
+#pragma unroll 1
+        for (int i = 2 * a.half + lane; i < a.dim; i += lanes) {
+            const float x = h.x[i];
+            take(i, x, norm ? pad_div_off(x, r.root, off, has_off) : x, h.dy[i]);
+        }
+        if (round == 0) dsquare = square_grad(a, f, r, group_sum(droot, lanes));
+    }
+}
+
+// ---------------------------------------------------------------- a group of lanes per head
+
+// What a lane has of a head: four pairs, or four values that are not rotated (in u[0]), or nothing.
+struct Unit {
+    bool there, rotates;
+    int first, second;                            // where its vectors begin
+    int table;                                    // ... in the tables' rows
+    __device__ __forceinline__ Unit(const RotaryArgs& a, int unit)
+    {
+        const int turning = a.half / 4, rest = (a.dim - 2 * a.half) / 4;
+        there = unit < turning + rest;
+        rotates = unit < turning;
+        table = min(unit, max(turning - 1, 0)) * 4;
+        first = rotates ? (a.interleaved ? 2 : 1) * table : 2 * a.half + (there ? unit - turning : 0) * 4;
+        second = rotates ? (a.interleaved ? first + 4 : first + a.half) : first;
+        if (!there) first = second = 0;
+    }
+};
+template <bool INTERLEAVED> __device__ __forceinline__ void to_pairs(const v4f (&u)[2], float (&z1)[4], float (&z2)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        z1[i] = INTERLEAVED ? u[i / 2][2 * (i % 2)] : u[0][i];
+        z2[i] = INTERLEAVED ? u[i / 2][2 * (i % 2) + 1] : u[1][i];
+    }
+}
+template <bool INTERLEAVED> __device__ __forceinline__ void from_pairs(const float (&z1)[4], const float (&z2)[4], v4f (&u)[2])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (INTERLEAVED) { u[i / 2][2 * (i % 2)] = z1[i]; u[i / 2][2 * (i % 2) + 1] = z2[i]; }
+        else { u[0][i] = z1[i]; u[1][i] = z2[i]; }
+    }
+}
+__device__ __forceinline__ void load_unit(const float* base, const Unit& at, v4f (&u)[2])
+{
+    u[0] = *reinterpret_cast<const v4f_any*>(base + at.first);
+    u[1] = *reinterpret_cast<const v4f_any*>(base + at.second);
+}
+__device__ __forceinline__ void store_unit(float* base, const Unit& at, const v4f (&u)[2])
+{
+    if (at.there) __builtin_nontemporal_store(u[0], reinterpret_cast<v4f_any*>(base + at.first));
+    if (at.rotates) __builtin_nontemporal_store(u[1], reinterpret_cast<v4f_any*>(base + at.second));
+}
+__device__ __forceinline__ void load_table(const Head& h, const Unit& at, bool any, v4f& c, v4f& s)
+{
+    const float nan = u2f(kQNaN);
+    c = s = v4f{nan, nan, nan, nan};
+    if (any && h.cos) { c = *reinterpret_cast<const v4f_any*>(h.cos + at.table); s = *reinterpret_cast<const v4f_any*>(h.sin + at.table); }
+}
+
+__device__ __forceinline__ float square_sum(const Raw& ar, const RotaryArgs& a, const Unit& at, const v4f (&x)[2])
+{
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[v] += ar.mul(x[v][i], x[v][i]);
+    return group_sum((at.there ? sum[0] : 0.0f) + (at.rotates ? sum[1] : 0.0f), a.lanes);
+}
+
+// root_of and the approximate square_grad as integer additions; `held`: all in their windows.
+struct RawRoot { float variance, root; bool held; };
+__device__ __forceinline__ RawRoot raw_root_of(const Raw& ar, const RotaryArgs& a, float sum)
+{
+    RawRoot r;
+    r.variance = ar.div(sum, (float)a.dim) + a.eps;
+    const float l = ar.div((float)((int)f2u(r.variance) - (int)kBias) * 0x1p-23f, 1.0f), t = ar.mul(ar.mul(l, 0.5f), 1.0f), whole = floorf(t);
+    r.root = u2f((uint32_t)((int)whole + 127) << 23) * ((1.0f + t) - whole);
+    WindowLog log;
+    WindowRoot root;
+    WindowPlain variance;
+    log.see(l); root.see(r.root); variance.see(r.variance);
+    r.held = log.held() && root.held() && variance.held() && r.variance > 0.0f;
+    return r;
+}
+__device__ __forceinline__ float raw_square_grad(const Raw& ar, const RotaryArgs& a, const RawRoot& r, float droot)
+{
+    const float dl = ar.mul(ar.mul(ar.mul(r.root, kActLn2), droot), 0.5f);
+    return ar.mul(ar.div(1.0f, (float)a.dim), ar.div(ar.div(dl, r.variance), kActLn2));
+}
+
+// The token at position 0 has sines of zero.  Its products with them are left out; the tests see one in their place.
+__device__ __forceinline__ bool stands_still(v4f& s)
+{
+    const bool still = ((f2u(s[0]) | f2u(s[1]) | f2u(s[2]) | f2u(s[3])) << 1) == 0u;
+    if (still) s = v4f{1.0f, 1.0f, 1.0f, 1.0f};
+    return still;
+}
+
+// Whether `here` is true in all lanes of the group.
+__device__ __forceinline__ bool in_group(bool here, int lanes)
+{
+    const uint64_t group = (lanes == 64 ? ~0ull : (1ull << lanes) - 1ull) << (threadIdx.x % 64 & ~(lanes - 1));
+    return (__ballot(here) & group) == group;
+}
+__device__ __forceinline__ bool all_zero(const v4f (&u)[2])
+{
+    uint32_t any = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) any |= f2u(u[i / 4][i % 4]);
+    return (any << 1) == 0u;
+}
+
+// What a lane knows of the head's weight: its values, and whether they are in their window.
+struct Weight { v4f w[2]; bool norm, held; };
+__device__ __forceinline__ Weight load_weight(const float* weight, const Unit& at)
+{
+    Weight r{{}, weight != nullptr, true};
+    if (!r.norm) return r;
+    load_unit(weight, at, r.w);
+    WindowW window;
+    window.see(r.w[0]); window.see(r.w[1]);
+    r.held = window.held();
+    return r;
+}
+// offsets that the windows above allow for
+__device__ __forceinline__ bool usual_offset(float off) { return off > 0.75f && off < 1.5f; }
+
+// y of a lane's unit; false if a value of the wavefront is outside its window, and y is then not computed.
+template <bool INTERLEAVED>
+__device__ __forceinline__ bool forward_head(const RotaryArgs& a, const Unit& at, const v4f (&x)[2], const Weight& w, const v4f& c, v4f s, v4f (&y)[2])
+{
+    const Raw ar(a.off);
+    const bool still = stands_still(s);
+    WindowTable tables;
+    if (at.rotates) { tables.see(c); tables.see(s); }
+    bool held = usual_offset(a.off) && tables.held() && w.held;
+    y[0] = x[0]; y[1] = x[1];
+    if (w.norm) {
+        WindowX seen;
+        seen.see(x[0]); seen.see(x[1]);
+        const RawRoot r = raw_root_of(ar, a, square_sum(ar, a, at, x));
+        held = held && seen.held() && r.held;
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[v][i] = ar.mul(ar.div(x[v][i], r.root), w.w[v][i]);
+    } else if (at.rotates) {
+        WindowPlain seen;
+        seen.see(x[0]); seen.see(x[1]);
+        held = held && seen.held();
+    }
+    if (at.rotates) {
+        float z1[4], z2[4], y1[4], y2[4];
+        to_pairs<INTERLEAVED>(y, z1, z2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y1[i] = ar.mul(z1[i], c[i]) - (still ? 0.0f : ar.mul(z2[i], s[i]));
+            y2[i] = ar.mul(z2[i], c[i]) + (still ? 0.0f : ar.mul(z1[i], s[i]));
+        }
+        from_pairs<INTERLEAVED>(y1, y2, y);
+    }
+    return __ballot(!held) == 0ull;
+}
+
+template <bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a)
+{
+    const bool other = (int)blockIdx.x >= a.part[0].groups;
+    const PartArgs& p = other ? a.part[1] : a.part[0];
+    const int lanes = a.lanes;
+    const Unit at(a, threadIdx.x & (lanes - 1));
+    // (lanes of heads past the end go along with the last head, for the sums over a group, and store nothing)
+    const uint32_t mine = (blockIdx.x - (other ? a.part[0].groups : 0)) * (kThreads / lanes) + threadIdx.x / lanes;
+    const Head h = find_head(a, p, min(mine, p.rows - 1));
+    v4f x[2], c, s, y[2];
+    load_unit(h.x, at, x);
+    const Weight w = load_weight(p.weight, at);
+    load_table(h, at, a.half > 0, c, s);
+    if (!forward_head<INTERLEAVED>(a, at, x, w, c, s, y)) forward_by_value(a, p.weight, h, threadIdx.x & (lanes - 1), lanes, mine < p.rows);
+    else if (mine < p.rows) store_unit(h.y, at, y);
+}
+
+// The gradient with all approximate slopes, where a product's is its other factor.  term: the weight's gradient.  False as above.
+template <bool INTERLEAVED>
+__device__ __forceinline__ bool backward_head(const RotaryArgs& a, const Unit& at, const v4f (&x)[2], v4f (&d)[2], const Weight& w, const v4f& c, v4f s,
+                                              v4f (&dx)[2], v4f (&term)[2])
+{
+    const Raw ar(a.off);
+    // (a token that the loss leaves out: behind a norm the gradients of such a head are zeros, the tests see ones in their place)
+    const bool nothing = w.norm && in_group(all_zero(d), a.lanes);
+    if (nothing) d[0] = d[1] = v4f{1.0f, 1.0f, 1.0f, 1.0f};
+    const bool still = stands_still(s);
+    bool held = usual_offset(a.off) && w.held;
+    dx[0] = d[0]; dx[1] = d[1];
+    if (at.rotates) {
+        WindowTable tables;
+        WindowPlain seen;
+        tables.see(c); tables.see(s); seen.see(d[0]); seen.see(d[1]);
+        held = held && tables.held() && seen.held();
+        float d1[4], d2[4], z1[4], z2[4];
+        to_pairs<INTERLEAVED>(d, d1, d2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            z1[i] = ar.mul(d1[i], c[i]) + (still ? 0.0f : ar.mul(d2[i], s[i]));
+            z2[i] = ar.mul(d2[i], c[i]) - (still ? 0.0f : ar.mul(d1[i], s[i]));
+        }
+        from_pairs<INTERLEAVED>(z1, z2, dx);
+    }
+    if (w.norm) {
+        WindowX seen;
+        WindowGrad grads;
+        seen.see(x[0]); seen.see(x[1]); grads.see(dx[0]); grads.see(dx[1]);
+        const RawRoot r = raw_root_of(ar, a, square_sum(ar, a, at, x));
+        float through[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float n = ar.div(x[v][i], r.root), dz = dx[v][i];
+                dx[v][i] = ar.mul(dz, w.w[v][i]);
+                term[v][i] = ar.mul(dz, n);
+                through[v] -= ar.mul(ar.div(n, r.root), dx[v][i]);
+            }
+        const float droot = group_sum((at.there ? through[0] : 0.0f) + (at.rotates ? through[1] : 0.0f), a.lanes);
+        const float dsquare = raw_square_grad(ar, a, r, droot), inverse = ar.div(1.0f, r.root);
+        WindowSquare squares;
+        WindowRootGrad root_grads;
+        squares.see(dsquare); root_grads.see(droot);
+        held = held && seen.held() && grads.held() && r.held && squares.held() && root_grads.held();
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float q = ar.mul(dsquare, x[v][i]);
+                dx[v][i] = nothing ? 0.0f : ar.mul(inverse, dx[v][i]) + (q + q);
+                term[v][i] = nothing ? 0.0f : term[v][i];
+            }
+    }
+    return __ballot(!held) == 0ull;
+}
+
+// LDS accesses of a wavefront's lanes to each other's values stay in order.
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wavefront notes the heads that it could not do by raw additions and computes them behind a run of kRun turns, where the
+// registers of the usual path are free.  (Within its loop the checked functions' many cases cost that path 137 registers and scalar
+// spills, three wavefronts per SIMD; called as a function, the callee's registers counted.)
+constexpr int kRun = 32;
+
+template <bool INTERLEAVED, bool APPROXIMATE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void rotary_bwd_kernel(RotaryArgs a)
+{
+    __shared__ float held[kThreads * 8];          // the weight's gradient of every group: at most 8 values a lane
+    const bool other = (int)blockIdx.x >= a.part[0].groups;
+    const PartArgs& p = other ? a.part[1] : a.part[0];
+    const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = kThreads / lanes;
+    const int work_group = (int)blockIdx.x - (other ? a.part[0].groups : 0);
+    const uint32_t rows = p.rows, step = (uint32_t)(p.groups * groups), first = (uint32_t)(work_group * groups + group);
+    const int turns = (int)((rows - (uint32_t)(work_group * groups) + step - 1) / step);
+    float* mine = held + group * a.dim;
+    for (int i = lane; i < a.dim; i += lanes) mine[i] = 0.0f;
+    wave_fence();
+    auto head = [&](int turn) __attribute__((always_inline)) {
+        return find_head(a, p, min(first + turn * step, rows - 1));      // (past the end: along with the last head, and nothing stored)
+    };
+#pragma unroll 1
+    for (int run = 0; run < turns; run += kRun) {
+        const int end = min(run + kRun, turns);
+        uint32_t odd = ~0u;
+        if constexpr (APPROXIMATE) {
+            odd = 0u;
+            const Unit at(a, lane);
+            const Weight w = load_weight(p.weight, at);
+            v4f sum[2] = {};
+#pragma unroll 1
+            for (int turn = run; turn < end; ++turn) {
+                const Head h = head(turn);
+                v4f x[2] = {}, d[2], c, s, dx[2], term[2] = {};
+                load_unit(h.dy, at, d);
+                if (w.norm) load_unit(h.x, at, x);
+                load_table(h, at, a.half > 0, c, s);
+                if (!backward_head<INTERLEAVED>(a, at, x, d, w, c, s, dx, term)) { odd |= 1u << (turn - run); continue; }
+                if (first + turn * step < rows) {
+                    store_unit(h.y, at, dx);
+                    sum[0] += term[0]; sum[1] += term[1];
+                }
+            }
+            if (p.sums) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (at.there) mine[at.first + i] += sum[0][i];
+                    if (at.rotates) mine[at.second + i] += sum[1][i];
+                }
+                wave_fence();                     // (below, a value of the head may be another lane's than here)
+            }
+        }
+        odd = __builtin_amdgcn_readfirstlane(odd);
+#pragma unroll 1
+        for (int turn = run; turn < end; ++turn)
+            if ((odd >> (turn - run)) & 1u)
+                backward_by_value<APPROXIMATE>(a, p.weight, head(turn), lane, lanes, first + turn * step < rows, [&](int i, float t) { mine[i] += t; });
+        wave_fence();
+    }
+    if (!p.sums) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.dim; i += kThreads) {
+        float total = held[i];
+        for (int g = 1; g < groups; ++g) total += held[g * a.dim + i];
+        p.sums[(long)work_group * a.dim + i] = total;
+    }
+}
+
+// ---------------------------------------------------------------- a wavefront per head: any size
+
+template <bool BACKWARD>
+__global__ __launch_bounds__(kThreads) void any_rotary_kernel(RotaryArgs a)
+{
+    const bool other = (int)blockIdx.x >= a.part[0].groups;
+    const PartArgs& p = other ? a.part[1] : a.part[0];
+    const uint32_t row = (blockIdx.x - (other ? a.part[0].groups : 0)) * kWaves + threadIdx.x / 64;
+    const int lane = threadIdx.x % 64;
+    if (row >= p.rows) return;
+    const Head h = find_head(a, p, row);
+    float* terms = p.sums ? p.sums + (long)row * a.dim : nullptr;      // (one row per head)
+    if (BACKWARD) backward_by_value<false>(a, p.weight, h, lane, 64, true, [&](int i, float t) { if (terms) terms[i] = t; });
+    else forward_by_value(a, p.weight, h, lane, 64, true);
+}
+
+// ---------------------------------------------------------------- host
+
+// Lanes of a group: the power of two that holds a head's units; 0: the head takes the kernels for any size.
+int lanes_for(long dim, long rotated)
+{
+    if (rotated % 8 != 0 || dim % 4 != 0) return 0;
+    const long units = rotated / 8 + (dim - rotated) / 4;
+    if (units > 64) return 0;
+    int lanes = 2;
+    while (lanes < units) lanes *= 2;
+    return lanes;
+}
+constexpr long kBackwardGroups = 1024;            // work-groups of a backward launch: the four per compute unit that are resident
+// work-groups of a part of `rows` heads, of `all` heads in the launch
+long backward_groups(long rows, long all, int lanes)
+{
+    const long whole = (rows + kThreads / lanes - 1) / (kThreads / lanes);
+    return all == 0 ? 0 : std::min(whole, std::max(1L, (long)((double)kBackwardGroups * (double)rows / (double)all)));
 }
 
 int fill(const char* what, RotaryArgs& a, const pam_hip_heads* parts, int count, const float* cos, const float* sin, long table_rows,
@@ -147,22 +542,41 @@ int fill(const char* what, RotaryArgs& a, const pam_hip_heads* parts, int count,
         return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: negative size", what);
     if (rotated % 2 != 0 || rotated > dim) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the rotated part is an even number of a head's values", what);
     const long heads = parts[0].heads + (count > 1 ? parts[1].heads : 0);
-    if (batch > (1L << 30) || tokens > (1L << 30) || dim > (1L << 20) || heads > (1L << 20) || (batch && tokens && heads > (1L << 40) / batch / tokens))
+    if (batch > (1L << 30) || tokens > (1L << 30) || dim > (1L << 20) || heads > (1L << 20) || (batch && tokens && heads > (1L << 30) / batch / tokens))
         return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: size out of range", what);
-    a.rows = batch * tokens * heads;
     for (int i = 0; i < 2; ++i) {
-        a.part[i] = i < count ? parts[i] : pam_hip_heads{};
-        a.terms[i] = nullptr;
-        if (a.rows && dim && a.part[i].heads && (!a.part[i].x || !a.part[i].y || (backward && !a.part[i].dy)))
-            return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
+        const pam_hip_heads h = i < count ? parts[i] : pam_hip_heads{};
+        a.part[i] = PartArgs{h.x, h.x_sb, h.x_st, h.x_sh, backward ? h.dy : nullptr, h.dy_sb, h.dy_st, h.dy_sh, h.weight, h.y, nullptr, (uint32_t)(batch * tokens * h.heads), (uint32_t)h.heads, 0};
+        if (a.part[i].rows && dim && (!h.x || !h.y || (backward && !h.dy))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
     }
-    if (a.rows && rotated && (!cos || !sin) && table_rows > 0) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
+    if (a.part[0].rows + a.part[1].rows && rotated && (!cos || !sin) && table_rows > 0) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
     a.cos = cos; a.sin = sin; a.table_rows = table_rows; a.positions = positions; a.p_sb = p_sb; a.p_st = p_st;
-    a.tokens = tokens; a.heads = (int)heads; a.dim = (int)dim; a.half = (int)(rotated / 2); a.interleaved = interleaved != 0;
+    a.tokens = (uint32_t)tokens; a.dim = (int)dim; a.half = (int)(rotated / 2); a.interleaved = interleaved != 0;
+    a.lanes = lanes_for(dim, rotated);
     a.eps = eps; a.off = offset; a.has_off = offset != 1.0f;
     a.flags = ApproxFlags{false, false, false};
-    if ((a.rows + kWaves - 1) / kWaves > INT_MAX) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: too many heads", what);
     return PAM_HIP_OK;
+}
+
+// Launches `grouped` kernels (or those for any size) over the parts' work-groups.
+template <class Kernel>
+int launch(const char* what, const RotaryArgs& a, Kernel kernel, void* stream)
+{
+    const long groups = (long)a.part[0].groups + a.part[1].groups;
+    if (groups == 0) return PAM_HIP_OK;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kThreads), 0, (hipStream_t)stream, a);
+    return pamhost::check_launch(what);
+}
+void whole_groups(RotaryArgs& a, int per_group) { for (PartArgs& p : a.part) p.groups = (int)((p.rows + per_group - 1) / per_group); }
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// Rows of sums that the backward pass leaves of a part: one per work-group, or per head.
+long sum_rows(const pam_hip_heads* parts, int count, int i, long batch, long tokens, long dim, long rotated)
+{
+    const long rows = batch * tokens * parts[i].heads, all = batch * tokens * (parts[0].heads + (count > 1 ? parts[1].heads : 0));
+    const int lanes = lanes_for(dim, rotated);
+    return lanes ? backward_groups(rows, all, lanes) : rows;
 }
 
 }  // namespace
@@ -175,20 +589,19 @@ int pam_hip_rotary_fwd(const pam_hip_heads* parts, int count, const float* cos, 
 {
     RotaryArgs a;
     const int rc = fill("rotary_fwd", a, parts, count, cos, sin, table_rows, positions, positions_sb, positions_st, batch, tokens, dim, rotated, interleaved, eps, offset, false);
-    if (rc != PAM_HIP_OK || a.rows == 0 || dim == 0) return rc;
-    hipLaunchKernelGGL(rotary_kernel, dim3((unsigned)((a.rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, (hipStream_t)stream, a);
-    return pamhost::check_launch("rotary_fwd");
+    if (rc != PAM_HIP_OK || dim == 0) return rc;
+    whole_groups(a, a.lanes ? kThreads / a.lanes : kWaves);
+    return launch("rotary_fwd", a, !a.lanes ? any_rotary_kernel<false> : interleaved ? rotary_kernel<true> : rotary_kernel<false>, stream);
 }
 
-static size_t terms_floats(const pam_hip_heads& p, long batch, long tokens, long dim) { return p.dweight ? (size_t)(batch * tokens * p.heads) * dim : 0; }
-
-size_t pam_hip_rotary_bwd_workspace_bytes(const pam_hip_heads* parts, int count, long batch, long tokens, long dim)
+size_t pam_hip_rotary_bwd_workspace_bytes(const pam_hip_heads* parts, int count, long batch, long tokens, long dim, long rotated)
 {
     size_t bytes = 0;
-    for (int i = 0; parts && i < count && i < 2; ++i) {
-        const long rows = batch * tokens * parts[i].heads;
-        if (parts[i].dweight) bytes += ((terms_floats(parts[i], batch, tokens, dim) * 4 + 255) & ~(size_t)255) + ((pam_hip_column_sums_workspace_bytes(rows, dim, 1) + 255) & ~(size_t)255);
-    }
+    for (int i = 0; parts && batch > 0 && tokens > 0 && i < count && i < 2; ++i)
+        if (parts[i].dweight) {
+            const long rows = sum_rows(parts, count, i, batch, tokens, dim, rotated);
+            bytes += align256((size_t)rows * dim * sizeof(float)) + align256(pam_hip_column_sums_workspace_bytes(rows, dim, 1));
+        }
     return bytes;
 }
 
@@ -200,24 +613,30 @@ int pam_hip_rotary_bwd(const pam_hip_heads* parts, int count, const float* cos, 
     int rc = fill("rotary_bwd", a, parts, count, cos, sin, table_rows, positions, positions_sb, positions_st, batch, tokens, dim, rotated, interleaved, eps, offset, true);
     if (rc != PAM_HIP_OK || dim == 0) return rc;
     a.flags = ApproxFlags{approx_a != 0, approx_b != 0, approx_exp != 0};
-    const size_t need = pam_hip_rotary_bwd_workspace_bytes(parts, count, batch, tokens, dim);
+    const size_t need = pam_hip_rotary_bwd_workspace_bytes(parts, count, batch, tokens, dim, rotated);
     if (need && (!workspace || workspace_bytes < need)) return pamhost::fail(PAM_HIP_ERR_WORKSPACE, "rotary_bwd: workspace of %zu bytes needed", need);
     char* at = (char*)workspace;
+    long rows[2] = {0, 0};
     for (int i = 0; i < count; ++i)
         if (parts[i].dweight) {
-            a.terms[i] = (float*)at;
-            at += (terms_floats(parts[i], batch, tokens, dim) * 4 + 255) & ~(size_t)255;
+            rows[i] = sum_rows(parts, count, i, batch, tokens, dim, rotated);
+            a.part[i].sums = (float*)at;
+            at += align256((size_t)rows[i] * dim * sizeof(float));
         }
-    if (a.rows) {
-        hipLaunchKernelGGL(rotary_bwd_kernel, dim3((unsigned)((a.rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, (hipStream_t)stream, a);
-        rc = pamhost::check_launch("rotary_bwd");
+    if (a.lanes) {
+        const long all = (long)a.part[0].rows + a.part[1].rows;
+        for (PartArgs& p : a.part) p.groups = (int)backward_groups(p.rows, all, a.lanes);
+        const bool approximate = a.flags.a && a.flags.b && a.flags.e;
+        rc = launch("rotary_bwd", a, !approximate ? rotary_bwd_kernel<false, false> : interleaved ? rotary_bwd_kernel<true, true> : rotary_bwd_kernel<false, true>, stream);
+    } else {
+        whole_groups(a, kWaves);
+        rc = launch("rotary_bwd", a, any_rotary_kernel<true>, stream);
     }
     for (int i = 0; i < count && rc == PAM_HIP_OK; ++i)
         if (parts[i].dweight) {
-            const long rows = batch * tokens * parts[i].heads;
-            const size_t bytes = pam_hip_column_sums_workspace_bytes(rows, dim, 1);
-            rc = pam_hip_column_sums(a.terms[i], dim, parts[i].dweight, nullptr, 0, nullptr, rows, dim, bytes ? at : nullptr, bytes, stream);
-            at += (bytes + 255) & ~(size_t)255;
+            const size_t bytes = pam_hip_column_sums_workspace_bytes(rows[i], dim, 1);
+            rc = pam_hip_column_sums(a.part[i].sums, dim, parts[i].dweight, nullptr, 0, nullptr, rows[i], dim, bytes ? at : nullptr, bytes, stream);
+            at += align256(bytes);
         }
     return rc;
 }
