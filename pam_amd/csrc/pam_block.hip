@@ -3,6 +3,7 @@
 
 #include "pam_activation.h"
 #include "pam_common.h"
+#include "pam_thin.h"
 
 using namespace pamdev;
 
@@ -74,6 +75,8 @@ int pam_hip_linear_act_fwd(const float* a, long a_sr, long a_sc, const float* w,
     if (rc != PAM_HIP_OK) return rc;
     if (m == 0 || n == 0) return PAM_HIP_OK;
     if (!y || (k > 0 && (!a || !w))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "linear_act_fwd: null pointer");
+    if (pamthin::takes(m, n, k, a_sc, w_sc))
+        return pamthin::launch("linear_act_fwd", pamthin::Layer{a, a_sr, w, w_sr, bias, residual, residual_sr, z, y, (int)m, (int)n, (int)k, activation, offset}, false, (hipStream_t)stream);
     float* sums = z ? z : y;
     rc = pam_hip_pam_linear_fwd(a, a_sr, a_sc, w, w_sc, w_sr, bias, sums, n, 1, m, n, k, offset, workspace, workspace_bytes, stream);
     if (rc != PAM_HIP_OK || (!z && !residual && activation == PAM_HIP_ACT_NONE)) return rc;
@@ -97,6 +100,8 @@ int pam_hip_gated_linear_fwd(const float* a, long a_sr, long a_sc, const float* 
     if (rc != PAM_HIP_OK) return rc;
     if (m == 0 || f == 0) return PAM_HIP_OK;
     if (!y || (k > 0 && (!a || !w))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "gated_linear_fwd: null pointer");
+    if (pamthin::takes(m, 2 * f, k, a_sc, w_sc))
+        return pamthin::launch("gated_linear_fwd", pamthin::Layer{a, a_sr, w, w_sr, bias, nullptr, 0, z, y, (int)m, (int)f, (int)k, activation, offset}, true, (hipStream_t)stream);
     if (!workspace || workspace_bytes < pam_hip_gated_linear_workspace_bytes(m, f, k))
         return pamhost::fail(PAM_HIP_ERR_WORKSPACE, "gated_linear_fwd: workspace of %zu bytes needed", pam_hip_gated_linear_workspace_bytes(m, f, k));
     const size_t held = align256((size_t)m * 2 * f * sizeof(float));
