@@ -29,39 +29,20 @@ def _flags(offset, approx_bwd):
     return float(_offset_value(offset)), bool(a), bool(b), bool(approx_bwd)
 
 
-def _rows(t, n, name):
-    if t.dim() < 1 or t.shape[-1] != n:
-        raise ValueError(f"{name}: the last dimension is {tuple(t.shape)[-1:]}, expected {n}")
-    return t.reshape(math.prod(t.shape[:-1]), n)
-
-
 def linear_act(X, W, bias=None, activation=None, residual=None, *, offset=None, approx_bwd=False, use_kernel=True):
     """activation(X W^T + bias) + residual in one product, X [..., d_in], W [d_out, d_in], residual of the result's shape.
 
     activation: None, "relu", "silu" (x over 1 + exp(-x), one quotient) or "gelu" (x over 1 + exp(-1.702 x)).  The sigmoid's
     exponent is held below 64, so that no x overflows it."""
     _require_kernel(X, use_kernel)
-    act = _activation(activation)
-    if W.dim() != 2:
-        raise ValueError(f"linear_act: the weight is a matrix, got {tuple(W.shape)}")
-    lead, n = X.shape[:-1], W.shape[0]
-    if residual is not None:
-        if residual.shape != (*lead, n):
-            raise ValueError(f"linear_act: the residual must have the shape of the result, got {tuple(residual.shape)} for {(*lead, n)}")
-        residual = _rows(residual, n, "linear_act")
-    out = _abi.host().layer(False, _rows(X, W.shape[1], "linear_act"), W, bias, act, residual, *_flags(offset, approx_bwd))
-    return out.view(*lead, n)
+    return _abi.host().layer(False, X, W, bias, _activation(activation), residual, *_flags(offset, approx_bwd))
 
 
 def gated_linear(X, W, bias=None, activation="silu", *, offset=None, approx_bwd=False, use_kernel=True):
     """activation(X Wg^T + bg) (*) (X Wu^T + bu): the first half of a gated feed-forward layer.  W [2 hidden, d_in] holds the
     gate's rows and then the other factor's, bias [2 hidden] likewise; the result is [..., hidden].  activation as for linear_act."""
     _require_kernel(X, use_kernel)
-    act = _activation(activation)
-    if W.dim() != 2 or W.shape[0] % 2:
-        raise ValueError(f"gated_linear: the weight is a matrix of the gate's rows and as many others, got {tuple(W.shape)}")
-    out = _abi.host().layer(True, _rows(X, W.shape[1], "gated_linear"), W, bias, act, None, *_flags(offset, approx_bwd))
-    return out.view(*X.shape[:-1], W.shape[0] // 2)
+    return _abi.host().layer(True, X, W, bias, _activation(activation), None, *_flags(offset, approx_bwd))
 
 
 def rotary_tables(positions, dim, base=10000.0, *, scaling=None, device=None):

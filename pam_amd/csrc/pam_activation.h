@@ -59,4 +59,93 @@ __device__ __forceinline__ float activation_grad(const Activation& act, float x,
     return div_grad_a(x, u, d, f.a, off, has_off) + mul_grad(x, c, dt, f.a, off, has_off);
 }
 
+// ---------------------------------------------------------------- the usual case
+
+// The primitives as single integer additions: with signs and exponents in place a (*) b is bits(a) + bits(b) - bias, a (/) b is
+// bits(a) - bits(b) + bias, and an offset, one more product or quotient of the result, is one more constant in either.  That holds while operands and results are normal numbers, which the
+// callers make sure of by windows on what goes in: exponents of [first, last) per kind of value, chosen so that no result of
+// a chain leaves the normal range, whatever the values in them.
+struct Raw {
+    uint32_t mul_add, div_add;
+    __device__ __forceinline__ explicit Raw(float off) : mul_add(f2u(off) - 2u * kBias), div_add(2u * kBias - f2u(off)) {}
+    __device__ __forceinline__ float mul(float a, float b) const { return u2f(f2u(a) + f2u(b) + mul_add); }
+    __device__ __forceinline__ float div(float a, float b) const { return u2f(f2u(a) - f2u(b) + div_add); }
+    // 2^t for |t| <= 126, t (*) 1 (*) offset first as the base-2 entry point has it
+    __device__ __forceinline__ float exp2(float t) const
+    {
+        const float x = mul(t, 1.0f), whole = floorf(x);
+        return u2f((uint32_t)((int)whole + 127) << 23) * ((1.0f + x) - whole);
+    }
+};
+template <int FIRST, int LAST>                    // magnitudes 2^FIRST <= |v| < 2^LAST: one shift-add and a max per value
+struct Window {
+    uint32_t most = 0;
+    __device__ __forceinline__ void see(float v) { most = max(most, (f2u(v) << 1) - ((uint32_t)(FIRST + 127) << 24)); }
+    __device__ __forceinline__ bool held() const { return most < ((uint32_t)(LAST - FIRST) << 24); }
+};
+// offsets that the windows allow for: at most a factor of 2^0.6 on each of a chain's results
+__device__ __forceinline__ bool usual_offset(float off) { return off > 0.75f && off < 1.5f; }
+
+__device__ __forceinline__ bool is_zero(float v) { return (f2u(v) << 1) == 0u; }
+// a (*) b by addition, zeros by the definition (the sign of the other operand)
+__device__ __forceinline__ float mul_or_zero(const Raw& ar, float a, float b)
+{
+    const bool za = is_zero(a), zb = is_zero(b);
+    const uint32_t sign = ((za ? 0u : f2u(a)) ^ (zb ? 0u : f2u(b))) & kSign;
+    return za || zb ? u2f(sign) : ar.mul(a, b);
+}
+
+// silu and gelu of zero and 2^-40 <= |x| < 16 by additions, with the offsets of usual_sigmoid_offset: t (*) offset lies within 44.3 of zero, u in
+// [1, 2^44.4), x (/) u in 2^[-41, 4).  For the gradient d, |d| in 2^[-40, 40), the smallest result is x (/) u (/) u (*) d at x = -16: above
+// 2^-125 with the largest offset, its own factors counted, and 2^-115 without one.  A zero x stands as 2^-40 (2^t is 1 there),
+// which leaves the gradient what it is.
+__device__ __forceinline__ bool usual_sigmoid_offset(float off) { return off > 0.9f && off < 1.06f; }
+typedef Window<-40, 4> WindowAct;
+typedef Window<-40, 40> WindowActGrad;
+struct RawSigmoid {
+    float x, t, e, u;
+    __device__ __forceinline__ RawSigmoid(const Raw& ar, float value, float scale)
+    {
+        x = is_zero(value) ? 0x1p-40f : value;
+        t = ar.mul(x, scale);
+        e = ar.exp2(t);
+        u = 1.0f + e;
+    }
+    __device__ __forceinline__ float result(const Raw& ar, float value) const { return is_zero(value) ? 0.0f : ar.div(x, u); }
+    __device__ __forceinline__ float grad(const Raw& ar, float d, float scale) const        // all slopes approximate; d not zero
+    {
+        const float du = -ar.mul(ar.div(ar.div(x, u), u), d), dt = ar.mul(ar.mul(e, kActLn2), du);
+        return ar.mul(ar.div(1.0f, u), d) + ar.mul(dt, scale);
+    }
+};
+
+// act(v) of a lane's values: by additions where all of the wavefront's are ordinary, else by the checked function, called.
+__device__ __noinline__ float any_activation(float x, int kind, float off) { return Activation{kind, off, off != 1.0f}(x); }
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int kind, float off)
+{
+    if (kind == PAM_HIP_ACT_NONE) return;
+    if (kind == PAM_HIP_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] <= 0.0f ? 0.0f : v[i];
+        return;
+    }
+    const float scale = kind == PAM_HIP_ACT_SILU ? kSiluScale : kGeluScale;
+    const Raw ar(off);
+    WindowAct seen;
+    float y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (!is_zero(v[i])) seen.see(v[i]);
+        y[i] = RawSigmoid(ar, v[i], scale).result(ar, v[i]);
+    }
+    if (__builtin_expect(__ballot(!seen.held() || !usual_sigmoid_offset(off)) == 0ull, 1)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = y[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = any_activation(v[i], kind, off);
+    }
+}
+
 }  // namespace pamdev

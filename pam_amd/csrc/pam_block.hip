@@ -3,6 +3,7 @@
 
 #include "pam_activation.h"
 #include "pam_common.h"
+#include "pam_gemm_layer.h"
 #include "pam_thin.h"
 
 using namespace pamdev;
@@ -13,44 +14,130 @@ constexpr int kThreads = 256;
 
 Activation activation_of(int kind, float offset) { return Activation{kind, offset, offset != 1.0f}; }
 bool known(int activation) { return activation >= PAM_HIP_ACT_NONE && activation <= PAM_HIP_ACT_GELU; }
-size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 unsigned groups_for(size_t values) { return (unsigned)std::min<size_t>((values + kThreads - 1) / kThreads, 1u << 20); }
 
-// y = act(z) + residual, m rows of n
-__global__ __launch_bounds__(kThreads) void act_kernel(const float* z, const float* __restrict__ residual, long residual_sr, float* y,
-                                                      size_t total, long n, Activation act)
+// The gradients for z: dz = [dg | du] of rows of f values (GATED), or of one row of all of them.
+//
+// Bound by memory, 12 bytes a value or 20 a gated one.  A lane takes four consecutive values (a row's last ones overlap the
+// ones before, written alike).  With all slopes approximate and every value of the
+// wavefront of ordinary size the chain is integer additions (pam_activation.h); otherwise the checked functions compute it value by value.
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+
+struct BwdArgs {
+    const float* z; const float* dy; float* dz;
+    long f;                                       // values of a row; GATED: of a half
+    uint32_t per_row, units;                      // lanes' shares of a row, of all rows
+    Activation act;
+    ApproxFlags flags;
+};
+
+template <bool GATED>
+__device__ __forceinline__ void bwd_value(const BwdArgs& a, float g, float u, float d, float& dg, float& du)
 {
-    for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (size_t)gridDim.x * kThreads) {
-        const float v = act(z[i]);
-        y[i] = residual ? v + residual[(long)(i / n) * residual_sr + (long)(i % n)] : v;
+    if (GATED) {
+        const float y = a.act(g);
+        du = mul_grad(u, y, d, a.flags.b, a.act.off, a.act.has_off);
+        d = mul_grad(y, u, d, a.flags.a, a.act.off, a.act.has_off);
+    }
+    dg = activation_grad(a.act, g, d, a.flags);
+}
+
+template <bool GATED>
+__global__ __launch_bounds__(kThreads) void act_bwd_kernel(BwdArgs a)
+{
+    const uint32_t unit = blockIdx.x * kThreads + threadIdx.x;
+    if (unit >= a.units) return;
+    const uint32_t row = GATED ? unit / a.per_row : 0u, share = GATED ? unit - row * a.per_row : unit;
+    const long column = min((long)share * 4, a.f - 4), at = (long)row * a.f + column, z_at = GATED ? at + (long)row * a.f : at;
+    const v4f g = *reinterpret_cast<const v4f_any*>(a.z + z_at), d = *reinterpret_cast<const v4f_any*>(a.dy + at);
+    const v4f u = GATED ? *reinterpret_cast<const v4f_any*>(a.z + z_at + a.f) : g;
+    v4f dg, du;
+    const bool sigmoid = a.act.kind >= PAM_HIP_ACT_SILU;
+    bool held = a.flags.a && a.flags.b && a.flags.e && usual_sigmoid_offset(a.act.off);
+    if (held) {
+        const Raw ar(a.act.off);
+        WindowAct gates;
+        WindowActGrad grads;                      // (and the gated product's operands: two of them make 2^[-80, 80))
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool nothing = is_zero(d[i]);
+            const RawSigmoid s(ar, g[i], a.act.scale());
+            float y = g[i], to_gate = d[i];
+            if (sigmoid) {
+                if (!is_zero(g[i])) gates.see(g[i]);
+                y = s.result(ar, g[i]);
+            } else if (a.act.kind == PAM_HIP_ACT_RELU) y = g[i] <= 0.0f ? 0.0f : g[i];
+            if (GATED) {
+                if (!nothing) grads.see(d[i]);
+                if (!sigmoid && !is_zero(y)) grads.see(y);
+                grads.see(u[i]);                  // (a zero there is left to the checked functions)
+                du[i] = mul_or_zero(ar, d[i], y);
+                to_gate = nothing ? u2f(f2u(u[i]) & kSign) : ar.mul(d[i], u[i]);
+            }
+            if (sigmoid) {
+                if (!nothing) grads.see(to_gate);
+                dg[i] = nothing ? 0.0f : s.grad(ar, to_gate, a.act.scale());
+            } else dg[i] = a.act.kind == PAM_HIP_ACT_RELU && g[i] <= 0.0f ? 0.0f : to_gate;
+        }
+        held = held && grads.held() && gates.held();
+    }
+    if (__ballot(!held) != 0ull) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float dgi, dui = 0.0f;
+            bwd_value<GATED>(a, g[i], u[i], d[i], dgi, dui);
+            dg[i] = dgi; du[i] = dui;
+        }
+    }
+    *reinterpret_cast<v4f_any*>(a.dz + z_at) = dg;
+    if (GATED) *reinterpret_cast<v4f_any*>(a.dz + z_at + a.f) = du;
+}
+
+// ... of rows of fewer than four values
+template <bool GATED>
+__global__ __launch_bounds__(kThreads) void short_act_bwd_kernel(BwdArgs a, long rows)
+{
+    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < rows * a.f; i += (long)gridDim.x * kThreads) {
+        const long row = i / a.f, z_at = GATED ? i + row * a.f : i;
+        float dg, du;
+        bwd_value<GATED>(a, a.z[z_at], GATED ? a.z[z_at + a.f] : 0.0f, a.dy[i], dg, du);
+        a.dz[z_at] = dg;
+        if (GATED) a.dz[z_at + a.f] = du;
     }
 }
 
-// y = act(g) (*) u, z = [g | u]
-__global__ __launch_bounds__(kThreads) void gate_kernel(const float* __restrict__ z, float* __restrict__ y, size_t total, long f, Activation act)
+template <bool GATED>
+int launch_bwd(const char* what, BwdArgs a, long rows, hipStream_t st)
 {
-    for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (size_t)gridDim.x * kThreads) {
-        const size_t at = i / f * (2 * f) + i % f;
-        y[i] = pam_mul_off(act(z[at]), z[at + f], act.off, act.has_off);
+    if (a.f < 4) {
+        hipLaunchKernelGGL((short_act_bwd_kernel<GATED>), dim3(groups_for((size_t)(rows * a.f))), dim3(kThreads), 0, st, a, rows);
+        return pamhost::check_launch(what);
     }
-}
-
-__global__ __launch_bounds__(kThreads) void act_bwd_kernel(const float* __restrict__ z, const float* __restrict__ dy, float* __restrict__ dz, size_t total,
-                                                          Activation act, ApproxFlags flags)
-{
-    for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (size_t)gridDim.x * kThreads)
-        dz[i] = activation_grad(act, z[i], dy[i], flags);
-}
-
-__global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const float* __restrict__ z, const float* __restrict__ dy, float* __restrict__ dz, size_t total,
-                                                           long f, Activation act, ApproxFlags flags)
-{
-    for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (size_t)gridDim.x * kThreads) {
-        const size_t at = i / f * (2 * f) + i % f;
-        const float g = z[at], u = z[at + f], d = dy[i], a = act(g);
-        dz[at] = activation_grad(act, g, mul_grad(a, u, d, flags.a, act.off, act.has_off), flags);
-        dz[at + f] = mul_grad(u, a, d, flags.b, act.off, act.has_off);
+    // (a launch counts its units in 32 bits: more rows, or a longer one, are several launches)
+    constexpr long kMost = 1L << 30;
+    if (GATED) {
+        a.per_row = (uint32_t)((a.f + 3) / 4);
+        for (long first = 0; first < rows; ) {
+            const long n = std::min(rows - first, std::max(1L, kMost / (long)a.per_row));
+            a.units = (uint32_t)(n * a.per_row);
+            hipLaunchKernelGGL((act_bwd_kernel<GATED>), dim3((a.units + kThreads - 1) / kThreads), dim3(kThreads), 0, st, a);
+            const int rc = pamhost::check_launch(what);
+            if (rc != PAM_HIP_OK) return rc;
+            first += n; a.z += n * 2 * a.f; a.dz += n * 2 * a.f; a.dy += n * a.f;
+        }
+        return PAM_HIP_OK;
     }
+    for (long left = a.f; left > 0; ) {
+        a.f = left - 4 * kMost < 4 ? left : 4 * kMost;                        // (a launch's row has at least four)
+        if (a.f > 4 * kMost) a.f = 2 * kMost;
+        a.per_row = a.units = (uint32_t)((a.f + 3) / 4);
+        hipLaunchKernelGGL((act_bwd_kernel<GATED>), dim3((a.units + kThreads - 1) / kThreads), dim3(kThreads), 0, st, a);
+        const int rc = pamhost::check_launch(what);
+        if (rc != PAM_HIP_OK) return rc;
+        left -= a.f; a.z += a.f; a.dz += a.f; a.dy += a.f;
+    }
+    return PAM_HIP_OK;
 }
 
 int check_sizes(const char* what, long m, long n, long k, int activation)
@@ -77,19 +164,13 @@ int pam_hip_linear_act_fwd(const float* a, long a_sr, long a_sc, const float* w,
     if (!y || (k > 0 && (!a || !w))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "linear_act_fwd: null pointer");
     if (pamthin::takes(m, n, k, a_sc, w_sc))
         return pamthin::launch("linear_act_fwd", pamthin::Layer{a, a_sr, w, w_sr, bias, residual, residual_sr, z, y, (int)m, (int)n, (int)k, activation, offset}, false, (hipStream_t)stream);
-    float* sums = z ? z : y;
-    rc = pam_hip_pam_linear_fwd(a, a_sr, a_sc, w, w_sc, w_sr, bias, sums, n, 1, m, n, k, offset, workspace, workspace_bytes, stream);
-    if (rc != PAM_HIP_OK || (!z && !residual && activation == PAM_HIP_ACT_NONE)) return rc;
-    const size_t total = (size_t)m * n;
-    hipLaunchKernelGGL(act_kernel, dim3(groups_for(total)), dim3(kThreads), 0, (hipStream_t)stream, sums, residual, residual_sr, y, total, n,
-                       activation_of(activation, offset));
-    return pamhost::check_launch("linear_act_fwd");
+    return pamgemm::layer_product("linear_act_fwd", false, a, a_sr, a_sc, w, w_sr, w_sc, bias, residual, residual_sr, activation, z, y, m, n, k, offset,
+                                  workspace, workspace_bytes, stream);
 }
 
 size_t pam_hip_gated_linear_workspace_bytes(long m, long f, long k)
 {
-    if (m <= 0 || f <= 0 || k < 0) return 0;
-    return align256((size_t)m * 2 * f * sizeof(float)) + pam_hip_gemm_workspace_bytes(1, m, 2 * f, k);
+    return m <= 0 || f <= 0 ? 0 : pam_hip_gemm_workspace_bytes(1, m, pamgemm::gated_columns(f), k);
 }
 
 int pam_hip_gated_linear_fwd(const float* a, long a_sr, long a_sc, const float* w, long w_sr, long w_sc, const float* bias,
@@ -102,15 +183,8 @@ int pam_hip_gated_linear_fwd(const float* a, long a_sr, long a_sc, const float* 
     if (!y || (k > 0 && (!a || !w))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "gated_linear_fwd: null pointer");
     if (pamthin::takes(m, 2 * f, k, a_sc, w_sc))
         return pamthin::launch("gated_linear_fwd", pamthin::Layer{a, a_sr, w, w_sr, bias, nullptr, 0, z, y, (int)m, (int)f, (int)k, activation, offset}, true, (hipStream_t)stream);
-    if (!workspace || workspace_bytes < pam_hip_gated_linear_workspace_bytes(m, f, k))
-        return pamhost::fail(PAM_HIP_ERR_WORKSPACE, "gated_linear_fwd: workspace of %zu bytes needed", pam_hip_gated_linear_workspace_bytes(m, f, k));
-    const size_t held = align256((size_t)m * 2 * f * sizeof(float));
-    float* sums = z ? z : (float*)workspace;
-    rc = pam_hip_pam_linear_fwd(a, a_sr, a_sc, w, w_sc, w_sr, bias, sums, 2 * f, 1, m, 2 * f, k, offset, (char*)workspace + held, workspace_bytes - held, stream);
-    if (rc != PAM_HIP_OK) return rc;
-    const size_t total = (size_t)m * f;
-    hipLaunchKernelGGL(gate_kernel, dim3(groups_for(total)), dim3(kThreads), 0, (hipStream_t)stream, sums, y, total, f, activation_of(activation, offset));
-    return pamhost::check_launch("gated_linear_fwd");
+    return pamgemm::layer_product("gated_linear_fwd", true, a, a_sr, a_sc, w, w_sr, w_sc, bias, nullptr, 0, activation, z, y, m, f, k, offset,
+                                  workspace, workspace_bytes, stream);
 }
 
 int pam_hip_act_bwd(const float* z, const float* dy, float* dz, size_t n, int activation, float offset, int approx_a, int approx_b,
@@ -119,9 +193,8 @@ int pam_hip_act_bwd(const float* z, const float* dy, float* dz, size_t n, int ac
     if (!known(activation) || n > (size_t)1 << 41) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "act_bwd: unknown activation %d or size out of range", activation);
     if (n == 0) return PAM_HIP_OK;
     if (!z || !dy || !dz) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "act_bwd: null pointer");
-    hipLaunchKernelGGL(act_bwd_kernel, dim3(groups_for(n)), dim3(kThreads), 0, (hipStream_t)stream, z, dy, dz, n, activation_of(activation, offset),
-                       ApproxFlags{approx_a != 0, approx_b != 0, approx_exp != 0});
-    return pamhost::check_launch("act_bwd");
+    return launch_bwd<false>("act_bwd", BwdArgs{z, dy, dz, (long)n, 0, 0, activation_of(activation, offset), ApproxFlags{approx_a != 0, approx_b != 0, approx_exp != 0}},
+                             1, (hipStream_t)stream);
 }
 
 int pam_hip_gated_bwd(const float* z, const float* dy, float* dz, long m, long f, int activation, float offset, int approx_a, int approx_b,
@@ -131,10 +204,8 @@ int pam_hip_gated_bwd(const float* z, const float* dy, float* dz, long m, long f
     if (rc != PAM_HIP_OK) return rc;
     if (m == 0 || f == 0) return PAM_HIP_OK;
     if (!z || !dy || !dz) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "gated_bwd: null pointer");
-    const size_t total = (size_t)m * f;
-    hipLaunchKernelGGL(gate_bwd_kernel, dim3(groups_for(total)), dim3(kThreads), 0, (hipStream_t)stream, z, dy, dz, total, f,
-                       activation_of(activation, offset), ApproxFlags{approx_a != 0, approx_b != 0, approx_exp != 0});
-    return pamhost::check_launch("gated_bwd");
+    return launch_bwd<true>("gated_bwd", BwdArgs{z, dy, dz, f, 0, 0, activation_of(activation, offset), ApproxFlags{approx_a != 0, approx_b != 0, approx_exp != 0}},
+                            m, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -8,6 +8,7 @@
 #include <random>
 
 #include "pam_gemm_kernel.h"
+#include "pam_gemm_layer.h"
 #include "../../include/pam_hip_extra.h"
 #include "../../include/pam_hip_probe.h"
 
@@ -330,6 +331,7 @@ __global__ __launch_bounds__(256) void empty_k_kernel(float* __restrict__ y, lon
 
 // Cut tiles of many pieces: the pieces of every tile added in ascending order from +0 by a kernel of its own, one
 // lane per 128-bit row of the tile (work-groups of 128 lanes, eight per tile); eight pieces' loads in flight.
+template <int WAY>
 __global__ __launch_bounds__(128) void fold_kernel(pamgemm::GemmArgs g)
 {
     using pamgemm::v4f;
@@ -350,11 +352,26 @@ __global__ __launch_bounds__(128) void fold_kernel(pamgemm::GemmArgs g)
     const pamgemm::LanePlace place = pamgemm::lane_place(tid, row0, col0, g.M, g.N);
     const int r = row0 + place.ty * 4 + i, c = col0 + place.tx * 4;
     if (r >= g.M) return;
+    if constexpr (WAY != WAY_PLAIN) {
+        const float sums[4] = {total.x, total.y, total.z, total.w};
+        if (c < g.N) finish_row<WAY>(g, r, c, g.N, sums);
+        return;
+    }
     float* dst = g.Y + (long)zb * g.y_sb + (long)r * g.y_sr + (long)c * g.y_sc;
     const float sums[4] = {total.x, total.y, total.z, total.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (c + j < g.N) dst[(long)j * g.y_sc] = g.bias ? sums[j] + g.bias[c + j] : sums[j];
+}
+
+// sums over nothing on their way through an activation: a lane per four columns
+template <int WAY>
+__global__ __launch_bounds__(256) void empty_layer_kernel(pamgemm::GemmArgs g)
+{
+    const int quads = (g.N + 3) / 4;
+    const long idx = (long)blockIdx.x * 256 + threadIdx.x;
+    const float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (idx < (long)g.M * quads) finish_row<WAY>(g, (int)(idx / quads), (int)(idx % quads) * 4, g.N, sums);
 }
 
 // Products of at most kFewRows rows and short sums (one decoding step of attention: a query against the keys and values of
@@ -487,7 +504,7 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
          const float* l, long l_sb, long l_sr, long l_sc, const float* r, long r_sb, long r_sr, long r_sc,
          const float* d, long d_sb, long d_sr, long d_sc, float* y, long y_sb, long y_sr, long y_sc,
          float offset, void* workspace, size_t workspace_bytes, void* stream, const ConvGeom* conv = nullptr,
-         const float* bias = nullptr)
+         const float* bias = nullptr, int way = WAY_PLAIN, const WayOut* way_out = nullptr)
 {
     if (batch < 0 || M < 0 || N < 0 || K < 0) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: negative size", what);
     if (batch == 0 || M == 0 || N == 0) return PAM_HIP_OK;
@@ -497,13 +514,13 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
         return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: dimension too large (sizes and batch <= 2^30, output tiles of all matrices < 2^31)", what);
     hipStream_t st = (hipStream_t)stream;
 
-    if (K == 0) {                                  // (the operands are empty, and may be null)
+    if (K == 0 && way == WAY_PLAIN) {              // (the operands are empty, and may be null)
         const long n = batch * M * N;
         hipLaunchKernelGGL(empty_k_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, y, y_sb, y_sr, y_sc, batch, (int)M, (int)N, bias);
         return pamhost::check_launch(what);
     }
     const bool usable = workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0;
-    Plan p = make_plan(batch, M, N, K, usable);
+    Plan p = make_plan(batch, M, N, K > 0 ? K : 1, usable);
     if (p.pieces > 1 && plan_space(p).total > workspace_bytes) p = make_plan(batch, M, N, K, false);       // whole tiles
     int lk = load_kind(l_sr, l_sc, l_sb, l, M, K);
     int rk = conv ? LOAD_CONV : load_kind(r_sc, r_sr, r_sb, r, N, K);
@@ -514,8 +531,9 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
         rk = LOAD_CONVR;
     else if (conv && conv->row_quads && conv->transposed && mode != MODE_STD && lk == LOAD_KVEC && K % 4 == 0)
         rk = LOAD_CONVK;
-    const bool few = mode == MODE_PAM && !conv && M <= kFewRows && K <= kFewLongest && p.pieces == 1 && offset == 1.0f && g_force_bk == 0 && g_force_pieces == 0;
-    p = launch_plan(p, mode == MODE_PAM && !few, conv != nullptr, lk != LOAD_ANY && rk != LOAD_ANY, batch, M, N, K);
+    if (way != WAY_PLAIN && (lk != rk || (lk != LOAD_KVEC && lk != LOAD_KODD))) lk = rk = LOAD_ANY;      // (both along k, or any)
+    const bool few = mode == MODE_PAM && way == WAY_PLAIN && !conv && M <= kFewRows && K <= kFewLongest && p.pieces == 1 && offset == 1.0f && g_force_bk == 0 && g_force_pieces == 0;
+    p = launch_plan(p, mode == MODE_PAM && way == WAY_PLAIN && !few, conv != nullptr, lk != LOAD_ANY && rk != LOAD_ANY, batch, M, N, K);
     const Space sp = plan_space(p);
 
     GemmArgs g;
@@ -543,6 +561,27 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
     }
 
     g.cv = conv ? *conv : ConvGeom{nullptr, nullptr, 0, 0, 0, 0, 0};
+    g.way = way_out ? *way_out : WayOut{nullptr, 0, nullptr, 0, 0};
+
+    if (way != WAY_PLAIN) {
+        if (K == 0) {
+            const long n = M * ((N + 3) / 4);
+            const dim3 grid((unsigned)((n + 255) / 256));
+            if (way == WAY_GATED) hipLaunchKernelGGL(empty_layer_kernel<WAY_GATED>, grid, dim3(256), 0, st, g);
+            else hipLaunchKernelGGL(empty_layer_kernel<WAY_LAYER>, grid, dim3(256), 0, st, g);
+            return pamhost::check_launch(what);
+        }
+        unsigned groups = (unsigned)p.units;
+        if (p.units >= 64 && (p.pieces == 1 || g.fold_here)) groups = spread_over_xcds(g);       // (as launch_mode)
+        if (way == WAY_GATED) { if (p.bk == 32) launch_layer<32, WAY_GATED>(lk, groups, st, g); else launch_layer<16, WAY_GATED>(lk, groups, st, g); }
+        else { if (p.bk == 32) launch_layer<32, WAY_LAYER>(lk, groups, st, g); else launch_layer<16, WAY_LAYER>(lk, groups, st, g); }
+        if (p.pieces > 1 && !g.fold_here) {
+            const dim3 grid((unsigned)(p.units / p.pieces * 8));
+            if (way == WAY_GATED) hipLaunchKernelGGL(fold_kernel<WAY_GATED>, grid, dim3(128), 0, st, g);
+            else hipLaunchKernelGGL(fold_kernel<WAY_LAYER>, grid, dim3(128), 0, st, g);
+        }
+        return pamhost::check_launch(what);
+    }
 
     if (few) {
         const unsigned groups = (unsigned)(batch * g.ntn);
@@ -562,7 +601,7 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
     default: launch_mode<MODE_BWD_DR>(p, lk, rk, st, g); break;
     }
     if (p.pieces > 1 && !g.fold_here)
-        hipLaunchKernelGGL(fold_kernel, dim3((unsigned)(p.units / p.pieces * 8)), dim3(128), 0, st, g);
+        hipLaunchKernelGGL(fold_kernel<WAY_PLAIN>, dim3((unsigned)(p.units / p.pieces * 8)), dim3(128), 0, st, g);
     return pamhost::check_launch(what);
 }
 
@@ -870,6 +909,21 @@ int scratch_address(const char* what, void** ptr)
 }
 
 }  // namespace
+
+namespace pamgemm {
+
+long gated_columns(long hidden) { return (hidden + 1) / 2 * 4; }
+
+int layer_product(const char* what, bool gated, const float* a, long a_sr, long a_sc, const float* w, long w_sr, long w_sc, const float* bias,
+                  const float* residual, long residual_sr, int activation, float* z, float* y, long m, long n, long k, float offset,
+                  void* workspace, size_t workspace_bytes, void* stream)
+{
+    const WayOut out{residual, residual_sr, z, activation, (int)n};
+    return gemm(what, MODE_PAM, 1, m, gated ? gated_columns(n) : n, k, a, 0, a_sr, a_sc, w, gated ? n * w_sr : 0, w_sc, w_sr, nullptr, 0, 0, 0,
+                y, 0, n, 1, offset, workspace, workspace_bytes, stream, nullptr, bias, gated ? WAY_GATED : WAY_LAYER, &out);
+}
+
+}  // namespace pamgemm
 
 extern "C" {
 

@@ -1,0 +1,4 @@
+// The matrix kernels with 32-deep k-tiles whose sums go out by WAY_LAYER (one file per pair: they compile side by side).
+#include "pam_gemm_kernel.h"
+
+template void pamgemm::launch_layer<32, pamgemm::WAY_LAYER>(int, unsigned, hipStream_t, const pamgemm::GemmArgs&);

@@ -100,13 +100,28 @@ bool wants_graph(std::initializer_list<const Tensor*> tensors)
     return false;
 }
 
+// ... of X [..., d_in], the residual of the result's shape
 Tensor call_layer(bool gated, const Tensor& X, const Tensor& W, const std::optional<Tensor>& bias, int64_t activation, const std::optional<Tensor>& residual,
                   double offset, bool a, bool b, bool e)
 {
+    const char* const name = gated ? "gated_linear" : "linear_act";
     const Tensor none;
-    if (!wants_graph({&X, &W, bias ? &*bias : &none, residual ? &*residual : &none}))
-        return layer(gated, row_major(X, 2), W, bias.value_or(none), (int)activation, residual.value_or(none), false, offset).y;
-    return LayerNode::apply(gated, X, W, bias, activation, residual, true, offset, a, b, e);
+    TORCH_CHECK_VALUE(W.dim() == 2, name, ": the weight is a matrix, got ", shape(W));
+    TORCH_CHECK_VALUE(!gated || W.size(0) % 2 == 0, name, ": the weight has the gate's rows and as many others, got ", shape(W));
+    TORCH_CHECK_VALUE(X.dim() >= 1 && X.size(-1) == W.size(1), name, ": shapes ", shape(X), " and ", shape(W), " do not multiply");
+    const int64_t n = gated ? W.size(0) / 2 : W.size(0);
+    const bool rows = X.dim() == 2;
+    std::vector<int64_t> sizes(X.sizes().begin(), X.sizes().end());
+    sizes.back() = n;
+    TORCH_CHECK_VALUE(!residual || residual->sizes() == at::IntArrayRef(sizes), name, ": the residual must have the shape of the result, got ", residual ? shape(*residual) : "");
+    const int64_t m = c10::multiply_integers(sizes.begin(), sizes.end() - 1);
+    const Tensor x = rows ? X : X.reshape({m, X.size(-1)});
+    std::optional<Tensor> r = residual;
+    if (r && !rows) r = r->reshape({m, n});
+    Tensor y;
+    if (wants_graph({&x, &W, bias ? &*bias : &none, r ? &*r : &none})) y = LayerNode::apply(gated, x, W, bias, activation, r, true, offset, a, b, e);
+    else y = layer(gated, row_major(x, 2), W, bias.value_or(none), (int)activation, r.value_or(none), false, offset).y;
+    return rows ? y : y.view(sizes);
 }
 
 // ---------------------------------------------------------------- rotation of queries and keys

@@ -45,26 +45,11 @@ struct RotaryArgs {
     ApproxFlags flags;
 };
 
-// The primitives as single integer additions: with signs and exponents in place a (*) b is bits(a) + bits(b) - bias, a (/) b is
-// bits(a) - bits(b) + bias, and an offset is one more constant in either.  That holds while operands and results are normal numbers, which the
-// callers make sure of by windows on what goes in: exponents of [first, last) per kind of value, chosen so that no result of
-// the chain leaves the normal range, whatever the values in them.
-struct Raw {
-    uint32_t mul_add, div_add;
-    __device__ __forceinline__ explicit Raw(float off) : mul_add(f2u(off) - 2u * kBias), div_add(f2u(off)) {}
-    __device__ __forceinline__ float mul(float a, float b) const { return u2f(f2u(a) + f2u(b) + mul_add); }
-    __device__ __forceinline__ float div(float a, float b) const { return u2f(f2u(a) - f2u(b) + div_add); }
-};
-template <int FIRST, int LAST>                    // magnitudes 2^FIRST <= |v| < 2^LAST: one shift-add and a max per value
-struct Window {
-    uint32_t most = 0;
-    __device__ __forceinline__ void see(float v) { most = max(most, (f2u(v) << 1) - ((uint32_t)(FIRST + 127) << 24)); }
-    __device__ __forceinline__ void see(const v4f& v) { see(v[0]); see(v[1]); see(v[2]); see(v[3]); }
-    __device__ __forceinline__ bool held() const { return most < ((uint32_t)(LAST - FIRST) << 24); }
-};
+// Windows of pam_activation.h on what goes into a chain of integer additions (Raw).
 // With x in 2^[-20, 20), its root in 2^[-14, 21), w in 2^[-10, 10), dz in 2^[-44, 20): x / root in 2^[-42, 35), x / root / root in
 // 2^[-64, 50), dz w in 2^[-55, 31), their product in 2^[-120, 82); the offset, between 3/4 and 3/2, is in at most five factors of it.  Heads
 // without a norm: x or dy in 2^[-60, 60), times a table's value.
+template <class W> __device__ __forceinline__ void see(W& window, const v4f& v) { window.see(v[0]); window.see(v[1]); window.see(v[2]); window.see(v[3]); }
 typedef Window<-20, 20> WindowX;
 typedef Window<-14, 21> WindowRoot;
 typedef Window<-10, 10> WindowW;
@@ -301,13 +286,10 @@ __device__ __forceinline__ Weight load_weight(const float* weight, const Unit& a
     if (!r.norm) return r;
     load_unit(weight, at, r.w);
     WindowW window;
-    window.see(r.w[0]); window.see(r.w[1]);
+    see(window, r.w[0]); see(window, r.w[1]);
     r.held = window.held();
     return r;
 }
-// offsets that the windows above allow for
-__device__ __forceinline__ bool usual_offset(float off) { return off > 0.75f && off < 1.5f; }
-
 // y of a lane's unit; false if a value of the wavefront is outside its window, and y is then not computed.
 template <bool INTERLEAVED>
 __device__ __forceinline__ bool forward_head(const RotaryArgs& a, const Unit& at, const v4f (&x)[2], const Weight& w, const v4f& c, v4f s, v4f (&y)[2])
@@ -315,12 +297,12 @@ __device__ __forceinline__ bool forward_head(const RotaryArgs& a, const Unit& at
     const Raw ar(a.off);
     const bool still = stands_still(s);
     WindowTable tables;
-    if (at.rotates) { tables.see(c); tables.see(s); }
+    if (at.rotates) { see(tables, c); see(tables, s); }
     bool held = usual_offset(a.off) && tables.held() && w.held;
     y[0] = x[0]; y[1] = x[1];
     if (w.norm) {
         WindowX seen;
-        seen.see(x[0]); seen.see(x[1]);
+        see(seen, x[0]); see(seen, x[1]);
         const RawRoot r = raw_root_of(ar, a, square_sum(ar, a, at, x));
         held = held && seen.held() && r.held;
 #pragma unroll
@@ -329,7 +311,7 @@ __device__ __forceinline__ bool forward_head(const RotaryArgs& a, const Unit& at
             for (int i = 0; i < 4; ++i) y[v][i] = ar.mul(ar.div(x[v][i], r.root), w.w[v][i]);
     } else if (at.rotates) {
         WindowPlain seen;
-        seen.see(x[0]); seen.see(x[1]);
+        see(seen, x[0]); see(seen, x[1]);
         held = held && seen.held();
     }
     if (at.rotates) {
@@ -378,7 +360,7 @@ __device__ __forceinline__ bool backward_head(const RotaryArgs& a, const Unit& a
     if (at.rotates) {
         WindowTable tables;
         WindowPlain seen;
-        tables.see(c); tables.see(s); seen.see(d[0]); seen.see(d[1]);
+        see(tables, c); see(tables, s); see(seen, d[0]); see(seen, d[1]);
         held = held && tables.held() && seen.held();
         float d1[4], d2[4], z1[4], z2[4];
         to_pairs<INTERLEAVED>(d, d1, d2);
@@ -392,7 +374,7 @@ __device__ __forceinline__ bool backward_head(const RotaryArgs& a, const Unit& a
     if (w.norm) {
         WindowX seen;
         WindowGrad grads;
-        seen.see(x[0]); seen.see(x[1]); grads.see(dx[0]); grads.see(dx[1]);
+        see(seen, x[0]); see(seen, x[1]); see(grads, dx[0]); see(grads, dx[1]);
         const RawRoot r = raw_root_of(ar, a, square_sum(ar, a, at, x));
         float through[2] = {0.0f, 0.0f};
 #pragma unroll

@@ -404,6 +404,35 @@ def test_normed_rotation_against_64_bits(batch, tokens, heads, kv, dim, rotated,
             assert abs(terms.sum() - slope) <= 1e-4 * np.abs(terms).sum() + 1e-5
 
 
+def chain_norm(x, weight, eps, kw):
+    """By primitives, the row's sum by torch."""
+    d = x.shape[-1]
+    total = pam.mul(x, x, **kw).sum(-1, keepdim=True)
+    root = pam.pow(pam.div(total, float(d), **kw) + eps, 0.5, **kw)
+    return pam.mul(pam.div(x, root.expand_as(x).contiguous(), **kw), weight.expand_as(x).contiguous(), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,rotated", [(64, 64), (80, 40), (18, 10), (256, 64)])
+@pytest.mark.parametrize("offset", [None, OFF, 1.4])
+def test_normed_rotation_is_the_chain(dim, rotated, offset):
+    """Up to the order of the head's sums: 2^-17 of the largest value, approximate gradients."""
+    rng = np.random.default_rng(dim)
+    kw = dict(offset=offset, approx_bwd=True)
+    angle = rng.uniform(-4, 4, (6, rotated // 2))
+    cos, sin = gpu(np.cos(angle).astype(np.float32)), gpu(np.sin(angle).astype(np.float32))
+    x, w = gpu(normal(rng, 2, 6, 3, dim), True), gpu(normal(rng, dim, std=0.1) + np.float32(1.0), True)
+    d = normal(rng, 2, 6, 3, dim, std=0.1)
+    d[0, 2], d[1, 4, 1] = 0.0, 0.0                       # a token and a head that the loss leaves out
+    y, _ = pam.rotary(x, None, cos, sin, q_weight=w, **kw)
+    want = chain_rotary(chain_norm(x, w, 1e-6, kw), cos, sin, False, kw)
+    got, expected = [y, *torch.autograd.grad(y, (x, w), gpu(d))], [want, *torch.autograd.grad(want, (x, w), gpu(d))]
+    for a, b in zip(got, expected):
+        a, b = host(a), host(b)
+        assert np.abs(a - b).max() <= 2.0 ** -17 * np.abs(b).max()
+    assert not host(got[1])[0, 2].any() and not host(got[1])[1, 4, 1].any()
+
+
 @pytest.mark.gpu
 def test_rotation_of_one_tensor_and_norm_of_the_other():
     rng = np.random.default_rng(4)
