@@ -11,6 +11,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <sstream>
@@ -539,7 +540,7 @@ py::tuple adam_collect(py::list params, size_t start, py::dict state)
 }  // namespace
 
 // The interpreter is free for other threads while an op checks, allocates and launches, each of which may wait (a full
-// launch queue, device memory, the table of workspaces); only adam_collect reads Python objects.
+// launch queue, device memory, the table of workspaces); only adam_collect and clip read Python objects.
 PYBIND11_MODULE(_pam_host, module)
 {
     const py::call_guard<py::gil_scoped_release> unlocked;
@@ -575,6 +576,6 @@ PYBIND11_MODULE(_pam_host, module)
     module.def("unary", [](const Tensor& x, int64_t op, double number, double offset, bool a, bool e) { return UnaryNode::apply(x, op, number, offset, a, e); }, unlocked);
     module.def("layer", &call_layer, unlocked);
     module.def("rotary", &call_rotary, unlocked);
-    module.def("clip", &clip, unlocked);
+    module.def("clip", &clip);
     module.def("adam_collect", &adam_collect);
 }

@@ -273,31 +273,77 @@ variable_list call_rotary(const Tensor& q, const std::optional<Tensor>& k, const
 
 // ---------------------------------------------------------------- clipping
 
-// The norm of all tensors; with `outs`, the clipped values there (a tensor may be its own output).  Each tensor's memory is
-// without gaps or overlaps, and an output has its tensor's strides.
-Tensor clip(const variable_list& ins, const variable_list& outs, double max_norm, double eps, double offset)
+// The norm of all tensors; with `outs`, the clipped values there (a tensor may be its own output).  Values are taken in the order of
+// memory where a tensor's memory is without gaps or overlaps and its output's strides are its own; others go through copies.
+// Whether memory that is written for one tensor also belongs to another one of the table.
+bool clip_overlaps(const std::vector<pam_hip_clip_tensor>& table)
 {
-    TORCH_CHECK_VALUE(!ins.empty(), "clip_grads: no tensors");
-    TORCH_CHECK_VALUE(outs.empty() || outs.size() == ins.size(), "clip_grads: as many outputs as tensors");
-    std::vector<pam_hip_clip_tensor> table;
-    table.reserve(ins.size());
-    for (size_t i = 0; i < ins.size(); ++i) {
-        check_tensor(ins[i]);
-        TORCH_CHECK_VALUE(ins[i].device() == ins[0].device(), "clip_grads: tensors are on different devices");
-        TORCH_CHECK_VALUE(ins[i].is_non_overlapping_and_dense(), "clip_grads: a tensor's memory has gaps or overlaps");
-        if (!outs.empty()) {
-            check_tensor(outs[i]);
-            TORCH_CHECK_VALUE(outs[i].sizes() == ins[i].sizes() && outs[i].device() == ins[i].device() && outs[i].is_non_overlapping_and_dense()
-                                  && (ins[i].strides() == outs[i].strides() || (ins[i].is_contiguous() && outs[i].is_contiguous())),
-                              "clip_grads: an output has its tensor's shape, strides and device");
-        }
-        const size_t n = (size_t)ins[i].numel();
-        if (n) table.push_back({data(ins[i]), outs.empty() ? nullptr : data(outs[i]), n});
+    struct Range { uintptr_t begin, end; bool written; };
+    std::vector<Range> ranges;
+    ranges.reserve(2 * table.size());
+    for (const pam_hip_clip_tensor& t : table) {
+        const size_t bytes = t.n * sizeof(float);
+        if (t.in != t.out) ranges.push_back({(uintptr_t)t.in, (uintptr_t)t.in + bytes, false});
+        if (t.out) ranges.push_back({(uintptr_t)t.out, (uintptr_t)t.out + bytes, true});
     }
-    const OnDevice on(ins[0]);
-    const Tensor norm = new_floats({}, ins[0]);
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    uintptr_t any = 0, written = 0;               // the furthest end of the ranges so far
+    for (const Range& r : ranges) {
+        if (r.begin < written || (r.written && r.begin < any)) return true;
+        any = std::max(any, r.end);
+        if (r.written) written = std::max(written, r.end);
+    }
+    return false;
+}
+
+// (the lists are read as Python holds them: a program's hundreds of tensors, twice, as vectors of references took longer than the kernels)
+Tensor clip(const py::list& ins, const py::list& outs, double max_norm, double eps, double offset)
+{
+    const size_t count = ins.size();
+    TORCH_CHECK_VALUE(count > 0, "clip_grads: no tensors");
+    TORCH_CHECK_VALUE(outs.empty() || outs.size() == count, "clip_grads: as many outputs as tensors");
+    const auto tensor = [](const py::list& list, size_t i) -> const Tensor& {
+        PyObject* item = PyList_GET_ITEM(list.ptr(), (Py_ssize_t)i);
+        TORCH_CHECK_TYPE(THPVariable_Check(item), "clip_grads: expected tensors");
+        return THPVariable_Unpack(item);
+    };
+    const at::AutoGradMode no_graph(false);
+    const Tensor& first = tensor(ins, 0);
+    std::vector<pam_hip_clip_tensor> table;
+    std::vector<std::pair<Tensor, Tensor>> copied;                   // (where the result belongs, where it is)
+    variable_list held;
+    table.reserve(count);
+    for (size_t i = 0; i < count; ++i) {
+        const Tensor* in = &tensor(ins, i);
+        check_tensor(*in);
+        TORCH_CHECK_VALUE(in->layout() == at::kStrided && in->device() == first.device(), "clip_grads: tensors are dense and on one device");
+        const at::IntArrayRef sizes = in->sizes();
+        if (!in->is_non_overlapping_and_dense()) {
+            held.reserve(count);                                     // (so that `in` stays where it is)
+            held.push_back(in->contiguous());
+            in = &held.back();
+        }
+        float* out_data = nullptr;
+        if (!outs.empty()) {
+            const Tensor& out = tensor(outs, i);
+            check_tensor(out);
+            TORCH_CHECK_VALUE(out.sizes() == sizes && out.device() == first.device(), "clip_grads: an output has its tensor's shape and device");
+            if (out.strides() == in->strides()) out_data = data(out);
+            else {
+                copied.emplace_back(out, at::empty_like(*in));
+                out_data = data(copied.back().second);
+            }
+        }
+        const size_t n = (size_t)in->numel();
+        if (n) table.push_back({data(*in), out_data, n});
+    }
+    TORCH_CHECK_VALUE(outs.empty() || !clip_overlaps(table), "clip_grads: outputs share memory with each other or with other tensors");
+    const py::gil_scoped_release unlocked;
+    const OnDevice on(first);
+    const Tensor norm = new_floats({}, first);
     const size_t bytes = pam_hip_clip_workspace_bytes(table.data(), (long)table.size());
-    const Tensor ws = new_floats({(int64_t)(bytes / 4)}, ins[0]);
+    const Tensor ws = new_floats({(int64_t)(bytes / 4)}, first);
     check_call(pam_hip_clip_many(table.data(), (long)table.size(), (float)max_norm, (float)eps, data(norm), (float)offset, data(ws), bytes, on.stream), "clip_many");
+    for (const auto& c : copied) c.first.copy_(c.second);
     return norm;
 }

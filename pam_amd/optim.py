@@ -160,16 +160,10 @@ def multiply_grads(params, c, op_dict):
 _CLIP_EPS = 1e-6
 
 
-def _dense(tensors):
-    """The tensors, copies in the place of those whose memory has gaps or overlaps."""
-    return [t if t.is_contiguous() or (t.layout is torch.strided and torch.ops.aten.is_non_overlapping_and_dense(t)) else t.contiguous() for t in tensors]
-
-
 def grad_norm(grads, *, offset=None):
     """pow(sum of g (*) g over all tensors, 0.5), a tensor of no dimensions: the global norm of many fp32 GPU tensors."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    with torch.no_grad():
-        return _abi.host().clip(_dense(grads), [], math.inf, _CLIP_EPS, 1.0 if offset is None else float(offset))
+    return _abi.host().clip(grads, [], math.inf, _CLIP_EPS, 1.0 if offset is None else float(offset))
 
 
 def clip_grads(grads, max_norm, *, out=None, offset=None):
@@ -182,17 +176,7 @@ def clip_grads(grads, max_norm, *, out=None, offset=None):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads: the bound is not negative, got {max_norm}")
-    if len(out) != len(grads):
-        raise ValueError("clip_grads: as many outputs as tensors")
-    with torch.no_grad():
-        ins, outs = _dense(grads), _dense(out)
-        ins = [g.contiguous() if g.stride() != o.stride() else g for g, o in zip(ins, outs)]
-        outs = [o if o.stride() == g.stride() or o.is_contiguous() else torch.empty_like(g) for g, o in zip(ins, outs)]
-        norm = _abi.host().clip(ins, outs, max_norm, _CLIP_EPS, 1.0 if offset is None else float(offset))
-        for target, result in zip(out, outs):
-            if target is not result:
-                target.copy_(result)
-    return norm
+    return _abi.host().clip(grads, out, max_norm, _CLIP_EPS, 1.0 if offset is None else float(offset))
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, *, offset=None):

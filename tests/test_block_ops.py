@@ -556,6 +556,17 @@ def test_clip_of_views():
     assert torch.equal(into, same.t())
 
 
+@pytest.mark.gpu
+def test_clip_refuses_shared_outputs():
+    flat = torch.ones(100, device="cuda")
+    for ins, outs in (([flat, flat], None), ([flat[:60], flat[50:]], None), ([flat[:50]], [flat[10:60]]), ([flat[:10], flat[10:20]], [flat[10:20], flat[30:40]]),
+                      ([flat[:10], flat[20:30]], [flat[40:50], flat[45:55]])):
+        with pytest.raises(ValueError):
+            optim.clip_grads(ins, 1.0, out=outs)
+    assert flat.eq(1.0).all()
+    assert float(optim.grad_norm([flat, flat])) > 10.0           # (only read)
+
+
 # ---------------------------------------------------------------- streams, graphs, repeats
 
 def _pass(seed):
