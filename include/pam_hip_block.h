@@ -40,6 +40,15 @@ int pam_hip_act_bwd(const float *z, const float *dy, float *dz, size_t n, int ac
 int pam_hip_gated_bwd(const float *z, const float *dy, float *dz, long m, long f, int activation, float offset,
                       int approx_a, int approx_b, int approx_exp, void *stream);
 
+/* The products of the layers' gradients, dX = dZ (x) W and dW^T = X^T (x) dZ: pam_hip_pam_matmul_fwd (kind 0, the approximate gradient,
+ * mo not read) or pam_hip_pam_matmul_bwd (kind 1: l is the upstream gradient, 2: r is), with the sums held to chains of
+ * 1024 terms: a chunk of pam_hip_gemm_plan that is longer is cut into equal ones of at most 1024, as the two forward products
+ * above do.  (Without a workspace, or in products of more than 8192 tiles of 64 x 64, chunks stay as planned.) */
+size_t pam_hip_layer_grad_workspace_bytes(long m, long n, long k);
+int pam_hip_layer_grad(const float *l, long l_sr, long l_sc, const float *r, long r_sr, long r_sc, const float *mo, long mo_sr, long mo_sc,
+                       float *dm, long dm_sr, long dm_sc, long m, long n, long k, int kind, float offset,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
 /* The rotation of heads by their positions, after an optional norm of each head.
  *   n = x (/) pow(mean(x (*) x) + eps, 0.5),  z = n (*) weight            (weight NULL: z = x)
  *   y1 = z1 (*) cos - z2 (*) sin,  y2 = z2 (*) cos + z1 (*) sin            for the pairs of the first `rotated` values of a head:

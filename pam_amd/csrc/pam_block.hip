@@ -152,7 +152,7 @@ int check_sizes(const char* what, long m, long n, long k, int activation)
 
 extern "C" {
 
-size_t pam_hip_linear_act_workspace_bytes(long m, long n, long k) { return pam_hip_gemm_workspace_bytes(1, m, n, k); }
+size_t pam_hip_linear_act_workspace_bytes(long m, long n, long k) { return pamgemm::layer_workspace(m, n, k); }
 
 int pam_hip_linear_act_fwd(const float* a, long a_sr, long a_sc, const float* w, long w_sr, long w_sc, const float* bias,
                            int activation, const float* residual, long residual_sr, float* z, float* y, long m, long n, long k,
@@ -170,7 +170,7 @@ int pam_hip_linear_act_fwd(const float* a, long a_sr, long a_sc, const float* w,
 
 size_t pam_hip_gated_linear_workspace_bytes(long m, long f, long k)
 {
-    return m <= 0 || f <= 0 ? 0 : pam_hip_gemm_workspace_bytes(1, m, pamgemm::gated_columns(f), k);
+    return m <= 0 || f <= 0 ? 0 : pamgemm::layer_workspace(m, pamgemm::gated_columns(f), k);
 }
 
 int pam_hip_gated_linear_fwd(const float* a, long a_sr, long a_sc, const float* w, long w_sr, long w_sc, const float* bias,

@@ -9,6 +9,7 @@
 
 #include "pam_gemm_kernel.h"
 #include "pam_gemm_layer.h"
+#include "../../include/pam_hip_block.h"
 #include "../../include/pam_hip_extra.h"
 #include "../../include/pam_hip_probe.h"
 
@@ -294,6 +295,22 @@ Plan launch_plan(Plan p, bool pam, bool conv, bool quads, long batch, long M, lo
     return p;
 }
 
+// The layers' products (pam_hip_block.h) hold a chain of sums to kLongestChain terms: a plan of longer pieces is cut further, where a
+// cut tile can be (a workspace, arrival words for the tiles).  A chain of k terms in float32 loses about sqrt(k) 2^-25 of the result,
+// 1.3e-6 at the 4096 terms of a gated layer's gradients; with 1024 it is 9e-7 at most, for 3 % of the time (4096 tokens, 1024 -> 2 x 2048, forward
+// and gradients 2000 -> 2060 us; chains of 512 6e-7 and 2110).
+constexpr long kLongestChain = 1024;
+void limit_chain(Plan& p, long batch, long M, long N)
+{
+    const long tiles = batch * ((M + 63) / 64) * ((N + 63) / 64);
+    if ((long)p.piece_kt * p.bk <= kLongestChain || tiles > kMostCutTiles) return;
+    const int most = (int)(kLongestChain / p.bk), pieces = (p.kt + most - 1) / most;
+    p.piece_kt = (p.kt + pieces - 1) / pieces;
+    p.pieces = (p.kt + p.piece_kt - 1) / p.piece_kt;
+    p.units = tiles * p.pieces;
+    p.free = FreeShape{0, 0};
+}
+
 // workspace of a plan that cuts tiles: [arrival words, one per tile][one piece per unit].  The words' part has one size
 // for every shape, so that products of different shapes that share a workspace never write pieces over each other's
 // words (a word that does not carry the launch's tag costs its first arriver two more round trips).
@@ -504,7 +521,7 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
          const float* l, long l_sb, long l_sr, long l_sc, const float* r, long r_sb, long r_sr, long r_sc,
          const float* d, long d_sb, long d_sr, long d_sc, float* y, long y_sb, long y_sr, long y_sc,
          float offset, void* workspace, size_t workspace_bytes, void* stream, const ConvGeom* conv = nullptr,
-         const float* bias = nullptr, int way = WAY_PLAIN, const WayOut* way_out = nullptr)
+         const float* bias = nullptr, bool layer = false, int way = WAY_PLAIN, const WayOut* way_out = nullptr)
 {
     if (batch < 0 || M < 0 || N < 0 || K < 0) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: negative size", what);
     if (batch == 0 || M == 0 || N == 0) return PAM_HIP_OK;
@@ -521,6 +538,7 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
     }
     const bool usable = workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0;
     Plan p = make_plan(batch, M, N, K > 0 ? K : 1, usable);
+    if (layer && usable) limit_chain(p, batch, M, N);
     if (p.pieces > 1 && plan_space(p).total > workspace_bytes) p = make_plan(batch, M, N, K, false);       // whole tiles
     int lk = load_kind(l_sr, l_sc, l_sb, l, M, K);
     int rk = conv ? LOAD_CONV : load_kind(r_sc, r_sr, r_sb, r, N, K);
@@ -920,12 +938,31 @@ int layer_product(const char* what, bool gated, const float* a, long a_sr, long 
 {
     const WayOut out{residual, residual_sr, z, activation, (int)n};
     return gemm(what, MODE_PAM, 1, m, gated ? gated_columns(n) : n, k, a, 0, a_sr, a_sc, w, gated ? n * w_sr : 0, w_sc, w_sr, nullptr, 0, 0, 0,
-                y, 0, n, 1, offset, workspace, workspace_bytes, stream, nullptr, bias, gated ? WAY_GATED : WAY_LAYER, &out);
+                y, 0, n, 1, offset, workspace, workspace_bytes, stream, nullptr, bias, true, gated ? WAY_GATED : WAY_LAYER, &out);
+}
+
+size_t layer_workspace(long m, long n, long k)
+{
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    Plan p = make_plan(1, m, n, k, true);
+    limit_chain(p, 1, m, n);
+    return plan_space(p).total;
 }
 
 }  // namespace pamgemm
 
 extern "C" {
+
+size_t pam_hip_layer_grad_workspace_bytes(long m, long n, long k) { return pamgemm::layer_workspace(m, n, k); }
+
+int pam_hip_layer_grad(const float* l, long l_sr, long l_sc, const float* r, long r_sr, long r_sc, const float* mo, long mo_sr, long mo_sc,
+                       float* dm, long dm_sr, long dm_sc, long m, long n, long k, int kind, float offset,
+                       void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (kind < 0 || kind > 2) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "layer_grad: unknown kind %d", kind);
+    return gemm("layer_grad", kind == 0 ? MODE_PAM : kind == 1 ? MODE_BWD_DL : MODE_BWD_DR, 1, m, n, k, l, 0, l_sr, l_sc, r, 0, r_sr, r_sc,
+                kind ? mo : nullptr, 0, mo_sr, mo_sc, dm, 0, dm_sr, dm_sc, offset, workspace, workspace_bytes, stream, nullptr, nullptr, true);
+}
 
 size_t pam_hip_gemm_workspace_bytes(long batch, long m, long n, long k)
 {

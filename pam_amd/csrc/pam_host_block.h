@@ -41,6 +41,30 @@ Layer layer(bool gated, const Tensor& X, const Tensor& W, const Tensor& bias, in
     return out;
 }
 
+// The gradients of Y = A (x) B, as product_grads, with the sums of pam_hip_layer_grad
+Tensor layer_grad(const Tensor& L, const Tensor& R, const Tensor& other, int kind, double offset)
+{
+    for (const Tensor* t : {&L, &R, &other}) check_tensor(*t);
+    const int64_t m = L.size(0), k = L.size(1), n = R.size(1);
+    TORCH_CHECK_VALUE(R.size(0) == k && other.size(0) == m && other.size(1) == n, "layer_grad: shapes ", shape(L), " and ", shape(R), " do not multiply to ", shape(other));
+    const OnDevice on(L);
+    const Tensor out = new_floats({m, n}, L);
+    if (out.numel() == 0) return out;
+    const size_t bytes = pam_hip_layer_grad_workspace_bytes(m, n, k);
+    Tensor ws;
+    if (bytes) ws = gemm_workspace(L, on.stream, bytes);
+    check_call(pam_hip_layer_grad(data(L), L.stride(0), L.stride(1), data(R), R.stride(0), R.stride(1), data(other), other.stride(0), other.stride(1),
+                                  data(out), out.stride(0), out.stride(1), m, n, k, kind, (float)offset, data_or_null(ws), bytes, on.stream), "layer_grad");
+    return out;
+}
+ProductGrads layer_grads(const Tensor& A, const Tensor& B, const Tensor& dY, const Approx& f, double offset, bool need_A, bool need_B)
+{
+    ProductGrads g;
+    if (need_A) g.dA = layer_grad(dY, row_major(B.t(), 2), A, f.a ? 0 : 1, offset);
+    if (need_B) g.dB = layer_grad(row_major(A.t(), 2), dY, B, f.b ? 0 : 2, offset);
+    return g;
+}
+
 struct LayerNode : torch::autograd::Function<LayerNode> {
     static Tensor forward(AutogradContext* ctx, bool gated, const Tensor& X_in, const Tensor& W, const std::optional<Tensor>& bias, int64_t activation,
                           const std::optional<Tensor>& residual, bool train, double offset, bool a, bool b, bool e)
@@ -83,7 +107,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
             }
             const Tensor X = row_major(saved[0], 2), Wt = row_major(saved[1].t(), 2);
             TORCH_CHECK_VALUE(X.size(0) == m && Wt.size(1) == rows, name, ": a saved tensor has not the shape that it was saved with");
-            const ProductGrads g = product_grads(X, Wt, dz, 2, f, offset, want_x, want_w);
+            const ProductGrads g = layer_grads(X, Wt, dz, f, offset, want_x, want_w);
             dX = g.dA;
             if (g.dB.defined()) dW = g.dB.t();
             if (want_b) db = sum_rows(dz);

@@ -2,7 +2,9 @@
 // activation, residual or the gated product behind the sums.
 //
 // Bound by reading w once.  33.5 MB of gated weights: one token 8.0 us (4.2 TB/s with the launch, copies reach 5.3), eight 10.7; the matrix
-// kernel, whose tiles have 64 rows, and a pass for the gate 26.  8.4 MB: one token 3.9 us, eight 5.6.
+// kernel, whose tiles have 64 rows, 25.  8.4 MB: one token 3.9 us, eight 5.6.
+// Up to eight tokens are one set of work-groups, up to 24 two or three, which read w from memory once between them (16 tokens through
+// 33.5 MB 17.7 us, the matrix kernel 25; through 8.4 MB 6.9 and 16; 24 tokens 25 and 26.5, 10.6 and 16.6; 32 tokens 32 and 26, 11.5 and 16.5).
 // A wavefront takes C rows of w and a part of k: its lanes lie along k with 128-bit loads, so that every load of a row is 1 KB in one
 // piece, and keep C x ROWS sums, which are added up over the lanes through LDS.  How many rows a wavefront takes and over how many of a
 // work-group's four wavefronts k is dealt out goes by the number of wavefronts (shape_for).  At these times a kernel's length counts:
@@ -89,14 +91,16 @@ __device__ __forceinline__ void add_products(const Quad (&x)[ROWS], const Quad (
 
 // S wavefronts along k: 1, 2 or 4.  GATED: the C rows of a wavefront are C / 2 of the gate's and the same ones of the other half.
 template <int ROWS, int C, bool GATED>
-__global__ __launch_bounds__(kThreads) void thin_kernel(pamthin::Layer g, int S)
+__global__ __launch_bounds__(kThreads) void thin_kernel(pamthin::Layer g, int S, int sets)
 {
     constexpr int kSums = ROWS * C;
     constexpr int kColumns = GATED ? C / 2 : C;
     __shared__ float sums[kWaves][kSums], lanes[kWaves][kSums * 65];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);      // (so the rows' addresses are scalars)
     const int share = wave % S, set = wave / S;                            // which part of k, which rows of w
-    const int column0 = ((int)blockIdx.x * (kWaves / S) + set) * kColumns;
+    // (work-groups go to the eight XCDs in turn: those that read the same rows of w for other tokens are eight apart, on one of them)
+    const int of_set = (int)blockIdx.x / (8 * sets) * 8 + (int)blockIdx.x % 8, row0 = (int)blockIdx.x / 8 % sets * ROWS;
+    const int column0 = (of_set * (kWaves / S) + set) * kColumns;
     const bool has_off = g.off != 1.0f;
     const float* wp[C];
     const float* ap[ROWS];
@@ -106,7 +110,7 @@ __global__ __launch_bounds__(kThreads) void thin_kernel(pamthin::Layer g, int S)
         wp[c] = g.w + (long)(GATED && c >= kColumns ? column + g.n : column) * g.w_sr;
     }
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) ap[r] = g.a + (long)min(r, g.m - 1) * g.a_sr;
+    for (int r = 0; r < ROWS; ++r) ap[r] = g.a + (long)min(row0 + r, g.m - 1) * g.a_sr;
     float acc[ROWS][C];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
@@ -157,7 +161,7 @@ __global__ __launch_bounds__(kThreads) void thin_kernel(pamthin::Layer g, int S)
         for (int s = 1; s < S; ++s) v += sums[wave + s][i];
         return v;
     };
-    const int r = lane / kColumns, c = column0 + lane % kColumns, at = lane / kColumns * C + lane % kColumns;
+    const int r = row0 + lane / kColumns, c = column0 + lane % kColumns, at = lane / kColumns * C + lane % kColumns;
     if (r >= g.m || c >= g.n) return;
     const Activation act{g.activation, g.off, has_off};
     float v = sum_of(at);
@@ -174,19 +178,19 @@ __global__ __launch_bounds__(kThreads) void thin_kernel(pamthin::Layer g, int S)
     }
 }
 
-constexpr long kMostRows = 8;
+constexpr long kMostRows = 24;
 
 // Rows of w per wavefront and wavefronts along k: from four rows and one wavefront on, until there are enough wavefronts, first by dealing
 // out k while a wavefront keeps two steps of it, then by taking fewer rows.  Enough keep the memory busy, sixteen on a compute
 // unit for one or two tokens (1024 -> 8192: 8.8 us with eight, 7.4); each reads all the tokens' rows, so that for more tokens eight do better
 // (33.5 MB, eight tokens: 10.7 us with eight, 13.5 with sixteen, 18.5 with thirty-two).
 struct Shape { int C, S; };
-Shape shape_for(long rows, long k, int tokens, bool gated)
+Shape shape_for(long rows, long k, int tokens, int sets, bool gated)
 {
     const long enough = tokens >= 4 ? 2048 : 4096;
     Shape s{4, 1};
     const long steps = (k + kStep - 1) / kStep, least = gated ? 2 : 1;
-    while ((rows + s.C - 1) / s.C * s.S < enough) {
+    while ((rows + s.C - 1) / s.C * s.S * sets < enough) {
         if (s.S < 4 && steps >= 2 * s.S) s.S *= 2;
         else if (s.C > least) s.C /= 2;
         else break;
@@ -205,12 +209,13 @@ bool takes(long m, long rows, long k, long a_sc, long w_sc)
 
 int launch(const char* what, const Layer& g, bool gated, hipStream_t st)
 {
-    const int rows = g.m <= 1 ? 1 : g.m <= 2 ? 2 : g.m <= 4 ? 4 : 8;
-    const Shape s = shape_for((long)g.n * (gated ? 2 : 1), g.k, rows, gated);
+    const int rows = g.m <= 1 ? 1 : g.m <= 2 ? 2 : g.m <= 4 ? 4 : 8, sets = (g.m + rows - 1) / rows;
+    const Shape s = shape_for((long)g.n * (gated ? 2 : 1), g.k, rows, sets, gated);
     const int columns = (gated ? s.C / 2 : s.C) * (kWaves / s.S);
-    const dim3 grid((unsigned)((g.n + columns - 1) / columns));
+    const unsigned each = (unsigned)((g.n + columns - 1) / columns);
+    const dim3 grid(sets == 1 ? each : (each + 7) / 8 * 8 * (unsigned)sets);
 #define PAM_THIN(ROWS, WIDE, GATED) \
-    if (rows == ROWS && s.C == WIDE && gated == GATED) hipLaunchKernelGGL((thin_kernel<ROWS, WIDE, GATED>), grid, dim3(kThreads), 0, st, g, s.S);
+    if (rows == ROWS && s.C == WIDE && gated == GATED) hipLaunchKernelGGL((thin_kernel<ROWS, WIDE, GATED>), grid, dim3(kThreads), 0, st, g, s.S, sets);
 #define PAM_THIN_ROWS(ROWS) PAM_THIN(ROWS, 1, false) PAM_THIN(ROWS, 2, false) PAM_THIN(ROWS, 4, false) PAM_THIN(ROWS, 2, true) PAM_THIN(ROWS, 4, true)
     PAM_THIN_ROWS(1) PAM_THIN_ROWS(2) PAM_THIN_ROWS(4) PAM_THIN_ROWS(8)
 #undef PAM_THIN_ROWS

@@ -1,7 +1,7 @@
 """The decoder block's operators: product with activation and residual, gated layer, rotation of queries and keys, clipping.
 
 Two references.  The chain of the package's own primitives, bit for bit where the order of the sums is the same (products of
-more than eight rows, rotations without a norm).  And the definition in 64 bits (tests/_block_ref.py), with these bounds, fixed
+more than 24 rows with sums of at most 1024 terms, rotations without a norm).  And the definition in 64 bits (tests/_block_ref.py), with these bounds, fixed
 before the first run:
   * a sum of K PAM terms in float32, in any order: off by at most K 2^-23 times the sum of the terms' magnitudes (the terms
     themselves are exact);
@@ -151,7 +151,7 @@ def same_with_grads(ours, chain, tensors, dy, what):
         assert_same_bits(host(g), host(c), f"{what}, gradient {i}")
 
 
-SHAPES = [(9, 4, 4), (17, 33, 20), (64, 64, 64), (70, 130, 132), (100, 515, 66), (300, 96, 8), (33, 40, 65)]
+SHAPES = [(29, 4, 4), (27, 33, 20), (64, 64, 64), (70, 130, 132), (100, 515, 66), (300, 96, 8), (33, 40, 65)]
 
 
 @pytest.mark.gpu
@@ -234,7 +234,7 @@ def act_slack(z, name):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 7, 8, 9, 16, 65])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 24, 25, 65])
 @pytest.mark.parametrize("k,n", [(1, 1), (3, 5), (64, 7), (129, 30), (257, 66), (1030, 12), (4096, 3)])
 def test_products_against_64_bits(m, k, n):
     rng = np.random.default_rng(m * 1000 + k + n)
