@@ -529,6 +529,7 @@ int fill(const char* what, RotaryArgs& a, const pam_hip_heads* parts, int count,
     for (int i = 0; i < 2; ++i) {
         const pam_hip_heads h = i < count ? parts[i] : pam_hip_heads{};
         a.part[i] = PartArgs{h.x, h.x_sb, h.x_st, h.x_sh, backward ? h.dy : nullptr, h.dy_sb, h.dy_st, h.dy_sh, h.weight, h.y, nullptr, (uint32_t)(batch * tokens * h.heads), (uint32_t)h.heads, 0};
+        if (backward && h.dweight && !h.weight) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the gradient of a weight that is not there", what);
         if (a.part[i].rows && dim && (!h.x || !h.y || (backward && !h.dy))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
     }
     if (a.part[0].rows + a.part[1].rows && rotated && (!cos || !sin) && table_rows > 0) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
