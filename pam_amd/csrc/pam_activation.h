@@ -77,6 +77,39 @@ struct Raw {
         return u2f((uint32_t)((int)whole + 127) << 23) * ((1.0f + x) - whole);
     }
 };
+// The gradients of the primitives by additions and, where a slope is exact, a product with a power of two (the formulas of
+// pam_mul_bwd, pad_div_bwd and the base-2 entry points for normal numbers).  APPROXIMATE: all are approximate; otherwise `approx` says.
+template <bool APPROXIMATE>
+struct RawGrad : Raw {
+    uint32_t off_add;                             // bits(b (*) offset) - bits(b)
+    __device__ __forceinline__ explicit RawGrad(float off) : Raw(off), off_add(f2u(off) - kBias) {}
+    __device__ __forceinline__ static float slope(uint32_t other, float own) { return u2f((other + (f2u(own) & kMant)) & ~kMant); }
+    __device__ __forceinline__ float of_mul(float own, float other, float d, bool approx) const
+    {
+        const float a = mul(d, other);
+        return APPROXIMATE || approx ? a : d * slope(f2u(other) + off_add, own);
+    }
+    __device__ __forceinline__ float of_dividend(float a, float inverse, float d, bool approx) const       // inverse: 1 (/) b
+    {
+        const float v = mul(inverse, d);
+        return APPROXIMATE || approx ? v : d * slope(f2u(inverse), a);
+    }
+    __device__ __forceinline__ float of_divisor(float quotient, float b, float d, bool approx) const       // b positive
+    {
+        const float a = mul(div(quotient, b), d);
+        return -(APPROXIMATE || approx ? a : d * u2f((f2u(quotient) & ~kMant) - (f2u(b) & kExpo) + kBias));
+    }
+    __device__ __forceinline__ float of_exp2(float t, float e, float d, bool approx) const
+    {
+        const float a = mul(mul(e, kActLn2), d);
+        return APPROXIMATE || approx ? a : u2f(f2u(e) & ~kMant) * d * slope(off_add + kBias, t);
+    }
+    __device__ __forceinline__ float of_log2(float v, float d, bool approx) const                          // v positive
+    {
+        const float a = div(div(d, v), kActLn2), log = (float)((int)f2u(v) - (int)kBias) * 0x1p-23f;
+        return APPROXIMATE || approx ? a : d * slope(f2u(div(1.0f, 1.0f)), log) * u2f((254u << 23) - (f2u(v) & kExpo));
+    }
+};
 template <int FIRST, int LAST>                    // magnitudes 2^FIRST <= |v| < 2^LAST: one shift-add and a max per value
 struct Window {
     uint32_t most = 0;
@@ -112,10 +145,11 @@ struct RawSigmoid {
         u = 1.0f + e;
     }
     __device__ __forceinline__ float result(const Raw& ar, float value) const { return is_zero(value) ? 0.0f : ar.div(x, u); }
-    __device__ __forceinline__ float grad(const Raw& ar, float d, float scale) const        // all slopes approximate; d not zero
+    template <bool APPROXIMATE>
+    __device__ __forceinline__ float grad(const RawGrad<APPROXIMATE>& ar, float d, float scale, const ApproxFlags& f) const        // d not zero
     {
-        const float du = -ar.mul(ar.div(ar.div(x, u), u), d), dt = ar.mul(ar.mul(e, kActLn2), du);
-        return ar.mul(ar.div(1.0f, u), d) + ar.mul(dt, scale);
+        const float du = ar.of_divisor(ar.div(x, u), u, d, f.b), dt = ar.of_exp2(t, e, du, f.e);
+        return ar.of_dividend(x, ar.div(1.0f, u), d, f.a) + ar.of_mul(x, scale, dt, f.a);
     }
 };
 

@@ -10,8 +10,7 @@
 // written and read back instead made the pass a third longer in bytes).
 // The chain of primitives is computed as one integer addition each (Raw), behind tests that what goes in is of ordinary size; a
 // wavefront that meets a zero, an infinity or an extreme exponent computes its heads by the checked functions, with the same results.
-// Heads that do not come in fours, or of more than 64 units, take a wavefront each by the checked functions; so does a group's lanes
-// an exact gradient.
+// Heads that do not come in fours, or of more than 64 units, take a wavefront each by the checked functions.
 #include <algorithm>
 
 #include "../../include/pam_hip_extra.h"
@@ -235,25 +234,29 @@ __device__ __forceinline__ float square_sum(const Raw& ar, const RotaryArgs& a, 
     return group_sum((at.there ? sum[0] : 0.0f) + (at.rotates ? sum[1] : 0.0f), a.lanes);
 }
 
-// root_of and the approximate square_grad as integer additions; `held`: all in their windows.
-struct RawRoot { float variance, root; bool held; };
+// root_of and square_grad as integer additions; `held`: all in their windows.
+struct RawRoot { float sum, variance, log, half, root; bool held; };
 __device__ __forceinline__ RawRoot raw_root_of(const Raw& ar, const RotaryArgs& a, float sum)
 {
     RawRoot r;
+    r.sum = sum;
     r.variance = ar.div(sum, (float)a.dim) + a.eps;
-    const float l = ar.div((float)((int)f2u(r.variance) - (int)kBias) * 0x1p-23f, 1.0f), t = ar.mul(ar.mul(l, 0.5f), 1.0f), whole = floorf(t);
-    r.root = u2f((uint32_t)((int)whole + 127) << 23) * ((1.0f + t) - whole);
+    r.log = ar.div((float)((int)f2u(r.variance) - (int)kBias) * 0x1p-23f, 1.0f);
+    r.half = ar.mul(r.log, 0.5f);
+    r.root = ar.exp2(r.half);
     WindowLog log;
     WindowRoot root;
     WindowPlain variance;
-    log.see(l); root.see(r.root); variance.see(r.variance);
+    log.see(r.log); root.see(r.root); variance.see(r.variance);
     r.held = log.held() && root.held() && variance.held() && r.variance > 0.0f;
     return r;
 }
-__device__ __forceinline__ float raw_square_grad(const Raw& ar, const RotaryArgs& a, const RawRoot& r, float droot)
+template <bool APPROXIMATE>
+__device__ __forceinline__ float raw_square_grad(const RawGrad<APPROXIMATE>& ar, const RotaryArgs& a, const RawRoot& r, float droot)
 {
-    const float dl = ar.mul(ar.mul(ar.mul(r.root, kActLn2), droot), 0.5f);
-    return ar.mul(ar.div(1.0f, (float)a.dim), ar.div(ar.div(dl, r.variance), kActLn2));
+    const ApproxFlags f = a.flags;
+    const float dl = ar.of_mul(r.log, 0.5f, ar.of_exp2(r.half, r.root, droot, f.e), f.a);
+    return ar.of_dividend(r.sum, ar.div(1.0f, (float)a.dim), ar.of_log2(r.variance, dl, f.e), f.a);
 }
 
 // The token at position 0 has sines of zero.  Its products with them are left out; the tests see one in their place.
@@ -345,59 +348,73 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a)
     else if (mine < p.rows) store_unit(h.y, at, y);
 }
 
-// The gradient with all approximate slopes, where a product's is its other factor.  term: the weight's gradient.  False as above.
-template <bool INTERLEAVED>
+// The gradient; APPROXIMATE: all slopes are, so that z is not needed.  term: the weight's gradient.  False as above.
+template <bool INTERLEAVED, bool APPROXIMATE>
 __device__ __forceinline__ bool backward_head(const RotaryArgs& a, const Unit& at, const v4f (&x)[2], v4f (&d)[2], const Weight& w, const v4f& c, v4f s,
                                               v4f (&dx)[2], v4f (&term)[2])
 {
-    const Raw ar(a.off);
+    const RawGrad<APPROXIMATE> ar(a.off);
+    const ApproxFlags f = a.flags;
     // (a token that the loss leaves out: behind a norm the gradients of such a head are zeros, the tests see ones in their place)
     const bool nothing = w.norm && in_group(all_zero(d), a.lanes);
     if (nothing) d[0] = d[1] = v4f{1.0f, 1.0f, 1.0f, 1.0f};
     const bool still = stands_still(s);
     bool held = usual_offset(a.off) && w.held;
+    RawRoot r{};
+    v4f z[2] = {x[0], x[1]};
+    if (w.norm) {
+        WindowX seen;
+        see(seen, x[0]); see(seen, x[1]);
+        r = raw_root_of(ar, a, square_sum(ar, a, at, x));
+        held = held && seen.held() && r.held;
+        if (!APPROXIMATE)
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[v][i] = ar.mul(ar.div(x[v][i], r.root), w.w[v][i]);
+    }
     dx[0] = d[0]; dx[1] = d[1];
     if (at.rotates) {
         WindowTable tables;
         WindowPlain seen;
         see(tables, c); see(tables, s); see(seen, d[0]); see(seen, d[1]);
+        if (!APPROXIMATE && !w.norm) { see(seen, x[0]); see(seen, x[1]); }
         held = held && tables.held() && seen.held();
-        float d1[4], d2[4], z1[4], z2[4];
+        float d1[4], d2[4], z1[4], z2[4], o1[4], o2[4];
         to_pairs<INTERLEAVED>(d, d1, d2);
+        to_pairs<INTERLEAVED>(z, z1, z2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            z1[i] = ar.mul(d1[i], c[i]) + (still ? 0.0f : ar.mul(d2[i], s[i]));
-            z2[i] = ar.mul(d2[i], c[i]) - (still ? 0.0f : ar.mul(d1[i], s[i]));
+            o1[i] = ar.of_mul(z1[i], c[i], d1[i], f.a) + (still ? 0.0f : ar.of_mul(z1[i], s[i], d2[i], f.a));
+            o2[i] = ar.of_mul(z2[i], c[i], d2[i], f.a) - (still ? 0.0f : ar.of_mul(z2[i], s[i], d1[i], f.a));
         }
-        from_pairs<INTERLEAVED>(z1, z2, dx);
+        from_pairs<INTERLEAVED>(o1, o2, dx);
     }
     if (w.norm) {
-        WindowX seen;
         WindowGrad grads;
-        see(seen, x[0]); see(seen, x[1]); see(grads, dx[0]); see(grads, dx[1]);
-        const RawRoot r = raw_root_of(ar, a, square_sum(ar, a, at, x));
+        see(grads, dx[0]); see(grads, dx[1]);
         float through[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < 2; ++v)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float n = ar.div(x[v][i], r.root), dz = dx[v][i];
-                dx[v][i] = ar.mul(dz, w.w[v][i]);
-                term[v][i] = ar.mul(dz, n);
-                through[v] -= ar.mul(ar.div(n, r.root), dx[v][i]);
+                dx[v][i] = ar.of_mul(n, w.w[v][i], dz, f.a);
+                term[v][i] = ar.of_mul(w.w[v][i], n, dz, f.b);
+                through[v] += ar.of_divisor(n, r.root, dx[v][i], f.b);
             }
         const float droot = group_sum((at.there ? through[0] : 0.0f) + (at.rotates ? through[1] : 0.0f), a.lanes);
         const float dsquare = raw_square_grad(ar, a, r, droot), inverse = ar.div(1.0f, r.root);
         WindowSquare squares;
         WindowRootGrad root_grads;
         squares.see(dsquare); root_grads.see(droot);
-        held = held && seen.held() && grads.held() && r.held && squares.held() && root_grads.held();
+        held = held && grads.held() && squares.held() && root_grads.held();
 #pragma unroll
         for (int v = 0; v < 2; ++v)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float q = ar.mul(dsquare, x[v][i]);
-                dx[v][i] = nothing ? 0.0f : ar.mul(inverse, dx[v][i]) + (q + q);
+                const float q = ar.of_mul(x[v][i], x[v][i], dsquare, f.a), q2 = APPROXIMATE ? q : ar.of_mul(x[v][i], x[v][i], dsquare, f.b);
+                dx[v][i] = nothing ? 0.0f : ar.of_dividend(x[v][i], inverse, dx[v][i], f.a) + (q + q2);
                 term[v][i] = nothing ? 0.0f : term[v][i];
             }
     }
@@ -435,9 +452,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 #pragma unroll 1
     for (int run = 0; run < turns; run += kRun) {
         const int end = min(run + kRun, turns);
-        uint32_t odd = ~0u;
-        if constexpr (APPROXIMATE) {
-            odd = 0u;
+        uint32_t odd = 0u;
+        {
             const Unit at(a, lane);
             const Weight w = load_weight(p.weight, at);
             v4f sum[2] = {};
@@ -446,9 +462,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
                 const Head h = head(turn);
                 v4f x[2] = {}, d[2], c, s, dx[2], term[2] = {};
                 load_unit(h.dy, at, d);
-                if (w.norm) load_unit(h.x, at, x);
+                if (w.norm || !APPROXIMATE) load_unit(h.x, at, x);
                 load_table(h, at, a.half > 0, c, s);
-                if (!backward_head<INTERLEAVED>(a, at, x, d, w, c, s, dx, term)) { odd |= 1u << (turn - run); continue; }
+                if (!backward_head<INTERLEAVED, APPROXIMATE>(a, at, x, d, w, c, s, dx, term)) { odd |= 1u << (turn - run); continue; }
                 if (first + turn * step < rows) {
                     store_unit(h.y, at, dx);
                     sum[0] += term[0]; sum[1] += term[1];
@@ -610,7 +626,8 @@ int pam_hip_rotary_bwd(const pam_hip_heads* parts, int count, const float* cos, 
         const long all = (long)a.part[0].rows + a.part[1].rows;
         for (PartArgs& p : a.part) p.groups = (int)backward_groups(p.rows, all, a.lanes);
         const bool approximate = a.flags.a && a.flags.b && a.flags.e;
-        rc = launch("rotary_bwd", a, !approximate ? rotary_bwd_kernel<false, false> : interleaved ? rotary_bwd_kernel<true, true> : rotary_bwd_kernel<false, true>, stream);
+        rc = launch("rotary_bwd", a, interleaved ? (approximate ? rotary_bwd_kernel<true, true> : rotary_bwd_kernel<true, false>)
+                                                 : (approximate ? rotary_bwd_kernel<false, true> : rotary_bwd_kernel<false, false>), stream);
     } else {
         whole_groups(a, kWaves);
         rc = launch("rotary_bwd", a, any_rotary_kernel<true>, stream);
