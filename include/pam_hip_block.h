@@ -1,7 +1,8 @@
 /*
  * pam_hip_block.h -- entry points of libpam_hip.so for the operators of a decoder block and its training step: a product with
  * an activation and a residual, the gated layer, the rotation of queries and keys, the clipping of gradients.  The reference
- * has no counterparts; each is a composition of the primitives of pam_hip.h.  Conventions as in pam_hip.h.
+ * has no counterparts; each is a composition of the primitives of pam_hip.h.  Conventions as in pam_hip.h.  Results share no memory
+ * with each other or with what is read, unless it is said that they may.
  */
 #ifndef PAM_HIP_BLOCK_H
 #define PAM_HIP_BLOCK_H
@@ -19,7 +20,9 @@ enum { PAM_HIP_ACT_NONE = 0, PAM_HIP_ACT_RELU = 1, PAM_HIP_ACT_SILU = 2, PAM_HIP
 
 /* y[m][n] = act(a[m][k] (x) w[n][k]^T + bias[n]) + residual[m][n].  y and z are contiguous; bias and residual may be NULL;
  * residual's rows are contiguous, residual_sr apart.  z, if not NULL, receives what the activation is applied to (a backward pass
- * reads it).  The offset goes to every PAM operation, as in the chain of primitives: folded into w for the products. */
+ * reads it).  The offset goes to every PAM operation, as in the chain of primitives: folded into w for the products.
+ * Sums: up to 24 rows of a, with a and w contiguous along k, are added up lane by lane along k; otherwise as pam_hip_pam_matmul_fwd
+ * adds them, in chains of at most 1024 terms (pam_hip_layer_grad).  The order depends on the sizes and strides, never on values. */
 size_t pam_hip_linear_act_workspace_bytes(long m, long n, long k);
 int pam_hip_linear_act_fwd(const float *a, long a_sr, long a_sc, const float *w, long w_sr, long w_sc, const float *bias,
                            int activation, const float *residual, long residual_sr, float *z, float *y, long m, long n, long k,

@@ -152,6 +152,8 @@ int check_sizes(const char* what, long m, long n, long k, int activation)
     return PAM_HIP_OK;
 }
 
+long both_halves(long f) { return f < 0 || f > (1L << 30) ? f : 2 * f; }      // (out of range as it is, not past a long)
+
 }  // namespace
 
 extern "C" {
@@ -181,7 +183,7 @@ int pam_hip_gated_linear_fwd(const float* a, long a_sr, long a_sc, const float* 
                              int activation, float* z, float* y, long m, long f, long k, float offset,
                              void* workspace, size_t workspace_bytes, void* stream)
 {
-    int rc = check_sizes("gated_linear_fwd", m, 2 * f, k, activation);
+    int rc = check_sizes("gated_linear_fwd", m, both_halves(f), k, activation);
     if (rc != PAM_HIP_OK) return rc;
     if (m == 0 || f == 0) return PAM_HIP_OK;
     if (!y || (k > 0 && (!a || !w))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "gated_linear_fwd: null pointer");
@@ -204,7 +206,7 @@ int pam_hip_act_bwd(const float* z, const float* dy, float* dz, size_t n, int ac
 int pam_hip_gated_bwd(const float* z, const float* dy, float* dz, long m, long f, int activation, float offset, int approx_a, int approx_b,
                       int approx_exp, void* stream)
 {
-    const int rc = check_sizes("gated_bwd", m, 2 * f, 0, activation);
+    const int rc = check_sizes("gated_bwd", m, both_halves(f), 0, activation);
     if (rc != PAM_HIP_OK) return rc;
     if (m == 0 || f == 0) return PAM_HIP_OK;
     if (!z || !dy || !dz) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "gated_bwd: null pointer");

@@ -107,69 +107,101 @@ __device__ __forceinline__ float square_grad(const RotaryArgs& a, const ApproxFl
 
 // ---------------------------------------------------------------- value by value, by the checked functions
 
-// A head's output, or its gradient with any slopes, computed by `lanes` lanes with a pair or a value at a time.
+// The lane's part of a head: pair(q) for its pairs, rest(i) for its values behind the rotated part.  GROUPED: those of its unit (below),
+// otherwise every `lanes`th.  Sums over them are kept in two parts as the groups' are (Sums), so that a head has the same sums, bit for bit,
+// whichever way its wavefront takes.
+template <bool GROUPED, class Pair, class Rest>
+__device__ __forceinline__ void each_value(const RotaryArgs& a, int lane, int lanes, Pair pair, Rest rest)
+{
+    const int turning = a.half / 4, behind = 2 * a.half + (GROUPED ? 4 * (lane - turning) : lane);
+    if (!GROUPED || lane < turning) {
+        const int end = GROUPED ? 4 * lane + 4 : a.half;
+#pragma unroll 1
+        for (int q = GROUPED ? 4 * lane : lane; q < end; q += GROUPED ? 1 : lanes) pair(q);
+    }
+    if (!GROUPED || lane >= turning) {
+        const int end = GROUPED ? min(behind + 4, a.dim) : a.dim;
+#pragma unroll 1
+        for (int i = behind; i < end; i += GROUPED ? 1 : lanes) rest(i);
+    }
+}
+struct Sums {
+    float part[2] = {0.0f, 0.0f};
+    __device__ __forceinline__ void add(bool second, float v) { if (second) part[1] += v; else part[0] += v; }
+    __device__ __forceinline__ float total(int lanes) const { return group_sum(part[0] + part[1], lanes); }
+};
+// Where a pair's values are, and the part of a sum that they are in: a unit's vectors hold firsts and seconds, or two pairs each.
+struct Pair {
+    int i, j; bool part_i, part_j;
+    __device__ __forceinline__ Pair(const RotaryArgs& a, int q)
+        : i(a.interleaved ? 2 * q : q), j(a.interleaved ? 2 * q + 1 : q + a.half), part_i(a.interleaved && (q & 2)), part_j(!a.interleaved || (q & 2)) {}
+};
+
+template <bool GROUPED>
 __device__ __forceinline__ Root head_root(const RotaryArgs& a, const float* x, int lane, int lanes)
 {
-    float sum = 0.0f;
-#pragma unroll 1
-    for (int i = lane; i < a.dim; i += lanes) sum += pam_mul_off(x[i], x[i], a.off, a.has_off);
-    return root_of(a, group_sum(sum, lanes));
+    Sums sum;
+    auto square = [&](bool second, float v) { sum.add(second, pam_mul_off(v, v, a.off, a.has_off)); };
+    each_value<GROUPED>(a, lane, lanes,
+        [&](int q) { const Pair p(a, q); square(p.part_i, x[p.i]); square(p.part_j, x[p.j]); },
+        [&](int i) { square(false, x[i]); });
+    return root_of(a, sum.total(lanes));
 }
 
+template <bool GROUPED>
 __device__ __forceinline__ void forward_by_value(const RotaryArgs& a, const float* weight, const Head& h, int lane, int lanes, bool store)
 {
-    const float root = weight ? head_root(a, h.x, lane, lanes).root : 1.0f;
+    const float root = weight ? head_root<GROUPED>(a, h.x, lane, lanes).root : 1.0f;
     if (!store) return;
     auto value = [&](int i) { return weight ? pam_mul_off(pad_div_off(h.x[i], root, a.off, a.has_off), weight[i], a.off, a.has_off) : h.x[i]; };
-#pragma unroll 1
-    for (int q = lane; q < a.half; q += lanes) {
-        const int i = a.interleaved ? 2 * q : q, j = a.interleaved ? 2 * q + 1 : q + a.half;
-        const float z1 = value(i), z2 = value(j);
-        const float c = h.cos ? h.cos[q] : u2f(kQNaN), s = h.sin ? h.sin[q] : u2f(kQNaN);
-        h.y[i] = pam_mul_off(z1, c, a.off, a.has_off) - pam_mul_off(z2, s, a.off, a.has_off);
-        h.y[j] = pam_mul_off(z2, c, a.off, a.has_off) + pam_mul_off(z1, s, a.off, a.has_off);
-    }
-#pragma unroll 1
-    for (int i = 2 * a.half + lane; i < a.dim; i += lanes) h.y[i] = value(i);
+    each_value<GROUPED>(a, lane, lanes,
+        [&](int q) {
+            const Pair p(a, q);
+            const float z1 = value(p.i), z2 = value(p.j);
+            const float c = h.cos ? h.cos[q] : u2f(kQNaN), s = h.sin ? h.sin[q] : u2f(kQNaN);
+            h.y[p.i] = pam_mul_off(z1, c, a.off, a.has_off) - pam_mul_off(z2, s, a.off, a.has_off);
+            h.y[p.j] = pam_mul_off(z2, c, a.off, a.has_off) + pam_mul_off(z1, s, a.off, a.has_off);
+        },
+        [&](int i) { h.y[i] = value(i); });
 }
 
 // term(i, t): the weight's gradient gets t at value i from this head.  APPROXIMATE: all slopes are.
-template <bool APPROXIMATE, class Term>
+template <bool GROUPED, bool APPROXIMATE, class Term>
 __device__ __forceinline__ void backward_by_value(const RotaryArgs& a, const float* weight, const Head& h, int lane, int lanes, bool store, Term term)
 {
     const float off = a.off;
     const bool has_off = a.has_off, norm = weight != nullptr;
     const ApproxFlags f = APPROXIMATE ? ApproxFlags{true, true, true} : a.flags;
-    const Root r = norm ? head_root(a, h.x, lane, lanes) : Root{0.0f, 0.0f, 1.0f};
-    float droot = 0.0f, dsquare = 0.0f;
+    const Root r = norm ? head_root<GROUPED>(a, h.x, lane, lanes) : Root{0.0f, 0.0f, 1.0f};
+    Sums droot;
+    float dsquare = 0.0f;
     // first the weight's gradient and the root's, then x's (one loop over both, so that the code is there once)
 #pragma unroll 1
     for (int round = norm ? 0 : 1; round < 2; ++round) {
-        auto take = [&](int i, float x, float n, float dz) {
+        auto take = [&](int i, bool second, float x, float n, float dz) {
             const float dn = norm ? mul_grad(n, weight[i], dz, f.a, off, has_off) : dz;
             if (round == 0) {
                 if (store) term(i, mul_grad(weight[i], n, dz, f.b, off, has_off));
-                droot += div_grad_b(x, r.root, dn, f.b, off, has_off);
+                droot.add(second, div_grad_b(x, r.root, dn, f.b, off, has_off));
             } else if (store) {
                 h.y[i] = norm ? div_grad_a(x, r.root, dn, f.a, off, has_off) + (mul_grad(x, x, dsquare, f.a, off, has_off) + mul_grad(x, x, dsquare, f.b, off, has_off)) : dn;
             }
         };
-#pragma unroll 1
-        for (int q = lane; q < a.half; q += lanes) {
-            const int i = a.interleaved ? 2 * q : q, j = a.interleaved ? 2 * q + 1 : q + a.half;
-            const float x1 = h.x[i], x2 = h.x[j], d1 = h.dy[i], d2 = h.dy[j];
-            const float n1 = norm ? pad_div_off(x1, r.root, off, has_off) : x1, n2 = norm ? pad_div_off(x2, r.root, off, has_off) : x2;
-            const float z1 = norm ? pam_mul_off(n1, weight[i], off, has_off) : x1, z2 = norm ? pam_mul_off(n2, weight[j], off, has_off) : x2;
-            const float c = h.cos ? h.cos[q] : u2f(kQNaN), s = h.sin ? h.sin[q] : u2f(kQNaN);
-            take(i, x1, n1, mul_grad(z1, c, d1, f.a, off, has_off) + mul_grad(z1, s, d2, f.a, off, has_off));
-            take(j, x2, n2, mul_grad(z2, c, d2, f.a, off, has_off) + mul_grad(z2, s, -d1, f.a, off, has_off));
-        }
-#pragma unroll 1
-        for (int i = 2 * a.half + lane; i < a.dim; i += lanes) {
-            const float x = h.x[i];
-            take(i, x, norm ? pad_div_off(x, r.root, off, has_off) : x, h.dy[i]);
-        }
-        if (round == 0) dsquare = square_grad(a, f, r, group_sum(droot, lanes));
+        each_value<GROUPED>(a, lane, lanes,
+            [&](int q) {
+                const Pair p(a, q);
+                const float x1 = h.x[p.i], x2 = h.x[p.j], d1 = h.dy[p.i], d2 = h.dy[p.j];
+                const float n1 = norm ? pad_div_off(x1, r.root, off, has_off) : x1, n2 = norm ? pad_div_off(x2, r.root, off, has_off) : x2;
+                const float z1 = norm ? pam_mul_off(n1, weight[p.i], off, has_off) : x1, z2 = norm ? pam_mul_off(n2, weight[p.j], off, has_off) : x2;
+                const float c = h.cos ? h.cos[q] : u2f(kQNaN), s = h.sin ? h.sin[q] : u2f(kQNaN);
+                take(p.i, p.part_i, x1, n1, mul_grad(z1, c, d1, f.a, off, has_off) + mul_grad(z1, s, d2, f.a, off, has_off));
+                take(p.j, p.part_j, x2, n2, mul_grad(z2, c, d2, f.a, off, has_off) + mul_grad(z2, s, -d1, f.a, off, has_off));
+            },
+            [&](int i) {
+                const float x = h.x[i];
+                take(i, false, x, norm ? pad_div_off(x, r.root, off, has_off) : x, h.dy[i]);
+            });
+        if (round == 0) dsquare = square_grad(a, f, r, droot.total(lanes));
     }
 }
 
@@ -344,7 +376,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a)
     load_unit(h.x, at, x);
     const Weight w = load_weight(p.weight, at);
     load_table(h, at, a.half > 0, c, s);
-    if (!forward_head<INTERLEAVED>(a, at, x, w, c, s, y)) forward_by_value(a, p.weight, h, threadIdx.x & (lanes - 1), lanes, mine < p.rows);
+    if (!forward_head<INTERLEAVED>(a, at, x, w, c, s, y)) forward_by_value<true>(a, p.weight, h, threadIdx.x & (lanes - 1), lanes, mine < p.rows);
     else if (mine < p.rows) store_unit(h.y, at, y);
 }
 
@@ -483,7 +515,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 #pragma unroll 1
         for (int turn = run; turn < end; ++turn)
             if ((odd >> (turn - run)) & 1u)
-                backward_by_value<APPROXIMATE>(a, p.weight, head(turn), lane, lanes, first + turn * step < rows, [&](int i, float t) { mine[i] += t; });
+                backward_by_value<true, APPROXIMATE>(a, p.weight, head(turn), lane, lanes, first + turn * step < rows, [&](int i, float t) { mine[i] += t; });
         wave_fence();
     }
     if (!p.sums) return;
@@ -507,8 +539,8 @@ __global__ __launch_bounds__(kThreads) void any_rotary_kernel(RotaryArgs a)
     if (row >= p.rows) return;
     const Head h = find_head(a, p, row);
     float* terms = p.sums ? p.sums + (long)row * a.dim : nullptr;      // (one row per head)
-    if (BACKWARD) backward_by_value<false>(a, p.weight, h, lane, 64, true, [&](int i, float t) { if (terms) terms[i] = t; });
-    else forward_by_value(a, p.weight, h, lane, 64, true);
+    if (BACKWARD) backward_by_value<false, false>(a, p.weight, h, lane, 64, true, [&](int i, float t) { if (terms) terms[i] = t; });
+    else forward_by_value<false>(a, p.weight, h, lane, 64, true);
 }
 
 // ---------------------------------------------------------------- host

@@ -147,6 +147,8 @@ __global__ __launch_bounds__(kThreads) void thin_kernel(pamthin::Layer g, int S,
     for (int r = 0; r < ROWS; ++r)
 #pragma unroll
         for (int c = 0; c < C; ++c) lanes[wave][(r * C + c) * 65 + lane] = acc[r][c];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");            // (a wavefront's LDS accesses are in order)
+    __builtin_amdgcn_wave_barrier();
     const float* part = lanes[wave] + lane / kLanes * 65 + lane % kLanes * kPart;
     float total = 0.0f;
 #pragma unroll 4

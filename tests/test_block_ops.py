@@ -434,6 +434,40 @@ def test_normed_rotation_is_the_chain(dim, rotated, offset):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,rotated", [(64, 64), (80, 40), (18, 10), (256, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("approx", [True, False])
+def test_heads_do_not_depend_on_each_other(dim, rotated, interleaved, approx):
+    """A head with values that take the full definitions changes no bit of its neighbours."""
+    rng = np.random.default_rng(dim + rotated)
+    angle = rng.uniform(-4, 4, (5, rotated // 2))
+    cos, sin = gpu(np.cos(angle).astype(np.float32)), gpu(np.sin(angle).astype(np.float32))
+    usual, w, d = normal(rng, 1, 5, 3, dim), gpu(normal(rng, dim, std=0.1) + np.float32(1.0)), gpu(normal(rng, 1, 5, 3, dim, std=0.1))
+    odd = usual.copy()
+    odd[0, ::2, 1, 0], odd[0, ::2, 1, 1], odd[0, ::2, 1, -1] = 0.0, 1e-39, -3e20
+    results = []
+    for values in (usual, odd):
+        x = gpu(values, True)
+        y, _ = pam.rotary(x, None, cos, sin, q_weight=w, interleaved=interleaved, approx_bwd=approx)
+        results.append([host(y), host(torch.autograd.grad(y, x, d)[0])])
+    for a, b in zip(*results):
+        assert_same_bits(a[:, :, ::2], b[:, :, ::2])
+        assert_same_bits(a[:, 1::2], b[:, 1::2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(3, 260, 20), (8, 1030, 40), (70, 260, 70)])
+def test_rows_do_not_depend_on_each_other(m, k, n):
+    rng = np.random.default_rng(m)
+    usual, w = normal(rng, m, k), gpu(normal(rng, 2 * n, k, std=0.1))
+    odd = usual.copy()
+    odd[1, 0], odd[1, 5], odd[1, k // 2], odd[1, -1] = 0.0, 1e-39, -3e30, 1e-25
+    for call in (lambda x: pam.linear_act(x, w, None, "silu"), lambda x: pam.gated_linear(x, w)):
+        a, b = host(call(gpu(usual))), host(call(gpu(odd)))
+        assert_same_bits(np.delete(a, 1, 0), np.delete(b, 1, 0))
+
+
+@pytest.mark.gpu
 def test_rotation_of_one_tensor_and_norm_of_the_other():
     rng = np.random.default_rng(4)
     q, k, w = gpu(normal(rng, 2, 3, 2, 16)), gpu(normal(rng, 2, 3, 1, 16)), gpu(normal(rng, 16))
