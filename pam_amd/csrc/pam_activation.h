@@ -153,8 +153,18 @@ struct RawSigmoid {
     }
 };
 
-// act(v) of a lane's values: by additions where all of the wavefront's are ordinary, else by the checked function, called.
+// act(v) of a lane's values: by additions where all of the wavefront's are ordinary, else by the checked function, called.  Four at a time, in a
+// loop that turns the array around, so that the code is there once (sixteen values written out: the same time, four times the code).
 __device__ __noinline__ float any_activation(float x, int kind, float off) { return Activation{kind, off, off != 1.0f}(x); }
+template <int N>
+__device__ __forceinline__ void turn(float (&v)[N], int by)
+{
+    float w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = v[(i + by) % N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = w[i];
+}
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], int kind, float off)
 {
@@ -164,21 +174,30 @@ __device__ __forceinline__ void activate(float (&v)[N], int kind, float off)
         for (int i = 0; i < N; ++i) v[i] = v[i] <= 0.0f ? 0.0f : v[i];
         return;
     }
+    constexpr int kWide = N < 4 ? N : 4;
     const float scale = kind == PAM_HIP_ACT_SILU ? kSiluScale : kGeluScale;
     const Raw ar(off);
-    WindowAct seen;
-    float y[N];
+#pragma unroll 1
+    for (int part = 0; part < N; part += kWide) {
+        WindowAct seen;
+        float y[kWide];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (!is_zero(v[i])) seen.see(v[i]);
-        y[i] = RawSigmoid(ar, v[i], scale).result(ar, v[i]);
-    }
-    if (__builtin_expect(__ballot(!seen.held() || !usual_sigmoid_offset(off)) == 0ull, 1)) {
+        for (int i = 0; i < kWide; ++i) {
+            if (!is_zero(v[i])) seen.see(v[i]);
+            y[i] = RawSigmoid(ar, v[i], scale).result(ar, v[i]);
+        }
+        if (__ballot(!seen.held() || !usual_sigmoid_offset(off)) != 0ull) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = y[i];
-    } else {
+            for (int i = 0; i < kWide; ++i) y[i] = v[i];
+#pragma unroll 1
+            for (int i = 0; i < kWide; ++i) {
+                y[0] = any_activation(y[0], kind, off);
+                turn(y, 1);
+            }
+        }
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = any_activation(v[i], kind, off);
+        for (int i = 0; i < kWide; ++i) v[i] = y[i];
+        turn(v, kWide);
     }
 }
 

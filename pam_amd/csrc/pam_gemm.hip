@@ -370,8 +370,8 @@ __global__ __launch_bounds__(128) void fold_kernel(pamgemm::GemmArgs g)
     const int r = row0 + place.ty * 4 + i, c = col0 + place.tx * 4;
     if (r >= g.M) return;
     if constexpr (WAY != WAY_PLAIN) {
-        const float sums[4] = {total.x, total.y, total.z, total.w};
-        if (c < g.N) finish_row<WAY>(g, r, c, g.N, sums);
+        const float sums[1][4] = {{total.x, total.y, total.z, total.w}};
+        if (c < g.N) finish_rows<WAY, 1>(g, r, c, g.M, g.N, sums);
         return;
     }
     float* dst = g.Y + (long)zb * g.y_sb + (long)r * g.y_sr + (long)c * g.y_sc;
@@ -387,8 +387,8 @@ __global__ __launch_bounds__(256) void empty_layer_kernel(pamgemm::GemmArgs g)
 {
     const int quads = (g.N + 3) / 4;
     const long idx = (long)blockIdx.x * 256 + threadIdx.x;
-    const float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (idx < (long)g.M * quads) finish_row<WAY>(g, (int)(idx / quads), (int)(idx % quads) * 4, g.N, sums);
+    const float sums[1][4] = {};
+    if (idx < (long)g.M * quads) finish_rows<WAY, 1>(g, (int)(idx / quads), (int)(idx % quads) * 4, g.M, g.N, sums);
 }
 
 // Products of at most kFewRows rows and short sums (one decoding step of attention: a query against the keys and values of
