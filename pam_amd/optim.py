@@ -174,6 +174,8 @@ def clip_grads(grads, max_norm, *, out=None, offset=None):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     out = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
     max_norm = float(max_norm)
+    if len(out) != len(grads):
+        raise ValueError(f"clip_grads: {len(grads)} tensors and {len(out)} outputs")
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads: the bound is not negative, got {max_norm}")
     return _abi.host().clip(grads, out, max_norm, _CLIP_EPS, 1.0 if offset is None else float(offset))
