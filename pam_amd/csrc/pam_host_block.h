@@ -116,8 +116,16 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
     }
 };
 
-bool wants_graph(std::initializer_list<const Tensor*> tensors)
+// A tensor that carries a forward-mode derivative is refused, also where nothing is recorded (it does not require a gradient): its result
+// would come without one, which counts as zero.
+void refuse_forward_mode(const char* name, const Tensor& t)
 {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name, ": no forward-mode derivatives");
+}
+
+bool wants_graph(const char* name, std::initializer_list<const Tensor*> tensors)
+{
+    for (const Tensor* t : tensors) refuse_forward_mode(name, *t);
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : tensors)
         if (t->defined() && t->requires_grad()) return true;
@@ -143,7 +151,7 @@ Tensor call_layer(bool gated, const Tensor& X, const Tensor& W, const std::optio
     std::optional<Tensor> r = residual;
     if (r && !rows) r = r->reshape({m, n});
     Tensor y;
-    if (wants_graph({&x, &W, bias ? &*bias : &none, r ? &*r : &none})) y = LayerNode::apply(gated, x, W, bias, activation, r, true, offset, a, b, e);
+    if (wants_graph(name, {&x, &W, bias ? &*bias : &none, r ? &*r : &none})) y = LayerNode::apply(gated, x, W, bias, activation, r, true, offset, a, b, e);
     else y = layer(gated, row_major(x, 2), W, bias.value_or(none), (int)activation, r.value_or(none), false, offset).y;
     return rows ? y : y.view(sizes);
 }
@@ -288,7 +296,7 @@ variable_list call_rotary(const Tensor& q, const std::optional<Tensor>& k, const
                           const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight, bool interleaved, double eps, double offset, bool a, bool b, bool e)
 {
     const Tensor none;
-    if (wants_graph({&q, k ? &*k : &none, &cos, &sin, q_weight ? &*q_weight : &none, k_weight ? &*k_weight : &none}))
+    if (wants_graph("rotary", {&q, k ? &*k : &none, &cos, &sin, q_weight ? &*q_weight : &none, k_weight ? &*k_weight : &none}))
         return RotaryNode::apply(q, k, cos, sin, positions, q_weight, k_weight, interleaved, eps, offset, a, b, e);
     variable_list x{q}, w{q_weight.value_or(none)};
     if (k) { x.push_back(*k); w.push_back(k_weight.value_or(none)); }
