@@ -339,6 +339,7 @@ Tensor clip(const py::list& ins, const py::list& outs, double max_norm, double e
         TORCH_CHECK_TYPE(THPVariable_Check(item), "clip_grads: expected tensors");
         return THPVariable_Unpack(item);
     };
+    const bool recording = at::GradMode::is_enabled();
     const at::AutoGradMode no_graph(false);
     const Tensor& first = tensor(ins, 0);
     std::vector<pam_hip_clip_tensor> table;
@@ -348,6 +349,9 @@ Tensor clip(const py::list& ins, const py::list& outs, double max_norm, double e
     for (size_t i = 0; i < count; ++i) {
         const Tensor* in = &tensor(ins, i);
         check_tensor(*in);
+        refuse_forward_mode(outs.empty() ? "grad_norm" : "clip_grads", *in);
+        TORCH_CHECK(!(recording && outs.empty() && in->requires_grad()),
+                    "grad_norm: the norm has no gradient, and a tensor requires one; detach it or call under torch.no_grad()");
         TORCH_CHECK_VALUE(in->layout() == at::kStrided && in->device() == first.device(), "clip_grads: tensors are dense and on one device");
         const at::IntArrayRef sizes = in->sizes();
         if (!in->is_non_overlapping_and_dense()) {

@@ -160,8 +160,15 @@ def multiply_grads(params, c, op_dict):
 _CLIP_EPS = 1e-6
 
 
+def _not_traced(name):
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{name} is not recorded by torch.jit.trace")
+
+
 def grad_norm(grads, *, offset=None):
-    """pow(sum of g (*) g over all tensors, 0.5), a tensor of no dimensions: the global norm of many fp32 GPU tensors."""
+    """pow(sum of g (*) g over all tensors, 0.5), a tensor of no dimensions: the global norm of many fp32 GPU tensors.  It has no
+    gradient: where autograd records, tensors that require one (gradients made with create_graph=True) are refused."""
+    _not_traced("grad_norm")
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     return _abi.host().clip(grads, [], math.inf, _CLIP_EPS, 1.0 if offset is None else float(offset))
 
@@ -169,8 +176,9 @@ def grad_norm(grads, *, offset=None):
 def clip_grads(grads, max_norm, *, out=None, offset=None):
     """Scales the tensors so that their global norm is at most max_norm: g (*) min(1, max_norm (/) (norm + 1e-6)), one pass for
     the norm and one for the products.  out: a list of tensors of the same shapes that takes the results; None: in place.
-    Returns the norm before, on the GPU (the host does not wait).  A norm that is not finite makes the gradients NaN, as an
+    Returns the norm before, on the GPU (the host does not wait).  Autograd records none of it, as it does not an ordinary clip.  A norm that is not finite makes the gradients NaN, as an
     ordinary clip does; a max_norm of infinity leaves them as they are."""
+    _not_traced("clip_grads")
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     out = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
     max_norm = float(max_norm)
@@ -194,6 +202,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         return torch.zeros(())
     if any(g.is_sparse for g in grads):
         raise RuntimeError("clip_grad_norm_ does not support sparse gradients")
-    if error_if_nonfinite and not bool(grad_norm(grads, offset=offset).isfinite()):
-        raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
+    if error_if_nonfinite:
+        with torch.no_grad():
+            finite = bool(grad_norm(grads, offset=offset).isfinite())
+        if not finite:
+            raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
     return clip_grads(grads, max_norm, offset=offset)

@@ -6,6 +6,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import pam_amd as pam
+from pam_amd import optim
 
 
 def ones(*shape):
@@ -31,3 +32,39 @@ def test_forward_mode_is_refused(recording):
             with pytest.raises(NotImplementedError):
                 call()
         assert pam.linear_act(x, w).shape == (3, 6) and pam.rotary(q, None, cos, sin)[0].shape == q.shape
+
+
+def test_clipping_is_not_traced():
+    for call in (lambda x: optim.grad_norm([x]), lambda x: optim.clip_grads([x], 1.0), lambda x: optim.clip_grad_norm_([_with_grad(x)], 1.0)):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, (torch.ones(3),), check_trace=False)
+
+
+def _with_grad(g):
+    p = torch.nn.Parameter(torch.zeros_like(g))
+    p.grad = g.detach()
+    return p
+
+
+@pytest.mark.gpu
+def test_the_norm_is_no_constant_of_a_graph():
+    """The norm of gradients that carry a graph is refused where it would silently leave that graph; clipping such gradients records
+    nothing, as torch.nn.utils.clip_grad_norm_ does not."""
+    w = ones(5).requires_grad_()
+    grad, = torch.autograd.grad((w ** 3).sum(), w, create_graph=True)
+    assert grad.requires_grad
+    for t in (grad, w):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            optim.grad_norm([ones(2), t])
+        with torch.no_grad():
+            assert float(optim.grad_norm([t])) > 0.0
+        assert not optim.grad_norm(t.detach()).requires_grad
+    out = torch.empty_like(grad, requires_grad=False)
+    assert not optim.clip_grads([grad], 0.5, out=[out]).requires_grad and float(out[0]) < 3.0
+    w.grad = grad
+    assert not optim.clip_grad_norm_([w], 0.5, error_if_nonfinite=True).requires_grad
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(ones(3), ones(3))
+        for call in (lambda: optim.grad_norm([ones(3), g]), lambda: optim.clip_grads([g], 1.0, out=[ones(3)])):
+            with pytest.raises(NotImplementedError):
+                call()
