@@ -374,6 +374,11 @@ Tensor clip(const py::list& ins, const py::list& outs, double max_norm, double e
         if (n) table.push_back({data(*in), out_data, n});
     }
     TORCH_CHECK_VALUE(outs.empty() || !clip_overlaps(table), "clip_grads: outputs share memory with each other or with other tensors");
+    // (written through their pointers: a graph that has saved one of them must not be run on the new values)
+    for (size_t i = 0; i < outs.size(); ++i) {
+        const Tensor& out = tensor(outs, i);
+        if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+    }
     const py::gil_scoped_release unlocked;
     const OnDevice on(first);
     const Tensor norm = new_floats({}, first);

@@ -68,3 +68,23 @@ def test_the_norm_is_no_constant_of_a_graph():
         for call in (lambda: optim.grad_norm([ones(3), g]), lambda: optim.clip_grads([g], 1.0, out=[ones(3)])):
             with pytest.raises(NotImplementedError):
                 call()
+
+
+@pytest.mark.gpu
+def test_clipped_tensors_count_as_modified():
+    """A graph that has saved a tensor is not run on the clipped values of it."""
+    def graph(saved):
+        return (saved * ones(4).requires_grad_()).sum()
+    g, out, kept = 3 * ones(4), ones(4), 3 * ones(4)
+    sums = [graph(t) for t in (g, out, kept)]
+    optim.clip_grads([g], 0.5)
+    optim.clip_grads([kept], 0.5, out=[out])
+    for y in sums[:2]:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    optim.grad_norm([kept])
+    sums[2].backward()                                   # only read
+    with torch.inference_mode():
+        t = 3 * ones(4)
+        optim.clip_grads([t], 0.5)
+        assert float(t[0]) < 3.0
