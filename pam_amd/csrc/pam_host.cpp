@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <numeric>
 #include <sstream>
 #include <string>
 #include <utility>

@@ -305,8 +305,6 @@ variable_list call_rotary(const Tensor& q, const std::optional<Tensor>& k, const
 
 // ---------------------------------------------------------------- clipping
 
-// The norm of all tensors; with `outs`, the clipped values there (a tensor may be its own output).  Values are taken in the order of
-// memory where a tensor's memory is without gaps or overlaps and its output's strides are its own; others go through copies.
 // Whether memory that is written for one tensor also belongs to another one of the table.
 bool clip_overlaps(const std::vector<pam_hip_clip_tensor>& table)
 {
@@ -328,6 +326,90 @@ bool clip_overlaps(const std::vector<pam_hip_clip_tensor>& table)
     return false;
 }
 
+// Whether a sum of x_i stride_i with 0 <= x_i <= most_i can be `target`: strides from the largest on, each x_i within what the smaller
+// ones can make up for.  Strides that enclose each other, as views of rows and columns have, leave one or two values to try; a search of
+// many steps counts as a yes.
+class Reach {
+public:
+    void add(int64_t stride, int64_t most) { if (stride > 0 && most > 0) terms[stride] += most; }
+    bool operator()(int64_t target)
+    {
+        int64_t reach = 0, divisor = 0;
+        rest.clear();
+        for (const auto& [stride, most] : terms) {               // (ascending)
+            reach += stride * most; divisor = std::gcd(divisor, stride);
+            rest.push_back({stride, most, reach, divisor});
+        }
+        steps = 0;
+        return search(rest.size(), target);
+    }
+private:
+    struct Term { int64_t stride, most, reach, divisor; };       // reach, divisor: of this and all smaller ones
+    bool search(size_t count, int64_t target)
+    {
+        if (target == 0 || ++steps > 10000) return true;
+        if (count == 0) return false;
+        const Term& t = rest[count - 1];
+        if (target < 0 || target > t.reach || target % t.divisor != 0) return false;
+        const int64_t below = t.reach - t.stride * t.most;
+        for (int64_t x = std::min(t.most, target / t.stride); x >= 0 && target - x * t.stride <= below; --x)
+            if (search(count - 1, target - x * t.stride)) return true;
+        return false;
+    }
+    std::map<int64_t, int64_t> terms;
+    std::vector<Term> rest;
+    int steps = 0;
+};
+// Whether two values of a tensor are at one address: differences of indices, the first of them at least one in dimension k, that sum to nothing.
+bool folds_on_itself(const Tensor& t)
+{
+    for (int64_t k = 0; k < t.dim(); ++k) {
+        if (t.size(k) <= 1) continue;
+        Reach reach;
+        int64_t others = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) {
+            reach.add(t.stride(i), i == k ? t.size(i) - 2 : 2 * (t.size(i) - 1));
+            if (i != k) others += (t.size(i) - 1) * t.stride(i);
+        }
+        if (reach(others - t.stride(k))) return true;
+    }
+    return false;
+}
+int64_t span(const Tensor& t)                                        // (floats from its first value to its last)
+{
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return last;
+}
+bool share_values(const Tensor& a, const Tensor& b)
+{
+    const intptr_t apart = (intptr_t)data(b) - (intptr_t)data(a);
+    Reach reach;
+    for (const Tensor* t : {&a, &b})
+        for (int64_t i = 0; i < t->dim(); ++i) reach.add(t->stride(i), t->size(i) - 1);
+    return apart % (intptr_t)sizeof(float) != 0 || reach(apart / (intptr_t)sizeof(float) + span(b));
+}
+// Whether an output that is written by a copy shares memory with itself or another output.  (Their inputs have been read by then.)
+bool copies_overlap(const std::vector<Tensor>& copied, const std::vector<Tensor>& direct)
+{
+    struct Output { const Tensor* t; uintptr_t begin, end; bool copied; };
+    std::vector<Output> outputs;
+    for (const auto* list : {&copied, &direct})
+        for (const Tensor& t : *list) {
+            if (t.numel() == 0) continue;
+            if (list == &copied && folds_on_itself(t)) return true;
+            const uintptr_t begin = (uintptr_t)data(t);
+            outputs.push_back({&t, begin, begin + (uintptr_t)(span(t) + 1) * sizeof(float), list == &copied});
+        }
+    std::sort(outputs.begin(), outputs.end(), [](const Output& a, const Output& b) { return a.begin < b.begin; });
+    for (size_t i = 0; i < outputs.size(); ++i)
+        for (size_t j = i + 1; j < outputs.size() && outputs[j].begin < outputs[i].end; ++j)
+            if ((outputs[i].copied || outputs[j].copied) && share_values(*outputs[i].t, *outputs[j].t)) return true;
+    return false;
+}
+
+// The norm of all tensors; with `outs`, the clipped values there (a tensor may be its own output).  Values are taken in the order of
+// memory where a tensor's memory is without gaps or overlaps and its output's strides are its own; others go through copies.
 // (the lists are read as Python holds them: a program's hundreds of tensors, twice, as vectors of references took longer than the kernels)
 Tensor clip(const py::list& ins, const py::list& outs, double max_norm, double eps, double offset)
 {
@@ -373,7 +455,16 @@ Tensor clip(const py::list& ins, const py::list& outs, double max_norm, double e
         const size_t n = (size_t)in->numel();
         if (n) table.push_back({data(*in), out_data, n});
     }
-    TORCH_CHECK_VALUE(outs.empty() || !clip_overlaps(table), "clip_grads: outputs share memory with each other or with other tensors");
+    bool shared = !outs.empty() && clip_overlaps(table);
+    if (!copied.empty() && !shared) {
+        variable_list by_copy, direct;
+        for (size_t i = 0; i < count; ++i) {
+            const Tensor& out = tensor(outs, i);
+            (by_copy.size() < copied.size() && copied[by_copy.size()].first.is_same(out) ? by_copy : direct).push_back(out);
+        }
+        shared = copies_overlap(by_copy, direct);
+    }
+    TORCH_CHECK_VALUE(!shared, "clip_grads: outputs share memory with each other, with other tensors or within themselves");
     // (written through their pointers: a graph that has saved one of them must not be run on the new values)
     for (size_t i = 0; i < outs.size(); ++i) {
         const Tensor& out = tensor(outs, i);

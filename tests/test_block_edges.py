@@ -1,6 +1,7 @@
 """The decoder block's operators where a call could go wrong without a word: derivatives that no kernel computes, shared memory,
 positions that no table has.
 """
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -88,3 +89,50 @@ def test_clipped_tensors_count_as_modified():
         t = 3 * ones(4)
         optim.clip_grads([t], 0.5)
         assert float(t[0]) < 3.0
+
+
+# ---------------------------------------------------------------- memory that outputs share
+
+@pytest.mark.gpu
+def test_clip_refuses_shared_outputs_of_other_strides():
+    """Outputs that are written by a copy are looked at where they are, not where the copy comes from."""
+    a, b, o = ones(10, 10), ones(10, 10), torch.full((10, 10), 7.0, device="cuda")
+    wide = torch.full((4, 12), 7.0, device="cuda")
+    for ins, outs in (([a, b], [o.t(), o.t()]), ([a, b], [o.t(), o]), ([a, b], [o, o.t()]), ([a[:4, :5], b[:4, :5]], [wide[:, :5], wide[:, 4:9]]),
+                      ([a[0, :4]], [o[0, :1].expand(4)]), ([a[:3, :3]], [torch.as_strided(o, (3, 3), (2, 1))])):
+        with pytest.raises(ValueError):
+            optim.clip_grads(ins, 1.0, out=outs)
+    row = torch.full((1, 4), 3.0, device="cuda")
+    with pytest.raises(ValueError):
+        optim.clip_grads([b, row.expand(5, 4)], 1.0)                 # in place, all rows one
+    assert o.eq(7.0).all() and wide.eq(7.0).all() and b.eq(1.0).all() and row.eq(3.0).all()          # and nothing written
+    # columns and halves of one buffer share its span, not its values
+    optim.clip_grads([a[:4, :6], b[:4, :6]], 1.0, out=[wide[:, ::2], wide[:, 1::2]])
+    assert wide.eq(wide[0, 0]).all() and float(wide[0, 0]) < 1.0
+    wide.fill_(1.0)
+    optim.clip_grads([wide[:, :6], wide[:, 6:]], 1.0)
+    assert wide.eq(wide[0, 0]).all() and float(wide[0, 0]) < 1.0
+
+
+@pytest.mark.gpu
+def test_shared_values_are_found_exactly():
+    """Drawn views of one buffer, their addresses written out: refused if and only if one address is there twice."""
+    rng = np.random.default_rng(11)
+    flat, refused = torch.zeros(400, device="cuda"), 0
+    for _ in range(400):
+        views, addresses = [], []
+        for _ in range(2):
+            sizes, strides = rng.integers(1, 5, 2), rng.integers(1, 13, 2)
+            start = int(rng.integers(0, 60))
+            views.append(torch.as_strided(flat, tuple(int(n) for n in sizes), tuple(int(n) for n in strides), start))
+            addresses += [start + i * int(strides[0]) + j * int(strides[1]) for i in range(sizes[0]) for j in range(sizes[1])]
+        grads = [ones(*v.shape) for v in views]
+        if len(set(addresses)) < len(addresses):
+            refused += 1
+            with pytest.raises(ValueError):
+                optim.clip_grads(grads, 0.5, out=views)
+        else:
+            flat.zero_()
+            optim.clip_grads(grads, 0.5, out=views)
+            assert all(v.eq(views[0].flatten()[0]).all() for v in views) and int(flat.ne(0).sum()) == len(addresses)
+    assert 50 < refused < 350
