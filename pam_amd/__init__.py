@@ -14,3 +14,5 @@ from . import pam_experimental  # noqa: F401
 from . import cuda_bindings     # noqa: F401
 from . import pam_ops           # noqa: F401
 from . import composites        # noqa: F401
+from . import optim             # noqa: F401
+from . import blocks            # noqa: F401
