@@ -53,6 +53,8 @@ class Attention(torch.nn.Module):
         qkv = block_ops.linear_act(self.norm(x), self.qkv, **self.kw).view(batch, tokens, -1, self.dim)
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), 2)
         seen = cache["k"].shape[1] if cache else 0
+        if seen + tokens > cos.shape[0]:
+            raise ValueError(f"Attention: {seen} tokens in the cache, {tokens} more, and tables of {cos.shape[0]} positions")
         positions = torch.arange(seen, seen + tokens, device=x.device) if seen else None
         q, k = block_ops.rotary(q, k, cos, sin, positions, q_weight=self.q_weight, k_weight=self.k_weight, **self.kw)
         if cache is not None:

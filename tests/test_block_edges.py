@@ -8,6 +8,7 @@ import torch.autograd.forward_ad as forward_ad
 
 import pam_amd as pam
 from pam_amd import optim
+from pam_amd.blocks import Attention
 
 
 def ones(*shape):
@@ -136,3 +137,20 @@ def test_shared_values_are_found_exactly():
             optim.clip_grads(grads, 0.5, out=views)
             assert all(v.eq(views[0].flatten()[0]).all() for v in views) and int(flat.ne(0).sum()) == len(addresses)
     assert 50 < refused < 350
+
+
+# ---------------------------------------------------------------- positions that no table has
+
+@pytest.mark.gpu
+def test_decoding_past_the_tables_is_refused():
+    """The rotation makes such positions NaN; the module knows how many tokens its cache has, and says so."""
+    attention = Attention(16, 2, 1, 8).cuda()
+    cos, sin = pam.rotary_tables(6, 8, device="cuda")
+    with torch.no_grad():
+        cache = {}
+        for tokens in (4, 1, 1):
+            assert attention(ones(2, tokens, 16), cos, sin, cache).isfinite().all()
+        for tokens, kept in ((1, cache), (7, None), (3, {k: v[:, :4] for k, v in cache.items()})):
+            with pytest.raises(ValueError):
+                attention(ones(2, tokens, 16), cos, sin, kept)
+    assert cache["k"].shape[1] == 6
