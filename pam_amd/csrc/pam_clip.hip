@@ -217,6 +217,7 @@ int each_table(const pam_hip_clip_tensor* tensors, long count, Table& table, F l
 {
     constexpr size_t kPart = (size_t)1 << 31;     // (a longer tensor enters the table in parts: counts are 32-bit ones)
     static_assert(kPart % kChunk == 0, "parts are whole chunks");
+    constexpr size_t kMostGroups = (size_t)1 << 23;          // (a launch counts its work-items in 32 bits)
     int held = 0;
     size_t groups = 0, before = 0;
     auto flush = [&]() -> int {
@@ -229,7 +230,7 @@ int each_table(const pam_hip_clip_tensor* tensors, long count, Table& table, F l
     for (long i = 0; i < count; ++i)
         for (size_t at = 0; at < tensors[i].n; at += kPart) {
             const size_t n = std::min(kPart, tensors[i].n - at), need = chunks(n);
-            if (held == Table::kTensors || groups + need > ((size_t)1 << 30)) { const int rc = flush(); if (rc != PAM_HIP_OK) return rc; }
+            if (held == Table::kTensors || groups + need > kMostGroups) { const int rc = flush(); if (rc != PAM_HIP_OK) return rc; }
             table.in[held] = tensors[i].in + at;
             set_out(table, held, tensors[i].out ? tensors[i].out + at : nullptr);
             table.n[held] = (unsigned)n; table.first[held] = (unsigned)groups;

@@ -381,14 +381,14 @@ __global__ __launch_bounds__(128) void fold_kernel(pamgemm::GemmArgs g)
         if (c + j < g.N) dst[(long)j * g.y_sc] = g.bias ? sums[j] + g.bias[c + j] : sums[j];
 }
 
-// sums over nothing on their way through an activation: a lane per four columns
+// sums over nothing on their way through an activation: a lane per four columns (of up to 2^31 lanes: a launch counts them in 32 bits)
 template <int WAY>
 __global__ __launch_bounds__(256) void empty_layer_kernel(pamgemm::GemmArgs g)
 {
     const int quads = (g.N + 3) / 4;
-    const long idx = (long)blockIdx.x * 256 + threadIdx.x;
     const float sums[1][4] = {};
-    if (idx < (long)g.M * quads) finish_rows<WAY, 1>(g, (int)(idx / quads), (int)(idx % quads) * 4, g.M, g.N, sums);
+    for (long idx = (long)blockIdx.x * 256 + threadIdx.x; idx < (long)g.M * quads; idx += (long)gridDim.x * 256)
+        finish_rows<WAY, 1>(g, (int)(idx / quads), (int)(idx % quads) * 4, g.M, g.N, sums);
 }
 
 // Products of at most kFewRows rows and short sums (one decoding step of attention: a query against the keys and values of
@@ -584,7 +584,7 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
     if (way != WAY_PLAIN) {
         if (K == 0) {
             const long n = M * ((N + 3) / 4);
-            const dim3 grid((unsigned)((n + 255) / 256));
+            const dim3 grid((unsigned)std::min((n + 255) / 256, 1L << 23));
             if (way == WAY_GATED) hipLaunchKernelGGL(empty_layer_kernel<WAY_GATED>, grid, dim3(256), 0, st, g);
             else hipLaunchKernelGGL(empty_layer_kernel<WAY_LAYER>, grid, dim3(256), 0, st, g);
             return pamhost::check_launch(what);

@@ -40,6 +40,7 @@ struct RotaryArgs {
     const long long* positions; long p_sb, p_st;
     uint32_t tokens;
     int dim, half, interleaved, lanes;            // lanes: of a group
+    int first_group;                              // of the launch, of all work-groups (see launch())
     float eps, off; bool has_off;
     ApproxFlags flags;
 };
@@ -365,12 +366,13 @@ __device__ __forceinline__ bool forward_head(const RotaryArgs& a, const Unit& at
 template <bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a)
 {
-    const bool other = (int)blockIdx.x >= a.part[0].groups;
+    const int block = a.first_group + (int)blockIdx.x;
+    const bool other = block >= a.part[0].groups;
     const PartArgs& p = other ? a.part[1] : a.part[0];
     const int lanes = a.lanes;
     const Unit at(a, threadIdx.x & (lanes - 1));
     // (lanes of heads past the end go along with the last head, for the sums over a group, and store nothing)
-    const uint32_t mine = (blockIdx.x - (other ? a.part[0].groups : 0)) * (kThreads / lanes) + threadIdx.x / lanes;
+    const uint32_t mine = (uint32_t)(block - (other ? a.part[0].groups : 0)) * (kThreads / lanes) + threadIdx.x / lanes;
     const Head h = find_head(a, p, min(mine, p.rows - 1));
     v4f x[2], c, s, y[2];
     load_unit(h.x, at, x);
@@ -532,9 +534,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 template <bool BACKWARD>
 __global__ __launch_bounds__(kThreads) void any_rotary_kernel(RotaryArgs a)
 {
-    const bool other = (int)blockIdx.x >= a.part[0].groups;
+    const int block = a.first_group + (int)blockIdx.x;
+    const bool other = block >= a.part[0].groups;
     const PartArgs& p = other ? a.part[1] : a.part[0];
-    const uint32_t row = (blockIdx.x - (other ? a.part[0].groups : 0)) * kWaves + threadIdx.x / 64;
+    const uint32_t row = (uint32_t)(block - (other ? a.part[0].groups : 0)) * kWaves + threadIdx.x / 64;
     const int lane = threadIdx.x % 64;
     if (row >= p.rows) return;
     const Head h = find_head(a, p, row);
@@ -589,14 +592,20 @@ int fill(const char* what, RotaryArgs& a, const pam_hip_heads* parts, int count,
     return PAM_HIP_OK;
 }
 
-// Launches `grouped` kernels (or those for any size) over the parts' work-groups.
+// Launches a kernel over the parts' work-groups (at most 2^28 and two).  A launch counts its work-items in 32 bits, so that more than 2^24
+// work-groups are several launches.
 template <class Kernel>
-int launch(const char* what, const RotaryArgs& a, Kernel kernel, void* stream)
+int launch(const char* what, RotaryArgs& a, Kernel kernel, void* stream)
 {
+    constexpr long kMost = 1L << 23;
     const long groups = (long)a.part[0].groups + a.part[1].groups;
-    if (groups == 0) return PAM_HIP_OK;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kThreads), 0, (hipStream_t)stream, a);
-    return pamhost::check_launch(what);
+    for (long first = 0; first < groups; first += kMost) {
+        a.first_group = (int)first;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(kMost, groups - first)), dim3(kThreads), 0, (hipStream_t)stream, a);
+        const int rc = pamhost::check_launch(what);
+        if (rc != PAM_HIP_OK) return rc;
+    }
+    return PAM_HIP_OK;
 }
 void whole_groups(RotaryArgs& a, int per_group) { for (PartArgs& p : a.part) p.groups = (int)((p.rows + per_group - 1) / per_group); }
 

@@ -204,9 +204,10 @@ Shape shape_for(long rows, long k, int tokens, int sets, bool gated)
 
 namespace pamthin {
 
+// (a work-group takes sixteen rows of w where there are many, and a launch counts its work-items in 32 bits, 2^24 work-groups)
 bool takes(long m, long rows, long k, long a_sc, long w_sc)
 {
-    return m <= kMostRows && k > 0 && k <= (1L << 28) && rows <= (1L << 30) && (a_sc == 1 || k == 1) && (w_sc == 1 || k == 1);
+    return m <= kMostRows && k > 0 && k <= (1L << 28) && rows * ((m + 7) / 8) <= (1L << 27) && (a_sc == 1 || k == 1) && (w_sc == 1 || k == 1);
 }
 
 int launch(const char* what, const Layer& g, bool gated, hipStream_t st)

@@ -7,6 +7,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import pam_amd as pam
+import _block_ref as ref
 from pam_amd import optim
 from pam_amd.blocks import Attention
 
@@ -154,3 +155,44 @@ def test_decoding_past_the_tables_is_refused():
             with pytest.raises(ValueError):
                 attention(ones(2, tokens, 16), cos, sin, kept)
     assert cache["k"].shape[1] == 6
+
+
+# ---------------------------------------------------------------- more work than one launch counts
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [2, 18])
+def test_rotation_of_more_heads_than_one_launch_takes(dim):
+    """2^26 heads of a size that takes a wavefront each are 2^32 work-items.  The input is one token, expanded."""
+    tokens, heads = (1 << 20) + 1, 64
+    cos, sin = pam.rotary_tables(4, dim, device="cuda")
+    generator = torch.Generator("cuda").manual_seed(1)
+    one, d = (torch.randn(1, 1, heads, dim, device="cuda", generator=generator) for _ in range(2))
+    x = one.clone().requires_grad_()
+    k = torch.randn(1, 1, 2, dim, device="cuda", generator=generator)
+    first = torch.full((1,), 3, device="cuda")
+    want, want_k = pam.rotary(x, k, cos, sin, first, approx_bwd=True)
+    dx, = torch.autograd.grad(want, x, d)
+    many = one.expand(1, tokens, heads, dim).requires_grad_()
+    y, yk = pam.rotary(many, k.expand(1, tokens, 2, dim), cos, sin, first.expand(tokens), approx_bwd=True)
+    assert y.eq(want).all() and yk.eq(want_k).all()
+    g, = torch.autograd.grad(y, many, d.expand(1, tokens, heads, dim))
+    assert g.eq(dx).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1 << 27, (1 << 27) + 8, (1 << 28) + 5])
+def test_one_row_through_more_weights_than_one_launch_takes(rows):
+    x, w = torch.full((1, 1), 1.5, device="cuda"), torch.full((1, 1), 1.25, device="cuda")
+    want = float(pam.mul(x, w))
+    y = pam.linear_act(x, w.expand(rows, 1))
+    assert y.shape == (1, rows) and y.eq(want).all()
+    h = pam.gated_linear(x, w.expand(rows // 2 * 2, 1), activation=None)
+    assert h.shape == (1, rows // 2) and h.eq(float(pam.mul(y[:, :1], y[:, :1]))).all()
+
+
+@pytest.mark.gpu
+def test_norm_of_more_values_than_one_launch_takes():
+    """33 times 2^31 values in one table, read from one tensor."""
+    t = torch.full((1 << 31,), 2.0 ** -10, device="cuda")
+    total = 33 * 2.0 ** 31 * 2.0 ** -20                  # (sums of equal powers of two, added in pairs: exact)
+    assert float(optim.grad_norm([t] * 33)) == float(ref.sqrt(np.array(total)))
