@@ -45,8 +45,9 @@ int pam_hip_gated_bwd(const float *z, const float *dy, float *dz, long m, long f
 
 /* The products of the layers' gradients, dX = dZ (x) W and dW^T = X^T (x) dZ: pam_hip_pam_matmul_fwd (kind 0, the approximate gradient,
  * mo not read) or pam_hip_pam_matmul_bwd (kind 1: l is the upstream gradient, 2: r is), with the sums held to chains of
- * 1024 terms: a chunk of pam_hip_gemm_plan that is longer is cut into equal ones of at most 1024, as the two forward products
- * above do.  (Without a workspace, or in products of more than 8192 tiles of 64 x 64, chunks stay as planned.) */
+ * 1024 terms, as in the two forward products above: a chunk of pam_hip_gemm_plan (or all of k, without a workspace) that is longer is
+ * added up in equal chains of whole 32 terms, at most 1024, each from +0, whose sums are added in ascending order from +0.  The
+ * workspaces of all three are those of the plain products. */
 size_t pam_hip_layer_grad_workspace_bytes(long m, long n, long k);
 int pam_hip_layer_grad(const float *l, long l_sr, long l_sc, const float *r, long r_sr, long r_sc, const float *mo, long mo_sr, long mo_sc,
                        float *dm, long dm_sr, long dm_sc, long m, long n, long k, int kind, float offset,

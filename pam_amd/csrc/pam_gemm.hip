@@ -295,20 +295,25 @@ Plan launch_plan(Plan p, bool pam, bool conv, bool quads, long batch, long M, lo
     return p;
 }
 
-// The layers' products (pam_hip_block.h) hold a chain of sums to kLongestChain terms: a plan of longer pieces is cut further, where a
-// cut tile can be (a workspace, arrival words for the tiles).  A chain of k terms in float32 loses about sqrt(k) 2^-25 of the result,
-// 1.3e-6 at the 4096 terms of a gated layer's gradients; with 1024 it is 9e-7 at most, for 3 % of the time (4096 tokens, 1024 -> 2 x 2048, forward
-// and gradients 2000 -> 2060 us; chains of 512 6e-7 and 2110).
+// The layers' products (pam_hip_block.h) hold a chain of sums to kLongestChain terms: longer pieces are added up chain by chain within their
+// unit (CHAIN in the kernel), so that the bound holds whatever the sizes and takes no scratch.  Products of standard normal values, 256 x 256
+// results: one chain of 1024 terms is off by 5.7e-7 of the results' root mean square, of 4096 by 1.1e-6, of 65536 by 4.6e-6, in chains of 1024
+// by 5.8e-7, 5.9e-7 at either length.  Over the tiles cut into pieces of 1024 terms instead: 4096 tokens, 1024 -> 2 x 2048, forward and
+// gradients 1959 -> 1926 us, exact ones 2526 -> 2458, 8192 tokens, 2048 -> 2 x 4096 15860 -> 15980; forty drawn layers 0.96 ... 1.03, in all 1.00.
+// Returns a chain's k-tiles, equal ones but the last; 0: the plan's pieces are short enough.
 constexpr long kLongestChain = 1024;
-void limit_chain(Plan& p, long batch, long M, long N)
+int chain_of(Plan& p, long batch, long M, long N, long K)
 {
-    const long tiles = batch * ((M + 63) / 64) * ((N + 63) / 64);
-    if ((long)p.piece_kt * p.bk <= kLongestChain || tiles > kMostCutTiles) return;
-    const int most = (int)(kLongestChain / p.bk), pieces = (p.kt + most - 1) / most;
-    p.piece_kt = (p.kt + pieces - 1) / pieces;
-    p.pieces = (p.kt + p.piece_kt - 1) / p.piece_kt;
-    p.units = tiles * p.pieces;
-    p.free = FreeShape{0, 0};
+    if ((long)p.piece_kt * p.bk <= kLongestChain) return 0;
+    if (p.bk != 32) {                                                  // (a forced depth, or short pieces of a small product: as many or fewer pieces)
+        p.bk = 32;
+        p.kt = (int)((K + 31) / 32); p.piece_kt = (p.piece_kt + 1) / 2; p.pieces = (p.kt + p.piece_kt - 1) / p.piece_kt;
+        p.units = batch * ((M + 63) / 64) * ((N + 63) / 64) * p.pieces;
+        p.free = FreeShape{0, 0};
+    }
+    constexpr int most = (int)(kLongestChain / 32);
+    const int chains = (p.piece_kt + most - 1) / most;
+    return chains > 1 ? (p.piece_kt + chains - 1) / chains : 0;
 }
 
 // workspace of a plan that cuts tiles: [arrival words, one per tile][one piece per unit].  The words' part has one size
@@ -504,7 +509,7 @@ unsigned spread_over_xcds(GemmArgs& g)
     return (unsigned)(g.xcd_chunk * XCDS);
 }
 
-template <int MODE>
+template <int MODE, bool CHAIN = false>
 void launch_mode(const Plan& p, int lk, int rk, hipStream_t st, const GemmArgs& g)
 {
     // Piece-major launches keep the launch order: all XCDs then work on the same few k ranges at a time (each L2 fetches them,
@@ -513,7 +518,8 @@ void launch_mode(const Plan& p, int lk, int rk, hipStream_t st, const GemmArgs& 
     GemmArgs ga = g;
     unsigned groups = (unsigned)p.units;
     if (p.units >= 64 && (p.pieces == 1 || g.fold_here)) groups = spread_over_xcds(ga);
-    if (p.bk == 32) pamgemm::launch_gemm<32, MODE>(lk, rk, groups, st, ga);
+    if constexpr (CHAIN) pamgemm::launch_gemm<32, MODE, true>(lk, rk, groups, st, ga);
+    else if (p.bk == 32) pamgemm::launch_gemm<32, MODE>(lk, rk, groups, st, ga);
     else pamgemm::launch_gemm<16, MODE>(lk, rk, groups, st, ga);
 }
 
@@ -538,8 +544,8 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
     }
     const bool usable = workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0;
     Plan p = make_plan(batch, M, N, K > 0 ? K : 1, usable);
-    if (layer && usable) limit_chain(p, batch, M, N);
     if (p.pieces > 1 && plan_space(p).total > workspace_bytes) p = make_plan(batch, M, N, K, false);       // whole tiles
+    const int chain_kt = layer ? chain_of(p, batch, M, N, K) : 0;
     int lk = load_kind(l_sr, l_sc, l_sb, l, M, K);
     int rk = conv ? LOAD_CONV : load_kind(r_sc, r_sr, r_sb, r, N, K);
     if (!conv && mode != MODE_STD) odd_lines(l_sr, l_sc, M, r_sc, r_sr, N, K, lk, rk);
@@ -580,6 +586,7 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
 
     g.cv = conv ? *conv : ConvGeom{nullptr, nullptr, 0, 0, 0, 0, 0};
     g.way = way_out ? *way_out : WayOut{nullptr, 0, nullptr, 0, 0};
+    g.chain_kt = chain_kt;
 
     if (way != WAY_PLAIN) {
         if (K == 0) {
@@ -591,7 +598,8 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
         }
         unsigned groups = (unsigned)p.units;
         if (p.units >= 64 && (p.pieces == 1 || g.fold_here)) groups = spread_over_xcds(g);       // (as launch_mode)
-        if (way == WAY_GATED) { if (p.bk == 32) launch_layer<32, WAY_GATED>(lk, groups, st, g); else launch_layer<16, WAY_GATED>(lk, groups, st, g); }
+        if (chain_kt > 0) { if (way == WAY_GATED) launch_layer<32, WAY_GATED, true>(lk, groups, st, g); else launch_layer<32, WAY_LAYER, true>(lk, groups, st, g); }
+        else if (way == WAY_GATED) { if (p.bk == 32) launch_layer<32, WAY_GATED>(lk, groups, st, g); else launch_layer<16, WAY_GATED>(lk, groups, st, g); }
         else { if (p.bk == 32) launch_layer<32, WAY_LAYER>(lk, groups, st, g); else launch_layer<16, WAY_LAYER>(lk, groups, st, g); }
         if (p.pieces > 1 && !g.fold_here) {
             const dim3 grid((unsigned)(p.units / p.pieces * 8));
@@ -612,11 +620,19 @@ int gemm(const char* what, int mode, long batch, long M, long N, long K,
         launch_free(odd_kind(lk), odd_kind(rk), groups, st, g);
         return pamhost::check_launch(what);
     }
-    switch (mode) {
-    case MODE_PAM: launch_mode<MODE_PAM>(p, lk, rk, st, g); break;
-    case MODE_STD: launch_mode<MODE_STD>(p, lk, rk, st, g); break;
-    case MODE_BWD_DL: launch_mode<MODE_BWD_DL>(p, lk, rk, st, g); break;
-    default: launch_mode<MODE_BWD_DR>(p, lk, rk, st, g); break;
+    if (chain_kt > 0) {
+        switch (mode) {
+        case MODE_PAM: launch_mode<MODE_PAM, true>(p, lk, rk, st, g); break;
+        case MODE_BWD_DL: launch_mode<MODE_BWD_DL, true>(p, lk, rk, st, g); break;
+        default: launch_mode<MODE_BWD_DR, true>(p, lk, rk, st, g); break;
+        }
+    } else {
+        switch (mode) {
+        case MODE_PAM: launch_mode<MODE_PAM>(p, lk, rk, st, g); break;
+        case MODE_STD: launch_mode<MODE_STD>(p, lk, rk, st, g); break;
+        case MODE_BWD_DL: launch_mode<MODE_BWD_DL>(p, lk, rk, st, g); break;
+        default: launch_mode<MODE_BWD_DR>(p, lk, rk, st, g); break;
+        }
     }
     if (p.pieces > 1 && !g.fold_here)
         hipLaunchKernelGGL(fold_kernel<WAY_PLAIN>, dim3((unsigned)(p.units / p.pieces * 8)), dim3(128), 0, st, g);
@@ -944,9 +960,7 @@ int layer_product(const char* what, bool gated, const float* a, long a_sr, long 
 size_t layer_workspace(long m, long n, long k)
 {
     if (m <= 0 || n <= 0 || k <= 0) return 0;
-    Plan p = make_plan(1, m, n, k, true);
-    limit_chain(p, 1, m, n);
-    return plan_space(p).total;
+    return plan_space(make_plan(1, m, n, k, true)).total;
 }
 
 }  // namespace pamgemm

@@ -1,0 +1,4 @@
+// The matrix kernels whose sums are chains of bounded length: exact gradients of the right operand (one file each: they compile side by side).
+#include "pam_gemm_kernel.h"
+
+template void pamgemm::launch_gemm<32, pamgemm::MODE_BWD_DR, true>(int, int, unsigned, hipStream_t, const pamgemm::GemmArgs&);

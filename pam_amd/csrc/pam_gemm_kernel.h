@@ -52,7 +52,8 @@
 //    activation and a residual, or as a gated layer's product ("what becomes of the sums" below).
 //  * Accumulation order: every output is summed by one lane per k chunk (piece), k ascending,
 //    from +0, and the chunks' sums are added in ascending order from +0 -- with one chunk
-//    this is the order of the reference kernel (pam/cuda_kernels.cu:601, 608-627);
+//    this is the order of the reference kernel (pam/cuda_kernels.cu:601, 608-627); the layers' products
+//    add up a long chunk in shorter chains (CHAIN below);
 //    pam_hip_gemm_plan reports the chunk length.
 #pragma once
 #include <cmath>
@@ -127,6 +128,7 @@ struct GemmArgs {
     float off; int has_off;      // has_off: 0 none, 1 a normal number (off_add = its bit-pattern increment), 2 any other value
     uint32_t off_add;
     WayOut way;
+    int chain_kt;                // CHAIN: k-tiles of a chain of sums
 };
 
 // Classifies and transforms one staged value.  MODE_PAM: R carries the bias subtraction, and
@@ -975,13 +977,17 @@ __device__ __forceinline__ void finish_rows(const A& a, int r, int c, int rows, 
 // FREE: tiles of free_r x free_c blocks of 4 x 4 outputs (at most BM x BN outputs) instead of 64 x 64.
 // CUT: the launch cuts its tiles' k ranges into pieces (an instance of its own, so that the kernel for whole tiles
 // carries none of the pieces' way out).
-template <int BM, int BN, int TM, int TN, int BK, int MODE, int LKIND, int RKIND, bool CUT, bool FREE = false, int WAY = WAY_PLAIN>
+// CHAIN: a unit's sums are chains of chain_kt k-tiles, each from +0, added up in ascending order from +0 as pieces are; the sums of the chains
+// that have ended wait in the lane's private memory, which a chain's end reads and writes once (sixteen more registers are not
+// there: LDS and registers are both full at four work-groups per compute unit).  CUT is set, and pieces may be 1 all the same.
+template <int BM, int BN, int TM, int TN, int BK, int MODE, int LKIND, int RKIND, bool CUT, bool FREE = false, int WAY = WAY_PLAIN, bool CHAIN = false>
 __global__ __launch_bounds__(256) PAM_GEMM_OCCUPANCY void gemm_kernel(GemmArgs g)
 {
     constexpr int NT = 256, NW = NT / 64;
     constexpr int GM = TM / 4, GN = TN / 4;               // 4-wide groups per micro-tile side
     constexpr int LDL = BM + PAD, LDR = BN + PAD;
     static_assert(TM == 4 && TN == 4 && (FREE ? !CUT && BK == 16 && MODE == MODE_PAM : BM == 64 && BN == 64), "a tile's piece is sixteen sums per lane of 256");
+    static_assert(!CHAIN || (CUT && !FREE), "chains are of fixed tiles");
 
     __shared__ __attribute__((aligned(16))) uint32_t lds_l[2][BK * LDL];
     __shared__ __attribute__((aligned(16))) uint32_t lds_r[2][BK * LDR];
@@ -1422,18 +1428,43 @@ __global__ __launch_bounds__(256) PAM_GEMM_OCCUPANCY void gemm_kernel(GemmArgs g
         }
     };
 
+    volatile v4f ended[CHAIN ? TM : 1];           // (volatile: in memory, not sixteen registers that the loops then lack)
+    auto end_chain = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const v4f sums = ended[CHAIN ? i : 0] + v4f{acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+            acc[i][0] = sums.x; acc[i][1] = sums.y; acc[i][2] = sums.z; acc[i][3] = sums.w;
+        }
+    };
+    int stop = ktiles;                            // where the chain ends
+    if constexpr (CHAIN) {
+        stop = min(stop, g.chain_kt);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) ended[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     int t = 0;
     while (t < ktiles) {
+        if constexpr (CHAIN) {
+            if (t == stop) {
+                end_chain();
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    ended[i] = v4f{acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+                    acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+                }
+                stop = min(ktiles, stop + late_args()->chain_kt);
+            }
+        }
         begin_tile(t);
         // Runs of full plain k-tiles -- nearly all of them -- are a loop of their own: the accumulators then stay
         // in the same registers from one k-tile to the next instead of being moved to where the other loops want them.
         while (verdict == 0 && kcount == BK) {
             plain_tile();
             end_tile(t);
-            if (++t == ktiles) break;
+            if (++t == stop) break;
             begin_tile(t);
         }
-        if (t == ktiles) break;
+        if (t == stop) continue;
         if (verdict == kIdle) { end_tile(t); ++t; continue; }
         // full k-tiles with zeros (activations after a ReLU, padding, pruned weights)
         if (kSkips && kcount == BK && verdict != 0 && verdict < kGuarded) {
@@ -1484,7 +1515,9 @@ __global__ __launch_bounds__(256) PAM_GEMM_OCCUPANCY void gemm_kernel(GemmArgs g
     // A piece of a cut tile goes to its slot of the workspace.  If that completes the tile (and the launch folds its
     // tiles itself), the pieces are added in ascending k order from +0.
     const LateArgs e = late_args();
-    if constexpr (CUT) {
+    if constexpr (CHAIN) end_chain();
+    const bool cut = CUT && (!CHAIN || e->pieces > 1);
+    if (cut) {
         if (!e->fold_here) {                       // a second kernel adds the pieces: ordinary stores, the launch's end publishes them
 #pragma unroll
             for (int i = 0; i < TM; ++i) *piece_row(e->partial, (long)flat * e->pieces + piece, i, tid) = v4f{acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
@@ -1548,12 +1581,13 @@ __global__ __launch_bounds__(256) PAM_GEMM_OCCUPANCY void gemm_kernel(GemmArgs g
     }
 }
 
-template <int BK, int MODE>
+template <int BK, int MODE, bool CHAIN = false>
 void launch_gemm(int lk, int rk, unsigned groups, hipStream_t st, const GemmArgs& g)
 {
 #define PAM_GEMM_CASE(LK, RK) \
     if (lk == LK && rk == RK) {                                                                                                   \
-        if (g.pieces > 1) hipLaunchKernelGGL((gemm_kernel<64, 64, 4, 4, BK, MODE, LK, RK, true>), dim3(groups), dim3(256), 0, st, g);  \
+        if constexpr (CHAIN) hipLaunchKernelGGL((gemm_kernel<64, 64, 4, 4, BK, MODE, LK, RK, true, false, WAY_PLAIN, true>), dim3(groups), dim3(256), 0, st, g);  \
+        else if (g.pieces > 1) hipLaunchKernelGGL((gemm_kernel<64, 64, 4, 4, BK, MODE, LK, RK, true>), dim3(groups), dim3(256), 0, st, g);  \
         else hipLaunchKernelGGL((gemm_kernel<64, 64, 4, 4, BK, MODE, LK, RK, false>), dim3(groups), dim3(256), 0, st, g);            \
         return;                                                                                                                   \
     }
@@ -1564,7 +1598,7 @@ void launch_gemm(int lk, int rk, unsigned groups, hipStream_t st, const GemmArgs
     if constexpr (MODE != MODE_STD) {                                  // lines at any float's address
         PAM_GEMM_CASE(LOAD_KODD, LOAD_KODD) PAM_GEMM_CASE(LOAD_KODD, LOAD_RODD) PAM_GEMM_CASE(LOAD_RODD, LOAD_KODD) PAM_GEMM_CASE(LOAD_RODD, LOAD_RODD)
     }
-    if constexpr (MODE != MODE_STD) {                                  // image patches as the right operand
+    if constexpr (MODE != MODE_STD && !CHAIN) {                        // image patches as the right operand
         PAM_GEMM_CASE(LOAD_KVEC, LOAD_CONV) PAM_GEMM_CASE(LOAD_RVEC, LOAD_CONV) PAM_GEMM_CASE(LOAD_ANY, LOAD_CONV)
         if constexpr (MODE == MODE_PAM) { PAM_GEMM_CASE(LOAD_KVEC, LOAD_CONVQ) }      // (forward products of patch embeddings)
         PAM_GEMM_CASE(LOAD_KVEC, LOAD_CONVR)                                          // (convolutions of horizontal stride 1)
@@ -1574,12 +1608,13 @@ void launch_gemm(int lk, int rk, unsigned groups, hipStream_t st, const GemmArgs
 }
 
 // The products with another way out: of operands contiguous along k, or any others value by value.
-template <int BK, int WAY>
+template <int BK, int WAY, bool CHAIN = false>
 void launch_layer(int kind, unsigned groups, hipStream_t st, const GemmArgs& g)
 {
 #define PAM_GEMM_CASE(KIND) \
     if (kind == KIND) {                                                                                                                      \
-        if (g.pieces > 1) hipLaunchKernelGGL((gemm_kernel<64, 64, 4, 4, BK, MODE_PAM, KIND, KIND, true, false, WAY>), dim3(groups), dim3(256), 0, st, g); \
+        if constexpr (CHAIN) hipLaunchKernelGGL((gemm_kernel<64, 64, 4, 4, BK, MODE_PAM, KIND, KIND, true, false, WAY, true>), dim3(groups), dim3(256), 0, st, g); \
+        else if (g.pieces > 1) hipLaunchKernelGGL((gemm_kernel<64, 64, 4, 4, BK, MODE_PAM, KIND, KIND, true, false, WAY>), dim3(groups), dim3(256), 0, st, g); \
         else hipLaunchKernelGGL((gemm_kernel<64, 64, 4, 4, BK, MODE_PAM, KIND, KIND, false, false, WAY>), dim3(groups), dim3(256), 0, st, g);   \
         return;                                                                                                                              \
     }
@@ -1599,5 +1634,11 @@ PAM_GEMM_EXTERN(16, MODE_BWD_DL) PAM_GEMM_EXTERN(32, MODE_BWD_DL) PAM_GEMM_EXTER
 #define PAM_GEMM_EXTERN(BK, WAY) extern template void launch_layer<BK, WAY>(int, unsigned, hipStream_t, const GemmArgs&);
 PAM_GEMM_EXTERN(16, WAY_LAYER) PAM_GEMM_EXTERN(32, WAY_LAYER) PAM_GEMM_EXTERN(16, WAY_GATED) PAM_GEMM_EXTERN(32, WAY_GATED)
 #undef PAM_GEMM_EXTERN
+// (chains are longer than 512 k, whose k-tiles are 32 deep)
+extern template void launch_gemm<32, MODE_PAM, true>(int, int, unsigned, hipStream_t, const GemmArgs&);
+extern template void launch_gemm<32, MODE_BWD_DL, true>(int, int, unsigned, hipStream_t, const GemmArgs&);
+extern template void launch_gemm<32, MODE_BWD_DR, true>(int, int, unsigned, hipStream_t, const GemmArgs&);
+extern template void launch_layer<32, WAY_LAYER, true>(int, unsigned, hipStream_t, const GemmArgs&);
+extern template void launch_layer<32, WAY_GATED, true>(int, unsigned, hipStream_t, const GemmArgs&);
 
 }  // namespace pamgemm
