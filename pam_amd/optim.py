@@ -15,6 +15,7 @@ import torch
 import yaml
 
 from . import _abi
+from .cuda_bindings import _is_tracing
 from .factories import get_function_dict
 
 __all__ = ["Adam", "multiply_grads", "grad_norm", "clip_grads", "clip_grad_norm_"]
@@ -161,7 +162,7 @@ _CLIP_EPS = 1e-6
 
 
 def _not_traced(name):
-    if torch.jit.is_tracing():
+    if _is_tracing():
         raise RuntimeError(f"{name} is not recorded by torch.jit.trace")
 
 
