@@ -99,7 +99,7 @@ struct ConvGeom { const int2* ktab; const int2* ltab; int H, W; int transposed; 
 // the columns alternate in twos between the gate's and the other factor's, g0 g1 u0 u1 g2 g3 u2 u3 ...: a lane's four columns are then both
 // factors of two outputs, and the gated layer is the plain product of its weight with the rows read in that order (R.sb apart).  In both z, if
 // given, receives what the activation is applied to, and Y and z have contiguous rows.  With z written, against a pass of its own behind the
-// product: 4096 tokens, 1024 -> 2 x 2048 gated 722 -> 684 us, 4096 x 512 -> 1024 with silu 112 -> 102, 771 x 300 -> 1001 with residual 32 -> 28.
+// product: 4096 tokens, 1024 -> 2 x 2048 gated 722 -> 684 us, 4096 x 512 -> 1024 with silu 112 -> 102, 771 x 300 -> 1001 with residual 32 -> 25.8.
 enum { WAY_PLAIN = 0, WAY_LAYER = 1, WAY_GATED = 2 };
 struct WayOut {
     const float* residual; long residual_sr;     // or null
@@ -884,7 +884,7 @@ __device__ __forceinline__ LateArgs late_args()
 
 // The sums of rows r ... r + ROWS - 1 (those below `rows` are there), columns c ... c + 3, on the ways through an activation.  The
 // rows' loads are all in flight at once: row after row, each waiting for its residual, 771 x 300 -> 1001 (208 tiles) took 28.4 us
-// instead of 26.4.  A: GemmArgs or its place among the kernel's arguments.
+// instead of 25.8.  A: GemmArgs or its place among the kernel's arguments.
 template <int WAY, int ROWS, class A>
 __device__ __forceinline__ void finish_rows(const A& a, int r, int c, int rows, int columns, const float (&sums)[ROWS][4])
 {

@@ -1,7 +1,7 @@
 // The rotation of queries' and keys' heads by their positions, after an optional norm of each head, and its gradient.
 //
 // Bound by memory: 8 bytes a value forward, 12 backward.  4 x 4096 tokens of 16 + 4 heads of 128, normed: forward 65 us (5.2 TB/s, what a
-// large copy reaches), forward and gradients with both weights' 182 us (160 at that rate).  A head is taken by a group of 2 ... 64 lanes, one unit each: four
+// large copy reaches), forward and gradients with both weights' 180 us (160 at that rate).  A head is taken by a group of 2 ... 64 lanes, one unit each: four
 // pairs of a rotated part (two 128-bit loads, `rotated / 2` apart or side by side) or four values of the rest, so that a
 // pair's two values meet in one lane and the only exchange is the norm's sum over the group.  cos and sin are read per head; the heads of a
 // token follow each other, so that all but the first find them in the cache next to the compute unit.  A work-group stays with

@@ -177,8 +177,9 @@ def grad_norm(grads, *, offset=None):
 def clip_grads(grads, max_norm, *, out=None, offset=None):
     """Scales the tensors so that their global norm is at most max_norm: g (*) min(1, max_norm (/) (norm + 1e-6)), one pass for
     the norm and one for the products.  out: a list of tensors of the same shapes that takes the results; None: in place.
-    Returns the norm before, on the GPU (the host does not wait).  Autograd records none of it, as it does not an ordinary clip.  A norm that is not finite makes the gradients NaN, as an
-    ordinary clip does; a max_norm of infinity leaves them as they are."""
+    Returns the norm before, on the GPU (the host does not wait).  Autograd records none of it, as it does not an ordinary clip.  A norm that is
+    not finite makes all gradients NaN, also where it overflowed (an ordinary clip scales by zero then: the root of an infinity is NaN here); a
+    max_norm of infinity leaves them as they are."""
     _not_traced("clip_grads")
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     out = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
