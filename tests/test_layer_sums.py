@@ -68,10 +68,10 @@ def one_chain(kind, left, right, forward):
     return out
 
 
-def in_order(kind, left, right, forward, n_planned=None):
+def in_order(kind, left, right, forward, n_planned=None, piece=None):
     """Pieces as the product's plan cuts them, each in equal chains of whole 32 terms, at most 1024; everything added from +0 upwards."""
     m, n, k = left.shape[0], right.shape[1], left.shape[1]
-    piece = min(_abi.gemm_plan(1, m, n_planned or n, k), (k + 31) // 32 * 32)
+    piece = piece or min(_abi.gemm_plan(1, m, n_planned or n, k), (k + 31) // 32 * 32)
     tiles = (piece + 31) // 32
     chain = piece if piece <= 1024 else -(-tiles // -(-tiles // 32)) * 32
     total = torch.zeros(m, n, device="cuda")
@@ -112,6 +112,23 @@ def test_gradients_are_added_in_chains(kind, m, n, k, layouts):
         got = layer_grad(kind, left, right, forward)
         same = (got.view(torch.int32) == want.view(torch.int32)) | (got.isnan() & want.isnan())
         assert same.all(), (left_how, right_how, int((~same).sum()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pieces,piece", [(1, 2528), (2, 1280), (3, 848)])
+def test_chains_of_a_forced_depth(pieces, piece):
+    """16-deep k-tiles, as a plan may have them: 157 in pieces of 157 and 79, which are longer than a chain and become 79 and 40 of 32, or 53."""
+    generator = torch.Generator("cuda").manual_seed(pieces)
+    left, right, forward = operand(generator, 100, 2500, "rows"), operand(generator, 2500, 70, "rows"), operand(generator, 100, 70, "rows")
+    for kind in (0, 1, 2):
+        want, _, chain = in_order(kind, left, right, forward, piece=piece)
+        assert chain in (864, 640, 848)
+        _abi.load_library().pam_hip_set_tuning(16, pieces)
+        try:
+            got = layer_grad(kind, left, right, forward)
+        finally:
+            _abi.load_library().pam_hip_set_tuning(0, 0)
+        assert ((got.view(torch.int32) == want.view(torch.int32)) | (got.isnan() & want.isnan())).all()
 
 
 @pytest.mark.gpu
