@@ -335,17 +335,19 @@ bool clip_overlaps(const std::vector<pam_hip_clip_tensor>& table)
 // many steps counts as a yes.
 class Reach {
 public:
-    void add(int64_t stride, int64_t most) { if (stride > 0 && most > 0) terms[stride] += most; }
+    void add(int64_t stride, int64_t most) { if (stride > 0 && most > 0) terms.push_back({stride, most, 0, 0}); }
     bool operator()(int64_t target)
     {
+        std::sort(terms.begin(), terms.end(), [](const Term& a, const Term& b) { return a.stride < b.stride; });
         int64_t reach = 0, divisor = 0;
-        rest.clear();
-        for (const auto& [stride, most] : terms) {               // (ascending)
-            reach += stride * most; divisor = std::gcd(divisor, stride);
-            rest.push_back({stride, most, reach, divisor});
+        size_t count = 0;
+        for (const Term& t : terms) {
+            if (count > 0 && terms[count - 1].stride == t.stride) terms[count - 1].most += t.most;       // (one choice instead of two)
+            else terms[count++] = t;
+            reach += t.stride * t.most; divisor = std::gcd(divisor, t.stride);
+            terms[count - 1].reach = reach; terms[count - 1].divisor = divisor;
         }
-        steps = 0;
-        return search(rest.size(), target);
+        return search(count, target);
     }
 private:
     struct Term { int64_t stride, most, reach, divisor; };       // reach, divisor: of this and all smaller ones
@@ -353,15 +355,14 @@ private:
     {
         if (target == 0 || ++steps > 10000) return true;
         if (count == 0) return false;
-        const Term& t = rest[count - 1];
+        const Term& t = terms[count - 1];
         if (target < 0 || target > t.reach || target % t.divisor != 0) return false;
         const int64_t below = t.reach - t.stride * t.most;
         for (int64_t x = std::min(t.most, target / t.stride); x >= 0 && target - x * t.stride <= below; --x)
             if (search(count - 1, target - x * t.stride)) return true;
         return false;
     }
-    std::map<int64_t, int64_t> terms;
-    std::vector<Term> rest;
+    c10::SmallVector<Term, 8> terms;
     int steps = 0;
 };
 // Whether two values of a tensor are at one address: differences of indices, the first of them at least one in dimension k, that sum to nothing.
@@ -396,19 +397,32 @@ bool share_values(const Tensor& a, const Tensor& b)
 // Whether an output that is written by a copy shares memory with itself or another output.  (Their inputs have been read by then.)
 bool copies_overlap(const std::vector<Tensor>& copied, const std::vector<Tensor>& direct)
 {
-    struct Output { const Tensor* t; uintptr_t begin, end; bool copied; };
+    struct Output {
+        const Tensor* t; uintptr_t begin, end; bool copied;
+        int64_t row = 0, width = 0;               // the largest stride, how far the other dimensions reach
+    };
     std::vector<Output> outputs;
     for (const auto* list : {&copied, &direct})
         for (const Tensor& t : *list) {
             if (t.numel() == 0) continue;
             if (list == &copied && folds_on_itself(t)) return true;
             const uintptr_t begin = (uintptr_t)data(t);
-            outputs.push_back({&t, begin, begin + (uintptr_t)(span(t) + 1) * sizeof(float), list == &copied});
+            Output o{&t, begin, begin + (uintptr_t)(span(t) + 1) * sizeof(float), list == &copied};
+            for (int64_t i = 0; i < t.dim(); ++i) if (t.size(i) > 1) o.row = std::max(o.row, t.stride(i));
+            for (int64_t i = 0; i < t.dim(); ++i) if (t.stride(i) < o.row) o.width += (t.size(i) - 1) * t.stride(i);
+            outputs.push_back(o);
         }
+    // (columns of one buffer, the common case, lie beside each other in its rows: 512 of them are 130 000 pairs)
+    const auto beside = [](const Output& a, const Output& b) {
+        const int64_t apart = (int64_t)(b.begin - a.begin);
+        if (a.row == 0 || a.row != b.row || apart % (int64_t)sizeof(float) != 0) return false;
+        const int64_t at = apart / (int64_t)sizeof(float) % a.row;
+        return at > a.width && at + b.width < a.row;
+    };
     std::sort(outputs.begin(), outputs.end(), [](const Output& a, const Output& b) { return a.begin < b.begin; });
     for (size_t i = 0; i < outputs.size(); ++i)
         for (size_t j = i + 1; j < outputs.size() && outputs[j].begin < outputs[i].end; ++j)
-            if ((outputs[i].copied || outputs[j].copied) && share_values(*outputs[i].t, *outputs[j].t)) return true;
+            if ((outputs[i].copied || outputs[j].copied) && !beside(outputs[i], outputs[j]) && share_values(*outputs[i].t, *outputs[j].t)) return true;
     return false;
 }
 
