@@ -15,7 +15,7 @@ x = cap (*) tanh(a (/) cap), tanh u = (1 - w) (/) (1 + w) with w = 2^-(u (*) 2 l
 over the keys j that query i sees; a query that sees none has the result zero.  A row's e and l may be scaled by a power of
 two, which moves no result.  With `own` false `run` computes this from elementary torch operations on the bit patterns, in 32
 bits; with `own` true by the package's kernels.  `exact` is the definition in 64 bits.  Gradients are the approximate ones that
-the training recipes use (the other factor for a product's slope).
+the training recipes use (the other factor for a product's slope, e itself for the slope of e^x).
 """
 import math
 
@@ -315,7 +315,7 @@ def _attend(q, k, v, see, far, slopes, cap, scale, dy=None):
     dn = _mul(_div(one, total), dy)
     dl = -_mul(_div(y, total), dy).sum(1, keepdim=True)
     de = _product(dn, v) + dl
-    da = _mul(_mul(_mul(e, _number(math.log(2.0), q)), de), log2e)
+    da = _mul(e, de)
     if cap:
         da = torch.where(see, _capped_grad(w, th, da, cap), 0.0)
     dq = _mul(_product(da, k.t()), scale)
@@ -493,7 +493,7 @@ def _exact_head(case, s, i, head, k, v, positions):
     through_n = D.mul(D.div(torch.ones_like(l), l), dy)
     through_l = -D.mul(D.div(y, l), dy).sum(1, keepdim=True)
     through_e = D.product(through_n, v.t()) + through_l
-    through_x = D.mul(D.mul(D.mul(e, _f32(math.log(2.0))), through_e), _f32(LOG2E))
+    through_x = D.mul(e, through_e)
     if case["cap"]:
         through_th = D.mul(through_x, c)
         through_w = -(D.mul(D.div(torch.ones_like(w), 1.0 + w), through_th) + D.mul(D.div(th, 1.0 + w), through_th))
