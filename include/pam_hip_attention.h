@@ -1,0 +1,57 @@
+/*
+ * pam_hip_attention.h -- entry points of libpam_hip.so for attention in one piece, its gradients, and the paged cache that a model
+ * reads while decoding.  The reference composes attention from its products and softmax.  Conventions as in pam_hip.h; results share
+ * no memory with each other or with what is read, unless it is said that they may.  Pointers to prefix, documents, slopes, pages, lengths
+ * and counts are device pointers.
+ */
+#ifndef PAM_HIP_ATTENTION_H
+#define PAM_HIP_ATTENTION_H
+
+#include <stddef.h>
+
+#include "pam_hip_block.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Values of every token's heads, [batch][tokens][heads][dim]: a head's values lie side by side, the other strides are free. */
+typedef struct { const float *p; long sb, st, sh; } pam_hip_tokens;
+
+/* What query i does with key j (positions: the queries are the last `tokens` of `keys` tokens):
+ *   a = sum over d of (q_d (*) scale) (*) k_d
+ *   cap > 0:  a = cap (*) tanh(a (/) cap) with tanh u = (1 - w) (/) (1 + w), w = 2^-(u (*) 2 log2 e), odd in u
+ *   slopes:   a = a - slopes[head] (*) |i - j|
+ *   e_ij = 2^(a (*) log2 e),   l_i = sum of e_ij,   y_id = (sum of e_ij (*) v_jd) (/) l_i
+ * over the keys that it sees: j <= i if causal; |i - j| < window if window > 0; those and all j < prefix[batch entry] if prefix; of those,
+ * if documents ([batch][keys]), the ones of its own document, which is not negative.  A query that sees no key has the result zero, and no
+ * gradients.  Keys' and values' heads are shared by heads / kv_heads queries' heads in a row.
+ * Weights below 2^-62 of the largest that came before them are none.  A score that is not a finite number, or is 2^127 or more, makes its query's
+ * results NaN.  offset multiplies every PAM product and quotient, and lies in (0.75, 1.5); scale lies in (2^-40, 2^40), cap is 0 or in
+ * (2^-20, 2^20).  dim is a multiple of four, up to 256, of which the first `values` values of every head
+ * count and the others (at most three) may be anything. */
+typedef struct {
+    long batch, tokens, keys, heads, kv_heads, dim, values;
+    float scale, cap, offset;
+    int causal;
+    long window;
+    const long long *prefix, *documents;
+    const float *slopes;
+} pam_hip_attention_shape;
+
+/* y is contiguous.  stats, if not NULL, receives two floats for every query's head, [batch][tokens][heads][2]: a backward pass reads them. */
+size_t pam_hip_attention_workspace_bytes(const pam_hip_attention_shape *shape);
+int pam_hip_attention_fwd(const pam_hip_attention_shape *shape, const pam_hip_tokens *q, const pam_hip_tokens *k, const pam_hip_tokens *v,
+                          float *y, float *stats, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gradients for q, k and v (contiguous; dq, or dk and dv, may be NULL) from that of y: the chain of the primitives' gradients, with the
+ * sums of heads that share a key.  y (contiguous) and stats are the forward pass's.  The approx flags are those of pam_hip_act_bwd. */
+size_t pam_hip_attention_bwd_workspace_bytes(const pam_hip_attention_shape *shape, int want_q, int want_kv);
+int pam_hip_attention_bwd(const pam_hip_attention_shape *shape, const pam_hip_tokens *q, const pam_hip_tokens *k, const pam_hip_tokens *v,
+                          const float *y, const float *stats, const pam_hip_tokens *dy, float *dq, float *dk, float *dv,
+                          int approx_a, int approx_b, int approx_exp, void *workspace, size_t workspace_bytes, void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* PAM_HIP_ATTENTION_H */

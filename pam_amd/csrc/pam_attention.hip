@@ -1,0 +1,295 @@
+// Attention's entry points, and the small kernels beside pam_attention_fwd.h and pam_attention_bwd.h: the rows' quantities that the gradients
+// start from, and the chunks' sums put together.
+#include <algorithm>
+
+#include "pam_attention.h"
+
+namespace pamatt {
+
+typedef void (*Kernel)(Args);
+struct Variant { int slices, quads; Kernel kernel; };
+extern const Variant kFwd1[], kFwd2[], kFwd4[], kDqApprox[], kDqExact[], kDkvApprox[], kDkvExact[];
+
+}  // namespace pamatt
+
+using namespace pamatt;
+
+namespace {
+
+// The chunks of a row: weights scaled to the largest M, sums added in ascending order.  A thread has a quad of a row.
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(Args a)
+{
+    const long quads = a.dim / 4, id = (long)blockIdx.x * kThreads + threadIdx.x, all = (long)a.batch * a.kv_heads * a.rows * quads;
+    if (id >= all) return;
+    const long at = id / quads, head = at / a.rows, row = at - head * a.rows;
+    const int d = (int)(id - at * quads) * 4;
+    float M = kNothing;
+    for (int c = 0; c < a.chunks; ++c) M = fmaxf(M, a.partial_stats[(head * a.chunks + c) * a.rows + row].y);
+    float l = 0.0f;
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < a.chunks; ++c) {
+        const long from = (head * a.chunks + c) * a.rows + row;
+        const float2 s = a.partial_stats[from];
+        if (s.y == kNothing) continue;
+        const float f = scale_between(s.y, M);
+        const v4f x = *reinterpret_cast<const v4f*>(a.partial + from * a.dim + d);
+        l += s.x * f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += x[i] * f;
+    }
+    const int b = (int)(head / a.kv_heads), kv = (int)(head - (long)b * a.kv_heads);
+    const long to = ((long)b * a.tokens + row / a.group) * a.heads + kv * a.group + row % a.group;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = M == kNothing ? 0.0f : pad_div_off(sum[i], l, a.off, a.off != 1.0f);
+    *reinterpret_cast<v4f_any*>(a.y + to * a.dim + d) = sum;
+    if (a.stats && d == 0) a.stats[to] = make_float2(l, M);
+}
+
+// A query's head: qs, dn and its record (see pam_attention_bwd.h).  Sixteen lanes have one.
+struct RowArgs { Args a; const float* y; Tokens dy; const float2* stats; float4* records; float* qs; float* dn; };
+__global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
+{
+    const Args& a = r.a;
+    const long all = (long)a.batch * a.tokens * a.heads, mine = (long)blockIdx.x * (kThreads / 16) + threadIdx.x / 16, id = min(mine, all - 1);
+    const int lane = threadIdx.x % 16;
+    const long token = id / a.heads, b = token / a.tokens, t = token - b * a.tokens;
+    const int head = (int)(id - token * a.heads), kv = head / a.group;
+    const long row = t * a.group + head % a.group, to = (b * a.kv_heads + kv) * a.rows + row;
+    const float off = a.off;
+    const bool has_off = off != 1.0f;
+    const float2 stats = r.stats[id];
+    const float* const q = a.q.p + b * a.q.sb + t * a.q.st + (long)head * a.q.sh;
+    const float* const dy = r.dy.p + b * r.dy.sb + t * r.dy.st + (long)head * r.dy.sh;
+    const float* const y = r.y + id * a.dim;
+    const bool sees = stats.y != kNothing;
+    const float l = sees ? stats.x : 1.0f, inverse = pad_div_off(1.0f, l, off, has_off);
+    const bool whole = fabsf(l) < u2f(kExpo);
+    float dl = 0.0f;
+    uint32_t most = 0u;
+    for (int d = lane; d < a.dim; d += 16) {
+        const bool there = d < a.values;
+        const float g = there ? dy[d] : 0.0f, out = there ? y[d] : 0.0f;
+        // (the sums that y was the quotient of: the same bits as far as they matter to a slope)
+        const float sums = whole ? pam_mul(has_off ? pam_mul(out, off) : out, l) : l;
+        const float dn = div_grad_a(sums, l, g, a.flags.a, off, has_off);
+        r.qs[to * a.dim + d] = there ? pam_mul_off(q[d], a.scale, off, has_off) : 1.0f;
+        r.dn[to * a.dim + d] = there ? dn : 1.0f;
+        if (!there) continue;
+        dl += a.flags.b ? -pam_mul_off(pad_div_off(out, l, off, has_off), g, off, has_off) : -(u2f(f2u(out) & ~kMant) / u2f(f2u(l) & kExpo)) * g;
+        most = max(most, f2u(dn) & ~kSign);
+    }
+    // (all sixteen lanes are there: a work-group past the end repeats the last row)
+    for (int s = 8; s >= 1; s /= 2) {
+        dl += __shfl_xor(dl, s, 16);
+        most = max(most, (uint32_t)__shfl_xor((int)most, s, 16));
+    }
+    if (lane != 0 || mine >= all) return;
+    // a query without a gradient counts as one that sees nothing: it has none to give
+    const bool none = !sees || (most == 0u && dl == 0.0f);
+    const int exponent = max(-86, min(60, (int)(most >> 23) - 127));
+    r.records[to] = make_float4(none ? u2f(kExpo) : stats.y, none ? 0.0f : dl, none ? -86.0f : (float)exponent, a.slopes ? held_slope(a.slopes[head]) : 0.0f);
+}
+
+// dq from the chunks' sums, through q (*) scale; or dk or dv: nothing behind the sums.
+__global__ __launch_bounds__(kThreads) void attention_sum_kernel(Args a, const float* parts, float* out, int of_keys)
+{
+    const long quads = a.dim / 4, id = (long)blockIdx.x * kThreads + threadIdx.x;
+    const long lanes = of_keys ? a.keys : a.rows, all = (long)a.batch * a.kv_heads * lanes * quads;
+    if (id >= all) return;
+    const long at = id / quads, head = at / lanes, row = at - head * lanes, b = head / a.kv_heads, kv = head - b * a.kv_heads;
+    const int d = (int)(id - at * quads) * 4;
+    v4f sum = *reinterpret_cast<const v4f*>(parts + (head * a.chunks * lanes + row) * a.dim + d);
+    for (int c = 1; c < a.chunks; ++c) sum += *reinterpret_cast<const v4f*>(parts + ((head * a.chunks + c) * lanes + row) * a.dim + d);
+    long to;
+    if (of_keys) to = (b * a.keys + row) * a.kv_heads + kv;
+    else {
+        const long t = row / a.group, h = kv * a.group + row % a.group;
+        const float* const q = a.q.p + b * a.q.sb + t * a.q.st + h * a.q.sh;
+        to = (b * a.tokens + t) * a.heads + h;
+        const bool has_off = a.off != 1.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (d + i < a.values) sum[i] = mul_grad(q[d + i], a.scale, sum[i], a.flags.a, a.off, has_off);
+    }
+    *reinterpret_cast<v4f_any*>(out + to * a.dim + d) = sum;
+}
+
+// ---------------------------------------------------------------- host
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+const Variant& variant_for(const Variant* list, int values)
+{
+    const Variant* v = list;
+    while (v[1].slices && v->slices * v->quads * 4 < values) ++v;
+    return *v;
+}
+const Variant& forward_variant(int values) { return variant_for(values <= 64 ? kFwd1 : values <= 128 ? kFwd2 : kFwd4, values); }
+
+// How the streamed rows are cut.  A chip with 256 compute units has 1024 SIMDs, of which each should have several wavefronts to choose from and
+// to finish at different times: `enough` of them in all.  A chunk is at least two spans.
+struct Plan { int tiles, chunks, chunk; };
+Plan plan_for(long heads, long lanes, int slices, long streamed, long enough)
+{
+    const long per_tile = (long)kWaves * (64 / slices), tiles = (lanes + per_tile - 1) / per_tile;
+    const long waves = heads * ((lanes + 64 / slices - 1) / (64 / slices));
+    long chunks = std::max(1L, std::min((enough + waves - 1) / std::max(1L, waves), (streamed + 2 * kSpan - 1) / (2 * kSpan)));
+    const long chunk = ((streamed + chunks - 1) / chunks + kSpan - 1) / kSpan * kSpan;
+    chunks = std::max(1L, (streamed + chunk - 1) / std::max(1L, chunk));
+    return Plan{(int)tiles, (int)chunks, (int)std::max((long)kSpan, chunk)};
+}
+constexpr long kEnough = 8192;
+
+int check(const char* what, const pam_hip_attention_shape* s, Args& a)
+{
+    if (!s) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
+    if (s->batch < 0 || s->tokens < 0 || s->keys < 0 || s->heads < 0 || s->kv_heads < 0 || s->window < 0)
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: negative size", what);
+    if (s->dim < 4 || s->dim > 256 || s->dim % 4 != 0 || s->values < 1 || s->values > s->dim || s->values <= s->dim - 4)
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: heads of %ld values in rows of %ld: up to 256, in rows of the next multiple of four", what, s->values, s->dim);
+    if (s->kv_heads == 0 ? s->heads != 0 : s->heads % s->kv_heads != 0)
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: %ld heads do not share %ld", what, s->heads, s->kv_heads);
+    if (s->batch > (1L << 20) || s->heads > (1L << 16) || s->tokens > (1L << 28) || s->keys > (1L << 28) || s->batch * s->kv_heads > (1L << 20)
+        || (s->kv_heads && s->heads / s->kv_heads * s->tokens > (1L << 30)) || s->batch * s->tokens * s->heads > (1L << 32))
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: size out of range", what);
+    if (!(s->scale > 0x1p-40f && s->scale < 0x1p40f)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the scale lies between 2^-40 and 2^40", what);
+    if (s->cap != 0.0f && !(s->cap > 0x1p-20f && s->cap < 0x1p20f)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the cap lies between 2^-20 and 2^20", what);
+    if (!(s->offset > 0.75f && s->offset < 1.5f)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the offset lies between 0.75 and 1.5", what);
+    if (s->documents && s->tokens > s->keys) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: more queries than keys, whose documents are given", what);
+    a.batch = (int)s->batch; a.tokens = (int)s->tokens; a.keys = (int)s->keys; a.heads = (int)s->heads; a.kv_heads = (int)s->kv_heads;
+    a.group = s->kv_heads ? (int)(s->heads / s->kv_heads) : 1; a.dim = (int)s->dim; a.values = (int)s->values;
+    a.rows = a.tokens * a.group; a.first = a.keys - a.tokens; a.causal = s->causal != 0; a.window = (int)std::min(s->window, 1L << 29);
+    a.prefix = s->prefix; a.documents = s->documents; a.slopes = s->slopes; a.scale = s->scale; a.cap = s->cap; a.off = s->offset;
+    return PAM_HIP_OK;
+}
+Tokens tokens_of(const pam_hip_tokens* t) { return Tokens{t->p, t->sb, t->st, t->sh}; }
+long heads_of(const Args& a) { return (long)a.batch * a.kv_heads; }
+
+// A launch counts its work-items in 32 bits.
+int launch(const char* what, Kernel kernel, const Args& a, hipStream_t st)
+{
+    const long groups = heads_of(a) * a.tiles * a.chunks;
+    if (groups > (1L << 23)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: size out of range", what);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kThreads), 0, st, a);
+    return pamhost::check_launch(what);
+}
+int groups_for(const char* what, long items, unsigned& groups)
+{
+    const long n = (items + kThreads - 1) / kThreads;
+    if (n > (1L << 23)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: size out of range", what);
+    groups = (unsigned)n;
+    return PAM_HIP_OK;
+}
+
+Plan forward_plan(const Args& a) { return plan_for(heads_of(a), a.rows, forward_variant(a.values).slices, a.keys, kEnough); }
+Plan dq_plan(const Args& a) { return plan_for(heads_of(a), a.rows, variant_for(kDqApprox, a.values).slices, a.keys, kEnough); }
+Plan dkv_plan(const Args& a) { return plan_for(heads_of(a), a.keys, variant_for(kDkvApprox, a.values).slices, a.rows, kEnough); }
+
+struct BackwardSpace { size_t records, qs, dn, dq, dk, dv, bytes; };
+BackwardSpace backward_space(const Args& a, bool want_q, bool want_kv)
+{
+    BackwardSpace s{};
+    const size_t rows = (size_t)heads_of(a) * a.rows, keys = (size_t)heads_of(a) * a.keys, row = (size_t)a.dim * sizeof(float);
+    size_t at = 0;
+    const auto take = [&](size_t n) { const size_t from = at; at += align256(n); return from; };
+    s.records = take(rows * sizeof(float4)); s.qs = take(rows * row); s.dn = take(rows * row);
+    if (want_q) s.dq = take(rows * row * dq_plan(a).chunks);
+    if (want_kv) { const size_t n = keys * row * dkv_plan(a).chunks; s.dk = take(n); s.dv = take(n); }
+    s.bytes = at;
+    return s;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pam_hip_attention_workspace_bytes(const pam_hip_attention_shape* shape)
+{
+    Args a{};
+    if (check("attention", shape, a) != PAM_HIP_OK || a.keys == 0) return 0;
+    const Plan p = forward_plan(a);
+    if (p.chunks == 1) return 0;
+    const size_t rows = (size_t)heads_of(a) * a.rows * p.chunks;
+    return align256(rows * sizeof(float2)) + align256(rows * a.dim * sizeof(float));
+}
+
+int pam_hip_attention_fwd(const pam_hip_attention_shape* shape, const pam_hip_tokens* q, const pam_hip_tokens* k, const pam_hip_tokens* v,
+                          float* y, float* stats, void* workspace, size_t workspace_bytes, void* stream)
+{
+    Args a{};
+    int rc = check("attention_fwd", shape, a);
+    if (rc != PAM_HIP_OK || a.batch == 0 || a.rows == 0) return rc;
+    if (!q || !k || !v || !q->p || !y || (a.keys && (!k->p || !v->p))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "attention_fwd: null pointer");
+    const size_t need = pam_hip_attention_workspace_bytes(shape);
+    if (need && (!workspace || workspace_bytes < need)) return pamhost::fail(PAM_HIP_ERR_WORKSPACE, "attention_fwd: workspace of %zu bytes needed", need);
+    a.q = tokens_of(q); a.k = tokens_of(k); a.v = tokens_of(v);
+    a.y = y; a.stats = reinterpret_cast<float2*>(stats);
+    const hipStream_t st = (hipStream_t)stream;
+    const Plan p = forward_plan(a);
+    a.tiles = p.tiles; a.chunks = p.chunks; a.chunk = p.chunk;
+    if (need) {
+        a.partial_stats = (float2*)workspace;
+        a.partial = (float*)((char*)workspace + align256((size_t)heads_of(a) * a.rows * p.chunks * sizeof(float2)));
+    }
+    unsigned groups = 0;
+    rc = groups_for("attention_fwd", heads_of(a) * a.rows * (a.dim / 4), groups);
+    if (rc == PAM_HIP_OK) rc = launch("attention_fwd", forward_variant(a.values).kernel, a, st);
+    if (rc != PAM_HIP_OK || !need) return rc;
+    hipLaunchKernelGGL(attention_join_kernel, dim3(groups), dim3(kThreads), 0, st, a);
+    return pamhost::check_launch("attention_fwd");
+}
+
+size_t pam_hip_attention_bwd_workspace_bytes(const pam_hip_attention_shape* shape, int want_q, int want_kv)
+{
+    Args a{};
+    if (check("attention_bwd", shape, a) != PAM_HIP_OK) return 0;
+    return backward_space(a, want_q != 0, want_kv != 0).bytes;
+}
+
+int pam_hip_attention_bwd(const pam_hip_attention_shape* shape, const pam_hip_tokens* q, const pam_hip_tokens* k, const pam_hip_tokens* v,
+                          const float* y, const float* stats, const pam_hip_tokens* dy, float* dq, float* dk, float* dv,
+                          int approx_a, int approx_b, int approx_exp, void* workspace, size_t workspace_bytes, void* stream)
+{
+    Args a{};
+    int rc = check("attention_bwd", shape, a);
+    if (rc != PAM_HIP_OK || a.batch == 0 || a.kv_heads == 0) return rc;
+    const bool want_kv = dk != nullptr;
+    if ((dk == nullptr) != (dv == nullptr)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "attention_bwd: the gradients of keys and values come together");
+    if (!q || !k || !v || !dy || (a.rows && (!q->p || !y || !stats || !dy->p)) || (a.keys && (!k->p || !v->p)))
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "attention_bwd: null pointer");
+    const BackwardSpace space = backward_space(a, dq != nullptr, want_kv);
+    if (space.bytes && (!workspace || workspace_bytes < space.bytes)) return pamhost::fail(PAM_HIP_ERR_WORKSPACE, "attention_bwd: workspace of %zu bytes needed", space.bytes);
+    char* const ws = (char*)workspace;
+    a.q = tokens_of(q); a.k = tokens_of(k); a.v = tokens_of(v);
+    a.flags = ApproxFlags{approx_a != 0, approx_b != 0, approx_exp != 0};
+    const bool approximate = approx_a && approx_b && approx_exp;
+    a.records = (const float4*)(ws + space.records); a.qs = (const float*)(ws + space.qs); a.dn = (const float*)(ws + space.dn);
+    const hipStream_t st = (hipStream_t)stream;
+    unsigned groups = 0, row_groups = 0, key_groups = 0;
+    if ((rc = groups_for("attention_bwd", heads_of(a) * a.rows * 16, groups)) || (rc = groups_for("attention_bwd", heads_of(a) * a.rows * (a.dim / 4), row_groups))
+        || (rc = groups_for("attention_bwd", heads_of(a) * a.keys * (a.dim / 4), key_groups))) return rc;
+    if (a.rows) {
+        const RowArgs r{a, y, tokens_of(dy), reinterpret_cast<const float2*>(stats), (float4*)(ws + space.records), (float*)(ws + space.qs), (float*)(ws + space.dn)};
+        hipLaunchKernelGGL(attention_rows_kernel, dim3(groups), dim3(kThreads), 0, st, r);
+        if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
+    }
+    if (dq && a.rows) {
+        Args d = a;
+        const Plan p = dq_plan(a);
+        d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.out0 = (float*)(ws + space.dq);
+        if ((rc = launch("attention_bwd", variant_for(approximate ? kDqApprox : kDqExact, a.values).kernel, d, st))) return rc;
+        hipLaunchKernelGGL(attention_sum_kernel, dim3(row_groups), dim3(kThreads), 0, st, d, d.out0, dq, 0);
+        if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
+    }
+    if (want_kv && a.keys) {
+        Args d = a;
+        const Plan p = dkv_plan(a);
+        d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.out0 = (float*)(ws + space.dk); d.out1 = (float*)(ws + space.dv);
+        if ((rc = launch("attention_bwd", variant_for(approximate ? kDkvApprox : kDkvExact, a.values).kernel, d, st))) return rc;
+        hipLaunchKernelGGL(attention_sum_kernel, dim3(key_groups), dim3(kThreads), 0, st, d, d.out0, dk, 1);
+        hipLaunchKernelGGL(attention_sum_kernel, dim3(key_groups), dim3(kThreads), 0, st, d, d.out1, dv, 1);
+        if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
+    }
+    return PAM_HIP_OK;
+}
+
+}  // extern "C"

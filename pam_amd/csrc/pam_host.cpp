@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "../../include/pam_hip.h"
+#include "../../include/pam_hip_attention.h"
 #include "../../include/pam_hip_block.h"
 #include "../../include/pam_hip_extra.h"
 
@@ -490,6 +491,7 @@ struct UnaryNode : torch::autograd::Function<UnaryNode> {
 };
 
 #include "pam_host_block.h"
+#include "pam_host_attention.h"
 
 // ---------------------------------------------------------------- optimizer
 
@@ -577,6 +579,7 @@ PYBIND11_MODULE(_pam_host, module)
     module.def("unary", [](const Tensor& x, int64_t op, double number, double offset, bool a, bool e) { return UnaryNode::apply(x, op, number, offset, a, e); }, unlocked);
     module.def("layer", &call_layer, unlocked);
     module.def("rotary", &call_rotary, unlocked);
+    module.def("attention", &call_attention, unlocked);
     module.def("clip", &clip);
     module.def("adam_collect", &adam_collect);
 }
