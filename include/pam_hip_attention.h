@@ -51,6 +51,35 @@ int pam_hip_attention_bwd(const pam_hip_attention_shape *shape, const pam_hip_to
                           const float *y, const float *stats, const pam_hip_tokens *dy, float *dq, float *dk, float *dv,
                           int approx_a, int approx_b, int approx_exp, void *workspace, size_t workspace_bytes, void *stream);
 
+/* A cache in pages: keys and values of [pages][page][kv_heads][dim], a head's values side by side, the other strides (the same for both) free.
+ * pages ([batch][per_sequence], contiguous): the page of a sequence's places 0 ... page - 1, then of the next ones.  lengths ([batch]): the tokens of
+ * every sequence that are in the cache already; token t of a call is at place lengths + t.  counts ([batch]) or NULL: how many of a call's tokens a
+ * sequence has; the others are padding.  dim: up to 256. */
+typedef struct {
+    long batch, tokens, heads, kv_heads, dim;
+    long page, pages, per_sequence;
+    float scale, cap, offset;
+    long window;
+    const float *slopes;
+} pam_hip_cache_shape;
+
+/* The rotation (and norm) of pam_hip_rotary_fwd for the new tokens' queries and keys, a token's row of the tables being its place; q's go to q->y
+ * (contiguous; padding's are zeros; q may be NULL), k's and, as they are, v's to their places in the cache.  A token whose place the table does not have, or whose
+ * page is not there, is written nowhere.  Places of two tokens of a call must differ, and the cache shares no memory with what is read.  k->y, v->y and
+ * v->weight are not read. */
+int pam_hip_rotary_append(const pam_hip_heads *q, const pam_hip_heads *k, const pam_hip_heads *v, const float *cos, const float *sin,
+                          long table_rows, float *cache_k, float *cache_v, long cache_sp, long cache_st, long cache_sh, long page,
+                          long pages, long per_sequence, const int *table, const long long *lengths, const long long *counts,
+                          long batch, long tokens, long dim, long rotated, int interleaved, float eps, float offset, void *stream);
+
+/* The new tokens' queries (already in the cache are their keys and values, too) over the places 0 ... lengths + t of their sequences, or the last
+ * `window` of those; scores, weights and results as above.  y [batch][tokens][heads][dim] is contiguous; padding's are zeros.  A place that the table does
+ * not have, or on a page that is not there, makes the results that see it NaN. */
+size_t pam_hip_cached_attention_workspace_bytes(const pam_hip_cache_shape *shape);
+int pam_hip_cached_attention_fwd(const pam_hip_cache_shape *shape, const pam_hip_tokens *q, const float *cache_k, const float *cache_v,
+                                 long cache_sp, long cache_st, long cache_sh, const int *pages, const long long *lengths,
+                                 const long long *counts, float *y, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,499 @@
+// Attention of a few new tokens over a paged cache (pam_attention.h has the formulas), for single tokens while decoding.
+//
+// Bound by reading the cache once.  A key's row is taken by a group of L lanes, a quad each (4 ... 64 lanes, so that a load is whole rows of a page),
+// and the rows of the queries' heads that share it (ROWS of them) are kept in registers beside it.  A wavefront takes 64 keys at a
+// time: their scores by sums over the groups' lanes, then a lane per key for the weights (over the groups they would cost as much as
+// the products), then the values' rows with the weights from LDS.  Every sequence's keys are cut into as many parts as there are work-groups for it,
+// by its own length; four wavefronts of a work-group take 64 keys in turn, their sums are put together through LDS, and the parts' by a
+// second kernel.  Scaling by powers of two is exact, so that none of this moves a result beyond the order of its sums.
+#include <algorithm>
+
+#include "pam_attention.h"
+
+using namespace pamatt;
+
+namespace {
+
+constexpr int kSteps = 4;                         // keys' rows in flight, of every lane
+constexpr int kMostParts = 128;
+
+struct CacheArgs {
+    Tokens q;
+    const float* k; const float* v; long c_sp, c_st, c_sh;      // pages, places in one, heads
+    const int* table; const long long* lengths; const long long* counts;
+    const float* slopes;
+    float* y;
+    float* partial; float2* partial_stats;        // [batch][kv_heads][rows][parts][quads of values], [...]: l, M; or null: parts is 1
+    int batch, tokens, heads, kv_heads, group, values, rows;
+    int page, pages, per_sequence, window, capacity;      // per_sequence: entries of the table; capacity: the places that they make
+    int lanes, parts, sets;
+    float scale, cap, off;
+};
+
+struct RowPlace { int token, head; };
+__device__ __forceinline__ RowPlace place_of(const CacheArgs& a, int kv, int row) { return RowPlace{row / a.group, kv * a.group + row % a.group}; }
+
+// The sum over a group of lanes, in all of them.
+template <int CTRL> __device__ __forceinline__ float across(float v) { return u2f((uint32_t)__builtin_amdgcn_mov_dpp((int)f2u(v), CTRL, 0xf, 0xf, true)); }
+template <int N> __device__ __forceinline__ void group_sums(float (&v)[N], int lanes)
+{
+    typedef unsigned int u2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += across<0xb1>(v[i]);                       // lane ^ 1
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += across<0x4e>(v[i]);                       // lane ^ 2
+    if (lanes >= 8)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += across<0x141>(v[i]);                  // the other four of eight
+    if (lanes >= 16)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += across<0x140>(v[i]);                  // the other eight of sixteen
+    if (lanes >= 32)
+#pragma unroll
+        for (int i = 0; i < N; ++i) { const u2 r = __builtin_amdgcn_permlane16_swap(f2u(v[i]), f2u(v[i]), false, false); v[i] = u2f(r.x) + u2f(r.y); }
+    if (lanes >= 64)
+#pragma unroll
+        for (int i = 0; i < N; ++i) { const u2 r = __builtin_amdgcn_permlane32_swap(f2u(v[i]), f2u(v[i]), false, false); v[i] = u2f(r.x) + u2f(r.y); }
+}
+
+// LDS accesses of a wavefront's lanes to each other's values stay in order.
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The lane's quads of kSteps keys' rows, ones behind a head's values.
+struct Lane { int first, values; bool streams; uint64_t streaming; };
+__device__ __forceinline__ void load_rows(const float* base, const long (&at)[kSteps], const Lane& here, v4f (&r)[kSteps])
+{
+    if (here.values % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) r[i] = *reinterpret_cast<const v4f_any*>(base + at[i] + here.first);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) r[i][d] = here.streams ? r[i][d] : 1.0f;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const bool there = here.streams && here.first + d < here.values;
+            const float x = base[at[i] + (there ? here.first + d : 0)];
+            r[i][d] = there ? x : 1.0f;
+        }
+}
+__device__ __forceinline__ bool ordinary(const v4f (&r)[kSteps])
+{
+    uint32_t most = 0u;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) most = max(most, (f2u(r[i][d]) << 1) - kStreamBase);
+    return __ballot(most >= kStreamSpan) == 0ull;
+}
+
+template <int ROWS>
+__global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : 4) void cached_attention_kernel(CacheArgs a)
+{
+    __shared__ float scores[kWaves][kSpan][ROWS];                                // of a wavefront's keys, then their weights
+    __shared__ float sums[ROWS][256 + 4];
+    __shared__ float2 stats[kWaves][ROWS];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), L = a.lanes, keys_a_step = 64 / L;
+    // (work-groups go to the eight XCDs in turn: those that read the same keys for other rows are eight apart, on one of them)
+    const int x = (int)blockIdx.x, unit = x / (8 * a.sets) * 8 + x % 8, row0 = x / 8 % a.sets * ROWS;
+    if (unit >= a.batch * a.kv_heads * a.parts) return;
+    const int part = unit % a.parts, head_at = unit / a.parts, b = head_at / a.kv_heads, kv = head_at % a.kv_heads;
+    const int here_rows = min(ROWS, a.rows - row0);
+    const bool has_off = a.off != 1.0f;
+    const uint32_t off_add = f2u(a.off) - kBias, mul_add = f2u(a.off) - 2u * kBias, log2e_add = f2u(kLog2e) - kBias + off_add;
+    Args scoring_args{};
+    scoring_args.cap = a.cap; scoring_args.off = a.off; scoring_args.slopes = a.slopes;
+    const Scoring scoring(scoring_args);
+    const Full full{a.off, has_off, 0u - mul_add, lane_pad(0u)};
+
+    // what the rows see: [low_of(r), position of r]
+    const int length = (int)max(0ll, min(a.lengths[b], 1ll << 30)), given = a.counts ? (int)max(0ll, min(a.counts[b], (long long)a.tokens)) : a.tokens;
+    const int last_token = min((row0 + here_rows - 1) / a.group, given - 1), first_token = row0 / a.group;
+    const bool any = first_token <= last_token;
+    // (no key behind the table's last place is looked for, however long a sequence says it is: a row that would see one is no number)
+    const int end_of_all = any ? min(length + last_token + 1, a.capacity) : 0;
+    const int begin_of_all = any && a.window ? min(max(0, length + first_token - a.window + 1), end_of_all) : 0;
+    // this part of them, whole spans
+    const int spans = (end_of_all + kSpan - 1) / kSpan - begin_of_all / kSpan, each = (spans + a.parts - 1) / a.parts;
+    const int begin = (begin_of_all / kSpan + part * each) * kSpan, end = min(end_of_all, begin + each * kSpan);
+
+    Lane here;
+    here.first = lane % L * 4; here.values = a.values;
+    here.streams = here.first < a.values;
+    if (!here.streams) here.first = 0;
+    here.streaming = __ballot(here.streams);
+    uint32_t q[ROWS][4];
+    float acc[ROWS][4], l[ROWS], M[ROWS];
+    bool odd = false;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const RowPlace at = place_of(a, kv, row0 + min(r, here_rows - 1));
+        const float* const from = a.q.p + (long)b * a.q.sb + (long)at.token * a.q.st + (long)at.head * a.q.sh;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const bool there = here.streams && here.first + d < a.values;
+            const float v = from[there ? here.first + d : 0];
+            const uint32_t scaled = (f2u(v) << 1) == 0u ? kStandIn : f2u(v) + (f2u(a.scale) - kBias + off_add);
+            const bool out = there && (scaled << 1) - kLaneBase >= kLaneSpan;
+            odd = odd || out;
+            q[r][d] = there ? (out ? f2u(pam_mul_off(v, a.scale, a.off, has_off)) : scaled) + mul_add : full.pad;
+            acc[r][d] = 0.0f;
+        }
+        l[r] = 0.0f; M[r] = kNothing;
+    }
+    const bool careful_rows = __ballot(odd) != 0ull;
+    const int* const table = a.table + (long)b * a.per_sequence;
+    const float* const k = a.k + (long)kv * a.c_sh;
+    const float* const v = a.v + (long)kv * a.c_sh;
+    uint32_t saw = 0u;                            // a bit for every row
+
+#pragma unroll 1
+    for (int j0 = begin + wave * kSpan; j0 < end; j0 += kWaves * kSpan) {
+        // a lane per key: where its row lies
+        const int j = j0 + lane;
+        const bool exists = j < end;
+        bool there = exists;
+        long at = 0;
+        if (there) {
+            const int of = table[j / a.page];
+            there = of >= 0 && of < a.pages;
+            at = there ? (long)of * a.c_sp + (long)(j % a.page) * a.c_st : 0;
+        }
+        const auto row_at = [&](int step, long (&out)[kSteps]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int from = (step + i) * keys_a_step + lane / L;
+                out[i] = (long)(((uint64_t)(uint32_t)__shfl((int)(at >> 32), from, 64) << 32) | (uint32_t)__shfl((int)at, from, 64));
+            }
+        };
+        v4f rows[kSteps];
+        long where[kSteps];
+        // scores
+#pragma unroll 1
+        for (int step = 0; step < L; step += kSteps) {
+            row_at(step, where);
+            load_rows(k, where, here, rows);
+            const bool careful = careful_rows || !ordinary(rows);
+#pragma unroll
+            for (int i0 = 0; i0 < kSteps; i0 += (ROWS > 8 ? 1 : 2)) {
+                constexpr int kTwo = ROWS > 8 ? 1 : 2;
+                float s[kTwo * ROWS];
+#pragma unroll
+                for (int i = 0; i < kTwo; ++i)
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) sum += u2f(f2u(rows[i0 + i][d]) + q[r][d]);
+                        s[i * ROWS + r] = sum;
+                    }
+                if (__builtin_expect(careful, 0)) {
+#pragma unroll 1
+                    for (int n = 0; n < kTwo * ROWS; ++n) {
+                        // (the row's and the key's values by selects: the arrays stay in registers)
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            uint32_t mine = q[0][d], theirs = f2u(rows[i0][d]);
+#pragma unroll
+                            for (int r = 1; r < ROWS; ++r) mine = n % ROWS == r ? q[r][d] : mine;
+#pragma unroll
+                            for (int i = 1; i < kTwo; ++i) theirs = n / ROWS == i ? f2u(rows[i0 + i][d]) : theirs;
+                            mine = (uint32_t)anew((int)mine);
+                            sum += full_product(full, mine == full.pad ? 0u : mine + full.raw, theirs);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        s[0] = sum;
+                        turned(s);
+                    }
+                }
+                group_sums(s, L);
+                if (lane % L == 0)
+#pragma unroll
+                    for (int i = 0; i < kTwo; ++i)
+#pragma unroll
+                        for (int r = 0; r < ROWS; ++r) scores[wave][(step + i0 + i) * keys_a_step + lane / L][r] = s[i * ROWS + r];
+            }
+        }
+        wave_fence();
+        // weights: a lane per key
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const int token = (row0 + min(r, here_rows - 1)) / a.group;
+            const int pos = length + token;
+            const bool sees = exists && token < given && j <= pos && (a.window == 0 || j > pos - a.window);
+            const float slope = a.slopes ? a.slopes[place_of(a, kv, row0 + min(r, here_rows - 1)).head] : 0.0f;
+            float t = scoring.exponent(scores[wave][lane][r], held_slope(slope), pos - j);
+            t = there && finite(slope) ? t : u2f(kQNaN);
+            float most = sees ? t : kNothing;
+            most = most != most ? kNothing : most;
+#pragma unroll
+            for (int s = 1; s < 64; s *= 2) most = fmaxf(most, __shfl_xor(most, s, 64));
+            if (most > M[r] + kLag) {              // (the same in all lanes)
+                const float raised = u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(floorf(most)))), f = scale_between(M[r], raised);
+                l[r] *= f;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) acc[r][d] *= f;
+                M[r] = raised;
+            }
+            const float power = sees ? t - M[r] : 2.0f * kLeast;
+            saw |= sees ? 1u << r : 0u;
+            const bool in = power >= kLeast;
+            const float e = power_of_two(fmaxf(power, kLeast));
+            l[r] += in ? e : power * 0.0f;        // (what is no number makes none of the sum)
+            scores[wave][lane][r] = in ? e : 0.0f;
+            __builtin_amdgcn_sched_barrier(0);    // (row by row: all of them side by side take the registers of the loops around)
+        }
+        wave_fence();
+        // values
+#pragma unroll 1
+        for (int step = 0; step < L; step += kSteps) {
+            row_at(step, where);
+            load_rows(v, where, here, rows);
+            const bool careful = !ordinary(rows);
+            if (__builtin_expect(careful, 0)) {
+#pragma unroll 1
+                for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+                        const float e = scores[wave][(step + i) * keys_a_step + lane / L][r];
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            const float c = full_product(full, f2u(e), f2u(rows[0][d]));
+                            acc[r][d] += e > 0.0f ? c : 0.0f;
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                    turned(rows);
+                }
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    const float e = scores[wave][(step + i) * keys_a_step + lane / L][r];
+                    const uint32_t weight = e > 0.0f ? f2u(e) + mul_add : 0u;
+                    const float one = e > 0.0f ? 1.0f : 0.0f;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) acc[r][d] = __builtin_fmaf(u2f(f2u(rows[i][d]) + weight), one, acc[r][d]);
+                }
+        }
+        wave_fence();                             // (the next span's scores go where these weights are)
+    }
+
+    // the groups of lanes, then the wavefronts one after the other, scaled to the largest M
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        for (int s = L; s < 64; s *= 2)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[r][d] += __shfl_xor(acc[r][d], s, 64);
+        for (int s = 1; s < 64; s *= 2) l[r] += __shfl_xor(l[r], s, 64);
+        const int token = (row0 + min(r, here_rows - 1)) / a.group;
+        const bool beyond = token < given && length + token >= a.capacity, some = beyond || __ballot((saw >> r) & 1u) != 0ull;
+        l[r] = beyond ? u2f(kQNaN) : l[r];
+        if (some && M[r] == kNothing) M[r] = 0.0f;                               // (seen, and no number)
+        if (lane == 0) stats[wave][r] = make_float2(some ? l[r] : 0.0f, some ? M[r] : kNothing);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) {
+        if (w == wave && lane < L)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                float most = kNothing;
+#pragma unroll
+                for (int o = 0; o < kWaves; ++o) most = fmaxf(most, stats[o][r].y);
+                const bool mine = stats[w][r].y != kNothing;
+                const float f = mine ? scale_between(stats[w][r].y, most) : 0.0f;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const float x = mine ? acc[r][d] * f : 0.0f;
+                    sums[r][lane * 4 + d] = w == 0 ? x : sums[r][lane * 4 + d] + x;
+                }
+            }
+        __syncthreads();
+    }
+    const int quads = (a.values + 3) / 4;
+    for (int i = threadIdx.x; i < here_rows * quads; i += kThreads) {
+        const int r = i / quads, d = i % quads * 4;
+        float most = kNothing, total = 0.0f;
+        const v4f sum = {sums[r][d], sums[r][d + 1], sums[r][d + 2], sums[r][d + 3]};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, stats[w][r].y);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float2 s = stats[w][r];
+            total += s.y == kNothing ? 0.0f : s.x * scale_between(s.y, most);
+        }
+        const RowPlace at = place_of(a, kv, row0 + r);
+        if (a.partial) {
+            const long to = ((long)head_at * a.rows + row0 + r) * a.parts + part;
+            *reinterpret_cast<v4f*>(a.partial + to * quads * 4 + d) = sum;
+            if (d == 0) a.partial_stats[to] = make_float2(total, most);
+        } else {
+            float* const to = a.y + (((long)b * a.tokens + at.token) * a.heads + at.head) * a.values + d;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (d + c < a.values) to[c] = most == kNothing ? 0.0f : pad_div_off(sum[c], total, a.off, has_off);
+        }
+    }
+}
+
+// The parts of a query's head, one work-group each: lanes along its quads, the rest of the threads along the parts.
+__global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs a)
+{
+    __shared__ v4f sums[kThreads];
+    __shared__ float totals[kMostParts], scales[kMostParts];
+    __shared__ float top;
+    const int quads = (a.values + 3) / 4, row = (int)blockIdx.x % a.rows, head_at = (int)blockIdx.x / a.rows, b = head_at / a.kv_heads, kv = head_at % a.kv_heads;
+    const long from = ((long)head_at * a.rows + row) * a.parts;
+    float2 mine = make_float2(0.0f, kNothing);
+    if ((int)threadIdx.x < a.parts) mine = a.partial_stats[from + threadIdx.x];
+    if (threadIdx.x < 64) {
+        float2 second = make_float2(0.0f, kNothing);
+        if ((int)threadIdx.x + 64 < a.parts) second = a.partial_stats[from + threadIdx.x + 64];
+        float most = fmaxf(mine.y, second.y);
+        for (int s = 1; s < 64; s *= 2) most = fmaxf(most, __shfl_xor(most, s, 64));
+        if (threadIdx.x == 0) top = most;
+    }
+    __syncthreads();
+    const float M = top;
+    if ((int)threadIdx.x < a.parts) {
+        scales[threadIdx.x] = mine.y == kNothing ? 0.0f : scale_between(mine.y, M);
+        totals[threadIdx.x] = mine.y == kNothing ? 0.0f : mine.x * scales[threadIdx.x];
+    }
+    __syncthreads();
+    int columns = 1;                              // lanes along the quads: a power of two
+    while (columns < quads) columns *= 2;
+    const int column = threadIdx.x % columns, shares = kThreads / columns, share = threadIdx.x / columns;
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (column < quads)
+#pragma unroll 4
+        for (int p = share; p < a.parts; p += shares) {
+            const v4f x = *reinterpret_cast<const v4f*>(a.partial + (from + p) * quads * 4 + column * 4);
+            const float f = scales[p];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] += f != 0.0f ? x[c] * f : 0.0f;
+        }
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (share != 0 || column >= quads) return;
+    float total = 0.0f;
+    for (int p = 0; p < a.parts; ++p) total += totals[p];
+    for (int s = 1; s < shares; ++s)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] += sums[s * columns + column][c];
+    const RowPlace at = place_of(a, kv, row);
+    float* const to = a.y + (((long)b * a.tokens + at.token) * a.heads + at.head) * a.values + column * 4;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (column * 4 + c < a.values) to[c] = M == kNothing ? 0.0f : pad_div_off(sum[c], total, a.off, a.off != 1.0f);
+}
+
+// ---------------------------------------------------------------- host
+
+// Rows of a work-group, how many work-groups the rows of a key head take, lanes of a group, parts of a sequence.
+struct CachePlan { int rows_each, sets, lanes, parts; };
+CachePlan cache_plan(long heads, long rows, long values, long capacity)
+{
+    CachePlan p;
+    p.rows_each = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    p.sets = (int)((rows + p.rows_each - 1) / p.rows_each);
+    p.lanes = 4;
+    while (p.lanes * 4 < values) p.lanes *= 2;
+    // (three work-groups for each of 256 compute units; a part of less than a span for each wavefront is not worth a second kernel)
+    const long units = std::max(1L, heads * p.sets), wanted = (768 + units - 1) / units, most = (capacity + kWaves * kSpan - 1) / (kWaves * kSpan);
+    p.parts = (int)std::max(1L, std::min({wanted, most, (long)kMostParts}));
+    return p;
+}
+long padded(long values) { return (values + 3) / 4 * 4; }
+size_t cache_bytes(const CachePlan& p, long heads, long rows, long values)
+{
+    if (p.parts == 1) return 0;
+    const size_t n = (size_t)heads * rows * p.parts;
+    return (n * sizeof(float2) + 255) / 256 * 256 + n * padded(values) * sizeof(float);
+}
+
+int check_cache(const char* what, const pam_hip_cache_shape* s)
+{
+    if (!s) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
+    if (s->batch < 0 || s->tokens < 0 || s->heads < 0 || s->kv_heads < 0 || s->pages < 0 || s->per_sequence < 0 || s->window < 0)
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: negative size", what);
+    if (s->dim < 1 || s->dim > 256) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: heads have up to 256 values, got %ld", what, s->dim);
+    if (s->kv_heads == 0 ? s->heads != 0 : s->heads % s->kv_heads != 0)
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: %ld heads do not share %ld", what, s->heads, s->kv_heads);
+    if (s->page < 1 || s->page > (1L << 20) || s->pages > (1L << 30) || s->per_sequence > (1L << 30) || s->batch > (1L << 20) || s->heads > (1L << 16)
+        || s->tokens > (1L << 20) || s->batch * s->heads > (1L << 20) || s->batch * s->heads * s->tokens > (1L << 23))
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: size out of range", what);
+    if (s->per_sequence * s->page > (1L << 30)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the table of pages has up to 2^30 places", what);
+    if (!(s->scale > 0x1p-40f && s->scale < 0x1p40f)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the scale lies between 2^-40 and 2^40", what);
+    if (s->cap != 0.0f && !(s->cap > 0x1p-20f && s->cap < 0x1p20f)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the cap lies between 2^-20 and 2^20", what);
+    if (!(s->offset > 0.75f && s->offset < 1.5f)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: the offset lies between 0.75 and 1.5", what);
+    return PAM_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pam_hip_cached_attention_workspace_bytes(const pam_hip_cache_shape* s)
+{
+    if (check_cache("cached_attention", s) != PAM_HIP_OK || s->batch * s->heads * s->tokens == 0) return 0;
+    const long heads = s->batch * s->kv_heads, rows = s->heads / s->kv_heads * s->tokens;
+    return cache_bytes(cache_plan(heads, rows, s->dim, s->per_sequence * s->page), heads, rows, s->dim);
+}
+
+int pam_hip_cached_attention_fwd(const pam_hip_cache_shape* s, const pam_hip_tokens* q, const float* cache_k, const float* cache_v, long cache_sp, long cache_st,
+                                 long cache_sh, const int* pages, const long long* lengths, const long long* counts, float* y, void* workspace, size_t workspace_bytes,
+                                 void* stream)
+{
+    const int rc = check_cache("cached_attention", s);
+    if (rc != PAM_HIP_OK || s->batch * s->heads * s->tokens == 0) return rc;
+    // (without pages every key is one that is not there; it is not read, but an address is computed)
+    if (!q || !q->p || !y || !lengths || (s->per_sequence && !pages) || (s->pages && (!cache_k || !cache_v)))
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "cached_attention: null pointer");
+    CacheArgs a{};
+    a.q = Tokens{q->p, q->sb, q->st, q->sh};
+    a.k = s->pages ? cache_k : q->p; a.v = s->pages ? cache_v : q->p;
+    a.c_sp = cache_sp; a.c_st = cache_st; a.c_sh = s->pages ? cache_sh : 0;
+    a.table = pages; a.lengths = lengths; a.counts = counts; a.slopes = s->slopes; a.y = y;
+    a.batch = (int)s->batch; a.tokens = (int)s->tokens; a.heads = (int)s->heads; a.kv_heads = (int)s->kv_heads; a.group = (int)(s->heads / s->kv_heads);
+    a.values = (int)s->dim; a.rows = a.group * a.tokens;
+    a.page = (int)s->page; a.pages = (int)s->pages; a.per_sequence = (int)s->per_sequence; a.capacity = (int)(s->per_sequence * s->page); a.window = (int)std::min(s->window, 1L << 30);
+    a.scale = s->scale; a.cap = s->cap; a.off = s->offset;
+    const long heads = s->batch * s->kv_heads;
+    const CachePlan p = cache_plan(heads, a.rows, a.values, s->per_sequence * s->page);
+    a.lanes = p.lanes; a.parts = p.parts; a.sets = p.sets;
+    const size_t need = cache_bytes(p, heads, a.rows, a.values);
+    if (need && (!workspace || workspace_bytes < need)) return pamhost::fail(PAM_HIP_ERR_WORKSPACE, "cached_attention: workspace of %zu bytes needed", need);
+    if (need) {
+        a.partial_stats = (float2*)workspace;
+        a.partial = (float*)((char*)workspace + ((size_t)heads * a.rows * p.parts * sizeof(float2) + 255) / 256 * 256);
+    }
+    const hipStream_t st = (hipStream_t)stream;
+    const long units = heads * p.parts, groups = (units + 7) / 8 * 8 * p.sets;
+    if (groups > (1L << 23)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "cached_attention: size out of range");
+    const dim3 grid((unsigned)groups);
+    switch (p.rows_each) {
+    case 1: hipLaunchKernelGGL((cached_attention_kernel<1>), grid, dim3(kThreads), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((cached_attention_kernel<2>), grid, dim3(kThreads), 0, st, a); break;
+    case 4: hipLaunchKernelGGL((cached_attention_kernel<4>), grid, dim3(kThreads), 0, st, a); break;
+    case 8: hipLaunchKernelGGL((cached_attention_kernel<8>), grid, dim3(kThreads), 0, st, a); break;
+    default: hipLaunchKernelGGL((cached_attention_kernel<16>), grid, dim3(kThreads), 0, st, a); break;
+    }
+    int done = pamhost::check_launch("cached_attention");
+    if (done != PAM_HIP_OK || !need) return done;
+    hipLaunchKernelGGL(cached_join_kernel, dim3((unsigned)(heads * a.rows)), dim3(kThreads), 0, st, a);
+    return pamhost::check_launch("cached_attention");
+}
+
+}  // extern "C"

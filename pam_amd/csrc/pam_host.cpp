@@ -580,6 +580,8 @@ PYBIND11_MODULE(_pam_host, module)
     module.def("layer", &call_layer, unlocked);
     module.def("rotary", &call_rotary, unlocked);
     module.def("attention", &call_attention, unlocked);
+    module.def("rotary_append", &call_rotary_append, unlocked);
+    module.def("cached_attention", &call_cached_attention, unlocked);
     module.def("clip", &clip);
     module.def("adam_collect", &adam_collect);
 }

@@ -130,3 +130,95 @@ Tensor call_attention(const Tensor& q, const Tensor& k, const Tensor& v, double 
     const AttentionCall c = attention_call(q, k, v, scale, causal, window, prefix.value_or(none), documents.value_or(none), slopes.value_or(none), cap, offset);
     return without_pad(attend(c, q, k, v, false).y, c.shape.values);
 }
+
+// ---------------------------------------------------------------- a paged cache
+
+// What keys and values of a cache look like, and the table that says where a sequence's are.
+struct Cache { Tensor pages, lengths, counts; int64_t per_sequence; };
+Cache checked_cache(const char* name, const Tensor& k, const Tensor& v, const Tensor& pages, const Tensor& lengths, const Tensor& counts, const Tensor& q, int64_t batch, int64_t dim)
+{
+    check_tensor(k); check_tensor(v);
+    TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && v.strides() == k.strides() && k.device() == q.device() && v.device() == q.device() && k.size(1) >= 1,
+                      name, ": a cache's keys and values are two tensors [pages, page, kv heads, dim] of the same strides on the tensors' device, got ", shape(k), " and ", shape(v));
+    TORCH_CHECK_VALUE(k.size(3) == dim && (dim <= 1 || k.stride(3) == 1), name, ": a head's values lie side by side in the cache, as many as a query has");
+    TORCH_CHECK_TYPE(pages.scalar_type() == at::kInt, name, ": the table of pages is int32");
+    TORCH_CHECK_VALUE(pages.dim() == 2 && pages.size(0) == batch && pages.device() == q.device(), name, ": the table of pages is [batch, pages of a sequence] on the tensors' device, got ", shape(pages));
+    Cache c;
+    c.pages = pages.contiguous(); c.per_sequence = pages.size(1);
+    c.lengths = checked_integers(name, "lengths", lengths, q, {batch});
+    if (counts.defined()) c.counts = checked_integers(name, "counts", counts, q, {batch});
+    return c;
+}
+const long long* integers(const Tensor& t) { return t.defined() ? reinterpret_cast<const long long*>(t.data_ptr<int64_t>()) : nullptr; }
+
+// Whether two tensors have a value in common.  (Mostly their memory is apart as a whole.)
+bool in_common(const Tensor& a, const Tensor& b)
+{
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const uintptr_t a0 = (uintptr_t)data(a), b0 = (uintptr_t)data(b);
+    return a0 < b0 + (uintptr_t)(span(b) + 1) * sizeof(float) && b0 < a0 + (uintptr_t)(span(a) + 1) * sizeof(float) && share_values(a, b);
+}
+
+Tensor call_rotary_append(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& cos, const Tensor& sin, const Tensor& cache_k, const Tensor& cache_v,
+                          const Tensor& pages, const Tensor& lengths, const std::optional<Tensor>& counts, const std::optional<Tensor>& q_weight,
+                          const std::optional<Tensor>& k_weight, bool interleaved, double eps, double offset)
+{
+    const char* const name = "rotary_append";
+    const Tensor none;
+    TORCH_CHECK(!wants_graph(name, {&q_in, &k_in, &v_in, &cos, &sin, &cache_k, &cache_v, q_weight ? &*q_weight : &none, k_weight ? &*k_weight : &none}),
+                "rotary_append: what goes into a cache has no gradient, and a tensor requires one; call it under torch.no_grad()");
+    variable_list x{q_in, k_in}, w{q_weight.value_or(none), k_weight.value_or(none)};
+    check_tensor(v_in);
+    const Rotation r = rotation(x, w, cos, sin, none, interleaved, eps, offset, /*by_row=*/false);
+    TORCH_CHECK_VALUE(v_in.sizes() == k_in.sizes() && v_in.device() == k_in.device(), name, ": keys and values have one shape, got ", shape(k_in), " and ", shape(v_in));
+    const Cache c = checked_cache(name, cache_k, cache_v, pages, lengths, counts.value_or(none), q_in, r.batch, r.dim);
+    TORCH_CHECK_VALUE(cache_k.size(2) == k_in.size(2), name, ": ", k_in.size(2), " keys' heads and a cache of ", cache_k.size(2));
+    bool shared = folds_on_itself(cache_k) || in_common(cache_k, cache_v);
+    for (const Tensor* t : {&q_in, &k_in, &v_in, &cos, &sin})
+        for (const Tensor* cache : {&cache_k, &cache_v}) shared = shared || in_common(*cache, *t);
+    for (const Tensor& t : w)
+        if (t.defined()) shared = shared || in_common(cache_k, t) || in_common(cache_v, t);
+    TORCH_CHECK_VALUE(!shared, name, ": the cache shares memory within itself or with what is read");
+    const OnDevice on(q_in);
+    for (size_t i = 0; i < 2; ++i) {
+        x[i] = heads_contiguous(x[i]);
+        if (w[i].defined()) w[i] = w[i].contiguous();
+    }
+    const Tensor v = heads_contiguous(v_in), y = new_floats(x[0].sizes(), x[0]);
+    // (written through their pointers: a graph that has saved one of them must not be run on the new values)
+    for (const Tensor* t : {&cache_k, &cache_v})
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    const pam_hip_heads of_q = heads_of(x[0], w[0], y), of_k = heads_of(x[1], w[1], cache_k), of_v = heads_of(v, none, cache_v);
+    check_call(pam_hip_rotary_append(&of_q, &of_k, &of_v, data(r.cos), data(r.sin), r.cos.size(0), data(cache_k), data(cache_v), cache_k.stride(0), cache_k.stride(1), cache_k.stride(2),
+                                     cache_k.size(1), cache_k.size(0), c.per_sequence, c.pages.data_ptr<int>(), integers(c.lengths), integers(c.counts), r.batch, r.tokens, r.dim,
+                                     r.rotated, r.interleaved, r.eps, r.offset, on.stream), name);
+    return y;
+}
+
+Tensor call_cached_attention(const Tensor& q_in, const Tensor& cache_k, const Tensor& cache_v, const Tensor& pages, const Tensor& lengths, const std::optional<Tensor>& counts,
+                             double scale, int64_t window, const std::optional<Tensor>& slopes, double cap, double offset)
+{
+    const char* const name = "cached_attention";
+    const Tensor none;
+    TORCH_CHECK(!wants_graph(name, {&q_in, &cache_k, &cache_v, slopes ? &*slopes : &none}),
+                "cached_attention: a cache's attention has no gradient, and a tensor requires one; call it under torch.no_grad()");
+    check_tensor(q_in);
+    TORCH_CHECK_VALUE(q_in.dim() == 4 && q_in.size(3) >= 1 && q_in.size(3) <= 256, name, ": queries are [batch, tokens, heads, dim], heads of up to 256 values, got ", shape(q_in));
+    const Cache c = checked_cache(name, cache_k, cache_v, pages, lengths, counts.value_or(none), q_in, q_in.size(0), q_in.size(3));
+    const int64_t kv_heads = cache_k.size(2);
+    TORCH_CHECK_VALUE(kv_heads == 0 ? q_in.size(2) == 0 : q_in.size(2) % kv_heads == 0, name, ": ", q_in.size(2), " heads do not share ", kv_heads);
+    TORCH_CHECK_VALUE(window >= 0, name, ": the window has at least one key");
+    const Tensor slope = slopes ? checked_slopes(name, *slopes, q_in, q_in.size(2)) : Tensor();
+    const OnDevice on(q_in);
+    const Tensor q = heads_contiguous(q_in), y = new_floats(q.sizes(), q);
+    pam_hip_cache_shape s{};
+    s.batch = q.size(0); s.tokens = q.size(1); s.heads = q.size(2); s.kv_heads = kv_heads; s.dim = q.size(3);
+    s.page = cache_k.size(1); s.pages = cache_k.size(0); s.per_sequence = c.per_sequence;
+    s.scale = (float)scale; s.cap = (float)cap; s.offset = (float)offset; s.window = window; s.slopes = data_or_null(slope);
+    const size_t bytes = pam_hip_cached_attention_workspace_bytes(&s);
+    const Tensor ws = scratch_bytes(bytes, q);
+    const pam_hip_tokens at = tokens_of(q);
+    check_call(pam_hip_cached_attention_fwd(&s, &at, data(cache_k), data(cache_v), cache_k.stride(0), cache_k.stride(1), cache_k.stride(2), c.pages.data_ptr<int>(),
+                                            integers(c.lengths), integers(c.counts), data(y), data_or_null(ws), bytes, on.stream), name);
+    return y;
+}

@@ -176,9 +176,10 @@ pam_hip_heads heads_of(const Tensor& x, const Tensor& weight, const Tensor& y)
     return h;
 }
 
-Rotation rotation(const variable_list& x, const variable_list& weights, const Tensor& cos, const Tensor& sin, const Tensor& positions, bool interleaved, double eps, double offset)
+Rotation rotation(const variable_list& x, const variable_list& weights, const Tensor& cos, const Tensor& sin, const Tensor& positions, bool interleaved, double eps, double offset,
+                  bool by_row = true)
 {
-    const char* const name = "rotary";
+    const char* const name = by_row ? "rotary" : "rotary_append";          // by_row: without positions token t is at the tables' row t
     Rotation r;
     r.batch = x[0].dim() == 4 ? x[0].size(0) : 0; r.tokens = x[0].dim() == 4 ? x[0].size(1) : 0; r.dim = x[0].dim() == 4 ? x[0].size(3) : 0;
     for (size_t i = 0; i < x.size(); ++i) {
@@ -193,7 +194,7 @@ Rotation rotation(const variable_list& x, const variable_list& weights, const Te
     TORCH_CHECK_VALUE(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.device() == x[0].device() && sin.device() == x[0].device(),
                       name, ": cos and sin are two tables of one shape on the tensors' device");
     TORCH_CHECK_VALUE(2 * cos.size(1) <= r.dim, name, ": the tables rotate ", 2 * cos.size(1), " values of a head that has ", r.dim);
-    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), "rotary: the tables have no gradient");
+    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), name, ": the tables have no gradient");
     r.cos = cos.contiguous(); r.sin = sin.contiguous();
     r.rotated = 2 * cos.size(1);
     if (positions.defined()) {
@@ -202,7 +203,7 @@ Rotation rotation(const variable_list& x, const variable_list& weights, const Te
                               && (positions.dim() == 1 || positions.size(0) == r.batch),
                           name, ": positions are [tokens] or [batch, tokens] on the tensors' device, got ", shape(positions));
         r.positions = positions;
-    } else {
+    } else if (by_row) {
         TORCH_CHECK_VALUE(r.tokens <= cos.size(0), name, ": ", r.tokens, " tokens and tables of ", cos.size(0), " positions");
     }
     r.interleaved = interleaved; r.eps = (float)eps; r.offset = (float)offset;

@@ -13,6 +13,7 @@
 // Heads that do not come in fours, or of more than 64 units, take a wavefront each by the checked functions.
 #include <algorithm>
 
+#include "../../include/pam_hip_attention.h"
 #include "../../include/pam_hip_extra.h"
 #include "pam_activation.h"
 #include "pam_common.h"
@@ -546,6 +547,87 @@ __global__ __launch_bounds__(kThreads) void any_rotary_kernel(RotaryArgs a)
     else forward_by_value<false>(a, p.weight, h, lane, 64, true);
 }
 
+// ---------------------------------------------------------------- into a paged cache
+
+// Queries (part 0) and keys (part 1) as above, at the positions behind their sequence's tokens; keys and values (part 2, copied) go to their places in
+// a cache's pages.  A token that its sequence does not have leaves zeros for its queries and writes nothing to the cache; neither does one whose place or
+// page is not there.
+struct AppendArgs {
+    RotaryArgs rotary;                            // its parts: queries, keys
+    PartArgs values;
+    float* cache_k; float* cache_v; long c_sp, c_st, c_sh;
+    const int* table; const long long* lengths; const long long* counts;
+    long page, pages, per_sequence;
+};
+struct AppendHead { Head head; bool there; };      // there: the sequence has the token; head.y null: nowhere to put it
+__device__ __forceinline__ AppendHead find_place(const AppendArgs& g, const PartArgs& p, int part, uint32_t row)
+{
+    const RotaryArgs& a = g.rotary;
+    const uint32_t token = row / p.heads, at = row - token * p.heads, b = token / a.tokens, t = token - b * a.tokens;
+    const long long length = min(g.lengths[b], 1ll << 60), pos = length + t;
+    AppendHead h;
+    h.there = !g.counts || (long long)t < g.counts[b];
+    h.head.x = p.x + (long)b * p.x_sb + (long)t * p.x_st + (long)at * p.x_sh;
+    h.head.dy = nullptr;
+    h.head.y = nullptr;
+    if (part == 0) h.head.y = p.y + (long)row * a.dim;
+    else if (length >= 0 && pos / g.page < g.per_sequence) {
+        const long long of = g.table[(long)b * g.per_sequence + pos / g.page];
+        if (of >= 0 && of < g.pages) h.head.y = (part == 1 ? g.cache_k : g.cache_v) + of * g.c_sp + pos % g.page * g.c_st + (long)at * g.c_sh;
+    }
+    const bool in_table = length >= 0 && pos < a.table_rows;
+    h.head.cos = in_table ? a.cos + pos * a.half : nullptr;
+    h.head.sin = in_table ? a.sin + pos * a.half : nullptr;
+    return h;
+}
+struct AppendPart { int part, block; };
+__device__ __forceinline__ AppendPart part_of(const AppendArgs& g)
+{
+    const int block = g.rotary.first_group + (int)blockIdx.x, second = g.rotary.part[0].groups, third = second + g.rotary.part[1].groups;
+    return block >= third ? AppendPart{2, block - third} : block >= second ? AppendPart{1, block - second} : AppendPart{0, block};
+}
+
+template <bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g)
+{
+    const RotaryArgs& a = g.rotary;
+    const AppendPart here = part_of(g);
+    const PartArgs& p = here.part == 2 ? g.values : here.part == 1 ? a.part[1] : a.part[0];
+    const int lanes = a.lanes;
+    const Unit at(a, threadIdx.x & (lanes - 1));
+    const uint32_t mine = (uint32_t)here.block * (kThreads / lanes) + threadIdx.x / lanes;
+    const AppendHead h = find_place(g, p, here.part, min(mine, p.rows - 1));
+    const bool store = mine < p.rows && h.there && h.head.y;
+    v4f x[2], c, s, y[2];
+    load_unit(h.head.x, at, x);
+    if (here.part == 2) {
+        if (store) store_unit(h.head.y, at, x);
+        return;
+    }
+    const Weight w = load_weight(p.weight, at);
+    load_table(h.head, at, a.half > 0, c, s);
+    if (!forward_head<INTERLEAVED>(a, at, x, w, c, s, y)) forward_by_value<true>(a, p.weight, h.head, threadIdx.x & (lanes - 1), lanes, store);
+    else if (store) store_unit(h.head.y, at, y);
+    if (here.part == 0 && mine < p.rows && !h.there) {
+        y[0] = y[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        store_unit(h.head.y, at, y);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void any_append_kernel(AppendArgs g)
+{
+    const RotaryArgs& a = g.rotary;
+    const AppendPart here = part_of(g);
+    const PartArgs& p = here.part == 2 ? g.values : here.part == 1 ? a.part[1] : a.part[0];
+    const uint32_t row = (uint32_t)here.block * kWaves + threadIdx.x / 64;
+    const int lane = threadIdx.x % 64;
+    if (row >= p.rows) return;
+    const AppendHead h = find_place(g, p, here.part, row);
+    if (h.there && h.head.y && here.part != 2) forward_by_value<false>(a, p.weight, h.head, lane, 64, true);
+    else if (h.head.y && (h.there || here.part == 0))
+        for (int i = lane; i < a.dim; i += 64) h.head.y[i] = h.there ? h.head.x[i] : 0.0f;
+}
+
 // ---------------------------------------------------------------- host
 
 // Lanes of a group: the power of two that holds a head's units; 0: the head takes the kernels for any size.
@@ -632,6 +714,42 @@ int pam_hip_rotary_fwd(const pam_hip_heads* parts, int count, const float* cos, 
     if (rc != PAM_HIP_OK || dim == 0) return rc;
     whole_groups(a, a.lanes ? kThreads / a.lanes : kWaves);
     return launch("rotary_fwd", a, !a.lanes ? any_rotary_kernel<false> : interleaved ? rotary_kernel<true> : rotary_kernel<false>, stream);
+}
+
+int pam_hip_rotary_append(const pam_hip_heads* q, const pam_hip_heads* k, const pam_hip_heads* v, const float* cos, const float* sin, long table_rows,
+                          float* cache_k, float* cache_v, long cache_sp, long cache_st, long cache_sh, long page, long pages, long per_sequence, const int* table,
+                          const long long* lengths, const long long* counts, long batch, long tokens, long dim, long rotated, int interleaved, float eps,
+                          float offset, void* stream)
+{
+    const char* const what = "rotary_append";
+    if (!k || !v || k->heads != v->heads) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: keys and values have as many heads", what);
+    if (page < 1 || page > (1L << 20) || pages < 0 || per_sequence < 0 || pages > (1L << 30) || per_sequence > (1L << 30))
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: size out of range", what);
+    // (keys and values go where the table says: fill() looks at their other pointers)
+    pam_hip_heads parts[2] = {q ? *q : pam_hip_heads{}, *k};
+    parts[1].y = cache_k ? cache_k : const_cast<float*>(k->x);
+    AppendArgs g{};
+    int rc = fill(what, g.rotary, parts, 2, cos, sin, table_rows, nullptr, 0, 0, batch, tokens, dim, rotated, interleaved, eps, offset, false);
+    if (rc != PAM_HIP_OK || dim == 0 || batch == 0 || tokens == 0) return rc;
+    const long heads = batch * tokens * k->heads;
+    if (!lengths || (per_sequence && !table) || (heads && (!v->x || (pages && (!cache_k || !cache_v)))))
+        return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: null pointer", what);
+    g.values = PartArgs{v->x, v->x_sb, v->x_st, v->x_sh, nullptr, 0, 0, 0, nullptr, nullptr, nullptr, (uint32_t)heads, (uint32_t)k->heads, 0};
+    g.cache_k = cache_k; g.cache_v = cache_v; g.c_sp = cache_sp; g.c_st = cache_st; g.c_sh = cache_sh;
+    g.table = table; g.lengths = lengths; g.counts = counts; g.page = page; g.pages = pages; g.per_sequence = per_sequence;
+    const int per_group = g.rotary.lanes ? kThreads / g.rotary.lanes : kWaves;
+    whole_groups(g.rotary, per_group);
+    g.values.groups = g.rotary.part[1].groups;
+    // (a launch counts its work-items in 32 bits)
+    constexpr long kMost = 1L << 23;
+    const long groups = (long)g.rotary.part[0].groups + 2L * g.values.groups;
+    for (long first = 0; first < groups; first += kMost) {
+        g.rotary.first_group = (int)first;
+        hipLaunchKernelGGL((!g.rotary.lanes ? any_append_kernel : interleaved ? append_kernel<true> : append_kernel<false>), dim3((unsigned)std::min(kMost, groups - first)),
+                           dim3(kThreads), 0, (hipStream_t)stream, g);
+        if ((rc = pamhost::check_launch(what)) != PAM_HIP_OK) return rc;
+    }
+    return PAM_HIP_OK;
 }
 
 size_t pam_hip_rotary_bwd_workspace_bytes(const pam_hip_heads* parts, int count, long batch, long tokens, long dim, long rotated)
