@@ -45,10 +45,12 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(Args a)
     if (a.stats && d == 0) a.stats[to] = make_float2(l, M);
 }
 
-// A query's head: qs, dn and its record (see pam_attention_bwd.h).  Sixteen lanes have one.
-struct RowArgs { Args a; const float* y; Tokens dy; const float2* stats; float4* records; float* qs; float* dn; };
+// A query's head: qs, dn and its record (see pam_attention_bwd.h).  Sixteen lanes have one.  dl's terms are added up in the order in which the passes
+// add up dn (*) v, each slice's of `width` values from the first to the last, so that the two cancel to nothing where a row sees a single key.
+struct RowArgs { Args a; const float* y; Tokens dy; const float2* stats; float4* records; float* qs; float* dn; int slices, width; };
 __global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
 {
+    __shared__ float terms[kThreads / 16][256 + 1];
     const Args& a = r.a;
     const long all = (long)a.batch * a.tokens * a.heads, mine = (long)blockIdx.x * (kThreads / 16) + threadIdx.x / 16, id = min(mine, all - 1);
     const int lane = threadIdx.x % 16;
@@ -75,14 +77,18 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
         r.qs[to * a.dim + d] = there ? pam_mul_off(q[d], a.scale, off, has_off) : 1.0f;
         r.dn[to * a.dim + d] = there ? dn : 1.0f;
         if (!there) continue;
-        dl += a.flags.b ? -pam_mul_off(pad_div_off(out, l, off, has_off), g, off, has_off) : -(u2f(f2u(out) & ~kMant) / u2f(f2u(l) & kExpo)) * g;
+        terms[threadIdx.x / 16][d] = a.flags.b ? -pam_mul_off(pad_div_off(out, l, off, has_off), g, off, has_off) : -(u2f(f2u(out) & ~kMant) / u2f(f2u(l) & kExpo)) * g;
         most = max(most, f2u(dn) & ~kSign);
     }
     // (all sixteen lanes are there: a work-group past the end repeats the last row)
-    for (int s = 8; s >= 1; s /= 2) {
-        dl += __shfl_xor(dl, s, 16);
-        most = max(most, (uint32_t)__shfl_xor((int)most, s, 16));
+    for (int s = 8; s >= 1; s /= 2) most = max(most, (uint32_t)__shfl_xor((int)most, s, 16));
+    __syncthreads();
+    if (lane < r.slices) {
+        const int end = min(a.values, (lane + 1) * r.width);
+#pragma unroll 8
+        for (int d = lane * r.width; d < end; ++d) dl += terms[threadIdx.x / 16][d];
     }
+    for (int s = 1; s < 4; s *= 2) dl += __shfl_xor(dl, s, 16);
     if (lane != 0 || mine >= all) return;
     // a query without a gradient counts as one that sees nothing: it has none to give
     const bool none = !sees || (most == 0u && dl == 0.0f);
@@ -268,7 +274,8 @@ int pam_hip_attention_bwd(const pam_hip_attention_shape* shape, const pam_hip_to
     if ((rc = groups_for("attention_bwd", heads_of(a) * a.rows * 16, groups)) || (rc = groups_for("attention_bwd", heads_of(a) * a.rows * (a.dim / 4), row_groups))
         || (rc = groups_for("attention_bwd", heads_of(a) * a.keys * (a.dim / 4), key_groups))) return rc;
     if (a.rows) {
-        const RowArgs r{a, y, tokens_of(dy), reinterpret_cast<const float2*>(stats), (float4*)(ws + space.records), (float*)(ws + space.qs), (float*)(ws + space.dn)};
+        const RowArgs r{a, y, tokens_of(dy), reinterpret_cast<const float2*>(stats), (float4*)(ws + space.records), (float*)(ws + space.qs), (float*)(ws + space.dn), variant_for(kDqApprox, a.values).slices,
+                        4 * variant_for(kDqApprox, a.values).quads};
         hipLaunchKernelGGL(attention_rows_kernel, dim3(groups), dim3(kThreads), 0, st, r);
         if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
     }

@@ -119,6 +119,17 @@ def test_rows_that_see_nothing():
 
 
 @gpu
+@pytest.mark.parametrize("dim", [1, 16, 18, 64, 100, 128, 130, 256])
+def test_rows_of_a_single_key_give_no_gradient(dim):
+    """Their weight is one whatever the score is: nothing for queries and keys, to the bit, and dy for the value."""
+    for seed, shape, more in ((1, (2, 1, 1, 4, 2, dim), {}), (2, (1, 70, 70, 4, 2, dim), dict(window=1)), (3, (1, 1, 33, 2, 1, dim), dict(window=1, cap=9.0))):
+        q, k, v, dy = _inputs(seed, *shape)
+        y, (dq, dk, dv) = _run(q, k, v, dy, more)
+        assert (dq == 0).all() and (dk == 0).all() and (dv[:, -1] != 0).all()
+        assert torch.equal(y, _cuda(v)[:, -shape[1]:].repeat_interleave(shape[3] // shape[4], 2))
+
+
+@gpu
 @pytest.mark.parametrize("what", ["zero_row", "zero_values", "zero_queries", "small", "large", "one_zero"])
 def test_values_out_of_the_ordinary(what):
     def change(q, k, v, dy):
