@@ -8,18 +8,19 @@
 // M has been on the way.  (The softmax of the primitives subtracts the largest of all rows' scores, which is no whole number, and moves the
 // result with it.)
 //
-// A wavefront's lanes own rows (queries; in the pass for dk and dv, keys), with a row's values in the lane's registers, and the
-// other side streams by.  A product takes two instructions on 64 lanes, an integer addition that reads the streamed value from another lane
-// of the 16 (a data-parallel primitive of the addition itself: row_newbcast) and a float addition: no LDS, no barriers, and a wavefront alone in its
-// work-group's progress.  A streamed row is one 128-bit load per lane, the same for the four sixteens of the wavefront.
-// Rows of more than 64 values (32 in the backward passes, which hold three or four of them per lane) are cut into NS slices of
-// at most 16 quads, each of which has its own sixteens of the wavefront, 64 / NS rows; a score's slices are added by lane swaps.
-// Values read through scalar registers instead of lanes waited for the scalar cache: 2.2 T products/s where this has 6.4 (8 heads of 4096 x 4096 x 64, one
-// wavefront on every second SIMD).
+// A wavefront's lanes own 64 rows (queries; in the pass for dk and dv, keys), a slice of at most 32 of a row's values in a lane's registers, and the
+// other side streams by in scalar registers, that all lanes read: a product takes two instructions on 64 lanes, an integer addition and
+// a float addition, and nothing else.  One piece of a streamed row (at most 20 values) is used while the next one is on its way, wherever that
+// is: in this row, the next or the next phase's.  Longer rows are cut into slices with a wavefront each, which add up their parts of a score
+// through LDS: wider slices would do less twice, but leave room for two wavefronts on a SIMD, which did not cover the scalar loads.
+// Rates of the inner loop alone, two wavefronts per SIMD: 28 T products/s; with the streamed values read from another lane inside the integer
+// addition (a data-parallel primitive: everything around it issues half as fast) 18.6; copied out of one once for four rows 20.5; by lane reads 12.
 //
 // The integer addition is the product while no exponent leaves the normal range.  Streamed values have to be in 2^[-40, 40), a lane's in 2^[-86, 80); a
-// lane's zero stands as 2^-86, which adds less to a sum than its rounding.  A streamed row that is all zeros is left out by selects; a
-// streamed block with anything else in it, or a wavefront with anything else in its rows, takes the full definition (`careful`).
+// lane's zero stands as 2^-86, which adds less to a sum than its rounding.  Streamed rows with zeros take a loop that leaves those out by a factor.
+// With anything else in a streamed row, or in a lane's, a unit begins again with the full definition (`careful`), a row at a time: kept apart
+// from the usual loops, because side by side with them it took their registers.
+// Every value of a block is looked at for that by one lane, with vector loads of its own.
 #pragma once
 #include "pam_activation.h"
 #include "pam_common.h"
@@ -28,8 +29,8 @@
 namespace pamatt {
 using namespace pamdev;
 
-constexpr int kThreads = 256, kWaves = 4;
-constexpr int kBlock = 8;                         // streamed rows at a time (four: 18.8 T products/s where eight have 20.9)
+constexpr int kThreads = 256, kWaves = 4;         // (of the small kernels and of a cache's)
+constexpr int kBlock = 8;                         // streamed rows at a time
 constexpr int kSpan = 64;                         // streamed rows per word of visibility
 constexpr int kLink = 1024;                       // terms of a chain of sums; chains are added up in memory
 constexpr float kLag = 8.0f;
@@ -74,87 +75,14 @@ template <int N, int END, class F> __device__ __forceinline__ void each(F&& f)
     if constexpr (N < END) { f(Index<N>{}); each<N + 1, END>(f); }
 }
 
-template <int NS> __device__ __forceinline__ float over_slices(float v)          // the slices' sum, in all of them
-{
-    typedef unsigned int u2 __attribute__((ext_vector_type(2)));
-    if constexpr (NS == 4) { const u2 r = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false); v = u2f(r.x) + u2f(r.y); }
-    if constexpr (NS >= 2) { const u2 r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false); v = u2f(r.x) + u2f(r.y); }
-    return v;
-}
-
 constexpr uint32_t kStreamBase = (uint32_t)(127 - 40) << 24, kStreamSpan = 80u << 24;      // 2^[-40, 40) of bits << 1
 constexpr uint32_t kLaneBase = (uint32_t)(127 - 86) << 24, kLaneSpan = 166u << 24;         // 2^[-86, 80)
 constexpr uint32_t kStandIn = (uint32_t)(127 - 86) << 23;
 
-template <int NS, int W4>
-struct Place {                                    // what a lane has to do with
-    int lane, row_in_wave, slice, at;             // at: the first value of its quad in a streamed row
-    bool streams;                                 // it holds a part of streamed rows
-    uint64_t streaming;                           // the lanes that do
-    __device__ __forceinline__ explicit Place(int values)
-    {
-        constexpr int kRows = 64 / NS;
-        lane = threadIdx.x % 64; row_in_wave = lane % kRows; slice = lane / kRows;
-        at = slice * 4 * W4 + lane % 16 * 4;
-        streams = lane % 16 < W4 && at < values;
-        if (!streams) at = 0;
-        streaming = __ballot(streams);
-    }
-};
-
 // (comparisons with it are made where they are used, instead of kept from the beginning of a kernel to its end)
 __device__ __forceinline__ int anew(int v) { asm volatile("" : "+v"(v)); return v; }
 
-// Behind a row's values streamed rows have what `shift` makes ones of, and lanes' rows what makes + 0 of that.
-__device__ __forceinline__ uint32_t stream_pad(uint32_t shift) { return kBias - shift; }
 __device__ __forceinline__ uint32_t lane_pad(uint32_t shift) { return shift - kBias; }
-
-// A lane's row: bits(value) + scale + add, zeros stood in for (unscaled).  scale: of a factor in 2^[-41, 41].  Returns false if a value,
-// scaled, is out of the window.
-template <int W4>
-__device__ __forceinline__ bool load_lane(const float* row, int first, int dim, int values, uint32_t scale, uint32_t add, uint32_t pad, uint32_t (&out)[4 * W4])
-{
-    uint32_t most = 0u;
-    first = anew(first);
-#pragma unroll
-    for (int n = 0; n < W4; ++n) {
-        const v4f x = *reinterpret_cast<const v4f_any*>(row + min(first + 4 * n, dim - 4));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t b = (f2u(x[i]) << 1) == 0u ? kStandIn : f2u(x[i]) + scale;
-            const bool there = first + 4 * n + i < values;
-            most = max(most, there ? (b << 1) - kLaneBase : 0u);
-            out[4 * n + i] = there ? b + add : pad;
-        }
-    }
-    return most < kLaneSpan;
-}
-
-// The quad that a lane holds of a streamed row.
-struct Stream {
-    const float* p; long st;                      // uniform
-    uint32_t at; int last, values; bool streams, whole;      // whole: all lanes below W4 have four values
-    // the rows j ... j + 7, past the end the last one again
-    __device__ __forceinline__ void rows(int j, v4f (&r)[kBlock]) const
-    {
-#pragma unroll
-        for (int i = 0; i < kBlock; ++i) r[i] = *reinterpret_cast<const v4f_any*>(p + (long)min(j + i, last) * st + at);
-    }
-    __device__ __forceinline__ void pad(uint32_t shift, v4f (&r)[kBlock]) const      // (where they are used)
-    {
-        if (whole) return;
-        const float one = u2f(stream_pad(shift));
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const bool there = streams && (int)at + d < values;
-#pragma unroll
-            for (int i = 0; i < kBlock; ++i) r[i][d] = there ? r[i][d] : one;
-        }
-    }
-};
-template <int NS, int W4>
-__device__ __forceinline__ Stream stream_of(const Place<NS, W4>& here, const float* p, long st, int values, int count)
-{ return Stream{p, st, (uint32_t)here.at, count - 1, values, here.streams, values == 4 * W4 * NS}; }
 
 template <int N, class T> __device__ __forceinline__ void turned(T (&v)[N])      // all one place down, the first to the end
 {
@@ -164,62 +92,287 @@ template <int N, class T> __device__ __forceinline__ void turned(T (&v)[N])     
     v[N - 1] = first;
 }
 
-// What is the matter with a block of streamed rows: `zero`, the rows that are all zeros (they become ones, and their products are to
-// be left out), `careful`, something else is.
-struct Verdict { uint32_t zero; bool careful; };
-__device__ __forceinline__ Verdict judge(uint64_t streaming, uint32_t shift, v4f (&r)[kBlock])
+// A lane's part of a row: bits(value) + scale + add, zeros and what lies behind the row's values stood in for (unscaled; 2^-86 itself counts as the next
+// number).  scale: of a factor in 2^[-41, 41].  Returns false if a value, scaled, is out of the window.
+template <int W4>
+__device__ __forceinline__ bool load_lane(const float* row, int first, int dim, int values, uint32_t scale, uint32_t add, uint32_t (&out)[4 * W4])
 {
     uint32_t most = 0u;
+    first = anew(first);
 #pragma unroll
-    for (int j = 0; j < kBlock; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) most = max(most, ((f2u(r[j][i]) + shift) << 1) - kStreamBase);
-    Verdict v{0u, false};
-    if (__builtin_expect((__ballot(most >= kStreamSpan) & streaming) == 0ull, 1)) return v;
-#pragma unroll 1
-    for (int j = 0; j < kBlock; ++j) {
-        bool all = true, odd = false;
+    for (int n = 0; n < W4; ++n) {
+        const v4f x = *reinterpret_cast<const v4f_any*>(row + min(first + 4 * n, dim - 4));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            all = all && (f2u(r[0][i]) << 1) == 0u;
-            odd = odd || ((f2u(r[0][i]) + shift) << 1) - kStreamBase >= kStreamSpan;
+            uint32_t b = f2u(x[i]) + scale;
+            b = (b & ~kSign) == kStandIn ? b + 1u : b;
+            b = (f2u(x[i]) << 1) == 0u || first + 4 * n + i >= values ? kStandIn : b;
+            most = max(most, (b << 1) - kLaneBase);
+            out[4 * n + i] = b + add;
         }
-        if ((__ballot(!all) & streaming) == 0ull) {
-            v.zero |= 1u << j;
+    }
+    return most < kLaneSpan;
+}
+
+// ---------------------------------------------------------------- streamed rows
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f16_any __attribute__((ext_vector_type(16), aligned(4)));
+typedef float f8_any __attribute__((ext_vector_type(8), aligned(4)));
+
+// Rows of one head, of which a slice takes the quads first ... first + W4 - 1.  Where a row has fewer, the last one stands for the missing: lanes hold nothing there.
+template <bool WHOLE> struct Stream {
+    const float* p; long st, bytes; int last, first, quads;   // uniform; bytes: st as such; p: where the slice begins in row 0, or, not WHOLE, that row; quads: of a row
+    __device__ __forceinline__ Stream(const float* base, long stride, int rows, int first_quad, int row_quads)
+        : p(WHOLE ? base + 4 * first_quad : base), st(stride), bytes(stride * (long)sizeof(float)), last(rows - 1), first(first_quad), quads(row_quads) {}
+    __device__ __forceinline__ const float* row(int j) const { return p + (long)min(j, last) * st; }
+    __device__ __forceinline__ const float* after(const float* at, int j) const { return (const float*)((const char*)at + (j < last ? bytes : 0l)); }      // row j + 1, at being row j
+    __device__ __forceinline__ int quad(int n) const { return WHOLE ? n : min(first + n, quads - 1); }
+    // a lane of each sixteen has a quad
+    template <int W4> __device__ __forceinline__ v4f across(int j) const
+    { return *reinterpret_cast<const v4f_any*>(row(j) + 4 * quad(min((int)threadIdx.x % 16, W4 - 1))); }
+};
+
+// Q quads of a row in scalar registers.
+struct Piece { f16v a; v4f b; };
+template <int Q, bool WHOLE> __device__ __forceinline__ Piece piece_of(const Stream<WHOLE>& s, const float* row, int quad)
+{
+    typedef const __attribute__((address_space(4))) f16_any* P16;
+    typedef const __attribute__((address_space(4))) f8_any* P8;
+    typedef const __attribute__((address_space(4))) v4f_any* P4;
+    Piece x;
+    if constexpr (WHOLE) {
+        const float* const p = row + 4 * quad;
+        static_assert(Q >= 3 && Q <= 5);
+        if constexpr (Q >= 4) x.a = *(P16)p;
+        if constexpr (Q == 5) x.b = *(P4)(p + 16);
+        if constexpr (Q == 3) {
+            const f8_any y = *(P8)p; const v4f z = *(P4)(p + 8);
+            const auto w = __builtin_shufflevector(z, z, 0, 1, 2, 3, 0, 1, 2, 3);
+            x.a = __builtin_shufflevector(y, w, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 8, 9, 10, 11);
+        }
+    } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[0][i] = u2f(stream_pad(shift));
-        } else if ((__ballot(odd) & streaming) != 0ull) v.careful = true;
-        turned(r);
+        for (int n = 0; n < Q; ++n) {
+            const v4f z = *(P4)(row + 4 * s.quad(quad + n));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { if (n < 4) x.a[n * 4 + i] = z[i]; else x.b[i] = z[i]; }
+        }
+    }
+    return x;
+}
+__device__ __forceinline__ float at(const Piece& x, int i) { return i < 16 ? x.a[i] : x.b[i - 16]; }
+
+// Blocks of rows by pieces.  What asks for a phase's last piece asks for the next phase's first one.
+template <int W4, bool WHOLE> struct Pipe {
+    static constexpr int kPieces = W4 > 10 ? W4 / 4 : W4 > 5 ? 2 : 1, kQuads = W4 / kPieces;
+    static_assert(kPieces * kQuads == W4);
+    Piece now;
+    const float* at;                              // the row that it is of
+    __device__ __forceinline__ void request(const Stream<WHOLE>& s, int j) { at = s.row(j); now = piece_of<kQuads, WHOLE>(s, at, 0); }
+    // f(row of the block, first value, piece) for the rows j1 ... j1 + 7 of s, whose first piece is asked for; then comes row j2 of `next`.
+    // rolled: f gets row 0 every time and turns its arrays around
+    template <class F> __device__ __forceinline__ void rolled(const Stream<WHOLE>& s, int j1, const Stream<WHOLE>& next, int j2, F&& f)
+    {
+#pragma unroll 1
+        for (int j = 0; j < kBlock; ++j)
+#pragma unroll
+            for (int h = 0; h < kPieces; ++h) {
+                const Piece x = piece_of<kQuads, WHOLE>(s, s.row(j1 + j), h * kQuads);
+                f(h, h * kQuads * 4, x);
+            }
+        request(next, j2);
+    }
+    template <class F> __device__ __forceinline__ void block(const Stream<WHOLE>& s, int j1, const Stream<WHOLE>& next, int j2, F&& f)
+    {
+#pragma unroll
+        for (int j = 0; j < kBlock; ++j) {
+            const float* const after = j + 1 < kBlock ? s.after(at, j1 + j) : next.row(j2);
+#pragma unroll
+            for (int h = 0; h < kPieces; ++h) {
+                if constexpr (kQuads > 4) asm volatile("" ::"s"(now.a), "s"(now.b));          // (the wait for it, before the next one is asked for: loads of this kind
+                else asm volatile("" ::"s"(now.a));                                           // come back in any order, so that a wait is for all of them)
+                __builtin_amdgcn_sched_barrier(0);
+                const Piece later = h + 1 < kPieces ? piece_of<kQuads, WHOLE>(s, at, (h + 1) * kQuads) : piece_of<kQuads, WHOLE>(j + 1 < kBlock ? s : next, after, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                f(j, h * kQuads * 4, now);
+                __builtin_amdgcn_sched_barrier(0);
+                now = later;
+            }
+            at = after;
+        }
+    }
+};
+
+// Eight values of a piece with eight of a lane's at a time, and what remains by four.  Written as instructions: the compiler gave each product the
+// register of the one before, and the order below keeps dependent ones apart.
+#define PAM_T8 [t0] "=&v"(t[0]), [t1] "=&v"(t[1]), [t2] "=&v"(t[2]), [t3] "=&v"(t[3]), [t4] "=&v"(t[4]), [t5] "=&v"(t[5]), [t6] "=&v"(t[6]), [t7] "=&v"(t[7])
+#define PAM_T4 [t0] "=&v"(t[0]), [t1] "=&v"(t[1]), [t2] "=&v"(t[2]), [t3] "=&v"(t[3])
+#define PAM_S4(n) [s0] "s"(at(x, n)), [s1] "s"(at(x, n + 1)), [s2] "s"(at(x, n + 2)), [s3] "s"(at(x, n + 3))
+#define PAM_S8(n) PAM_S4(n), [s4] "s"(at(x, n + 4)), [s5] "s"(at(x, n + 5)), [s6] "s"(at(x, n + 6)), [s7] "s"(at(x, n + 7))
+#define PAM_M4(n) [m0] "v"(m[n]), [m1] "v"(m[n + 1]), [m2] "v"(m[n + 2]), [m3] "v"(m[n + 3])
+#define PAM_M8(n) PAM_M4(n), [m4] "v"(m[n + 4]), [m5] "v"(m[n + 5]), [m6] "v"(m[n + 6]), [m7] "v"(m[n + 7])
+#define PAM_O4(n) [o0] "+v"(o[n]), [o1] "+v"(o[n + 1]), [o2] "+v"(o[n + 2]), [o3] "+v"(o[n + 3])
+#define PAM_O8(n) PAM_O4(n), [o4] "+v"(o[n + 4]), [o5] "+v"(o[n + 5]), [o6] "+v"(o[n + 6]), [o7] "+v"(o[n + 7])
+#define PAM_EACH4(op) op("0") op("1") op("2") op("3")
+#define PAM_EACH8(op) PAM_EACH4(op) op("4") op("5") op("6") op("7")
+// the product of a streamed value and a lane's, of a streamed one and the lane's weight, of the lane's weight and a lane's
+#define PAM_OF_ROW(i) "v_add_u32 %[t" i "], %[s" i "], %[m" i "]\n"
+#define PAM_OF_WEIGHT(i) "v_add_u32 %[t" i "], %[s" i "], %[w]\n"
+#define PAM_OF_LANE(i) "v_add_u32 %[t" i "], %[w], %[m" i "]\n"
+#define PAM_POWER(i) "v_and_b32 %[t" i "], %[mask], %[t" i "]\n"
+#define PAM_SUM(i) "v_add_f32 %[sum], %[sum], %[t" i "]\n"
+#define PAM_SUM_BY_LANE(i) "v_fmac_f32 %[sum], %[t" i "], %[m" i "]\n"
+#define PAM_SUM_BY_ROW(i) "v_fmac_f32 %[sum], %[s" i "], %[t" i "]\n"
+#define PAM_ADD(i) "v_fmac_f32 %[o" i "], %[f], %[t" i "]\n"
+#define PAM_ADD_BY_ROW(i) "v_fmac_f32 %[o" i "], %[s" i "], %[t" i "]\n"
+
+// sum over d of row (*) lane: `m` as load_lane left it with add = bits(offset) - 2 bias
+template <int N> __device__ __forceinline__ void dot_piece(const Piece& x, const uint32_t* m, float& sum)
+{
+    float t[8];
+#pragma unroll
+    for (int n = 0; n + 8 <= N; n += 8) asm(PAM_EACH8(PAM_OF_ROW) PAM_EACH8(PAM_SUM) : [sum] "+v"(sum), PAM_T8 : PAM_S8(n), PAM_M8(n));
+    if constexpr (N % 8 != 0) asm(PAM_EACH4(PAM_OF_ROW) PAM_EACH4(PAM_SUM) : [sum] "+v"(sum), PAM_T4 : PAM_S4(N - 4), PAM_M4(N - 4));
+}
+// out_d += f * (weight (*) row's d), the weight's bits with that added, f 0 or 1
+template <int N> __device__ __forceinline__ void add_piece(const Piece& x, uint32_t w, float f, float* o)
+{
+    float t[8];
+#pragma unroll
+    for (int n = 0; n + 8 <= N; n += 8) asm(PAM_EACH8(PAM_OF_WEIGHT) PAM_EACH8(PAM_ADD) : PAM_O8(n), PAM_T8 : PAM_S8(n), [w] "v"(w), [f] "v"(f));
+    if constexpr (N % 8 != 0) asm(PAM_EACH4(PAM_OF_WEIGHT) PAM_EACH4(PAM_ADD) : PAM_O4(N - 4), PAM_T4 : PAM_S4(N - 4), [w] "v"(w), [f] "v"(f));
+}
+
+// ... of a row with zeros, whose products count for nothing
+template <int N> __device__ __forceinline__ void dot_piece_with_zeros(const Piece& x, const uint32_t* m, float& sum)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool none = (f2u(at(x, i)) << 1) == 0u;
+        sum = __builtin_fmaf(u2f((none ? kBias : f2u(at(x, i))) + m[i]), none ? 0.0f : 1.0f, sum);
+    }
+}
+template <int N> __device__ __forceinline__ void add_piece_with_zeros(const Piece& x, uint32_t w, float f, float* o)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool none = (f2u(at(x, i)) << 1) == 0u;
+        o[i] = __builtin_fmaf(u2f((none ? kBias : f2u(at(x, i))) + w) * f, none ? 0.0f : 1.0f, o[i]);
+    }
+}
+
+// By the slopes of the pieces that the factors are in (a slope is a product's power of two over the own factor's, so that it takes the product without its
+// mantissa; what it is to be over comes at the end).  mask: of the power, or zero where the product does not count.
+// sum over d of power(weight (*) row's d) * lane's d
+template <int N> __device__ __forceinline__ void dot_power_piece(const Piece& x, uint32_t w, uint32_t mask, const uint32_t* m, float& sum)
+{
+    float t[8];
+#pragma unroll
+    for (int n = 0; n + 8 <= N; n += 8)
+        asm(PAM_EACH8(PAM_OF_WEIGHT) PAM_EACH8(PAM_POWER) PAM_EACH8(PAM_SUM_BY_LANE) : [sum] "+v"(sum), PAM_T8 : PAM_S8(n), PAM_M8(n), [w] "v"(w), [mask] "v"(mask));
+    if constexpr (N % 8 != 0)
+        asm(PAM_EACH4(PAM_OF_WEIGHT) PAM_EACH4(PAM_POWER) PAM_EACH4(PAM_SUM_BY_LANE) : [sum] "+v"(sum), PAM_T4 : PAM_S4(N - 4), PAM_M4(N - 4), [w] "v"(w), [mask] "v"(mask));
+}
+// sum over d of power(weight (*) lane's d) * row's d
+template <int N> __device__ __forceinline__ void dot_lane_power_piece(const Piece& x, uint32_t w, uint32_t mask, const uint32_t* m, float& sum)
+{
+    float t[8];
+#pragma unroll
+    for (int n = 0; n + 8 <= N; n += 8)
+        asm(PAM_EACH8(PAM_OF_LANE) PAM_EACH8(PAM_POWER) PAM_EACH8(PAM_SUM_BY_ROW) : [sum] "+v"(sum), PAM_T8 : PAM_S8(n), PAM_M8(n), [w] "v"(w), [mask] "v"(mask));
+    if constexpr (N % 8 != 0)
+        asm(PAM_EACH4(PAM_OF_LANE) PAM_EACH4(PAM_POWER) PAM_EACH4(PAM_SUM_BY_ROW) : [sum] "+v"(sum), PAM_T4 : PAM_S4(N - 4), PAM_M4(N - 4), [w] "v"(w), [mask] "v"(mask));
+}
+// out_d += f * power(row's d (*) lane's d)
+template <int N> __device__ __forceinline__ void add_power_piece(const Piece& x, float f, uint32_t mask, const uint32_t* m, float* o)
+{
+    float t[8];
+#pragma unroll
+    for (int n = 0; n + 8 <= N; n += 8)
+        asm(PAM_EACH8(PAM_OF_ROW) PAM_EACH8(PAM_POWER) PAM_EACH8(PAM_ADD) : PAM_O8(n), PAM_T8 : PAM_S8(n), PAM_M8(n), [f] "v"(f), [mask] "v"(mask));
+    if constexpr (N % 8 != 0)
+        asm(PAM_EACH4(PAM_OF_ROW) PAM_EACH4(PAM_POWER) PAM_EACH4(PAM_ADD) : PAM_O4(N - 4), PAM_T4 : PAM_S4(N - 4), PAM_M4(N - 4), [f] "v"(f), [mask] "v"(mask));
+}
+// out_d += row's d * power(weight (*) lane's d)
+template <int N> __device__ __forceinline__ void add_lane_power_piece(const Piece& x, uint32_t w, uint32_t mask, const uint32_t* m, float* o)
+{
+    float t[8];
+#pragma unroll
+    for (int n = 0; n + 8 <= N; n += 8)
+        asm(PAM_EACH8(PAM_OF_LANE) PAM_EACH8(PAM_POWER) PAM_EACH8(PAM_ADD_BY_ROW) : PAM_O8(n), PAM_T8 : PAM_S8(n), PAM_M8(n), [w] "v"(w), [mask] "v"(mask));
+    if constexpr (N % 8 != 0)
+        asm(PAM_EACH4(PAM_OF_LANE) PAM_EACH4(PAM_POWER) PAM_EACH4(PAM_ADD_BY_ROW) : PAM_O4(N - 4), PAM_T4 : PAM_S4(N - 4), PAM_M4(N - 4), [w] "v"(w), [mask] "v"(mask));
+}
+
+// A row's block as one lane in eight sees it: every value of the slice in one lane.
+template <int W4, bool WHOLE> struct Look {
+    static constexpr int kParts = (W4 + 7) / 8;
+    v4f r[kParts];
+    __device__ __forceinline__ static int mine(int i) { return min((int)threadIdx.x % 8 + 8 * i, W4 - 1); }
+    __device__ __forceinline__ void load(const Stream<WHOLE>& s, int j1)
+    {
+        const float* const row = s.row(j1 + (int)threadIdx.x % 64 / 8);
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) r[i] = *reinterpret_cast<const v4f_any*>(row + 4 * s.quad(mine(i)));
+    }
+    // (behind a head's values its last quad counts as the values in it)
+    __device__ __forceinline__ void fill(const Stream<WHOLE>& s, int values)
+    {
+        if (values == 4 * s.quads) return;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            const int d = 4 * min(s.first + mine(i), s.quads - 1);
+#pragma unroll
+            for (int c = 1; c < 4; ++c) r[i][c] = d + c < values ? r[i][c] : r[i][0];
+        }
+    }
+};
+// What is the matter with a block: zeros in it, or something else.
+struct Verdict { bool zeros, wild; };
+template <int W4, bool WHOLE> __device__ __forceinline__ Verdict judge(Look<W4, WHOLE>& look, const Stream<WHOLE>& s, int values, uint32_t shift)
+{
+    look.fill(s, values);
+    uint32_t most = 0u;
+#pragma unroll
+    for (int i = 0; i < Look<W4, WHOLE>::kParts; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) most = max(most, ((f2u(look.r[i][c]) + shift) << 1) - kStreamBase);
+    Verdict v{__ballot(most >= kStreamSpan) != 0ull, false};
+    if (__builtin_expect(v.zeros, 0)) {
+        bool wild = false;
+#pragma unroll
+        for (int i = 0; i < Look<W4, WHOLE>::kParts; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) wild = wild || ((f2u(look.r[i][c]) << 1) != 0u && ((f2u(look.r[i][c]) + shift) << 1) - kStreamBase >= kStreamSpan);
+        v.wild = __ballot(wild) != 0ull;
     }
     return v;
 }
 
-// sum over d of a lane's values with a streamed row's: `mine` as load_lane left them with add = bits(offset) - 2 bias
-template <int W4> __device__ __forceinline__ float dot(const v4f& row, const uint32_t (&mine)[4 * W4])
+// ... where values are only factors of a float product: zeros and small ones are as good as any
+template <int W4, bool WHOLE> __device__ __forceinline__ bool all_finite(Look<W4, WHOLE>& look, const Stream<WHOLE>& s, int values)
 {
-    float sum = 0.0f;
-    each<0, W4>([&](auto n) __attribute__((always_inline)) {
+    look.fill(s, values);
+    uint32_t most = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += u2f(from_lane<decltype(n)::value>(row[i]) + mine[4 * n.value + i]);
-    });
-    return sum;
-}
-// out_d += f * (weight (*) a streamed row's d), weight as above; f is 0 or 1
-template <int W4> __device__ __forceinline__ void add_row(const v4f& row, uint32_t weight, float f, float (&out)[4 * W4])
-{
-    each<0, W4>([&](auto n) __attribute__((always_inline)) {
+    for (int i = 0; i < Look<W4, WHOLE>::kParts; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[4 * n.value + i] = __builtin_fmaf(u2f(from_lane<decltype(n)::value>(row[i]) + weight), f, out[4 * n.value + i]);
-    });
+        for (int c = 0; c < 4; ++c) most = max(most, f2u(look.r[i][c]) << 1);
+    return __ballot(most >= kExpo << 1) == 0ull;
 }
 
-// The same by the full definition, what turns `mine` back into a value's bits being `raw`.  One row's code each, in loops that turn the arrays
-// around.
-struct Full { float off; bool has_off; uint32_t raw, pad; };
+// The same products by the full definition, for a row that lanes hold a quad each of.  raw: what turns `mine` back into a value's bits.
+struct Full { float off; bool has_off; uint32_t raw; };
 __device__ __forceinline__ float full_product(const Full& f, uint32_t a, uint32_t b)
 {
     const float c = pam_general(a, b);
     return f.has_off ? pam_general(f2u(c), f2u(f.off)) : c;
+}
+__device__ __forceinline__ uint32_t real_bits(const Full& f, uint32_t mine)
+{
+    const uint32_t m = (uint32_t)anew((int)mine) + f.raw;      // (taken apart here and not, for all rows, before the loop)
+    return m == kStandIn ? 0u : m;
 }
 template <int W4> __device__ __forceinline__ float careful_dot(const Full& f, const v4f& row, const uint32_t (&mine)[4 * W4])
 {
@@ -227,8 +380,7 @@ template <int W4> __device__ __forceinline__ float careful_dot(const Full& f, co
     each<0, W4>([&](auto n) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t m = (uint32_t)anew((int)mine[4 * n.value + i]);      // (taken apart here and not, for all rows, before the loop)
-            sum += full_product(f, m == f.pad ? 0u : m + f.raw, from_lane<decltype(n)::value>(row[i]));
+            sum += full_product(f, real_bits(f, mine[4 * n.value + i]), from_lane<decltype(n)::value>(row[i]));
             __builtin_amdgcn_sched_barrier(0);    // (rare code: side by side the products took registers from the usual loops)
         }
     });
@@ -246,47 +398,79 @@ template <int W4> __device__ __forceinline__ void careful_add_row(const Full& f,
     });
 }
 
-// A block's scores (their slices added up).
-template <int NS, int W4>
-__device__ __forceinline__ void block_dots(const Full& f, bool careful, uint32_t zero, float scale, v4f (&r)[kBlock], const uint32_t (&mine)[4 * W4], float (&sum)[kBlock])
+// A block's sums of products with the rows of s; then comes row j2 of `next`.
+template <int W4, bool WHOLE>
+__device__ __forceinline__ void block_dots(Pipe<W4, WHOLE>& pipe, const Stream<WHOLE>& s, int j1, const Stream<WHOLE>& next, int j2, bool zeros, const uint32_t (&mine)[4 * W4], float (&sum)[kBlock])
 {
-    if (__builtin_expect(careful, 0)) {
-#pragma unroll 1
-        for (int j = 0; j < kBlock; ++j) {
-            sum[0] = careful_dot<W4>(f, r[0], mine) * scale;
-            turned(r); turned(sum);
-        }
-    } else {
+    constexpr int N = 4 * Pipe<W4, WHOLE>::kQuads;
 #pragma unroll
-        for (int j = 0; j < kBlock; ++j) sum[j] = dot<W4>(r[j], mine);
-    }
-#pragma unroll
-    for (int j = 0; j < kBlock; ++j) sum[j] = over_slices<NS>(sum[j]);
-    if (__builtin_expect(zero != 0u, 0)) {
-#pragma unroll
-        for (int j = 0; j < kBlock; ++j) sum[j] = (zero >> j) & 1u ? 0.0f : sum[j];
-    }
-}
-// out += the block's weights times its rows; a weight that does not count is anything.  add: as in load_lane.
-template <int W4>
-__device__ __forceinline__ void block_add(const Full& f, bool careful, uint32_t zero, float scale, v4f (&r)[kBlock], float (&weight)[kBlock], uint32_t add, uint32_t counts,
-                                          float (&out)[4 * W4])
-{
-    counts &= ~zero;
-    if (__builtin_expect(careful, 0)) {
-#pragma unroll 1
-        for (int j = 0; j < kBlock; ++j) {
-            careful_add_row<W4>(f, r[0], weight[0], (counts >> j) & 1u, scale, out);
-            turned(r); turned(weight);
-        }
+    for (int j = 0; j < kBlock; ++j) sum[j] = 0.0f;
+    if (__builtin_expect(zeros, 0)) {
+        pipe.rolled(s, j1, next, j2, [&](int h, int d, const Piece& x) __attribute__((always_inline)) {
+            dot_piece_with_zeros<N>(x, mine + d, sum[0]);
+            if (h == Pipe<W4, WHOLE>::kPieces - 1) turned(sum);
+        });
         return;
     }
-#pragma unroll
-    for (int j = 0; j < kBlock; ++j) {
-        const bool in = (counts >> j) & 1u;
-        add_row<W4>(r[j], in ? f2u(weight[j]) + add : 0u, in ? 1.0f : 0.0f, out);
-    }
+    pipe.block(s, j1, next, j2, [&](int j, int d, const Piece& x) __attribute__((always_inline)) { dot_piece<N>(x, mine + d, sum[j]); });
 }
+// out += the block's weights times its rows; a weight that does not count is anything.  add: as in load_lane.
+template <int W4, bool WHOLE>
+__device__ __forceinline__ void block_add(Pipe<W4, WHOLE>& pipe, const Stream<WHOLE>& s, int j1, const Stream<WHOLE>& next, int j2, bool zeros, float (&weight)[kBlock], uint32_t add, uint32_t counts,
+                                          float (&out)[4 * W4])
+{
+    constexpr int N = 4 * Pipe<W4, WHOLE>::kQuads;
+    if (__builtin_expect(zeros, 0)) {
+        pipe.rolled(s, j1, next, j2, [&](int h, int d, const Piece& x) __attribute__((always_inline)) {
+            const bool in = counts & 1u;
+            add_piece_with_zeros<N>(x, in ? f2u(weight[0]) + add : 0u, in ? 1.0f : 0.0f, out + d);
+            if (h == Pipe<W4, WHOLE>::kPieces - 1) { turned(weight); counts >>= 1; }
+        });
+        return;
+    }
+    pipe.block(s, j1, next, j2, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+        const bool in = (counts >> j) & 1u;
+        add_piece<N>(x, in ? f2u(weight[j]) + add : 0u, in ? 1.0f : 0.0f, out + d);
+    });
+}
+
+// A work-group is four wavefronts (eight, where a row has eight slices): NS of them for each of kTiles tiles of 64 rows, which stream the same rows by.  With
+// slices all wavefronts have the same barriers: `Team` says what one of them found to all.
+template <int NS> constexpr int kTiles = NS >= 4 ? 1 : 4 / NS;
+template <int NS> constexpr int kWaveCount = NS * kTiles<NS>;
+template <int NS> __device__ __forceinline__ bool in_team(bool x) { return NS == 1 ? __ballot(x) != 0ull : __syncthreads_or(x) != 0; }
+
+// Slices' sums, in all of their wavefronts and in one order, and whether a wavefront of the team met something wild.  Two buffers in turn: who writes one
+// again has passed the barrier before which the others read it.
+template <int NS, int N> struct Slices {
+    v4f part[2][kTiles<NS>][NS][N / 4][64];
+    int wild[2][kWaveCount<NS>];
+    __device__ __forceinline__ bool add_up(int turn, int wave, float (&v)[N], bool is_wild)
+    {
+        const int lane = (int)threadIdx.x % 64, tile = wave / NS, slice = wave % NS;
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) part[turn][tile][slice][i][lane] = v4f{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        if (lane == 0) wild[turn][wave] = is_wild;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            v4f x[NS];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) x[s] = part[turn][tile][s][i][lane];
+#pragma unroll
+            for (int n = NS; n > 1; n /= 2)
+#pragma unroll
+                for (int s = 0; s < n / 2; ++s) x[s] = x[2 * s] + x[2 * s + 1];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[4 * i + c] = x[0][c];
+        }
+        int any = 0;
+#pragma unroll
+        for (int s = 0; s < kWaveCount<NS>; ++s) any |= wild[turn][s];
+        return __builtin_amdgcn_readfirstlane(any) != 0;
+    }
+};
+template <int N> struct Slices<1, N> { __device__ __forceinline__ bool add_up(int, int, float (&)[N], bool is_wild) { return is_wild; } };
 
 // ---------------------------------------------------------------- which streamed rows a lane's row goes with
 
@@ -303,6 +487,17 @@ struct Sight {
 #pragma unroll
         for (int s = 1; s < 64; s *= 2) { a = min(a, __shfl_xor(a, s, 64)); b = max(b, __shfl_xor(b, s, 64)); }
         first = __builtin_amdgcn_readfirstlane(a); last = __builtin_amdgcn_readfirstlane(b);
+    }
+    template <int NS> __device__ __forceinline__ void close_team()
+    {
+        if constexpr (NS > 1) {
+            __shared__ int ends[kWaveCount<NS>][2];
+            if (threadIdx.x % 64 == 0) { ends[threadIdx.x / 64][0] = first; ends[threadIdx.x / 64][1] = last; }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaveCount<NS>; ++w) { first = min(first, ends[w][0]); last = max(last, ends[w][1]); }
+            first = __builtin_amdgcn_readfirstlane(first); last = __builtin_amdgcn_readfirstlane(last);
+        }
     }
     static __device__ __forceinline__ uint64_t bits_of(int from, int to)
     {

@@ -1,14 +1,15 @@
 // Attention's entry points, and the small kernels beside pam_attention_fwd.h and pam_attention_bwd.h: the rows' quantities that the gradients
 // start from, and the chunks' sums put together.
 #include <algorithm>
+#include <cmath>
 
 #include "pam_attention.h"
 
 namespace pamatt {
 
 typedef void (*Kernel)(Args);
-struct Variant { int slices, quads; Kernel kernel; };
-extern const Variant kFwd1[], kFwd2[], kFwd4[], kDqApprox[], kDqExact[], kDkvApprox[], kDkvExact[];
+struct Variant { int slices, quads; bool whole; Kernel kernel; };
+extern const Variant kForward[], kDqApprox[], kDqExact[], kDkvApprox[], kDkvExact[];
 
 }  // namespace pamatt
 
@@ -53,7 +54,7 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
     __shared__ float terms[kThreads / 16][256 + 1];
     const Args& a = r.a;
     const long all = (long)a.batch * a.tokens * a.heads, mine = (long)blockIdx.x * (kThreads / 16) + threadIdx.x / 16, id = min(mine, all - 1);
-    const int lane = threadIdx.x % 16;
+    const int lane = threadIdx.x % 16, last = a.values - 1;
     const long token = id / a.heads, b = token / a.tokens, t = token - b * a.tokens;
     const int head = (int)(id - token * a.heads), kv = head / a.group;
     const long row = t * a.group + head % a.group, to = (b * a.kv_heads + kv) * a.rows + row;
@@ -70,12 +71,12 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
     uint32_t most = 0u;
     for (int d = lane; d < a.dim; d += 16) {
         const bool there = d < a.values;
-        const float g = there ? dy[d] : 0.0f, out = there ? y[d] : 0.0f;
+        const float g = dy[min(d, last)], out = y[min(d, last)];
         // (the sums that y was the quotient of: the same bits as far as they matter to a slope)
         const float sums = whole ? pam_mul(has_off ? pam_mul(out, off) : out, l) : l;
         const float dn = div_grad_a(sums, l, g, a.flags.a, off, has_off);
-        r.qs[to * a.dim + d] = there ? pam_mul_off(q[d], a.scale, off, has_off) : 1.0f;
-        r.dn[to * a.dim + d] = there ? dn : 1.0f;
+        r.qs[to * a.dim + d] = pam_mul_off(q[min(d, last)], a.scale, off, has_off);          // (behind the values the last one again)
+        r.dn[to * a.dim + d] = dn;
         if (!there) continue;
         terms[threadIdx.x / 16][d] = a.flags.b ? -pam_mul_off(pad_div_off(out, l, off, has_off), g, off, has_off) : -(u2f(f2u(out) & ~kMant) / u2f(f2u(l) & kExpo)) * g;
         most = max(most, f2u(dn) & ~kSign);
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
 #pragma unroll 8
         for (int d = lane * r.width; d < end; ++d) dl += terms[threadIdx.x / 16][d];
     }
-    for (int s = 1; s < 4; s *= 2) dl += __shfl_xor(dl, s, 16);
+    for (int s = 1; s < 8; s *= 2) dl += __shfl_xor(dl, s, 16);
     if (lane != 0 || mine >= all) return;
     // a query without a gradient counts as one that sees nothing: it has none to give
     const bool none = !sees || (most == 0u && dl == 0.0f);
@@ -123,27 +124,53 @@ __global__ __launch_bounds__(kThreads) void attention_sum_kernel(Args a, const f
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-const Variant& variant_for(const Variant* list, int values)
+// Of the kernels' instances the one whose slices have just a row's quads, or else the first one wide enough of those that may have more.  (All lists
+// are the same, so that all passes add up a row's products in one order.)
+const Variant& variant_for(const Variant* list, long dim)
 {
-    const Variant* v = list;
-    while (v[1].slices && v->slices * v->quads * 4 < values) ++v;
-    return *v;
+    for (const Variant* v = list; v->slices; ++v)
+        if (v->whole ? 4L * v->slices * v->quads == dim : 4L * v->slices * v->quads >= dim) return *v;
+    return list[0];                               // (no call: rows have up to 256 values)
 }
-const Variant& forward_variant(int values) { return variant_for(values <= 64 ? kFwd1 : values <= 128 ? kFwd2 : kFwd4, values); }
 
-// How the streamed rows are cut.  A chip with 256 compute units has 1024 SIMDs, of which each should have several wavefronts to choose from and
-// to finish at different times: `enough` of them in all.  A chunk is at least two spans.
+// How the streamed rows are cut.  All units of a launch run at once or in a few turns of `slots` of them, so that a last turn of a few units costs as
+// much as a full one: among the cuts that fill one, two, ... turns the one is taken whose turns times its spans are least.  (4096 causal tokens, 8 heads over 2:
+// chunks of 256 keys, two turns and a bit, 0.70 ms.)  Which spans a tile sees is what the order and the window say; prefixes and documents are on the device.
+// A chunk is at least two spans, what a unit does besides its spans counts as a fifth of one.
 struct Plan { int tiles, chunks, chunk; };
-Plan plan_for(long heads, long lanes, int slices, long streamed, long enough)
+long tiles_of(int slices) { return slices >= 4 ? 1 : 4 / slices; }              // of a work-group (kTiles)
+template <class Range>                            // range(first, last row of a tile, low, high): the streamed rows that those see
+Plan plan_for(long heads, long lanes, int slices, long streamed, int waves_per_simd, Range range)
 {
-    const long per_tile = (long)kWaves * (64 / slices), tiles = (lanes + per_tile - 1) / per_tile;
-    const long waves = heads * ((lanes + 64 / slices - 1) / (64 / slices));
-    long chunks = std::max(1L, std::min((enough + waves - 1) / std::max(1L, waves), (streamed + 2 * kSpan - 1) / (2 * kSpan)));
-    const long chunk = ((streamed + chunks - 1) / chunks + kSpan - 1) / kSpan * kSpan;
-    chunks = std::max(1L, (streamed + chunk - 1) / std::max(1L, chunk));
-    return Plan{(int)tiles, (int)chunks, (int)std::max((long)kSpan, chunk)};
+    const long per_tile = 64 * tiles_of(slices), tiles = (lanes + per_tile - 1) / per_tile, spans = std::max(1L, (streamed + kSpan - 1) / kSpan);
+    const long slots = 256L * 4 * waves_per_simd / (slices * tiles_of(slices)), samples = std::min(tiles, 32L);
+    long low[32], high[32], total = 0;            // of tiles evenly spread, in spans
+    for (long n = 0; n < samples; ++n) {
+        const long tile = (2 * n + 1) * tiles / (2 * samples);
+        long from = 0, to = streamed;
+        range(tile * per_tile, std::min(lanes, (tile + 1) * per_tile) - 1, from, to);
+        low[n] = std::max(0L, from) / kSpan; high[n] = std::max(low[n], (std::min(to, streamed) + kSpan - 1) / kSpan);
+        total += high[n] - low[n];
+    }
+    const double each = samples ? (double)heads * tiles / samples : 0.0;
+    double best = 0.0;
+    long chosen = spans;
+    for (int turns = 1; turns <= 6; ++turns) {
+        long size = std::max(2L, (long)(each * total / (turns * slots)));
+        double units = 0.0;
+        for (int tries = 0; tries < 12; ++tries, size += 1 + size / 16) {
+            units = 0.0;
+            for (long n = 0; n < samples; ++n) units += high[n] == low[n] ? 0.0 : (double)((high[n] - 1) / size - low[n] / size + 1);
+            units *= each;
+            if (units <= turns * slots || size >= spans) break;
+        }
+        size = std::min(size, spans);
+        const double cost = std::ceil(units / slots) * (size + 0.2);
+        if (turns == 1 || cost < best * 0.97) { best = cost; chosen = size; }
+        if (size <= 2) break;
+    }
+    return Plan{(int)tiles, (int)((spans + chosen - 1) / chosen), (int)(chosen * kSpan)};
 }
-constexpr long kEnough = 8192;
 
 int check(const char* what, const pam_hip_attention_shape* s, Args& a)
 {
@@ -171,11 +198,11 @@ Tokens tokens_of(const pam_hip_tokens* t) { return Tokens{t->p, t->sb, t->st, t-
 long heads_of(const Args& a) { return (long)a.batch * a.kv_heads; }
 
 // A launch counts its work-items in 32 bits.
-int launch(const char* what, Kernel kernel, const Args& a, hipStream_t st)
+int launch(const char* what, const Variant& v, const Args& a, hipStream_t st)
 {
     const long groups = heads_of(a) * a.tiles * a.chunks;
     if (groups > (1L << 23)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "%s: size out of range", what);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(v.kernel, dim3((unsigned)groups), dim3(64 * v.slices * tiles_of(v.slices)), 0, st, a);
     return pamhost::check_launch(what);
 }
 int groups_for(const char* what, long items, unsigned& groups)
@@ -186,9 +213,34 @@ int groups_for(const char* what, long items, unsigned& groups)
     return PAM_HIP_OK;
 }
 
-Plan forward_plan(const Args& a) { return plan_for(heads_of(a), a.rows, forward_variant(a.values).slices, a.keys, kEnough); }
-Plan dq_plan(const Args& a) { return plan_for(heads_of(a), a.rows, variant_for(kDqApprox, a.values).slices, a.keys, kEnough); }
-Plan dkv_plan(const Args& a) { return plan_for(heads_of(a), a.keys, variant_for(kDkvApprox, a.values).slices, a.rows, kEnough); }
+// What a tile of queries' rows, or of keys, sees.
+struct OfRows {
+    const Args& a;
+    void operator()(long from, long to, long& low, long& high) const
+    {
+        const long first = a.first + from / a.group, last = a.first + to / a.group;
+        if (a.window && !a.prefix) low = first - a.window + 1;
+        if (a.causal) high = last + 1;
+        else if (a.window) high = last + a.window;
+    }
+};
+struct OfKeys {
+    const Args& a;
+    void operator()(long from, long to, long& low, long& high) const
+    {
+        if (a.prefix) return;
+        if (a.causal) low = (from - a.first) * a.group;
+        else if (a.window) low = (from - a.window + 1 - a.first) * a.group;
+        if (a.window) high = (to + a.window - a.first) * a.group;
+    }
+};
+Plan forward_plan(const Args& a)
+{
+    const Variant& v = variant_for(kForward, a.dim);
+    return plan_for(heads_of(a), a.rows, v.slices, a.keys, v.quads > 8 ? 2 : 3, OfRows{a});
+}
+Plan dq_plan(const Args& a) { return plan_for(heads_of(a), a.rows, variant_for(kDqApprox, a.dim).slices, a.keys, 3, OfRows{a}); }
+Plan dkv_plan(const Args& a) { return plan_for(heads_of(a), a.keys, variant_for(kDkvApprox, a.dim).slices, a.rows, 2, OfKeys{a}); }
 
 struct BackwardSpace { size_t records, qs, dn, dq, dk, dv, bytes; };
 BackwardSpace backward_space(const Args& a, bool want_q, bool want_kv)
@@ -238,7 +290,7 @@ int pam_hip_attention_fwd(const pam_hip_attention_shape* shape, const pam_hip_to
     }
     unsigned groups = 0;
     rc = groups_for("attention_fwd", heads_of(a) * a.rows * (a.dim / 4), groups);
-    if (rc == PAM_HIP_OK) rc = launch("attention_fwd", forward_variant(a.values).kernel, a, st);
+    if (rc == PAM_HIP_OK) rc = launch("attention_fwd", variant_for(kForward, a.dim), a, st);
     if (rc != PAM_HIP_OK || !need) return rc;
     hipLaunchKernelGGL(attention_join_kernel, dim3(groups), dim3(kThreads), 0, st, a);
     return pamhost::check_launch("attention_fwd");
@@ -274,8 +326,8 @@ int pam_hip_attention_bwd(const pam_hip_attention_shape* shape, const pam_hip_to
     if ((rc = groups_for("attention_bwd", heads_of(a) * a.rows * 16, groups)) || (rc = groups_for("attention_bwd", heads_of(a) * a.rows * (a.dim / 4), row_groups))
         || (rc = groups_for("attention_bwd", heads_of(a) * a.keys * (a.dim / 4), key_groups))) return rc;
     if (a.rows) {
-        const RowArgs r{a, y, tokens_of(dy), reinterpret_cast<const float2*>(stats), (float4*)(ws + space.records), (float*)(ws + space.qs), (float*)(ws + space.dn), variant_for(kDqApprox, a.values).slices,
-                        4 * variant_for(kDqApprox, a.values).quads};
+        const RowArgs r{a, y, tokens_of(dy), reinterpret_cast<const float2*>(stats), (float4*)(ws + space.records), (float*)(ws + space.qs), (float*)(ws + space.dn), variant_for(kDqApprox, a.dim).slices,
+                        4 * variant_for(kDqApprox, a.dim).quads};
         hipLaunchKernelGGL(attention_rows_kernel, dim3(groups), dim3(kThreads), 0, st, r);
         if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
     }
@@ -283,7 +335,7 @@ int pam_hip_attention_bwd(const pam_hip_attention_shape* shape, const pam_hip_to
         Args d = a;
         const Plan p = dq_plan(a);
         d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.out0 = (float*)(ws + space.dq);
-        if ((rc = launch("attention_bwd", variant_for(approximate ? kDqApprox : kDqExact, a.values).kernel, d, st))) return rc;
+        if ((rc = launch("attention_bwd", variant_for(approximate ? kDqApprox : kDqExact, a.dim), d, st))) return rc;
         hipLaunchKernelGGL(attention_sum_kernel, dim3(row_groups), dim3(kThreads), 0, st, d, d.out0, dq, 0);
         if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
     }
@@ -291,7 +343,7 @@ int pam_hip_attention_bwd(const pam_hip_attention_shape* shape, const pam_hip_to
         Args d = a;
         const Plan p = dkv_plan(a);
         d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.out0 = (float*)(ws + space.dk); d.out1 = (float*)(ws + space.dv);
-        if ((rc = launch("attention_bwd", variant_for(approximate ? kDkvApprox : kDkvExact, a.values).kernel, d, st))) return rc;
+        if ((rc = launch("attention_bwd", variant_for(approximate ? kDkvApprox : kDkvExact, a.dim), d, st))) return rc;
         hipLaunchKernelGGL(attention_sum_kernel, dim3(key_groups), dim3(kThreads), 0, st, d, d.out0, dk, 1);
         hipLaunchKernelGGL(attention_sum_kernel, dim3(key_groups), dim3(kThreads), 0, st, d, d.out1, dv, 1);
         if ((rc = pamhost::check_launch("attention_bwd"))) return rc;

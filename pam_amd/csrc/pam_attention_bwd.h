@@ -54,141 +54,221 @@ struct PairGrad {
 __device__ __forceinline__ float exact_term(const Full& f, float own, float other, float delta)
 { return pam_mul_bwd(own, other, delta, f.off, f.has_off); }
 
-template <int NS, int W4, bool APPROXIMATE>
-__global__ __launch_bounds__(kThreads, W4 > 12 ? 1 : 2) void attention_dq_kernel(Args a)
+// The usual way's sums of slopes are kept times the own factor's power until the end.
+constexpr uint32_t kPower = ~kMant;
+__device__ __forceinline__ float over_power(float sum, uint32_t own) { return sum * u2f((2u * kBias - (own & kExpo)) | (own & kSign)); }
+
+// The slopes of a row that lanes hold a quad each of, by the full definition.
+template <int W4, class F> __device__ __forceinline__ void each_of_row(const v4f& row, F&& f)
 {
-    constexpr int kRows = 64 / NS, W = 4 * W4;
-    const Place<NS, W4> here(a.values);
+    each<0, W4>([&](auto n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f(4 * n.value + i, u2f(from_lane<decltype(n)::value>(row[i])));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    });
+}
+
+// All blocks of a chunk of streamed rows, sums joined in memory after kLink of them; false: one block did not want to.
+template <int NS, int W4, int SUMS, class Start, class Block>
+__device__ __forceinline__ bool all_blocks(const Sight& sight, int begin, int end, float* const (&to)[SUMS], int first, int dim, bool exists, float (&out)[SUMS][4 * W4], Start&& start,
+                                           Block&& block)
+{
+    bool folded = false;
+    int terms = 0;
+#pragma unroll
+    for (int n = 0; n < SUMS; ++n)
+#pragma unroll
+        for (int d = 0; d < 4 * W4; ++d) out[n][d] = 0.0f;
+    const auto with_memory = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < SUMS; ++n)
+            row_in_memory<W4>(to[n], first, dim, exists, [&](int quad, v4f& x) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { float in_memory = x[i]; f(in_memory, out[n][4 * quad + i]); x[i] = in_memory; }
+            });
+    };
+#pragma unroll 1
+    for (int j0 = begin; j0 < end; j0 += kSpan) {
+        const uint64_t see = sight.span(j0);
+        if (!in_team<NS>(see != 0ull)) continue;
+        const bool all = __ballot(see != ~0ull) == 0ull;
+        if (terms >= kLink) {
+            with_memory([&](float& in_memory, float& sum) __attribute__((always_inline)) { in_memory = (folded ? in_memory : 0.0f) + sum; sum = 0.0f; });
+            folded = true; terms = 0;
+        }
+        terms += kSpan;
+        start(j0);
+#pragma unroll 1
+        for (int i0 = 0; i0 < kSpan; i0 += kBlock)
+            if (!block(j0 + i0, (uint32_t)(see >> i0) & 0xffu, all)) return false;
+    }
+    if (folded) with_memory([&](float& in_memory, float& sum) __attribute__((always_inline)) { sum += in_memory; });
+    return true;
+}
+
+template <int NS, int W4, bool WHOLE, bool APPROXIMATE>
+__global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Args a)
+{
+    constexpr int W = 4 * W4, N = 4 * Pipe<W4, WHOLE>::kQuads;
+    __shared__ Slices<NS, kBlock> slices_s, slices_de;
     const Unit u = unit_of(a);
-    const int row0 = (u.tile * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * kRows;
-    if (row0 >= a.rows) return;
-    const int mine = row0 + here.row_in_wave, row = min(mine, a.rows - 1), first = here.slice * W;
+    const int wave = wave_of(), slice = wave % NS, row0 = (u.tile * kTiles<NS> + wave / NS) * 64, mine = row0 + (int)threadIdx.x % 64, row = min(mine, a.rows - 1), first = slice * W;
     const bool exists = mine < a.rows;
     const int pos = a.first + row / a.group;
     const Scoring scoring(a);
     const PairGrad<APPROXIMATE> pair{scoring, a.flags};
-    const Full full{a.off, a.off != 1.0f, 0u - scoring.mul_add, lane_pad(0u)};
+    const uint32_t dn_add = APPROXIMATE ? scoring.mul_add : 0u;
+    const Full full{a.off, a.off != 1.0f, 0u - scoring.mul_add}, full_dn{a.off, a.off != 1.0f, 0u - dn_add};
     const float4 record = a.records[(long)u.head * a.rows + row];
     const float M = record.x, unit = u2f((uint32_t)(127 - (int)record.z) << 23), dl = record.y * unit, slope = record.w;
     uint32_t q[W], dn[W];
     const long at = ((long)u.head * a.rows + row) * a.dim;
-    bool odd = !load_lane<W4>(a.qs + at, first, a.dim, a.values, 0u, scoring.mul_add, lane_pad(0u), q);
-    odd = !load_lane<W4>(a.dn + at, first, a.dim, a.values, 0u - ((uint32_t)(int)record.z << 23), scoring.mul_add, lane_pad(0u), dn) || odd;
+    bool odd = !load_lane<W4>(a.qs + at, first, a.dim, a.values, 0u, scoring.mul_add, q);
+    odd = !load_lane<W4>(a.dn + at, first, a.dim, a.values, 0u - ((uint32_t)(int)record.z << 23), dn_add, dn) || odd;
     odd = odd || !finite(dl);
-    const bool careful_lanes = __ballot(odd && M != u2f(kExpo)) != 0ull;
+    // (all slopes, and no offset: what the usual way of the other kernel has)
+    const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
+    bool careful = in_team<NS>(odd && M != u2f(kExpo)) || unusual;
     Sight sight = sight_of_row(a, u.b, row);
-    const Stream keys = stream_of(here, a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.values, a.keys);
-    const Stream values = stream_of(here, a.v.p + (long)u.b * a.v.sb + (long)u.kv * a.v.sh, a.v.st, a.values, a.keys);
-    float out[W];
-#pragma unroll
-    for (int d = 0; d < W; ++d) out[d] = 0.0f;
-    float* const to = a.out0 + (((long)u.head * a.chunks + u.chunk) * a.rows + row) * a.dim;
-    bool folded = false;
-    int terms = 0;
+    sight.close_team<NS>();
+    const Stream<WHOLE> keys(a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.keys, slice * W4, a.dim / 4);
+    const Stream<WHOLE> values(a.v.p + (long)u.b * a.v.sb + (long)u.kv * a.v.sh, a.v.st, a.keys, slice * W4, a.dim / 4);
+    float out[1][W];
+    float* const to[1] = {a.out0 + (((long)u.head * a.chunks + u.chunk) * a.rows + row) * a.dim};
     const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
-#pragma unroll 1
-    for (int j0 = begin; j0 < end; j0 += kSpan) {
-        const uint64_t see = sight.span(j0);
-        if (__ballot(see != 0ull) == 0ull) continue;
-        const bool all = __ballot(see != ~0ull) == 0ull;
-        if (terms >= kLink) {
-            row_in_memory<W4>(to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
+    int turn = 0;
+    // weights from scores, and which ones count (what is no number does)
+    const auto weigh = [&](const float (&s)[kBlock], float (&e)[kBlock], uint32_t sees, bool all, int j1, bool& wrong) __attribute__((always_inline)) {
+        uint32_t counts = 0u;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = (folded ? x[i] : 0.0f) + out[4 * n + i];
+        for (int j = 0; j < kBlock; ++j) {
+            float power = scoring.exponent(s[j], slope, pos - (j1 + j)) - M;
+            if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
+            wrong = wrong || power != power;
+            counts |= power < kLeast ? 0u : 1u << j;
+            e[j] = power_of_two(fminf(fmaxf(power, kLeast), 60.0f));
+            e[j] = power != power ? power : e[j];
+        }
+        return counts;
+    };
+    bool gave_up = false;                         // (what all of a tile's slices find behind the sums goes with the next ones)
+    const auto skip = [&](float (&s)[kBlock], float (&de)[kBlock]) __attribute__((always_inline)) {      // (no row of the tile sees the block: its barriers)
+        const bool wild = slices_s.add_up(turn, wave, s, gave_up);
+        if (wild) { turn ^= 1; return false; }
+        slices_de.add_up(turn, wave, de, false);
+        turn ^= 1;
+        return true;
+    };
+    const auto score_gradient = [&](float s, float e, float de, int far) __attribute__((always_inline)) {
+        float x = s;
+        if (!APPROXIMATE && !a.flags.e) {                          // (the score as log2 e multiplies it)
+            x = scoring.cap != 0.0f ? scoring.capped(x) : x;
+            if (scoring.slopes) x = scoring.biased(x, slope, far);
+        }
+        return pair.checked(s, x, e, de + dl);
+    };
+    if (!careful) {
+        Pipe<W4, WHOLE> pipe;
+        Look<W4, WHOLE> look_k, look_v;
+        careful = !all_blocks<NS, W4, 1>(sight, begin, end, to, first, a.dim, exists, out,
+            [&](int j0) __attribute__((always_inline)) { pipe.request(keys, j0); look_k.load(keys, j0); look_v.load(values, j0); },
+            [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
+                float s[kBlock], de[kBlock], e[kBlock];
+                if (!all && __ballot(sees != 0u) == 0ull) {
+                    pipe.request(keys, j1 + kBlock); look_k.load(keys, j1 + kBlock); look_v.load(values, j1 + kBlock);
+                    return skip(s, de);
+                }
+                const Verdict kv = judge(look_k, keys, a.values, 0u), vv = judge(look_v, values, a.values, 0u);
+                look_k.load(keys, j1 + kBlock);
+                look_v.load(values, j1 + kBlock);
+                bool wrong = false;
+                block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, APPROXIMATE && kv.zeros, q, s);
+                bool wild = slices_s.add_up(turn, wave, s, gave_up || kv.wild || vv.wild || (!APPROXIMATE && (kv.zeros || vv.zeros)));
+                if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
+                uint32_t counts = weigh(s, e, sees, all, j1, wrong);
+                if constexpr (APPROXIMATE) block_dots<W4, WHOLE>(pipe, values, j1, keys, j1, vv.zeros, dn, de);
+                else {
+#pragma unroll
+                    for (int j = 0; j < kBlock; ++j) de[j] = 0.0f;
+                    pipe.block(values, j1, keys, j1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+                        dot_power_piece<N>(x, f2u(e[j]) + scoring.mul_add, counts >> j & 1u ? kPower : 0u, dn + d, de[j]);
+                    });
+#pragma unroll
+                    for (int j = 0; j < kBlock; ++j) de[j] = over_power(de[j], f2u(e[j]));
+                }
+                slices_de.add_up(turn, wave, de, false);
+                turn ^= 1;
+#pragma unroll
+                for (int j = 0; j < kBlock; ++j) {
+                    de[j] = score_gradient(s[j], e[j], de[j], pos - (j1 + j));
+                    if (APPROXIMATE) {
+                        // (less than 2^-86 is nothing beside |dn| of 1 and values of at least 2^-40)
+                        wrong = wrong || ((counts >> j) & 1u && !(fabsf(de[j]) < 0x1p80f));
+                        counts &= fabsf(de[j]) < 0x1p-86f ? ~(1u << j) : ~0u;
+                    }
+                }
+                gave_up = gave_up || __ballot(wrong) != 0ull;
+                if (NS == 1 && __builtin_expect(gave_up, 0)) return false;
+                if constexpr (APPROXIMATE) block_add<W4, WHOLE>(pipe, keys, j1, keys, j1 + kBlock, kv.zeros, de, scoring.mul_add, counts, out[0]);
+                else
+                    pipe.block(keys, j1, keys, j1 + kBlock, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+                        const bool in = counts >> j & 1u;
+                        add_power_piece<N>(x, in ? de[j] : 0.0f, in ? kPower : 0u, q + d, out[0] + d);
+                    });
+                return true;
             });
+        careful = careful || in_team<NS>(gave_up);
+        if (!APPROXIMATE)
 #pragma unroll
-            for (int d = 0; d < W; ++d) out[d] = 0.0f;
-            folded = true; terms = 0;
-        }
-        terms += kSpan;
-        v4f kr[kBlock], vr[kBlock];
-#pragma unroll 1
-        for (int i0 = 0; i0 < kSpan; i0 += kBlock) {
-            const uint32_t sees = (uint32_t)(see >> i0) & 0xffu;
-            if (!all && __ballot(sees != 0u) == 0ull) continue;
-            keys.rows(j0 + i0, kr);
-            values.rows(j0 + i0, vr);
-            keys.pad(0u, kr);
-            const Verdict kv = judge(here.streaming, 0u, kr);
-            float s[kBlock], de[kBlock], e[kBlock];
-            block_dots<NS, W4>(full, careful_lanes || kv.careful, kv.zero, 1.0f, kr, q, s);
-            uint32_t counts = 0u;
-            bool wrong = false;
-#pragma unroll
-            for (int j = 0; j < kBlock; ++j) {
-                float power = scoring.exponent(s[j], slope, pos - (j0 + i0 + j)) - M;
-                if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
-                wrong = wrong || power != power;
-                counts |= power < kLeast ? 0u : 1u << j;          // (what is no number counts)
-                e[j] = power_of_two(fminf(fmaxf(power, kLeast), 60.0f));
-                e[j] = power != power ? power : e[j];
-            }
-            values.pad(0u, vr);
-            const Verdict vv = judge(here.streaming, 0u, vr);
-            if (APPROXIMATE || a.flags.a) {
-                block_dots<NS, W4>(full, careful_lanes || vv.careful, vv.zero, 1.0f, vr, dn, de);
-            } else {
-#pragma unroll 1
-                for (int j = 0; j < kBlock; ++j) {
-                    float sum = 0.0f;
-                    each<0, W4>([&](auto n) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t m = (uint32_t)anew((int)dn[4 * n.value + i]);
-                            const bool is_zero = m - scoring.mul_add == kStandIn;
-                            const float term = exact_term(full, e[0], u2f(from_lane<decltype(n)::value>(vr[0][i])), m == full.pad || is_zero ? 0.0f : u2f(m + full.raw));
-                            sum += term;
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    });
-                    de[0] = (vv.zero >> j) & 1u ? 0.0f : over_slices<NS>(sum);
-                    turned(vr); turned(e); turned(de);
-                }
-            }
-            const bool small = careful_lanes || vv.careful;
-#pragma unroll
-            for (int j = 0; j < kBlock; ++j) {
-                float x = s[j];
-                if (!APPROXIMATE && !a.flags.e) {                  // (the score as log2 e multiplies it)
-                    x = scoring.cap != 0.0f ? scoring.capped(x) : x;
-                    if (scoring.slopes) x = scoring.biased(x, slope, pos - (j0 + i0 + j));
-                }
-                de[j] = pair.checked(s[j], x, e[j], de[j] + dl);
-                // (less than 2^-86 is nothing beside |dn| of 1 and values of at least 2^-40; with smaller ones it may be all there is)
-                const bool tiny = fabsf(de[j]) < 0x1p-86f;
-                wrong = wrong || ((counts >> j) & 1u && (!(fabsf(de[j]) < 0x1p80f) || (small && tiny)));
-                counts &= tiny && !small ? ~(1u << j) : ~0u;
-            }
-            const bool careful = careful_lanes || kv.careful || __ballot(wrong) != 0ull;
-            if (APPROXIMATE || a.flags.a) {
-                block_add<W4>(full, careful, kv.zero, 1.0f, kr, de, scoring.mul_add, counts, out);
-            } else {
-#pragma unroll 1
-                for (int j = 0; j < kBlock; ++j) {
-                    const bool in = ((counts & ~kv.zero) >> j) & 1u;
-                    each<0, W4>([&](auto n) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t m = (uint32_t)anew((int)q[4 * n.value + i]);
-                            const float term = exact_term(full, m == full.pad ? 1.0f : u2f(m + full.raw), u2f(from_lane<decltype(n)::value>(kr[0][i])), de[0]);
-                            out[4 * n.value + i] += in ? term : 0.0f;
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    });
-                    turned(kr); turned(de);
-                }
-            }
-        }
+            for (int d = 0; d < W; ++d) out[0][d] = over_power(out[0][d], q[d] + full.raw);
     }
-    if (folded)
-        row_in_memory<W4>(to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
+    gave_up = false;
+    if (__builtin_expect(careful, 0))
+        all_blocks<NS, W4, 1>(sight, begin, end, to, first, a.dim, exists, out, [](int) {}, [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
+            float s[kBlock], de[kBlock], e[kBlock];
+            if (!all && __ballot(sees != 0u) == 0ull) { skip(s, de); return true; }
+            bool wrong = false;
+#pragma unroll 1
+            for (int j = 0; j < kBlock; ++j) {
+                s[0] = careful_dot<W4>(full, keys.template across<W4>(j1 + j), q);
+                turned(s);
+            }
+            slices_s.add_up(turn, wave, s, false);
+            const uint32_t counts = weigh(s, e, sees, all, j1, wrong);
+#pragma unroll 1
+            for (int j = 0; j < kBlock; ++j) {
+                const v4f row = values.template across<W4>(j1 + j);
+                if (APPROXIMATE || a.flags.a) de[0] = careful_dot<W4>(full_dn, row, dn);
+                else {
+                    de[0] = 0.0f;
+                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) { de[0] += exact_term(full, e[0], x, u2f(real_bits(full_dn, dn[d]))); });
+                }
+                turned(de); turned(e);
+            }
+            slices_de.add_up(turn, wave, de, false);
+            turn ^= 1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[4 * n + i] += x[i];
+            for (int j = 0; j < kBlock; ++j) de[j] = score_gradient(s[j], e[j], de[j], pos - (j1 + j));
+#pragma unroll 1
+            for (int j = 0; j < kBlock; ++j) {
+                const v4f row = keys.template across<W4>(j1 + j);
+                const bool in = (counts >> j) & 1u;
+                if (APPROXIMATE || a.flags.a) careful_add_row<W4>(full, row, de[0], in, 1.0f, out[0]);
+                else
+                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) {
+                        const float term = exact_term(full, u2f(real_bits(full, q[d])), x, de[0]);
+                        out[0][d] += in ? term : 0.0f;
+                    });
+                turned(de);
+            }
+            return true;
         });
     const float back = 1.0f / unit;
 #pragma unroll
-    for (int d = 0; d < W; ++d) out[d] *= back;
-    store_row<W4>(to, first, a.dim, exists, out);
+    for (int d = 0; d < W; ++d) out[0][d] *= back;
+    store_row<W4>(to[0], first, a.dim, exists, out[0]);
 }
 
 // What a key's lane sees: the rows of its head's queries.
@@ -207,186 +287,199 @@ __device__ __forceinline__ Sight sight_of_key(const Args& a, int b, int key)
     return s;
 }
 
-template <int NS, int W4, bool APPROXIMATE>
-__global__ __launch_bounds__(kThreads, W4 > 8 ? 1 : 2) void attention_dkv_kernel(Args a)
+
+template <int NS, int W4, bool WHOLE, bool APPROXIMATE>
+__global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(Args a)
 {
-    constexpr int kRows = 64 / NS, W = 4 * W4;
-    const Place<NS, W4> here(a.values);
+    constexpr int W = 4 * W4, N = 4 * Pipe<W4, WHOLE>::kQuads;
+    __shared__ Slices<NS, kBlock> slices_s, slices_de;
     Unit u = unit_of(a);
     u.tile = a.tiles - 1 - u.tile;                // (the first keys have most queries where the order is causal)
-    const int key0 = (u.tile * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * kRows;
-    if (key0 >= a.keys) return;
-    const int mine = key0 + here.row_in_wave, key = min(mine, a.keys - 1), first = here.slice * W;
+    const int wave = wave_of(), slice = wave % NS, lane = (int)threadIdx.x % 64, key0 = (u.tile * kTiles<NS> + wave / NS) * 64, mine = key0 + lane, key = min(mine, a.keys - 1), first = slice * W;
     const bool exists = mine < a.keys;
     const Scoring scoring(a);
     const PairGrad<APPROXIMATE> pair{scoring, a.flags};
     typedef const __attribute__((address_space(4))) float4* Records;
     const float4* const all_records = a.records + (long)u.head * a.rows;
+    const auto record = [&](int r) __attribute__((always_inline)) { const Records from = (Records)(all_records + min(r, a.rows - 1)); return make_float4(from->x, from->y, from->z, from->w); };
     const int chunk_begin = u.chunk * a.chunk, chunk_end = min(a.rows, chunk_begin + a.chunk);
     // the largest |dn| of the chunk's rows is scaled to [1, 2)
     int most = -86;
-    for (int r = chunk_begin + here.lane; r < chunk_end; r += 64) most = max(most, (int)all_records[r].z);
+    for (int r = chunk_begin + lane; r < chunk_end; r += 64) most = max(most, (int)all_records[r].z);
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) most = max(most, __shfl_xor(most, s, 64));
-    most = __builtin_amdgcn_readfirstlane(most);
+    most = APPROXIMATE ? __builtin_amdgcn_readfirstlane(most) : 0;
     const uint32_t shift = 0u - ((uint32_t)most << 23);
     const float unit = u2f((uint32_t)(127 - most) << 23);
-    const Full full_q{a.off, a.off != 1.0f, 0u - scoring.mul_add, lane_pad(0u)}, full_n{a.off, a.off != 1.0f, 0u - scoring.mul_add - shift, lane_pad(shift)};
+    const Full full_q{a.off, a.off != 1.0f, 0u - scoring.mul_add}, full_n{a.off, a.off != 1.0f, 0u - scoring.mul_add - shift};
     uint32_t k[W], v[W];
-    bool odd = !load_lane<W4>(a.k.p + (long)u.b * a.k.sb + (long)key * a.k.st + (long)u.kv * a.k.sh, first, a.dim, a.values, 0u, scoring.mul_add, lane_pad(0u), k);
-    odd = !load_lane<W4>(a.v.p + (long)u.b * a.v.sb + (long)key * a.v.st + (long)u.kv * a.v.sh, first, a.dim, a.values, 0u, scoring.mul_add + shift, lane_pad(shift), v) || odd;
-    const bool careful_lanes = __ballot(odd) != 0ull;
+    bool odd = !load_lane<W4>(a.k.p + (long)u.b * a.k.sb + (long)key * a.k.st + (long)u.kv * a.k.sh, first, a.dim, a.values, 0u, scoring.mul_add, k);
+    odd = !load_lane<W4>(a.v.p + (long)u.b * a.v.sb + (long)key * a.v.st + (long)u.kv * a.v.sh, first, a.dim, a.values, 0u, scoring.mul_add + shift, v) || odd;
+    const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
+    bool careful = in_team<NS>(odd) || unusual;
     Sight sight = sight_of_key(a, u.b, key);
-    const Stream queries = stream_of(here, a.qs + (long)u.head * a.rows * a.dim, a.dim, a.values, a.rows);
-    const Stream grads = stream_of(here, a.dn + (long)u.head * a.rows * a.dim, a.dim, a.values, a.rows);
-    float dk[W], dv[W];
-#pragma unroll
-    for (int d = 0; d < W; ++d) dk[d] = dv[d] = 0.0f;
-    const long to = (((long)u.head * a.chunks + u.chunk) * a.keys + key) * a.dim;
-    bool folded = false;
-    int terms = 0;
+    sight.close_team<NS>();
+    const Stream<WHOLE> queries(a.qs + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);
+    const Stream<WHOLE> grads(a.dn + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);
+    float out[2][W];                              // dk, dv
+    const long at = (((long)u.head * a.chunks + u.chunk) * a.keys + key) * a.dim;
+    float* const to[2] = {a.out0 + at, a.out1 + at};
     const int begin = max(sight.first / kSpan * kSpan, chunk_begin), end = min(min(sight.last, a.rows), chunk_begin + a.chunk);
-#pragma unroll 1
-    for (int r0 = begin; r0 < end; r0 += kSpan) {
-        const uint64_t see = sight.span(r0);
-        if (__ballot(see != 0ull) == 0ull) continue;
-        const bool all = __ballot(see != ~0ull) == 0ull;
-        if (terms >= kLink) {
-            row_in_memory<W4>(a.out0 + to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
+    int turn = 0;
+    const auto weigh = [&](const float (&s)[kBlock], float (&e)[kBlock], uint32_t sees, bool all, int r1, bool& wrong) __attribute__((always_inline)) {
+        uint32_t counts = 0u;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = (folded ? x[i] : 0.0f) + dk[4 * n + i];
-            });
-            row_in_memory<W4>(a.out1 + to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = (folded ? x[i] : 0.0f) + dv[4 * n + i];
-            });
-#pragma unroll
-            for (int d = 0; d < W; ++d) dk[d] = dv[d] = 0.0f;
-            folded = true; terms = 0;
+        for (int j = 0; j < kBlock; ++j) {
+            const float4 of = record(r1 + j);
+            float power = scoring.exponent(s[j], of.w, a.first + (r1 + j) / a.group - key) - of.x;
+            if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
+            wrong = wrong || power != power;
+            counts |= power < kLeast ? 0u : 1u << j;
+            e[j] = power_of_two(fminf(fmaxf(power, kLeast), 60.0f));
+            e[j] = power != power ? power : e[j];
         }
-        terms += kSpan;
-        v4f qr[kBlock], nr[kBlock];
-#pragma unroll 1
-        for (int i0 = 0; i0 < kSpan; i0 += kBlock) {
-            const uint32_t sees = (uint32_t)(see >> i0) & 0xffu;
-            if (!all && __ballot(sees != 0u) == 0ull) continue;
-            queries.rows(r0 + i0, qr);
-            grads.rows(r0 + i0, nr);
-            float4 record[kBlock];
+        return counts;
+    };
+    bool gave_up = false;                         // (what all of a tile's slices find behind the sums goes with the next ones)
+    const auto skip = [&](float (&s)[kBlock], float (&de)[kBlock]) __attribute__((always_inline)) {      // (no row of the tile sees the block: its barriers)
+        const bool wild = slices_s.add_up(turn, wave, s, gave_up);
+        if (wild) { turn ^= 1; return false; }
+        slices_de.add_up(turn, wave, de, false);
+        turn ^= 1;
+        return true;
+    };
+    const auto score_gradient = [&](float s, float e, float de, int r) __attribute__((always_inline)) {
+        const float4 of = record(r);
+        float x = s;
+        if (!APPROXIMATE && !a.flags.e) {
+            x = scoring.cap != 0.0f ? scoring.capped(x) : x;
+            if (scoring.slopes) x = scoring.biased(x, of.w, a.first + r / a.group - key);
+        }
+        return pair.checked(s, x, e, de + of.y * unit);
+    };
+    if (!careful) {
+        Pipe<W4, WHOLE> pipe;
+        Look<W4, WHOLE> look_q, look_n;
+        careful = !all_blocks<NS, W4, 2>(sight, begin, end, to, first, a.dim, exists, out,
+            [&](int r0) __attribute__((always_inline)) { pipe.request(queries, r0); look_q.load(queries, r0); look_n.load(grads, r0); },
+            [&](int r1, uint32_t sees, bool all) __attribute__((always_inline)) {
+                float s[kBlock], de[kBlock], e[kBlock];
+                if (!all && __ballot(sees != 0u) == 0ull) {
+                    pipe.request(queries, r1 + kBlock); look_q.load(queries, r1 + kBlock); look_n.load(grads, r1 + kBlock);
+                    return skip(s, de);
+                }
+                const Verdict qv = judge(look_q, queries, a.values, 0u);
+                Verdict nv{false, false};
+                if (APPROXIMATE) nv = judge(look_n, grads, a.values, shift);
+                else nv.wild = !all_finite(look_n, grads, a.values);
+                look_q.load(queries, r1 + kBlock);
+                look_n.load(grads, r1 + kBlock);
+                bool wrong = false;
+                block_dots<W4, WHOLE>(pipe, queries, r1, grads, r1, APPROXIMATE && qv.zeros, k, s);
+                const bool wild = slices_s.add_up(turn, wave, s, gave_up || qv.wild || nv.wild || (!APPROXIMATE && qv.zeros));
+                if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
+                uint32_t counts = weigh(s, e, sees, all, r1, wrong);
+                if constexpr (APPROXIMATE) block_dots<W4, WHOLE>(pipe, grads, r1, grads, r1, nv.zeros, v, de);
+                else {
 #pragma unroll
-            for (int j = 0; j < kBlock; ++j) {
-                const Records from = (Records)(all_records + min(r0 + i0 + j, a.rows - 1));
-                record[j] = make_float4(from->x, from->y, from->z, from->w);
-            }
-            queries.pad(0u, qr);
-            const Verdict qv = judge(here.streaming, 0u, qr);
+                    for (int j = 0; j < kBlock; ++j) de[j] = 0.0f;
+                    pipe.block(grads, r1, grads, r1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+                        dot_lane_power_piece<N>(x, f2u(e[j]), counts >> j & 1u ? kPower : 0u, v + d, de[j]);
+                    });
+#pragma unroll
+                    for (int j = 0; j < kBlock; ++j) de[j] = over_power(de[j], f2u(e[j]));
+                }
+                slices_de.add_up(turn, wave, de, false);
+                turn ^= 1;
+                const uint32_t counts_e = counts;
+#pragma unroll
+                for (int j = 0; j < kBlock; ++j) {
+                    de[j] = score_gradient(s[j], e[j], de[j], r1 + j);
+                    if (APPROXIMATE) {
+                        wrong = wrong || ((counts >> j) & 1u && !(fabsf(de[j]) < 0x1p80f));
+                        counts &= fabsf(de[j]) < 0x1p-86f ? ~(1u << j) : ~0u;
+                    }
+                }
+                gave_up = gave_up || __ballot(wrong) != 0ull;
+                if (NS == 1 && __builtin_expect(gave_up, 0)) return false;
+                // dv: e (*) dn, dk: da (*) qs
+                if constexpr (APPROXIMATE) {
+                    block_add<W4, WHOLE>(pipe, grads, r1, queries, r1, nv.zeros, e, scoring.mul_add + shift, counts_e, out[1]);
+                    block_add<W4, WHOLE>(pipe, queries, r1, queries, r1 + kBlock, qv.zeros, de, scoring.mul_add, counts, out[0]);
+                } else {
+                    pipe.block(grads, r1, queries, r1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+                        add_lane_power_piece<N>(x, f2u(e[j]), counts_e >> j & 1u ? kPower : 0u, v + d, out[1] + d);
+                    });
+                    pipe.block(queries, r1, queries, r1 + kBlock, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+                        const bool in = counts >> j & 1u;
+                        add_power_piece<N>(x, in ? de[j] : 0.0f, in ? kPower : 0u, k + d, out[0] + d);
+                    });
+                }
+                return true;
+            });
+        careful = careful || in_team<NS>(gave_up);
+        if (!APPROXIMATE)
+#pragma unroll
+            for (int d = 0; d < W; ++d) { out[0][d] = over_power(out[0][d], k[d] + full_q.raw); out[1][d] = over_power(out[1][d], v[d] + full_n.raw); }
+    }
+    gave_up = false;
+    if (__builtin_expect(careful, 0))
+        all_blocks<NS, W4, 2>(sight, begin, end, to, first, a.dim, exists, out, [](int) {}, [&](int r1, uint32_t sees, bool all) __attribute__((always_inline)) {
             float s[kBlock], de[kBlock], e[kBlock];
-            block_dots<NS, W4>(full_q, careful_lanes || qv.careful, qv.zero, 1.0f, qr, k, s);
-            uint32_t counts = 0u;
+            if (!all && __ballot(sees != 0u) == 0ull) { skip(s, de); return true; }
             bool wrong = false;
-#pragma unroll
+#pragma unroll 1
             for (int j = 0; j < kBlock; ++j) {
-                const int pos = a.first + (r0 + i0 + j) / a.group;
-                float power = scoring.exponent(s[j], record[j].w, pos - key) - record[j].x;
-                if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
-                wrong = wrong || power != power;
-                counts |= power < kLeast ? 0u : 1u << j;
-                e[j] = power_of_two(fminf(fmaxf(power, kLeast), 60.0f));
-                e[j] = power != power ? power : e[j];
+                s[0] = careful_dot<W4>(full_q, queries.template across<W4>(r1 + j), k);
+                turned(s);
             }
-            grads.pad(shift, nr);
-            const Verdict nv = judge(here.streaming, shift, nr);
-            const bool weights_wrong = __ballot(wrong) != 0ull;
-            if (APPROXIMATE || a.flags.a) {
-                block_dots<NS, W4>(full_n, careful_lanes || nv.careful, nv.zero, unit, nr, v, de);
-            } else {
+            slices_s.add_up(turn, wave, s, false);
+            const uint32_t counts = weigh(s, e, sees, all, r1, wrong);
 #pragma unroll 1
-                for (int j = 0; j < kBlock; ++j) {
-                    float sum = 0.0f;
-                    each<0, W4>([&](auto n) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t m = (uint32_t)anew((int)v[4 * n.value + i]);
-                            const float other = m == full_n.pad || m - scoring.mul_add - shift == kStandIn ? 0.0f : u2f(m + full_n.raw);
-                            sum += exact_term(full_n, e[0], other, u2f(from_lane<decltype(n)::value>(nr[0][i])) * unit);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    });
-                    de[0] = (nv.zero >> j) & 1u ? 0.0f : over_slices<NS>(sum);
-                    turned(nr); turned(e); turned(de);
-                }
-            }
-            // dv: e (*) dn
-            if (APPROXIMATE || a.flags.b) {
-                block_add<W4>(full_n, careful_lanes || nv.careful || weights_wrong, nv.zero, unit, nr, e, scoring.mul_add + shift, counts, dv);
-            } else {
-#pragma unroll 1
-                for (int j = 0; j < kBlock; ++j) {
-                    const bool in = ((counts & ~nv.zero) >> j) & 1u;
-                    each<0, W4>([&](auto n) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t m = (uint32_t)anew((int)v[4 * n.value + i]);
-                            const float own = m == full_n.pad ? 1.0f : u2f(m + full_n.raw);
-                            const float term = exact_term(full_n, own, e[0], u2f(from_lane<decltype(n)::value>(nr[0][i])) * unit);
-                            dv[4 * n.value + i] += in ? term : 0.0f;
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    });
-                    turned(nr); turned(e);
-                }
-            }
-            const bool small = careful_lanes || nv.careful;
-#pragma unroll
             for (int j = 0; j < kBlock; ++j) {
-                float x = s[j];
-                if (!APPROXIMATE && !a.flags.e) {
-                    x = scoring.cap != 0.0f ? scoring.capped(x) : x;
-                    if (scoring.slopes) x = scoring.biased(x, record[j].w, a.first + (r0 + i0 + j) / a.group - key);
+                const v4f row = grads.template across<W4>(r1 + j);
+                const bool in = (counts >> j) & 1u;
+                if (APPROXIMATE || a.flags.a) de[0] = careful_dot<W4>(full_n, row, v) * unit;
+                else {
+                    de[0] = 0.0f;
+                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) { de[0] += exact_term(full_n, e[0], u2f(real_bits(full_n, v[d])), x * unit); });
                 }
-                de[j] = pair.checked(s[j], x, e[j], de[j] + record[j].y * unit);
-                // (less than 2^-86 is nothing beside |dn| of 1 and values of at least 2^-40; with smaller ones it may be all there is)
-                const bool tiny = fabsf(de[j]) < 0x1p-86f;
-                wrong = wrong || ((counts >> j) & 1u && (!(fabsf(de[j]) < 0x1p80f) || (small && tiny)));
-                counts &= tiny && !small ? ~(1u << j) : ~0u;
-            }
-            // dk: da (*) qs
-            if (APPROXIMATE || a.flags.b) {
-                block_add<W4>(full_q, careful_lanes || qv.careful || __ballot(wrong) != 0ull, qv.zero, 1.0f, qr, de, scoring.mul_add, counts, dk);
-            } else {
-#pragma unroll 1
-                for (int j = 0; j < kBlock; ++j) {
-                    const bool in = ((counts & ~qv.zero) >> j) & 1u;
-                    each<0, W4>([&](auto n) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t m = (uint32_t)anew((int)k[4 * n.value + i]);
-                            const float own = m == full_q.pad ? 1.0f : u2f(m + full_q.raw);
-                            const float term = exact_term(full_q, own, u2f(from_lane<decltype(n)::value>(qr[0][i])), de[0]);
-                            dk[4 * n.value + i] += in ? term : 0.0f;
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
+                if (APPROXIMATE || a.flags.b) careful_add_row<W4>(full_n, row, e[0], in, unit, out[1]);
+                else
+                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) {
+                        const float term = exact_term(full_n, u2f(real_bits(full_n, v[d])), e[0], x * unit);
+                        out[1][d] += in ? term : 0.0f;
                     });
-                    turned(qr); turned(de);
-                }
+                turned(de); turned(e);
             }
-        }
-    }
-    if (folded) {
-        row_in_memory<W4>(a.out0 + to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
+            slices_de.add_up(turn, wave, de, false);
+            turn ^= 1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dk[4 * n + i] += x[i];
+            for (int j = 0; j < kBlock; ++j) de[j] = score_gradient(s[j], e[j], de[j], r1 + j);
+#pragma unroll 1
+            for (int j = 0; j < kBlock; ++j) {
+                const v4f row = queries.template across<W4>(r1 + j);
+                const bool in = (counts >> j) & 1u;
+                if (APPROXIMATE || a.flags.b) careful_add_row<W4>(full_q, row, de[0], in, 1.0f, out[0]);
+                else
+                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) {
+                        const float term = exact_term(full_q, u2f(real_bits(full_q, k[d])), x, de[0]);
+                        out[0][d] += in ? term : 0.0f;
+                    });
+                turned(de);
+            }
+            return true;
         });
-        row_in_memory<W4>(a.out1 + to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dv[4 * n + i] += x[i];
-        });
-    }
     const float back = 1.0f / unit;
 #pragma unroll
-    for (int d = 0; d < W; ++d) { dk[d] *= back; dv[d] *= back; }
-    store_row<W4>(a.out0 + to, first, a.dim, exists, dk);
-    store_row<W4>(a.out1 + to, first, a.dim, exists, dv);
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int d = 0; d < W; ++d) out[n][d] *= back;
+        store_row<W4>(to[n], first, a.dim, exists, out[n]);
+    }
 }
+
+template <int NS, int W4, bool WHOLE, bool APPROXIMATE> constexpr Variant dq_of() { return Variant{NS, W4, WHOLE, attention_dq_kernel<NS, W4, WHOLE, APPROXIMATE>}; }
+template <int NS, int W4, bool WHOLE, bool APPROXIMATE> constexpr Variant dkv_of() { return Variant{NS, W4, WHOLE, attention_dkv_kernel<NS, W4, WHOLE, APPROXIMATE>}; }
 
 }  // namespace pamatt

@@ -3,15 +3,20 @@
 
 namespace pamatt {
 extern const Variant kDqApprox[] = {
-    {1, 4, attention_dq_kernel<1, 4, true>},
-    {1, 8, attention_dq_kernel<1, 8, true>},
-    {2, 6, attention_dq_kernel<2, 6, true>},
-    {2, 8, attention_dq_kernel<2, 8, true>},
-    {4, 5, attention_dq_kernel<4, 5, true>},
-    {4, 6, attention_dq_kernel<4, 6, true>},
-    {4, 8, attention_dq_kernel<4, 8, true>},
-    {4, 12, attention_dq_kernel<4, 12, true>},
-    {4, 16, attention_dq_kernel<4, 16, true>},
-    {0, 0, nullptr},
+    dq_of<1, 4, true, true>(),
+    dq_of<1, 8, true, true>(),
+    dq_of<2, 6, true, true>(),
+    dq_of<2, 8, true, true>(),
+    dq_of<4, 5, true, true>(),
+    dq_of<4, 6, true, true>(),
+    dq_of<4, 8, true, true>(),
+    dq_of<8, 6, true, true>(),
+    dq_of<8, 8, true, true>(),
+    dq_of<1, 4, false, true>(),
+    dq_of<1, 8, false, true>(),
+    dq_of<2, 8, false, true>(),
+    dq_of<4, 8, false, true>(),
+    dq_of<8, 8, false, true>(),
+    {0, 0, false, nullptr},
 };
 }  // namespace pamatt

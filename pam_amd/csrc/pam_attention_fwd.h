@@ -1,4 +1,4 @@
-// The forward pass of pam_attention.h: a wavefront's 64 / NS rows over a chunk of the keys.
+// The forward pass of pam_attention.h: tiles of 64 rows over a chunk of the keys, a wavefront for each slice.
 #pragma once
 #include "pam_attention.h"
 
@@ -50,18 +50,20 @@ __device__ __forceinline__ void over_total(float (&out)[N], float l, float off)
     }
 }
 
-// A unit of a launch: the tile of rows, the chunk, the batch entry and key head.  Consecutive work-groups take different heads, so that
-// a head's keys stay with few of the XCDs' caches, and the last tiles, which see most keys where the order is causal, come first.
+// A unit of a launch, a work-group: the tiles of 64 rows, the chunk, the batch entry and key head.  Consecutive work-groups take different heads, so that
+// a head's keys stay with few of the XCDs' caches, and the last tiles, which see most keys where the order is causal, come first.  Work-groups go
+// to the XCDs in turn, and a tile begins with another chunk than the one before: else an XCD had the same chunks of all of them, seen by all rows or by few.
 struct Unit { int head, b, kv, tile, chunk; };
 __device__ __forceinline__ Unit unit_of(const Args& a)
 {
     Unit u;
-    const uint32_t heads = (uint32_t)(a.batch * a.kv_heads), at = blockIdx.x / heads;
+    const uint32_t heads = (uint32_t)(a.batch * a.kv_heads), at = blockIdx.x / heads, tile = at / (uint32_t)a.chunks;
     u.head = (int)(blockIdx.x - at * heads);
     u.b = u.head / a.kv_heads; u.kv = u.head - u.b * a.kv_heads;
-    u.tile = a.tiles - 1 - (int)(at / (uint32_t)a.chunks); u.chunk = (int)(at % (uint32_t)a.chunks);
+    u.tile = a.tiles - 1 - (int)tile; u.chunk = (int)((at + tile) % (uint32_t)a.chunks);
     return u;
 }
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
 
 // What a query's row sees: its keys.
 __device__ __forceinline__ Sight sight_of_row(const Args& a, int b, int row)
@@ -78,27 +80,25 @@ __device__ __forceinline__ Sight sight_of_row(const Args& a, int b, int row)
     return s;
 }
 
-template <int NS, int W4>
-__global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a)
+template <int NS, int W4, bool WHOLE>
+__global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention_kernel(Args a)
 {
-    constexpr int kRows = 64 / NS, W = 4 * W4;
-    const Place<NS, W4> here(a.values);
+    constexpr int W = 4 * W4;
+    __shared__ Slices<NS, kBlock> slices;
     const Unit u = unit_of(a);
-    const int row0 = (u.tile * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64)) * kRows;
-    if (row0 >= a.rows) return;                   // (no barriers below)
-    const int mine = row0 + here.row_in_wave, row = min(mine, a.rows - 1);
+    const int wave = wave_of(), slice = wave % NS, row0 = (u.tile * kTiles<NS> + wave / NS) * 64, mine = row0 + (int)threadIdx.x % 64, row = min(mine, a.rows - 1), first = slice * W;
     const bool exists = mine < a.rows;
-    const int token = row / a.group, head = u.kv * a.group + row % a.group, pos = a.first + token, first = here.slice * W;
+    const int token = row / a.group, head = u.kv * a.group + row % a.group, pos = a.first + token;
     const Scoring scoring(a);
-    const Full full{a.off, a.off != 1.0f, 0u - scoring.mul_add, lane_pad(0u)};
+    const Full full{a.off, a.off != 1.0f, 0u - scoring.mul_add};
     uint32_t q[W];
-    bool odd = false;
+    bool careful;
     {
         // (q (*) scale first, by the full definition where it takes that)
         const float* from = a.q.p + (long)u.b * a.q.sb + (long)token * a.q.st + (long)head * a.q.sh;
         const uint32_t scale_add = f2u(a.scale) - kBias + scoring.off_add;
-        odd = !load_lane<W4>(from, first, a.dim, a.values, scale_add, scoring.mul_add, lane_pad(0u), q);
-        if (__ballot(odd) != 0ull) {
+        careful = in_team<NS>(!load_lane<W4>(from, first, a.dim, a.values, scale_add, scoring.mul_add, q));
+        if (careful) {
 #pragma unroll 1
             for (int d = 0; d < W; ++d) {
                 if (first + d < a.values) q[0] = f2u(pam_mul_off(from[first + d], a.scale, a.off, full.has_off)) + scoring.mul_add;
@@ -106,88 +106,130 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a)
             }
         }
     }
-    const bool careful_lanes = __ballot(odd) != 0ull;
     float slope = 0.0f, wrong = 0.0f;             // wrong: becomes NaN with the first number that is none
     if (scoring.slopes) { slope = held_slope(a.slopes[head]); wrong = finite(a.slopes[head]) ? 0.0f : u2f(kQNaN); }
-    const Sight sight = sight_of_row(a, u.b, row);
-    const Stream keys = stream_of(here, a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.values, a.keys);
-    const Stream values = stream_of(here, a.v.p + (long)u.b * a.v.sb + (long)u.kv * a.v.sh, a.v.st, a.values, a.keys);
-
-    float out[W], l = 0.0f, l_before = 0.0f, M = kNothing, M_folded = kNothing;
-    bool some = false, folded = false;
-#pragma unroll
-    for (int d = 0; d < W; ++d) out[d] = 0.0f;
+    Sight sight = sight_of_row(a, u.b, row);
+    sight.close_team<NS>();
+    const Stream<WHOLE> keys(a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.keys, slice * W4, a.dim / 4);
+    const Stream<WHOLE> values(a.v.p + (long)u.b * a.v.sb + (long)u.kv * a.v.sh, a.v.st, a.keys, slice * W4, a.dim / 4);
     const long stat = ((long)u.head * a.chunks + u.chunk) * a.rows + row;
     float* const to = a.partial ? a.partial + stat * a.dim : a.y + (((long)u.b * a.tokens + token) * a.heads + head) * a.dim;
-    int terms = 0;
     const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
-#pragma unroll 1
-    for (int j0 = begin; j0 < end; j0 += kSpan) {
-        const uint64_t see = sight.span(j0);
-        if (__ballot(see != 0ull) == 0ull) continue;
-        some = some || see != 0ull;
-        const bool all = __ballot(see != ~0ull) == 0ull;
-        if (terms >= kLink) {                     // the chain of sums so far joins those before it, in memory
-            const float f = scale_between(M_folded, M);
-            row_in_memory<W4>(to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
+
+    float out[W], l, l_before, M, M_folded;
+    bool some, folded;
+    int terms, turn = 0;
+    // scores to weights, M raised where one is far above it; returns which ones count
+    const auto weigh = [&](float (&t)[kBlock], uint32_t sees, bool all, int j1) __attribute__((always_inline)) {
+        float most = kNothing;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { x[i] = (folded ? x[i] * f : 0.0f) + out[4 * n + i]; }
+        for (int j = 0; j < kBlock; ++j) t[j] = scoring.exponent(t[j], slope, pos - (j1 + j));
+        if (all)
+#pragma unroll
+            for (int j = 0; j < kBlock; ++j) most = fmaxf(most, t[j]);
+        else
+#pragma unroll
+            for (int j = 0; j < kBlock; ++j) most = fmaxf(most, (sees >> j) & 1u ? t[j] : kNothing);
+        if (__ballot(most > M + kLag) != 0ull) {
+            const float raised = most > M + kLag ? floorf(most) : M, f = scale_between(M, raised);
+            l *= f; l_before *= f;
+#pragma unroll
+            for (int d = 0; d < W; ++d) out[d] *= f;
+            M = raised;
+        }
+        uint32_t counts = 0u;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kBlock; ++j) {
+            float power = t[j] - M;
+            if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
+            wrong = __builtin_fmaf(power, 0.0f, wrong);
+            const bool in = power >= kLeast;
+            t[j] = power_of_two(fmaxf(power, kLeast));
+            sum += in ? t[j] : 0.0f;
+            counts |= in ? 1u << j : 0u;
+        }
+        l += sum;
+        return counts;
+    };
+    // all blocks of the chunk; false: one of them did not want to
+    const auto run = [&](auto&& start, auto&& block) __attribute__((always_inline)) {
+        l = l_before = 0.0f; M = M_folded = kNothing;
+        some = folded = false; terms = 0;
+#pragma unroll
+        for (int d = 0; d < W; ++d) out[d] = 0.0f;
+#pragma unroll 1
+        for (int j0 = begin; j0 < end; j0 += kSpan) {
+            const uint64_t see = sight.span(j0);
+            if (!in_team<NS>(see != 0ull)) continue;
+            some = some || see != 0ull;
+            const bool all = __ballot(see != ~0ull) == 0ull;
+            if (terms >= kLink) {                 // the chain of sums so far joins those before it, in memory
+                const float f = scale_between(M_folded, M);
+                row_in_memory<W4>(to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { x[i] = (folded ? x[i] * f : 0.0f) + out[4 * n + i]; }
+                });
+#pragma unroll
+                for (int d = 0; d < W; ++d) out[d] = 0.0f;
+                l_before += l; l = 0.0f;
+                M_folded = M; folded = true; terms = 0;
+            }
+            terms += kSpan;
+            start(j0);
+#pragma unroll 1
+            for (int i0 = 0; i0 < kSpan; i0 += kBlock)
+                if (!block(j0 + i0, (uint32_t)(see >> i0) & 0xffu, all)) return false;
+        }
+        return true;
+    };
+    if (!careful) {
+        Pipe<W4, WHOLE> pipe;
+        Look<W4, WHOLE> look_k, look_v;
+        careful = !run([&](int j0) __attribute__((always_inline)) { pipe.request(keys, j0); look_k.load(keys, j0); look_v.load(values, j0); },
+            [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
+                float t[kBlock];
+                if (!all && __ballot(sees != 0u) == 0ull) {
+                    pipe.request(keys, j1 + kBlock); look_k.load(keys, j1 + kBlock); look_v.load(values, j1 + kBlock);
+                    const bool wild = slices.add_up(turn, wave, t, false);
+                    turn ^= 1;
+                    return !wild;
+                }
+                const Verdict kv = judge(look_k, keys, a.values, 0u), vv = judge(look_v, values, a.values, 0u);
+                look_k.load(keys, j1 + kBlock);      // (the next block's; past the end the last key again)
+                look_v.load(values, j1 + kBlock);
+                block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, kv.zeros, q, t);
+                const bool wild = slices.add_up(turn, wave, t, kv.wild || vv.wild);
+                turn ^= 1;
+                if (__builtin_expect(wild, 0)) return false;
+                const uint32_t counts = weigh(t, sees, all, j1);
+                block_add<W4, WHOLE>(pipe, values, j1, keys, j1 + kBlock, vv.zeros, t, scoring.mul_add, counts, out);
+                return true;
             });
-#pragma unroll
-            for (int d = 0; d < W; ++d) out[d] = 0.0f;
-            l_before += l; l = 0.0f;
-            M_folded = M; folded = true; terms = 0;
-        }
-        terms += kSpan;
-        v4f kr[kBlock], vr[kBlock];
-        keys.rows(j0, kr);
-#pragma unroll 1
-        for (int i0 = 0; i0 < kSpan; i0 += kBlock) {
-            const uint32_t sees = (uint32_t)(see >> i0) & 0xffu;
-            if (!all && __ballot(sees != 0u) == 0ull) {
-                keys.rows(j0 + i0 + kBlock, kr);
-                continue;
-            }
-            values.rows(j0 + i0, vr);
-            keys.pad(0u, kr);
-            const Verdict kv = judge(here.streaming, 0u, kr);
-            float t[kBlock];
-            block_dots<NS, W4>(full, careful_lanes || kv.careful, kv.zero, 1.0f, kr, q, t);
-            keys.rows(j0 + i0 + kBlock, kr);          // (the next block's; past the end the last key again)
-            float most = kNothing;
-#pragma unroll
-            for (int j = 0; j < kBlock; ++j) t[j] = scoring.exponent(t[j], slope, pos - (j0 + i0 + j));
-            if (all)
-#pragma unroll
-                for (int j = 0; j < kBlock; ++j) most = fmaxf(most, t[j]);
-            else
-#pragma unroll
-                for (int j = 0; j < kBlock; ++j) most = fmaxf(most, (sees >> j) & 1u ? t[j] : kNothing);
-            if (__ballot(most > M + kLag) != 0ull) {
-                const float raised = most > M + kLag ? floorf(most) : M, f = scale_between(M, raised);
-                l *= f; l_before *= f;
-#pragma unroll
-                for (int d = 0; d < W; ++d) out[d] *= f;
-                M = raised;
-            }
-            uint32_t counts = 0u;
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kBlock; ++j) {
-                float power = t[j] - M;
-                if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
-                wrong = __builtin_fmaf(power, 0.0f, wrong);
-                const bool in = power >= kLeast;
-                t[j] = power_of_two(fmaxf(power, kLeast));
-                sum += in ? t[j] : 0.0f;
-                counts |= in ? 1u << j : 0u;
-            }
-            l += sum;
-            values.pad(0u, vr);
-            const Verdict vv = judge(here.streaming, 0u, vr);
-            block_add<W4>(full, vv.careful, vv.zero, 1.0f, vr, t, scoring.mul_add, counts, out);
-        }
     }
+    if (__builtin_expect(careful, 0))
+        run([](int) {}, [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
+            float t[kBlock];
+            if (!all && __ballot(sees != 0u) == 0ull) {
+                slices.add_up(turn, wave, t, false);
+                turn ^= 1;
+                return true;
+            }
+#pragma unroll 1
+            for (int j = 0; j < kBlock; ++j) {
+                t[0] = careful_dot<W4>(full, keys.template across<W4>(j1 + j), q);
+                turned(t);
+            }
+            slices.add_up(turn, wave, t, false);
+            turn ^= 1;
+            const uint32_t counts = weigh(t, sees, all, j1);
+#pragma unroll 1
+            for (int j = 0; j < kBlock; ++j) {
+                careful_add_row<W4>(full, values.template across<W4>(j1 + j), t[0], (counts >> j) & 1u, 1.0f, out);
+                turned(t);
+            }
+            return true;
+        });
     if (folded) {
         const float f = scale_between(M_folded, M);
         row_in_memory<W4>(to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {
@@ -200,16 +242,18 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(Args a)
     l = some ? l + wrong : 0.0f;
     M = some ? (M == kNothing ? 0.0f : M) : kNothing;
     if (a.partial) {
-        if (exists && here.slice == 0) a.partial_stats[stat] = make_float2(l, M);
+        if (exists && slice == 0) a.partial_stats[stat] = make_float2(l, M);
         if (__ballot(some) != 0ull) store_row<W4>(to, first, a.dim, exists, out);
         return;
     }
-    if (a.stats && exists && here.slice == 0) a.stats[((long)u.b * a.tokens + token) * a.heads + head] = make_float2(l, M);
+    if (a.stats && exists && slice == 0) a.stats[((long)u.b * a.tokens + token) * a.heads + head] = make_float2(l, M);
     over_total(out, some ? l : 1.0f, a.off);
     store_row<W4>(to, first, a.dim, exists, out);
 }
 
 typedef void (*Kernel)(Args);
-struct Variant { int slices, quads; Kernel kernel; };
+struct Variant { int slices, quads; bool whole; Kernel kernel; };      // whole: for rows of just these quads
+
+template <int NS, int W4, bool WHOLE> constexpr Variant forward_of() { return Variant{NS, W4, WHOLE, attention_kernel<NS, W4, WHOLE>}; }
 
 }  // namespace pamatt

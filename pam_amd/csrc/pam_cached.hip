@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : 4) void cached_attention_k
     Args scoring_args{};
     scoring_args.cap = a.cap; scoring_args.off = a.off; scoring_args.slopes = a.slopes;
     const Scoring scoring(scoring_args);
-    const Full full{a.off, has_off, 0u - mul_add, lane_pad(0u)};
+    const Full full{a.off, has_off, 0u - mul_add};
 
     // what the rows see: [low_of(r), position of r]
     const int length = (int)max(0ll, min(a.lengths[b], 1ll << 30)), given = a.counts ? (int)max(0ll, min(a.counts[b], (long long)a.tokens)) : a.tokens;
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : 4) void cached_attention_k
             const uint32_t scaled = (f2u(v) << 1) == 0u ? kStandIn : f2u(v) + (f2u(a.scale) - kBias + off_add);
             const bool out = there && (scaled << 1) - kLaneBase >= kLaneSpan;
             odd = odd || out;
-            q[r][d] = there ? (out ? f2u(pam_mul_off(v, a.scale, a.off, has_off)) : scaled) + mul_add : full.pad;
+            q[r][d] = there ? (out ? f2u(pam_mul_off(v, a.scale, a.off, has_off)) : scaled) + mul_add : lane_pad(0u);
             acc[r][d] = 0.0f;
         }
         l[r] = 0.0f; M[r] = kNothing;
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : 4) void cached_attention_k
 #pragma unroll
                             for (int i = 1; i < kTwo; ++i) theirs = n / ROWS == i ? f2u(rows[i0 + i][d]) : theirs;
                             mine = (uint32_t)anew((int)mine);
-                            sum += full_product(full, mine == full.pad ? 0u : mine + full.raw, theirs);
+                            sum += full_product(full, mine == lane_pad(0u) ? 0u : mine + full.raw, theirs);
                             __builtin_amdgcn_sched_barrier(0);
                         }
                         s[0] = sum;
