@@ -97,18 +97,24 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
     r.records[to] = make_float4(none ? u2f(kExpo) : stats.y, none ? 0.0f : dl, none ? -86.0f : (float)exponent, a.slopes ? held_slope(a.slopes[head]) : 0.0f);
 }
 
-// dq from the chunks' sums, through q (*) scale; or dk or dv: nothing behind the sums.
-__global__ __launch_bounds__(kThreads) void attention_sum_kernel(Args a, const float* parts, float* out, int of_keys)
+// dq from the chunks' sums, through q (*) scale; or dk and dv (the second half of the launch): nothing behind the sums.
+struct SumArgs { Args a; const float* parts[2]; float* out[2]; int of_keys; };
+__global__ __launch_bounds__(kThreads) void attention_sum_kernel(SumArgs s)
 {
-    const long quads = a.dim / 4, id = (long)blockIdx.x * kThreads + threadIdx.x;
-    const long lanes = of_keys ? a.keys : a.rows, all = (long)a.batch * a.kv_heads * lanes * quads;
-    if (id >= all) return;
+    const Args& a = s.a;
+    const long quads = a.dim / 4, lanes = s.of_keys ? a.keys : a.rows, all = (long)a.batch * a.kv_heads * lanes * quads;
+    long id = (long)blockIdx.x * kThreads + threadIdx.x;
+    const int which = id >= all;
+    if (which) id -= all;
+    if (id >= all || (which && !s.of_keys)) return;
+    const float* const parts = which ? s.parts[1] : s.parts[0];
     const long at = id / quads, head = at / lanes, row = at - head * lanes, b = head / a.kv_heads, kv = head - b * a.kv_heads;
     const int d = (int)(id - at * quads) * 4;
     v4f sum = *reinterpret_cast<const v4f*>(parts + (head * a.chunks * lanes + row) * a.dim + d);
+#pragma unroll 4
     for (int c = 1; c < a.chunks; ++c) sum += *reinterpret_cast<const v4f*>(parts + ((head * a.chunks + c) * lanes + row) * a.dim + d);
     long to;
-    if (of_keys) to = (b * a.keys + row) * a.kv_heads + kv;
+    if (s.of_keys) to = (b * a.keys + row) * a.kv_heads + kv;
     else {
         const long t = row / a.group, h = kv * a.group + row % a.group;
         const float* const q = a.q.p + b * a.q.sb + t * a.q.st + h * a.q.sh;
@@ -117,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void attention_sum_kernel(Args a, const f
 #pragma unroll
         for (int i = 0; i < 4; ++i) if (d + i < a.values) sum[i] = mul_grad(q[d + i], a.scale, sum[i], a.flags.a, a.off, has_off);
     }
-    *reinterpret_cast<v4f_any*>(out + to * a.dim + d) = sum;
+    *reinterpret_cast<v4f_any*>((which ? s.out[1] : s.out[0]) + to * a.dim + d) = sum;
 }
 
 // ---------------------------------------------------------------- host
@@ -250,8 +256,10 @@ BackwardSpace backward_space(const Args& a, bool want_q, bool want_kv)
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t from = at; at += align256(n); return from; };
     s.records = take(rows * sizeof(float4)); s.qs = take(rows * row); s.dn = take(rows * row);
-    if (want_q) s.dq = take(rows * row * dq_plan(a).chunks);
-    if (want_kv) { const size_t n = keys * row * dkv_plan(a).chunks; s.dk = take(n); s.dv = take(n); }
+    // (a pass of one chunk writes its gradients itself)
+    const int of_q = want_q ? dq_plan(a).chunks : 1, of_kv = want_kv ? dkv_plan(a).chunks : 1;
+    if (of_q > 1) s.dq = take(rows * row * of_q);
+    if (of_kv > 1) { s.dk = take(keys * row * of_kv); s.dv = take(keys * row * of_kv); }
     s.bytes = at;
     return s;
 }
@@ -324,30 +332,25 @@ int pam_hip_attention_bwd(const pam_hip_attention_shape* shape, const pam_hip_to
     const hipStream_t st = (hipStream_t)stream;
     unsigned groups = 0, row_groups = 0, key_groups = 0;
     if ((rc = groups_for("attention_bwd", heads_of(a) * a.rows * 16, groups)) || (rc = groups_for("attention_bwd", heads_of(a) * a.rows * (a.dim / 4), row_groups))
-        || (rc = groups_for("attention_bwd", heads_of(a) * a.keys * (a.dim / 4), key_groups))) return rc;
+        || (rc = groups_for("attention_bwd", 2 * heads_of(a) * a.keys * (a.dim / 4), key_groups))) return rc;
     if (a.rows) {
-        const RowArgs r{a, y, tokens_of(dy), reinterpret_cast<const float2*>(stats), (float4*)(ws + space.records), (float*)(ws + space.qs), (float*)(ws + space.dn), variant_for(kDqApprox, a.dim).slices,
-                        4 * variant_for(kDqApprox, a.dim).quads};
+        const Variant& v = variant_for(kDqApprox, a.dim);
+        const RowArgs r{a, y, tokens_of(dy), reinterpret_cast<const float2*>(stats), (float4*)(ws + space.records), (float*)(ws + space.qs), (float*)(ws + space.dn), v.slices, 4 * v.quads};
         hipLaunchKernelGGL(attention_rows_kernel, dim3(groups), dim3(kThreads), 0, st, r);
         if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
     }
-    if (dq && a.rows) {
+    const auto pass = [&](const Variant* list, const Plan& p, float* part0, float* part1, float* out0, float* out1, int of_keys, unsigned sum_groups) {
         Args d = a;
-        const Plan p = dq_plan(a);
-        d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.out0 = (float*)(ws + space.dq);
-        if ((rc = launch("attention_bwd", variant_for(approximate ? kDqApprox : kDqExact, a.dim), d, st))) return rc;
-        hipLaunchKernelGGL(attention_sum_kernel, dim3(row_groups), dim3(kThreads), 0, st, d, d.out0, dq, 0);
-        if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
-    }
-    if (want_kv && a.keys) {
-        Args d = a;
-        const Plan p = dkv_plan(a);
-        d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.out0 = (float*)(ws + space.dk); d.out1 = (float*)(ws + space.dv);
-        if ((rc = launch("attention_bwd", variant_for(approximate ? kDkvApprox : kDkvExact, a.dim), d, st))) return rc;
-        hipLaunchKernelGGL(attention_sum_kernel, dim3(key_groups), dim3(kThreads), 0, st, d, d.out0, dk, 1);
-        hipLaunchKernelGGL(attention_sum_kernel, dim3(key_groups), dim3(kThreads), 0, st, d, d.out1, dv, 1);
-        if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
-    }
+        d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.whole = p.chunks == 1;
+        d.out0 = d.whole ? out0 : part0; d.out1 = d.whole ? out1 : part1;
+        const int failed = launch("attention_bwd", variant_for(list, a.dim), d, st);
+        if (failed || d.whole) return failed;
+        hipLaunchKernelGGL(attention_sum_kernel, dim3(sum_groups), dim3(kThreads), 0, st, SumArgs{d, {part0, part1}, {out0, out1}, of_keys});
+        return pamhost::check_launch("attention_bwd");
+    };
+    if (dq && a.rows && (rc = pass(approximate ? kDqApprox : kDqExact, dq_plan(a), (float*)(ws + space.dq), nullptr, dq, nullptr, 0, row_groups))) return rc;
+    if (want_kv && a.keys
+        && (rc = pass(approximate ? kDkvApprox : kDkvExact, dkv_plan(a), (float*)(ws + space.dk), (float*)(ws + space.dv), dk, dv, 1, key_groups))) return rc;
     return PAM_HIP_OK;
 }
 

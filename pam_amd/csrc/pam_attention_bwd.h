@@ -136,7 +136,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     const Stream<WHOLE> keys(a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.keys, slice * W4, a.dim / 4);
     const Stream<WHOLE> values(a.v.p + (long)u.b * a.v.sb + (long)u.kv * a.v.sh, a.v.st, a.keys, slice * W4, a.dim / 4);
     float out[1][W];
-    float* const to[1] = {a.out0 + (((long)u.head * a.chunks + u.chunk) * a.rows + row) * a.dim};
+    const int head = u.kv * a.group + row % a.group;
+    float* const to[1] = {a.out0 + (a.whole ? ((long)u.b * a.tokens + row / a.group) * a.heads + head : ((long)u.head * a.chunks + u.chunk) * a.rows + row) * a.dim};
     const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
     int turn = 0;
     // weights from scores, and which ones count (what is no number does)
@@ -268,6 +269,14 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     const float back = 1.0f / unit;
 #pragma unroll
     for (int d = 0; d < W; ++d) out[0][d] *= back;
+    if (a.whole) {                                // (else where the chunks are put together)
+        const float* const from = a.q.p + (long)u.b * a.q.sb + (long)(row / a.group) * a.q.st + (long)head * a.q.sh;
+#pragma unroll 1
+        for (int d = 0; d < W; ++d) {
+            if (first + d < a.values) out[0][0] = mul_grad(from[first + d], a.scale, out[0][0], a.flags.a, a.off, a.off != 1.0f);
+            turned(out[0]);
+        }
+    }
     store_row<W4>(to[0], first, a.dim, exists, out[0]);
 }
 
@@ -322,7 +331,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     const Stream<WHOLE> queries(a.qs + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);
     const Stream<WHOLE> grads(a.dn + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);
     float out[2][W];                              // dk, dv
-    const long at = (((long)u.head * a.chunks + u.chunk) * a.keys + key) * a.dim;
+    const long at = (a.whole ? ((long)u.b * a.keys + key) * a.kv_heads + u.kv : ((long)u.head * a.chunks + u.chunk) * a.keys + key) * a.dim;
     float* const to[2] = {a.out0 + at, a.out1 + at};
     const int begin = max(sight.first / kSpan * kSpan, chunk_begin), end = min(min(sight.last, a.rows), chunk_begin + a.chunk);
     int turn = 0;
