@@ -1,11 +1,13 @@
 // Attention of a few new tokens over a paged cache (pam_attention.h has the formulas), for single tokens while decoding.
 //
-// Bound by reading the cache once.  A key's row is taken by a group of L lanes, a quad each (4 ... 64 lanes, so that a load is whole rows of a page),
-// and the rows of the queries' heads that share it (ROWS of them) are kept in registers beside it.  A wavefront takes 64 keys at a
-// time: their scores by sums over the groups' lanes, then a lane per key for the weights (over the groups they would cost as much as
-// the products), then the values' rows with the weights from LDS.  Every sequence's keys are cut into as many parts as there are work-groups for it,
-// by its own length; four wavefronts of a work-group take 64 keys in turn, their sums are put together through LDS, and the parts' by a
-// second kernel.  Scaling by powers of two is exact, so that none of this moves a result beyond the order of its sums.
+// Bound by reading the cache once, or, where many rows share it, by the products.  A wavefront takes 64 keys at a time.  For the scores a lane owns a key, 32 of
+// its values in registers while the queries' rows come by in scalar registers (pam_attention.h): two instructions a product and no sums over
+// lanes, so that the keys are read once for up to 20 rows.  Then a lane per key makes the weights, and for the results a group of L lanes
+// owns a key's row of values, a quad each (4 ... 64 lanes), and reads the rows' weights from LDS.  Every sequence's keys are cut into as
+// many parts as there are work-groups for it, by its own length; four wavefronts of a work-group take 64 keys in turn, their sums are put
+// together through LDS, and the parts' by a second kernel.  Scaling by powers of two is exact, so that none of this moves a result beyond the
+// order of its sums.
+// Heads that are no whole quads take a kernel in which groups of lanes own keys for the scores, too.
 #include <algorithm>
 
 #include "pam_attention.h"
@@ -15,7 +17,8 @@ using namespace pamatt;
 namespace {
 
 constexpr int kSteps = 4;                         // keys' rows in flight, of every lane
-constexpr int kMostParts = 128;
+constexpr int kMostParts = 128, kMostRows = 20;
+typedef void (*Kernel)(struct CacheArgs);
 
 struct CacheArgs {
     Tokens q;
@@ -95,35 +98,122 @@ __device__ __forceinline__ bool ordinary(const v4f (&r)[kSteps])
     return __ballot(most >= kStreamSpan) == 0ull;
 }
 
+// What a kernel's work-group is there for.
+struct Share {
+    int row0, here_rows, part, head_at, b, kv, length, given, begin, end;
+    __device__ __forceinline__ Share(const CacheArgs& a, int rows_each)
+    {
+        // (work-groups go to the eight XCDs in turn: those that read the same keys for other rows are eight apart, on one of them)
+        const int x = (int)blockIdx.x, unit = x / (8 * a.sets) * 8 + x % 8;
+        row0 = x / 8 % a.sets * rows_each;
+        here_rows = unit < a.batch * a.kv_heads * a.parts ? min(rows_each, a.rows - row0) : 0;
+        part = unit % a.parts; head_at = unit / a.parts; b = min(head_at / a.kv_heads, a.batch - 1); kv = head_at % a.kv_heads;
+        length = (int)max(0ll, min(a.lengths[b], 1ll << 30));
+        given = a.counts ? (int)max(0ll, min(a.counts[b], (long long)a.tokens)) : a.tokens;
+        const int last_token = min((row0 + here_rows - 1) / a.group, given - 1), first_token = row0 / a.group;
+        const bool any = first_token <= last_token;
+        // (no key behind the table's last place is looked for, however long a sequence says it is: a row that would see one is no number)
+        const int end_of_all = any ? min(length + last_token + 1, a.capacity) : 0;
+        const int begin_of_all = any && a.window ? min(max(0, length + first_token - a.window + 1), end_of_all) : 0;
+        // this part of them, whole spans
+        const int spans = (end_of_all + kSpan - 1) / kSpan - begin_of_all / kSpan, each = (spans + a.parts - 1) / a.parts;
+        begin = (begin_of_all / kSpan + part * each) * kSpan; end = min(end_of_all, begin + each * kSpan);
+    }
+};
+// Where a key's row lies, and whether it does.
+struct KeyPlace { long at; bool there; };
+__device__ __forceinline__ KeyPlace key_place(const CacheArgs& a, const int* table, int j, bool exists)
+{
+    KeyPlace p{0, exists};
+    if (exists) {
+        const int of = table[j / a.page];
+        p.there = of >= 0 && of < a.pages;
+        p.at = p.there ? (long)of * a.c_sp + (long)(j % a.page) * a.c_st : 0;
+    }
+    return p;
+}
+
+// The wavefronts' sums (each lane's quad of `acc`, over groups of L lanes) and what they are over, put together and written.
 template <int ROWS>
-__global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : 4) void cached_attention_kernel(CacheArgs a)
+__device__ __forceinline__ void finish(const CacheArgs& a, const Share& me, float (&acc)[ROWS][4], float (&l)[ROWS], const float (&M_of)[ROWS], uint32_t saw,
+                                       float (&sums)[ROWS][256 + 4], float2 (&stats)[kWaves][ROWS])
+{
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), L = a.lanes;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        for (int s = L; s < 64; s *= 2)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[r][d] += __shfl_xor(acc[r][d], s, 64);
+        for (int s = 1; s < 64; s *= 2) l[r] += __shfl_xor(l[r], s, 64);
+        const int token = (me.row0 + min(r, me.here_rows - 1)) / a.group;
+        const bool beyond = token < me.given && me.length + token >= a.capacity, some = beyond || __ballot((saw >> r) & 1u) != 0ull;
+        l[r] = beyond ? u2f(kQNaN) : l[r];
+        const float M = some && M_of[r] == kNothing ? 0.0f : M_of[r];            // (seen, and no number)
+        if (lane == 0) stats[wave][r] = make_float2(some ? l[r] : 0.0f, some ? M : kNothing);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) {
+        if (w == wave && lane < L)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                float most = kNothing;
+#pragma unroll
+                for (int o = 0; o < kWaves; ++o) most = fmaxf(most, stats[o][r].y);
+                const bool mine = stats[w][r].y != kNothing;
+                const float f = mine ? scale_between(stats[w][r].y, most) : 0.0f;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const float x = mine ? acc[r][d] * f : 0.0f;
+                    sums[r][lane * 4 + d] = w == 0 ? x : sums[r][lane * 4 + d] + x;
+                }
+            }
+        __syncthreads();
+    }
+    const int quads = (a.values + 3) / 4;
+    for (int i = threadIdx.x; i < me.here_rows * quads; i += kThreads) {
+        const int r = i / quads, d = i % quads * 4;
+        float most = kNothing, total = 0.0f;
+        const v4f sum = {sums[r][d], sums[r][d + 1], sums[r][d + 2], sums[r][d + 3]};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, stats[w][r].y);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float2 s = stats[w][r];
+            total += s.y == kNothing ? 0.0f : s.x * scale_between(s.y, most);
+        }
+        const RowPlace at = place_of(a, me.kv, me.row0 + r);
+        if (a.partial) {
+            const long to = ((long)me.head_at * a.rows + me.row0 + r) * a.parts + me.part;
+            *reinterpret_cast<v4f*>(a.partial + to * quads * 4 + d) = sum;
+            if (d == 0) a.partial_stats[to] = make_float2(total, most);
+        } else {
+            float* const to = a.y + (((long)me.b * a.tokens + at.token) * a.heads + at.head) * a.values + d;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (d + c < a.values) to[c] = most == kNothing ? 0.0f : pad_div_off(sum[c], total, a.off, a.off != 1.0f);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- heads of any size
+
+template <int ROWS>
+__global__ __launch_bounds__(kThreads, 4) void cached_attention_kernel(CacheArgs a)
 {
     __shared__ float scores[kWaves][kSpan][ROWS];                                // of a wavefront's keys, then their weights
     __shared__ float sums[ROWS][256 + 4];
     __shared__ float2 stats[kWaves][ROWS];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), L = a.lanes, keys_a_step = 64 / L;
-    // (work-groups go to the eight XCDs in turn: those that read the same keys for other rows are eight apart, on one of them)
-    const int x = (int)blockIdx.x, unit = x / (8 * a.sets) * 8 + x % 8, row0 = x / 8 % a.sets * ROWS;
-    if (unit >= a.batch * a.kv_heads * a.parts) return;
-    const int part = unit % a.parts, head_at = unit / a.parts, b = head_at / a.kv_heads, kv = head_at % a.kv_heads;
-    const int here_rows = min(ROWS, a.rows - row0);
+    const Share me(a, ROWS);
+    if (me.here_rows <= 0) return;
+    const int row0 = me.row0, here_rows = me.here_rows, b = me.b, kv = me.kv, length = me.length, given = me.given, begin = me.begin, end = me.end;
     const bool has_off = a.off != 1.0f;
-    const uint32_t off_add = f2u(a.off) - kBias, mul_add = f2u(a.off) - 2u * kBias, log2e_add = f2u(kLog2e) - kBias + off_add;
+    const uint32_t off_add = f2u(a.off) - kBias, mul_add = f2u(a.off) - 2u * kBias;
     Args scoring_args{};
     scoring_args.cap = a.cap; scoring_args.off = a.off; scoring_args.slopes = a.slopes;
     const Scoring scoring(scoring_args);
     const Full full{a.off, has_off, 0u - mul_add};
-
-    // what the rows see: [low_of(r), position of r]
-    const int length = (int)max(0ll, min(a.lengths[b], 1ll << 30)), given = a.counts ? (int)max(0ll, min(a.counts[b], (long long)a.tokens)) : a.tokens;
-    const int last_token = min((row0 + here_rows - 1) / a.group, given - 1), first_token = row0 / a.group;
-    const bool any = first_token <= last_token;
-    // (no key behind the table's last place is looked for, however long a sequence says it is: a row that would see one is no number)
-    const int end_of_all = any ? min(length + last_token + 1, a.capacity) : 0;
-    const int begin_of_all = any && a.window ? min(max(0, length + first_token - a.window + 1), end_of_all) : 0;
-    // this part of them, whole spans
-    const int spans = (end_of_all + kSpan - 1) / kSpan - begin_of_all / kSpan, each = (spans + a.parts - 1) / a.parts;
-    const int begin = (begin_of_all / kSpan + part * each) * kSpan, end = min(end_of_all, begin + each * kSpan);
 
     Lane here;
     here.first = lane % L * 4; here.values = a.values;
@@ -160,13 +250,9 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : 4) void cached_attention_k
         // a lane per key: where its row lies
         const int j = j0 + lane;
         const bool exists = j < end;
-        bool there = exists;
-        long at = 0;
-        if (there) {
-            const int of = table[j / a.page];
-            there = of >= 0 && of < a.pages;
-            at = there ? (long)of * a.c_sp + (long)(j % a.page) * a.c_st : 0;
-        }
+        const KeyPlace place = key_place(a, table, j, exists);
+        const bool there = place.there;
+        const long at = place.at;
         const auto row_at = [&](int step, long (&out)[kSteps]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
@@ -290,62 +376,246 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : 4) void cached_attention_k
         wave_fence();                             // (the next span's scores go where these weights are)
     }
 
-    // the groups of lanes, then the wavefronts one after the other, scaled to the largest M
+    finish<ROWS>(a, me, acc, l, M, saw, sums, stats);
+}
+
+// ---------------------------------------------------------------- heads of whole quads
+
+constexpr int kSlice = 8;                         // quads of a key in a lane's registers
+
+// Rows of queries, one after the other: a token's heads of this key head, then the next token's; the last one again behind the last.
+struct Queries {
+    const char* first; long step, wrap; int group, head0, count;                 // uniform
+    __device__ __forceinline__ Queries(const CacheArgs& a, const Share& me)
+    {
+        const RowPlace at = place_of(a, me.kv, me.row0);
+        first = (const char*)(a.q.p + (long)me.b * a.q.sb + (long)at.token * a.q.st + (long)at.head * a.q.sh);
+        step = a.q.sh * (long)sizeof(float); wrap = (a.q.st - (a.group - 1) * a.q.sh) * (long)sizeof(float);
+        group = a.group; head0 = me.row0 % a.group; count = me.here_rows;
+    }
+    __device__ __forceinline__ const char* after(const char* at, int& head, int r) const          // row r + 1, at being row r and `head` its head
+    {
+        const bool over = head + 1 == group;
+        const long by = over ? wrap : step;
+        head = over ? 0 : head + 1;
+        return at + (r + 1 < count ? by : 0l);
+    }
+};
+
+template <int ROWS, bool WHOLE>
+__global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : ROWS > 4 ? 3 : 4) void cached_rows_kernel(CacheArgs a)
+{
+    constexpr int kPad = ROWS < 4 ? ROWS : (ROWS + 3) / 4 * 4;
+    __shared__ float weights[kWaves][kSpan][kPad];                               // a key's, of all rows: bits(weight) + mul_add
+    __shared__ float sums[ROWS][256 + 4];
+    __shared__ float2 stats[kWaves][ROWS];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), L = a.lanes, keys_a_step = 64 / L, quads = a.values / 4;
+    const Share me(a, ROWS);
+    if (me.here_rows <= 0) return;
+    const bool has_off = a.off != 1.0f;
+    Args scoring_args{};
+    scoring_args.cap = a.cap; scoring_args.off = a.off; scoring_args.slopes = a.slopes;
+    const Scoring scoring(scoring_args);
+    const Full full{a.off, has_off, 0u};
+    const uint32_t scale_add = f2u(a.scale) - kBias + scoring.off_add, key_add = scale_add + scoring.mul_add, mul_add = scoring.mul_add;
+    const Queries queries(a, me);
+    // the queries, scaled, have to be in the streamed values' window; zeros are left out by factors
+    bool q_zeros = false, q_wild = false;
+    for (int i = threadIdx.x; i < me.here_rows * quads; i += kThreads) {
+        const RowPlace at = place_of(a, me.kv, me.row0 + i / quads);
+        const v4f x = *reinterpret_cast<const v4f_any*>(a.q.p + (long)me.b * a.q.sb + (long)at.token * a.q.st + (long)at.head * a.q.sh + i % quads * 4);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const bool zero = (f2u(x[c]) << 1) == 0u;
+            q_zeros = q_zeros || zero;
+            q_wild = q_wild || (!zero && ((f2u(x[c]) + scale_add) << 1) - kStreamBase >= kStreamSpan);
+        }
+    }
+    q_zeros = __syncthreads_or(q_zeros) != 0; q_wild = __syncthreads_or(q_wild) != 0;
+
+    float acc[ROWS][4], l[ROWS], M[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        for (int s = L; s < 64; s *= 2)
+        l[r] = 0.0f; M[r] = kNothing;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) acc[r][d] += __shfl_xor(acc[r][d], s, 64);
-        for (int s = 1; s < 64; s *= 2) l[r] += __shfl_xor(l[r], s, 64);
-        const int token = (row0 + min(r, here_rows - 1)) / a.group;
-        const bool beyond = token < given && length + token >= a.capacity, some = beyond || __ballot((saw >> r) & 1u) != 0ull;
-        l[r] = beyond ? u2f(kQNaN) : l[r];
-        if (some && M[r] == kNothing) M[r] = 0.0f;                               // (seen, and no number)
-        if (lane == 0) stats[wave][r] = make_float2(some ? l[r] : 0.0f, some ? M[r] : kNothing);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int d = 0; d < 4; ++d) acc[r][d] = 0.0f;
     }
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) {
-        if (w == wave && lane < L)
+    const int* const table = a.table + (long)me.b * a.per_sequence;
+    const float* const k = a.k + (long)me.kv * a.c_sh;
+    const float* const v = a.v + (long)me.kv * a.c_sh;
+    const int own = min(lane % L, quads - 1) * 4;                                // of a row of values
+    const bool streams = lane % L < quads;
+    uint32_t saw = 0u;                            // a bit for every row
+
+    const auto load_keys = [&](long at, int slice, v4f (&x)[kSlice]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                float most = kNothing;
+        for (int n = 0; n < kSlice; ++n) x[n] = *reinterpret_cast<const v4f_any*>(k + at + 4 * (WHOLE ? slice * kSlice + n : min(slice * kSlice + n, quads - 1)));
+    };
+#pragma unroll 1
+    for (int j0 = me.begin + wave * kSpan; j0 < me.end; j0 += kWaves * kSpan) {
+        const int j = j0 + lane;
+        const bool exists = j < me.end;
+        const KeyPlace place = key_place(a, table, min(j, me.end - 1), true);      // (behind the last key that one again)
+        const auto row_at = [&](int step, long (&out)[kSteps]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int o = 0; o < kWaves; ++o) most = fmaxf(most, stats[o][r].y);
-                const bool mine = stats[w][r].y != kNothing;
-                const float f = mine ? scale_between(stats[w][r].y, most) : 0.0f;
+            for (int i = 0; i < kSteps; ++i) {
+                const int from = (step + i) * keys_a_step + lane / L;
+                out[i] = (long)(((uint64_t)(uint32_t)__shfl((int)(place.at >> 32), from, 64) << 32) | (uint32_t)__shfl((int)place.at, from, 64));
+            }
+        };
+        const auto load_values = [&](int step, v4f (&x)[kSteps]) __attribute__((always_inline)) {
+            long where[kSteps];
+            row_at(min(step, L - kSteps), where);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const float x = mine ? acc[r][d] * f : 0.0f;
-                    sums[r][lane * 4 + d] = w == 0 ? x : sums[r][lane * 4 + d] + x;
+            for (int i = 0; i < kSteps; ++i) x[i] = *reinterpret_cast<const v4f_any*>(v + where[i] + own);
+        };
+        // scores
+        float s[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) s[r] = 0.0f;
+        const int slices = (quads + kSlice - 1) / kSlice;
+        v4f next[kSlice];
+        load_keys(place.at, 0, next);
+        uint32_t odd = 0u;
+#pragma unroll 1
+        for (int slice = 0; slice < slices; ++slice) {
+            uint32_t mine[4 * kSlice];
+#pragma unroll
+            for (int n = 0; n < kSlice; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x = f2u(next[n][c]);
+                    x = (x << 1) == 0u || (!WHOLE && slice * kSlice + n >= quads) ? kStandIn : x;
+                    odd = max(odd, (x << 1) - kLaneBase);
+                    mine[4 * n + c] = x + key_add;
+                }
+            if (slice + 1 < slices) load_keys(place.at, slice + 1, next);
+            const Stream<WHOLE> layout(nullptr, 0, 1, WHOLE ? 0 : slice * kSlice, quads);
+            const char* row = queries.first + (WHOLE ? slice * kSlice * 16l : 0l);
+            int head = queries.head0;
+            Piece now = piece_of<4, WHOLE>(layout, (const float*)row, 0);
+            if (__builtin_expect(!q_zeros, 1)) {
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    const char* const after = queries.after(row, head, r);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        asm volatile("" ::"s"(now.a));
+                        __builtin_amdgcn_sched_barrier(0);
+                        const Piece later = h == 0 ? piece_of<4, WHOLE>(layout, (const float*)row, 4) : piece_of<4, WHOLE>(layout, (const float*)after, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                        dot_piece<16>(now, mine + 16 * h, s[r]);
+                        __builtin_amdgcn_sched_barrier(0);
+                        now = later;
+                    }
+                    row = after;
+                }
+            } else {
+#pragma unroll 1
+                for (int r = 0; r < ROWS; ++r) {
+                    dot_piece_with_zeros<16>(now, mine, s[0]);
+                    now = piece_of<4, WHOLE>(layout, (const float*)row, 4);
+                    dot_piece_with_zeros<16>(now, mine + 16, s[0]);
+                    row = queries.after(row, head, r);
+                    now = piece_of<4, WHOLE>(layout, (const float*)row, 0);
+                    turned(s);
                 }
             }
-        __syncthreads();
-    }
-    const int quads = (a.values + 3) / 4;
-    for (int i = threadIdx.x; i < here_rows * quads; i += kThreads) {
-        const int r = i / quads, d = i % quads * 4;
-        float most = kNothing, total = 0.0f;
-        const v4f sum = {sums[r][d], sums[r][d + 1], sums[r][d + 2], sums[r][d + 3]};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, stats[w][r].y);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float2 s = stats[w][r];
-            total += s.y == kNothing ? 0.0f : s.x * scale_between(s.y, most);
         }
-        const RowPlace at = place_of(a, kv, row0 + r);
-        if (a.partial) {
-            const long to = ((long)head_at * a.rows + row0 + r) * a.parts + part;
-            *reinterpret_cast<v4f*>(a.partial + to * quads * 4 + d) = sum;
-            if (d == 0) a.partial_stats[to] = make_float2(total, most);
-        } else {
-            float* const to = a.y + (((long)b * a.tokens + at.token) * a.heads + at.head) * a.values + d;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (d + c < a.values) to[c] = most == kNothing ? 0.0f : pad_div_off(sum[c], total, a.off, has_off);
+        if (__builtin_expect(q_wild || __ballot(odd >= kLaneSpan) != 0ull, 0)) {
+            // the full definition
+            const char* row = queries.first;
+            int head = queries.head0;
+#pragma unroll 1
+            for (int r = 0; r < ROWS; ++r) {
+                s[0] = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < a.values; ++d) {
+                    const float query = reinterpret_cast<const float*>(row)[d];
+                    s[0] += full_product(full, f2u(pam_mul_off(query, a.scale, a.off, has_off)), f2u(k[place.at + d]));
+                }
+                row = queries.after(row, head, r);
+                turned(s);
+            }
         }
+        v4f rows[kSteps];
+        load_values(0, rows);
+        // weights: a lane per key
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const int token = (me.row0 + min(r, me.here_rows - 1)) / a.group, pos = me.length + token;
+            const bool sees = exists && token < me.given && j <= pos && (a.window == 0 || j > pos - a.window);
+            const float slope = a.slopes ? a.slopes[place_of(a, me.kv, me.row0 + min(r, me.here_rows - 1)).head] : 0.0f;
+            float t = scoring.exponent(s[r], held_slope(slope), pos - j);
+            t = place.there && finite(slope) ? t : u2f(kQNaN);
+            float most = sees ? t : kNothing;
+            most = most != most ? kNothing : most;
+            if (__ballot(most > M[r] + kLag) != 0ull) {
+#pragma unroll
+                for (int n = 1; n < 64; n *= 2) most = fmaxf(most, __shfl_xor(most, n, 64));
+                const float raised = u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(floorf(most)))), f = scale_between(M[r], raised);
+                l[r] *= f;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) acc[r][d] *= f;
+                M[r] = raised;
+            }
+            const float power = sees ? t - M[r] : 2.0f * kLeast;
+            saw |= sees ? 1u << r : 0u;
+            const bool in = power >= kLeast;
+            const float e = power_of_two(fmaxf(power, kLeast));
+            l[r] += in ? e : power * 0.0f;        // (what is no number makes none of the sum)
+            // (one that does not count stands as 2^-86: nothing beside the largest, which is at least 2^-8)
+            weights[wave][lane][r] = u2f((in ? f2u(e) : kStandIn) + mul_add);
+            __builtin_amdgcn_sched_barrier(0);    // (row by row: all of them side by side take the registers of the loops around)
+        }
+        wave_fence();
+        // values
+#pragma unroll 1
+        for (int step = 0; step < L; step += kSteps) {
+            v4f later[kSteps];
+            load_values(step + kSteps, later);
+            uint32_t most = 0u;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) most = max(most, (f2u(rows[i][d]) << 1) - kStreamBase);
+            if (__builtin_expect((__ballot(most >= kStreamSpan && streams)) != 0ull, 0)) {
+                // zeros, or something else: by the full definition
+#pragma unroll 1
+                for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+                        const uint32_t weight = f2u(weights[wave][(step + i) * keys_a_step + lane / L][r]) - mul_add;
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            const float c = full_product(full, weight, f2u(rows[0][d]));
+                            acc[r][d] += weight != kStandIn ? c : 0.0f;
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                    turned(rows);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const float* const of = weights[wave][(step + i) * keys_a_step + lane / L];
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) acc[r][d] += u2f(f2u(rows[i][d]) + f2u(of[r]));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) rows[i] = later[i];
+        }
+        wave_fence();                             // (the next span's weights go where these are)
     }
+    if (!streams)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[r][d] = 0.0f;
+    finish<ROWS>(a, me, acc, l, M, saw, sums, stats);
 }
 
 // The parts of a query's head, one work-group each: lanes along its quads, the rest of the threads along the parts.
@@ -406,7 +676,12 @@ struct CachePlan { int rows_each, sets, lanes, parts; };
 CachePlan cache_plan(long heads, long rows, long values, long capacity)
 {
     CachePlan p;
-    p.rows_each = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    if (values % 4 != 0) p.rows_each = rows <= 1 ? 1 : 4;
+    else {
+        // (rows in as few sets as there can be, of one size)
+        const long sets = (rows + kMostRows - 1) / kMostRows, each = (rows + sets - 1) / std::max(1L, sets);
+        p.rows_each = each <= 1 ? 1 : each <= 2 ? 2 : (int)((each + 3) / 4 * 4);
+    }
     p.sets = (int)((rows + p.rows_each - 1) / p.rows_each);
     p.lanes = 4;
     while (p.lanes * 4 < values) p.lanes *= 2;
@@ -483,13 +758,20 @@ int pam_hip_cached_attention_fwd(const pam_hip_cache_shape* s, const pam_hip_tok
     const long units = heads * p.parts, groups = (units + 7) / 8 * 8 * p.sets;
     if (groups > (1L << 23)) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "cached_attention: size out of range");
     const dim3 grid((unsigned)groups);
-    switch (p.rows_each) {
-    case 1: hipLaunchKernelGGL((cached_attention_kernel<1>), grid, dim3(kThreads), 0, st, a); break;
-    case 2: hipLaunchKernelGGL((cached_attention_kernel<2>), grid, dim3(kThreads), 0, st, a); break;
-    case 4: hipLaunchKernelGGL((cached_attention_kernel<4>), grid, dim3(kThreads), 0, st, a); break;
-    case 8: hipLaunchKernelGGL((cached_attention_kernel<8>), grid, dim3(kThreads), 0, st, a); break;
-    default: hipLaunchKernelGGL((cached_attention_kernel<16>), grid, dim3(kThreads), 0, st, a); break;
-    }
+    const bool whole = a.values % (4 * kSlice) == 0;
+    Kernel kernel = nullptr;
+    if (a.values % 4 != 0) kernel = p.rows_each == 1 ? cached_attention_kernel<1> : cached_attention_kernel<4>;
+    else
+        switch (p.rows_each) {
+        case 1: kernel = whole ? cached_rows_kernel<1, true> : cached_rows_kernel<1, false>; break;
+        case 2: kernel = whole ? cached_rows_kernel<2, true> : cached_rows_kernel<2, false>; break;
+        case 4: kernel = whole ? cached_rows_kernel<4, true> : cached_rows_kernel<4, false>; break;
+        case 8: kernel = whole ? cached_rows_kernel<8, true> : cached_rows_kernel<8, false>; break;
+        case 12: kernel = whole ? cached_rows_kernel<12, true> : cached_rows_kernel<12, false>; break;
+        case 16: kernel = whole ? cached_rows_kernel<16, true> : cached_rows_kernel<16, false>; break;
+        default: kernel = whole ? cached_rows_kernel<kMostRows, true> : cached_rows_kernel<kMostRows, false>; break;
+        }
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, a);
     int done = pamhost::check_launch("cached_attention");
     if (done != PAM_HIP_OK || !need) return done;
     hipLaunchKernelGGL(cached_join_kernel, dim3((unsigned)(heads * a.rows)), dim3(kThreads), 0, st, a);
