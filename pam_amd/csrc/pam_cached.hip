@@ -17,7 +17,7 @@ using namespace pamatt;
 namespace {
 
 constexpr int kSteps = 4;                         // keys' rows in flight, of every lane
-constexpr int kMostParts = 128, kMostRows = 20;
+constexpr int kMostParts = 512, kMostRows = 20;
 typedef void (*Kernel)(struct CacheArgs);
 
 struct CacheArgs {
@@ -381,6 +381,9 @@ __global__ __launch_bounds__(kThreads, 4) void cached_attention_kernel(CacheArgs
 
 // ---------------------------------------------------------------- heads of whole quads
 
+// Work-groups that a compute unit has at once: two leave the registers that keep eight kilobytes of every wavefront on their way (three, with less on
+// its way: 16 sequences of up to 4000 tokens 55 us where two take 51).
+constexpr int kGroupsAtOnce = 2;
 constexpr int kSlice = 8;                         // quads of a key in a lane's registers
 
 // Rows of queries, one after the other: a token's heads of this key head, then the next token's; the last one again behind the last.
@@ -403,8 +406,10 @@ struct Queries {
 };
 
 template <int ROWS, bool WHOLE>
-__global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : ROWS > 4 ? 3 : 4) void cached_rows_kernel(CacheArgs a)
+__global__ __launch_bounds__(kThreads, kGroupsAtOnce) void cached_rows_kernel(CacheArgs a)
 {
+    constexpr bool kEarly = ROWS <= 8;            // the next span's keys are asked for before this one's values are added up (more rows have no registers for them)
+    constexpr int kAhead = kEarly ? 8 : 4;        // rows of values that a lane has on their way
     constexpr int kPad = ROWS < 4 ? ROWS : (ROWS + 3) / 4 * 4;
     __shared__ float weights[kWaves][kSpan][kPad];                               // a key's, of all rows: bits(weight) + mul_add
     __shared__ float sums[ROWS][256 + 4];
@@ -419,6 +424,18 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : ROWS > 4 ? 3 : 4) void cac
     const Full full{a.off, has_off, 0u};
     const uint32_t scale_add = f2u(a.scale) - kBias + scoring.off_add, key_add = scale_add + scoring.mul_add, mul_add = scoring.mul_add;
     const Queries queries(a, me);
+    const int* const table = a.table + (long)me.b * a.per_sequence;
+    const float* const k = a.k + (long)me.kv * a.c_sh;
+    const float* const v = a.v + (long)me.kv * a.c_sh;
+    // the first span's keys, and every other's while the values of the one before are added up, are on their way before anything waits
+    const auto load_keys = [&](long at, int slice, v4f (&x)[kSlice]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < kSlice; ++n) x[n] = *reinterpret_cast<const v4f_any*>(k + at + 4 * (WHOLE ? slice * kSlice + n : min(slice * kSlice + n, quads - 1)));
+    };
+    const auto place_of_span = [&](int j0) __attribute__((always_inline)) { return key_place(a, table, max(0, min(j0 + lane, me.end - 1)), me.begin < me.end); };      // (behind the last key that one again)
+    KeyPlace place = place_of_span(me.begin + wave * kSpan);
+    v4f next[kSlice];
+    load_keys(place.at, 0, next);
     // the queries, scaled, have to be in the streamed values' window; zeros are left out by factors
     bool q_zeros = false, q_wild = false;
     for (int i = threadIdx.x; i < me.here_rows * quads; i += kThreads) {
@@ -440,42 +457,32 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : ROWS > 4 ? 3 : 4) void cac
 #pragma unroll
         for (int d = 0; d < 4; ++d) acc[r][d] = 0.0f;
     }
-    const int* const table = a.table + (long)me.b * a.per_sequence;
-    const float* const k = a.k + (long)me.kv * a.c_sh;
-    const float* const v = a.v + (long)me.kv * a.c_sh;
     const int own = min(lane % L, quads - 1) * 4;                                // of a row of values
     const bool streams = lane % L < quads;
     uint32_t saw = 0u;                            // a bit for every row
 
-    const auto load_keys = [&](long at, int slice, v4f (&x)[kSlice]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < kSlice; ++n) x[n] = *reinterpret_cast<const v4f_any*>(k + at + 4 * (WHOLE ? slice * kSlice + n : min(slice * kSlice + n, quads - 1)));
-    };
 #pragma unroll 1
     for (int j0 = me.begin + wave * kSpan; j0 < me.end; j0 += kWaves * kSpan) {
         const int j = j0 + lane;
         const bool exists = j < me.end;
-        const KeyPlace place = key_place(a, table, min(j, me.end - 1), true);      // (behind the last key that one again)
-        const auto row_at = [&](int step, long (&out)[kSteps]) __attribute__((always_inline)) {
+        const auto row_at = [&](int step, long (&out)[kAhead]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
+            for (int i = 0; i < kAhead; ++i) {
                 const int from = (step + i) * keys_a_step + lane / L;
                 out[i] = (long)(((uint64_t)(uint32_t)__shfl((int)(place.at >> 32), from, 64) << 32) | (uint32_t)__shfl((int)place.at, from, 64));
             }
         };
-        const auto load_values = [&](int step, v4f (&x)[kSteps]) __attribute__((always_inline)) {
-            long where[kSteps];
-            row_at(min(step, L - kSteps), where);
+        const auto load_values = [&](int step, v4f (&x)[kAhead]) __attribute__((always_inline)) {
+            long where[kAhead];
+            row_at(min(step, L - kAhead), where);
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) x[i] = *reinterpret_cast<const v4f_any*>(v + where[i] + own);
+            for (int i = 0; i < kAhead; ++i) x[i] = *reinterpret_cast<const v4f_any*>(v + where[i] + own);
         };
         // scores
         float s[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) s[r] = 0.0f;
         const int slices = (quads + kSlice - 1) / kSlice;
-        v4f next[kSlice];
-        load_keys(place.at, 0, next);
         uint32_t odd = 0u;
 #pragma unroll 1
         for (int slice = 0; slice < slices; ++slice) {
@@ -538,8 +545,10 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : ROWS > 4 ? 3 : 4) void cac
                 turned(s);
             }
         }
-        v4f rows[kSteps];
+        v4f rows[kAhead];
         load_values(0, rows);
+        const KeyPlace after = place_of_span(j0 + kWaves * kSpan);
+        if (kEarly) load_keys(after.at, 0, next);
         // weights: a lane per key
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -571,33 +580,51 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : ROWS > 4 ? 3 : 4) void cac
         wave_fence();
         // values
 #pragma unroll 1
-        for (int step = 0; step < L; step += kSteps) {
-            v4f later[kSteps];
-            load_values(step + kSteps, later);
+        for (int step = 0; step < L; step += kAhead) {
+            v4f later[kAhead];
+            load_values(step + kAhead, later);
             uint32_t most = 0u;
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
+            for (int i = 0; i < kAhead; ++i)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) most = max(most, (f2u(rows[i][d]) << 1) - kStreamBase);
             if (__builtin_expect((__ballot(most >= kStreamSpan && streams)) != 0ull, 0)) {
-                // zeros, or something else: by the full definition
+                // zeros are left out by factors, anything else takes the full definition
+                bool odd_value = false;
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) odd_value = odd_value || ((f2u(rows[i][d]) << 1) != 0u && (f2u(rows[i][d]) << 1) - kStreamBase >= kStreamSpan);
+                const bool wild = __ballot(odd_value && streams) != 0ull;
 #pragma unroll 1
-                for (int i = 0; i < kSteps; ++i) {
+                for (int i = 0; i < kAhead; ++i) {
+                    const float* const of = weights[wave][(step + i) * keys_a_step + lane / L];
+                    if (!wild) {
+                        v4f x = rows[0], f;
 #pragma unroll
-                    for (int r = 0; r < ROWS; ++r) {
-                        const uint32_t weight = f2u(weights[wave][(step + i) * keys_a_step + lane / L][r]) - mul_add;
+                        for (int d = 0; d < 4; ++d) { f[d] = (f2u(x[d]) << 1) == 0u ? 0.0f : 1.0f; x[d] = (f2u(x[d]) << 1) == 0u ? 1.0f : x[d]; }
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) {
-                            const float c = full_product(full, weight, f2u(rows[0][d]));
-                            acc[r][d] += weight != kStandIn ? c : 0.0f;
-                            __builtin_amdgcn_sched_barrier(0);
+                        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) acc[r][d] = __builtin_fmaf(u2f(f2u(x[d]) + f2u(of[r])), f[d], acc[r][d]);
+                    } else {
+#pragma unroll 1
+                        for (int r = 0; r < ROWS; ++r) {
+                            const uint32_t weight = f2u(of[r]) - mul_add;
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) {
+                                const float c = full_product(full, weight, f2u(rows[0][d]));
+#pragma unroll
+                                for (int n = 0; n < ROWS; ++n) acc[n][d] += n == r && weight != kStandIn ? c : 0.0f;
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
                         }
                     }
                     turned(rows);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
+                for (int i = 0; i < kAhead; ++i) {
                     const float* const of = weights[wave][(step + i) * keys_a_step + lane / L];
 #pragma unroll
                     for (int r = 0; r < ROWS; ++r)
@@ -606,9 +633,11 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : ROWS > 4 ? 3 : 4) void cac
                 }
             }
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) rows[i] = later[i];
+            for (int i = 0; i < kAhead; ++i) rows[i] = later[i];
         }
         wave_fence();                             // (the next span's weights go where these are)
+        place = after;
+        if (!kEarly) load_keys(place.at, 0, next);
     }
     if (!streams)
 #pragma unroll
@@ -622,25 +651,32 @@ __global__ __launch_bounds__(kThreads, ROWS > 8 ? 2 : ROWS > 4 ? 3 : 4) void cac
 __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs a)
 {
     __shared__ v4f sums[kThreads];
-    __shared__ float totals[kMostParts], scales[kMostParts];
-    __shared__ float top;
+    __shared__ float scales[kMostParts], tops[kWaves], totals[kWaves];
     const int quads = (a.values + 3) / 4, row = (int)blockIdx.x % a.rows, head_at = (int)blockIdx.x / a.rows, b = head_at / a.kv_heads, kv = head_at % a.kv_heads;
     const long from = ((long)head_at * a.rows + row) * a.parts;
-    float2 mine = make_float2(0.0f, kNothing);
-    if ((int)threadIdx.x < a.parts) mine = a.partial_stats[from + threadIdx.x];
-    if (threadIdx.x < 64) {
-        float2 second = make_float2(0.0f, kNothing);
-        if ((int)threadIdx.x + 64 < a.parts) second = a.partial_stats[from + threadIdx.x + 64];
-        float most = fmaxf(mine.y, second.y);
-        for (int s = 1; s < 64; s *= 2) most = fmaxf(most, __shfl_xor(most, s, 64));
-        if (threadIdx.x == 0) top = most;
+    float2 mine[kMostParts / kThreads];
+    float M = kNothing;
+#pragma unroll
+    for (int i = 0; i < kMostParts / kThreads; ++i) {
+        const int p = (int)threadIdx.x + i * kThreads;
+        mine[i] = p < a.parts ? a.partial_stats[from + p] : make_float2(0.0f, kNothing);
+        M = fmaxf(M, mine[i].y);
     }
+    for (int s = 1; s < 64; s *= 2) M = fmaxf(M, __shfl_xor(M, s, 64));
+    if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = M;
     __syncthreads();
-    const float M = top;
-    if ((int)threadIdx.x < a.parts) {
-        scales[threadIdx.x] = mine.y == kNothing ? 0.0f : scale_between(mine.y, M);
-        totals[threadIdx.x] = mine.y == kNothing ? 0.0f : mine.x * scales[threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, tops[w]);
+    float part_sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMostParts / kThreads; ++i) {
+        const int p = (int)threadIdx.x + i * kThreads;
+        const float f = mine[i].y == kNothing ? 0.0f : scale_between(mine[i].y, M);
+        if (p < a.parts) scales[p] = f;
+        part_sum += mine[i].y == kNothing ? 0.0f : mine[i].x * f;
     }
+    for (int s = 1; s < 64; s *= 2) part_sum += __shfl_xor(part_sum, s, 64);
+    if (threadIdx.x % 64 == 0) totals[threadIdx.x / 64] = part_sum;
     __syncthreads();
     int columns = 1;                              // lanes along the quads: a power of two
     while (columns < quads) columns *= 2;
@@ -658,7 +694,7 @@ __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs a)
     __syncthreads();
     if (share != 0 || column >= quads) return;
     float total = 0.0f;
-    for (int p = 0; p < a.parts; ++p) total += totals[p];
+    for (int w = 0; w < kWaves; ++w) total += totals[w];
     for (int s = 1; s < shares; ++s)
 #pragma unroll
         for (int c = 0; c < 4; ++c) sum[c] += sums[s * columns + column][c];
@@ -683,10 +719,10 @@ CachePlan cache_plan(long heads, long rows, long values, long capacity)
         p.rows_each = each <= 1 ? 1 : each <= 2 ? 2 : (int)((each + 3) / 4 * 4);
     }
     p.sets = (int)((rows + p.rows_each - 1) / p.rows_each);
-    p.lanes = 4;
+    p.lanes = values % 4 ? 4 : 8;
     while (p.lanes * 4 < values) p.lanes *= 2;
-    // (three work-groups for each of 256 compute units; a part of less than a span for each wavefront is not worth a second kernel)
-    const long units = std::max(1L, heads * p.sets), wanted = (768 + units - 1) / units, most = (capacity + kWaves * kSpan - 1) / (kWaves * kSpan);
+    // (the work-groups that 256 compute units have at once; a part of less than a span for each wavefront is not worth a second kernel)
+    const long units = std::max(1L, heads * p.sets), wanted = 256 * kGroupsAtOnce / units, most = (capacity + kWaves * kSpan - 1) / (kWaves * kSpan);
     p.parts = (int)std::max(1L, std::min({wanted, most, (long)kMostParts}));
     return p;
 }
