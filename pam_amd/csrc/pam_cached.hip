@@ -26,10 +26,10 @@ struct CacheArgs {
     const int* table; const long long* lengths; const long long* counts;
     const float* slopes;
     float* y;
-    float* partial; float2* partial_stats;        // [batch][kv_heads][rows][parts][quads of values], [...]: l, M; or null: parts is 1
+    float* partial; float2* partial_stats;        // [kv_heads][batch x parts][rows][quads of values], [...]: l, M; or null: parts is 1
     int batch, tokens, heads, kv_heads, group, values, rows;
     int page, pages, per_sequence, window, capacity;      // per_sequence: entries of the table; capacity: the places that they make
-    int lanes, parts, sets;
+    int lanes, parts, sets, rows_each;            // parts: on average, of a sequence
     float scale, cap, off;
 };
 
@@ -98,26 +98,70 @@ __device__ __forceinline__ bool ordinary(const v4f (&r)[kSteps])
     return __ballot(most >= kStreamSpan) == 0ull;
 }
 
+// Which spans of a sequence the rows row0 ... row0 + count - 1 see.
+struct Spans {
+    int length, given, begin, end;                // keys; the first one's span is where the count begins
+    __device__ __forceinline__ Spans(const CacheArgs& a, int b, int row0, int count)
+    {
+        length = (int)max(0ll, min(a.lengths[b], 1ll << 30));
+        given = a.counts ? (int)max(0ll, min(a.counts[b], (long long)a.tokens)) : a.tokens;
+        const int last_token = min((row0 + count - 1) / a.group, given - 1), first_token = row0 / a.group;
+        const bool any = first_token <= last_token;
+        // (no key behind the table's last place is looked for, however long a sequence says it is: a row that would see one is no number)
+        end = any ? min(length + last_token + 1, a.capacity) : 0;
+        begin = any && a.window ? min(max(0, length + first_token - a.window + 1), end) : 0;
+    }
+    __device__ __forceinline__ int count() const { return (end + kSpan - 1) / kSpan - begin / kSpan; }
+};
+// How the parts of a key head's work-groups (batch x parts) go to the sequences: up to 64 sequences share them by their lengths, so that each part has
+// the same number of spans for every wavefront; more have a fixed number each.  (16 sequences of 4000 tokens and less, 512 work-groups: 48 us
+// with a fixed number.)
+struct Cut { int b, first, parts, each; };        // of sequence b: its first part, how many, the spans in one
+__device__ __forceinline__ Cut cut_of(const CacheArgs& a, int row0, int count, bool by_part, int which)          // by_part: of the sequence that has part `which`
+{
+    Cut c;
+    if (a.batch > 64 || a.parts == 1) {
+        c.b = by_part ? which / a.parts : which; c.first = c.b * a.parts; c.parts = a.parts;
+        c.each = (Spans(a, c.b, row0, count).count() + a.parts - 1) / a.parts;
+        return c;
+    }
+    const int lane = threadIdx.x % 64, all = a.batch * a.parts;
+    const int spans = lane < a.batch ? Spans(a, lane, row0, count).count() : 0;
+    const auto sum = [](int v) { for (int s = 1; s < 64; s *= 2) v += __shfl_xor(v, s, 64); return v; };
+    int each = max(kWaves, (sum(spans) / all + kWaves - 1) / kWaves * kWaves), parts = 0;
+    for (;; each += max(kWaves, each / 8 / kWaves * kWaves)) {                   // (ends: parts <= sum / each + batch, and there are at least twice batch)
+        parts = lane < a.batch ? max(1, (spans + each - 1) / each) : 0;
+        if (__builtin_amdgcn_readfirstlane(sum(parts)) <= all) break;
+    }
+    int upto = parts;
+    for (int s = 1; s < 64; s *= 2) { const int x = __shfl_up(upto, s, 64); upto += lane >= s ? x : 0; }
+    c.b = __builtin_amdgcn_readfirstlane(by_part ? (int)__popcll(__ballot(lane < a.batch && upto <= which)) : which);
+    c.parts = __shfl(parts, min(c.b, 63), 64);
+    c.first = __builtin_amdgcn_readfirstlane(__shfl(upto, min(c.b, 63), 64) - c.parts);
+    c.parts = __builtin_amdgcn_readfirstlane(c.parts);
+    c.each = __builtin_amdgcn_readfirstlane(each);
+    return c;
+}
 // What a kernel's work-group is there for.
 struct Share {
-    int row0, here_rows, part, head_at, b, kv, length, given, begin, end;
+    int row0, here_rows, slot, b, kv, length, given, begin, end;                 // slot: where its sums go
     __device__ __forceinline__ Share(const CacheArgs& a, int rows_each)
     {
         // (work-groups go to the eight XCDs in turn: those that read the same keys for other rows are eight apart, on one of them)
-        const int x = (int)blockIdx.x, unit = x / (8 * a.sets) * 8 + x % 8;
+        const int x = (int)blockIdx.x, all = a.batch * a.parts;
+        slot = x / (8 * a.sets) * 8 + x % 8;
         row0 = x / 8 % a.sets * rows_each;
-        here_rows = unit < a.batch * a.kv_heads * a.parts ? min(rows_each, a.rows - row0) : 0;
-        part = unit % a.parts; head_at = unit / a.parts; b = min(head_at / a.kv_heads, a.batch - 1); kv = head_at % a.kv_heads;
-        length = (int)max(0ll, min(a.lengths[b], 1ll << 30));
-        given = a.counts ? (int)max(0ll, min(a.counts[b], (long long)a.tokens)) : a.tokens;
-        const int last_token = min((row0 + here_rows - 1) / a.group, given - 1), first_token = row0 / a.group;
-        const bool any = first_token <= last_token;
-        // (no key behind the table's last place is looked for, however long a sequence says it is: a row that would see one is no number)
-        const int end_of_all = any ? min(length + last_token + 1, a.capacity) : 0;
-        const int begin_of_all = any && a.window ? min(max(0, length + first_token - a.window + 1), end_of_all) : 0;
-        // this part of them, whole spans
-        const int spans = (end_of_all + kSpan - 1) / kSpan - begin_of_all / kSpan, each = (spans + a.parts - 1) / a.parts;
-        begin = (begin_of_all / kSpan + part * each) * kSpan; end = min(end_of_all, begin + each * kSpan);
+        here_rows = 0;
+        kv = slot / all;
+        if (kv >= a.kv_heads) return;
+        const int count = min(rows_each, a.rows - row0);
+        const Cut cut = cut_of(a, row0, count, true, slot - kv * all);
+        b = cut.b;
+        if (b >= a.batch) return;                 // (more parts than the sequences need)
+        here_rows = count;
+        const Spans of(a, b, row0, count);
+        length = of.length; given = of.given;
+        begin = (of.begin / kSpan + (slot - kv * all - cut.first) * cut.each) * kSpan; end = min(of.end, begin + cut.each * kSpan);
     }
 };
 // Where a key's row lies, and whether it does.
@@ -184,7 +228,7 @@ __device__ __forceinline__ void finish(const CacheArgs& a, const Share& me, floa
         }
         const RowPlace at = place_of(a, me.kv, me.row0 + r);
         if (a.partial) {
-            const long to = ((long)me.head_at * a.rows + me.row0 + r) * a.parts + me.part;
+            const long to = (long)me.slot * a.rows + me.row0 + r;
             *reinterpret_cast<v4f*>(a.partial + to * quads * 4 + d) = sum;
             if (d == 0) a.partial_stats[to] = make_float2(total, most);
         } else {
@@ -653,13 +697,15 @@ __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs a)
     __shared__ v4f sums[kThreads];
     __shared__ float scales[kMostParts], tops[kWaves], totals[kWaves];
     const int quads = (a.values + 3) / 4, row = (int)blockIdx.x % a.rows, head_at = (int)blockIdx.x / a.rows, b = head_at / a.kv_heads, kv = head_at % a.kv_heads;
-    const long from = ((long)head_at * a.rows + row) * a.parts;
+    const int row0 = row / a.rows_each * a.rows_each;
+    const Cut cut = cut_of(a, row0, min(a.rows_each, a.rows - row0), false, b);
+    const auto at_part = [&](int p) { return ((long)kv * a.batch * a.parts + cut.first + p) * a.rows + row; };
     float2 mine[kMostParts / kThreads];
     float M = kNothing;
 #pragma unroll
     for (int i = 0; i < kMostParts / kThreads; ++i) {
         const int p = (int)threadIdx.x + i * kThreads;
-        mine[i] = p < a.parts ? a.partial_stats[from + p] : make_float2(0.0f, kNothing);
+        mine[i] = p < cut.parts ? a.partial_stats[at_part(p)] : make_float2(0.0f, kNothing);
         M = fmaxf(M, mine[i].y);
     }
     for (int s = 1; s < 64; s *= 2) M = fmaxf(M, __shfl_xor(M, s, 64));
@@ -672,7 +718,7 @@ __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs a)
     for (int i = 0; i < kMostParts / kThreads; ++i) {
         const int p = (int)threadIdx.x + i * kThreads;
         const float f = mine[i].y == kNothing ? 0.0f : scale_between(mine[i].y, M);
-        if (p < a.parts) scales[p] = f;
+        if (p < cut.parts) scales[p] = f;
         part_sum += mine[i].y == kNothing ? 0.0f : mine[i].x * f;
     }
     for (int s = 1; s < 64; s *= 2) part_sum += __shfl_xor(part_sum, s, 64);
@@ -684,8 +730,8 @@ __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs a)
     v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
     if (column < quads)
 #pragma unroll 4
-        for (int p = share; p < a.parts; p += shares) {
-            const v4f x = *reinterpret_cast<const v4f*>(a.partial + (from + p) * quads * 4 + column * 4);
+        for (int p = share; p < cut.parts; p += shares) {
+            const v4f x = *reinterpret_cast<const v4f*>(a.partial + at_part(p) * quads * 4 + column * 4);
             const float f = scales[p];
 #pragma unroll
             for (int c = 0; c < 4; ++c) sum[c] += f != 0.0f ? x[c] * f : 0.0f;
@@ -709,7 +755,7 @@ __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs a)
 
 // Rows of a work-group, how many work-groups the rows of a key head take, lanes of a group, parts of a sequence.
 struct CachePlan { int rows_each, sets, lanes, parts; };
-CachePlan cache_plan(long heads, long rows, long values, long capacity)
+CachePlan cache_plan(long batch, long heads, long rows, long values, long capacity)
 {
     CachePlan p;
     if (values % 4 != 0) p.rows_each = rows <= 1 ? 1 : 4;
@@ -723,7 +769,7 @@ CachePlan cache_plan(long heads, long rows, long values, long capacity)
     while (p.lanes * 4 < values) p.lanes *= 2;
     // (the work-groups that 256 compute units have at once; a part of less than a span for each wavefront is not worth a second kernel)
     const long units = std::max(1L, heads * p.sets), wanted = 256 * kGroupsAtOnce / units, most = (capacity + kWaves * kSpan - 1) / (kWaves * kSpan);
-    p.parts = (int)std::max(1L, std::min({wanted, most, (long)kMostParts}));
+    p.parts = (int)std::max(1L, std::min({wanted, most, (long)kMostParts / std::max(1L, std::min(batch, 64L))}));
     return p;
 }
 long padded(long values) { return (values + 3) / 4 * 4; }
@@ -760,7 +806,7 @@ size_t pam_hip_cached_attention_workspace_bytes(const pam_hip_cache_shape* s)
 {
     if (check_cache("cached_attention", s) != PAM_HIP_OK || s->batch * s->heads * s->tokens == 0) return 0;
     const long heads = s->batch * s->kv_heads, rows = s->heads / s->kv_heads * s->tokens;
-    return cache_bytes(cache_plan(heads, rows, s->dim, s->per_sequence * s->page), heads, rows, s->dim);
+    return cache_bytes(cache_plan(s->batch, heads, rows, s->dim, s->per_sequence * s->page), heads, rows, s->dim);
 }
 
 int pam_hip_cached_attention_fwd(const pam_hip_cache_shape* s, const pam_hip_tokens* q, const float* cache_k, const float* cache_v, long cache_sp, long cache_st,
@@ -782,8 +828,8 @@ int pam_hip_cached_attention_fwd(const pam_hip_cache_shape* s, const pam_hip_tok
     a.page = (int)s->page; a.pages = (int)s->pages; a.per_sequence = (int)s->per_sequence; a.capacity = (int)(s->per_sequence * s->page); a.window = (int)std::min(s->window, 1L << 30);
     a.scale = s->scale; a.cap = s->cap; a.off = s->offset;
     const long heads = s->batch * s->kv_heads;
-    const CachePlan p = cache_plan(heads, a.rows, a.values, s->per_sequence * s->page);
-    a.lanes = p.lanes; a.parts = p.parts; a.sets = p.sets;
+    const CachePlan p = cache_plan(s->batch, heads, a.rows, a.values, s->per_sequence * s->page);
+    a.lanes = p.lanes; a.parts = p.parts; a.sets = p.sets; a.rows_each = p.rows_each;
     const size_t need = cache_bytes(p, heads, a.rows, a.values);
     if (need && (!workspace || workspace_bytes < need)) return pamhost::fail(PAM_HIP_ERR_WORKSPACE, "cached_attention: workspace of %zu bytes needed", need);
     if (need) {

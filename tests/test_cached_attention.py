@@ -70,6 +70,9 @@ def _compare(batch, tokens, heads, kv_heads, dim, page, lengths, counts=None, se
 CASES = [  # batch, tokens, heads, kv heads, dim, page, lengths, counts
     (1, 1, 1, 1, 4, 1, [0], None), (1, 1, 4, 2, 64, 16, [37], None), (3, 1, 8, 2, 128, 64, [0, 63, 300], None), (2, 5, 3, 1, 80, 17, [100, 7], None),
     (2, 9, 4, 2, 32, 16, [5, 40], [9, 2]), (2, 3, 2, 1, 256, 4, [70, 0], [0, 3]), (1, 2, 6, 2, 100, 256, [513], None), (2, 1, 3, 3, 18, 5, [9, 64], None),
+    (70, 1, 2, 1, 32, 16, [(i * 37) % 300 for i in range(70)], None), (64, 1, 2, 2, 16, 16, [(i * 91) % 1100 for i in range(64)], [i % 2 for i in range(64)]),
+    (9, 6, 4, 1, 64, 32, [1500, 0, 700, 3, 64, 63, 65, 1, 128], [6, 6, 1, 2, 6, 6, 6, 0, 5]), (2, 11, 2, 1, 96, 16, [900, 100], None), (3, 2, 4, 1, 66, 16, [700, 64, 1], None),
+    (1, 5, 5, 1, 128, 64, [2000], None), (1, 3, 4, 1, 112, 64, [800], None), (1, 2, 8, 1, 8, 64, [800], None), (1, 1, 20, 1, 256, 64, [300], None),
     (1, 7, 6, 1, 48, 32, [129], None), (1, 1, 1, 1, 1, 3, [10], None), (1, 1, 2, 1, 16, 8, [5000], None), (4, 4, 16, 4, 24, 16, [1, 2, 3, 400], [4, 3, 1, 4]),
 ]
 
@@ -107,6 +110,12 @@ def test_values_out_of_the_ordinary(what):
             q[:, :, 1] = 0
     for rows in ((2, 1, 4, 2, 64), (1, 6, 4, 1, 64)):
         _compare(*rows, 8, [130] * rows[0], seed=6, change=change)
+
+
+@gpu
+@pytest.mark.parametrize("window", [1, 64, 65, 700])
+def test_windows_over_parts(window):
+    _compare(5, 2, 8, 2, 32, 16, [1400, 90, 0, 777, 64], [2, 2, 1, 2, 0], seed=9, window=window)
 
 
 @gpu
