@@ -2,7 +2,7 @@
 //
 // Bound by reading the cache once, or, where many rows share it, by the products.  A wavefront takes 64 keys at a time.  For the scores a lane owns a key, 32 of
 // its values in registers while the queries' rows come by in scalar registers (pam_attention.h): two instructions a product and no sums over
-// lanes, so that the keys are read once for up to 20 rows.  Then a lane per key makes the weights, and for the results a group of L lanes
+// lanes, so that the keys are read once for up to 12 rows.  Then a lane per key makes the weights, and for the results a group of L lanes
 // owns a key's row of values, a quad each (4 ... 64 lanes), and reads the rows' weights from LDS.  Every sequence's keys are cut into as
 // many parts as there are work-groups for it, by its own length; four wavefronts of a work-group take 64 keys in turn, their sums are put
 // together through LDS, and the parts' by a second kernel.  Scaling by powers of two is exact, so that none of this moves a result beyond the
@@ -17,7 +17,7 @@ using namespace pamatt;
 namespace {
 
 constexpr int kSteps = 4;                         // keys' rows in flight, of every lane
-constexpr int kMostParts = 512, kMostRows = 20;
+constexpr int kMostParts = 512, kMostRows = 12;
 typedef void (*Kernel)(struct CacheArgs);
 
 struct CacheArgs {
@@ -425,9 +425,9 @@ __global__ __launch_bounds__(kThreads, 4) void cached_attention_kernel(CacheArgs
 
 // ---------------------------------------------------------------- heads of whole quads
 
-// Work-groups that a compute unit has at once: two leave the registers that keep eight kilobytes of every wavefront on their way (three, with less on
-// its way: 16 sequences of up to 4000 tokens 55 us where two take 51).
-constexpr int kGroupsAtOnce = 2;
+// Work-groups that a compute unit has at once, what the registers leave room for.  (The next span's keys asked for before this one's values are added up, in two:
+// 16 sequences of up to 4000 tokens 47 us where three take 42; keys read a line by eight lanes and passed on through LDS 49.)
+constexpr int groups_at_once(int rows) { return rows <= 4 ? 3 : 2; }
 constexpr int kSlice = 8;                         // quads of a key in a lane's registers
 
 // Rows of queries, one after the other: a token's heads of this key head, then the next token's; the last one again behind the last.
@@ -450,10 +450,9 @@ struct Queries {
 };
 
 template <int ROWS, bool WHOLE>
-__global__ __launch_bounds__(kThreads, kGroupsAtOnce) void cached_rows_kernel(CacheArgs a)
+__global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_kernel(CacheArgs a)
 {
-    constexpr bool kEarly = ROWS <= 8;            // the next span's keys are asked for before this one's values are added up (more rows have no registers for them)
-    constexpr int kAhead = kEarly ? 8 : 4;        // rows of values that a lane has on their way
+    constexpr int kAhead = ROWS <= 4 ? 8 : 4;     // rows of values that a lane has on their way
     constexpr int kPad = ROWS < 4 ? ROWS : (ROWS + 3) / 4 * 4;
     __shared__ float weights[kWaves][kSpan][kPad];                               // a key's, of all rows: bits(weight) + mul_add
     __shared__ float sums[ROWS][256 + 4];
@@ -471,7 +470,7 @@ __global__ __launch_bounds__(kThreads, kGroupsAtOnce) void cached_rows_kernel(Ca
     const int* const table = a.table + (long)me.b * a.per_sequence;
     const float* const k = a.k + (long)me.kv * a.c_sh;
     const float* const v = a.v + (long)me.kv * a.c_sh;
-    // the first span's keys, and every other's while the values of the one before are added up, are on their way before anything waits
+    // the first span's keys are on their way before anything waits
     const auto load_keys = [&](long at, int slice, v4f (&x)[kSlice]) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < kSlice; ++n) x[n] = *reinterpret_cast<const v4f_any*>(k + at + 4 * (WHOLE ? slice * kSlice + n : min(slice * kSlice + n, quads - 1)));
@@ -591,8 +590,7 @@ __global__ __launch_bounds__(kThreads, kGroupsAtOnce) void cached_rows_kernel(Ca
         }
         v4f rows[kAhead];
         load_values(0, rows);
-        const KeyPlace after = place_of_span(j0 + kWaves * kSpan);
-        if (kEarly) load_keys(after.at, 0, next);
+        const KeyPlace after = place_of_span(j0 + kWaves * kSpan);               // (the table is read while the values are)
         // weights: a lane per key
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -681,7 +679,7 @@ __global__ __launch_bounds__(kThreads, kGroupsAtOnce) void cached_rows_kernel(Ca
         }
         wave_fence();                             // (the next span's weights go where these are)
         place = after;
-        if (!kEarly) load_keys(place.at, 0, next);
+        load_keys(place.at, 0, next);
     }
     if (!streams)
 #pragma unroll
@@ -768,7 +766,7 @@ CachePlan cache_plan(long batch, long heads, long rows, long values, long capaci
     p.lanes = values % 4 ? 4 : 8;
     while (p.lanes * 4 < values) p.lanes *= 2;
     // (the work-groups that 256 compute units have at once; a part of less than a span for each wavefront is not worth a second kernel)
-    const long units = std::max(1L, heads * p.sets), wanted = 256 * kGroupsAtOnce / units, most = (capacity + kWaves * kSpan - 1) / (kWaves * kSpan);
+    const long units = std::max(1L, heads * p.sets), wanted = 256 * groups_at_once(p.rows_each) / units, most = (capacity + kWaves * kSpan - 1) / (kWaves * kSpan);
     p.parts = (int)std::max(1L, std::min({wanted, most, (long)kMostParts / std::max(1L, std::min(batch, 64L))}));
     return p;
 }
@@ -849,8 +847,6 @@ int pam_hip_cached_attention_fwd(const pam_hip_cache_shape* s, const pam_hip_tok
         case 2: kernel = whole ? cached_rows_kernel<2, true> : cached_rows_kernel<2, false>; break;
         case 4: kernel = whole ? cached_rows_kernel<4, true> : cached_rows_kernel<4, false>; break;
         case 8: kernel = whole ? cached_rows_kernel<8, true> : cached_rows_kernel<8, false>; break;
-        case 12: kernel = whole ? cached_rows_kernel<12, true> : cached_rows_kernel<12, false>; break;
-        case 16: kernel = whole ? cached_rows_kernel<16, true> : cached_rows_kernel<16, false>; break;
         default: kernel = whole ? cached_rows_kernel<kMostRows, true> : cached_rows_kernel<kMostRows, false>; break;
         }
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, a);
