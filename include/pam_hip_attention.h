@@ -29,7 +29,7 @@ typedef struct { const float *p; long sb, st, sh; } pam_hip_tokens;
  * Weights below 2^-62 of the largest that came before them are none.  A score that is not a finite number, or is 2^127 or more, makes its query's
  * results NaN.  offset multiplies every PAM product and quotient, and lies in (0.75, 1.5); scale lies in (2^-40, 2^40), cap is 0 or in
  * (2^-20, 2^20).  dim is a multiple of four, up to 256, of which the first `values` values of every head
- * count and the others (at most three) may be anything. */
+ * count; the others (at most three) have to be 1 in keys and values and may be anything elsewhere. */
 typedef struct {
     long batch, tokens, keys, heads, kv_heads, dim, values;
     float scale, cap, offset;

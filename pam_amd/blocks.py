@@ -1,12 +1,12 @@
 """Modules of a decoder-only transformer in PAM arithmetic, made of the operators that a step of one runs next to each other:
-layer_norm, linear_act, rotary with the heads' norms, bmm and softmax, gated_linear.  For a training step the optimizer's side is
+layer_norm, linear_act, rotary with the heads' norms, bmm and softmax or attention, gated_linear.  For a training step the optimizer's side is
 `pam_amd.optim.clip_grad_norm_` and `pam_amd.optim.Adam`.
 """
 import math
 
 import torch
 
-from . import block_ops
+from . import attention_ops, block_ops
 from .composites import LayerNorm, softmax
 from .pam_ops import bmm, mul
 
@@ -35,14 +35,15 @@ class GatedFeedForward(torch.nn.Module):
 
 class Attention(torch.nn.Module):
     """x + out(attention(norm(x))), causal, `kv_heads` keys' and values' heads shared by `heads` queries' heads, queries and keys
-    normed per head and rotated.  cache: a dict that keeps keys and values of the tokens so far from call to call."""
+    normed per head and rotated.  cache: a dict that keeps keys and values of the tokens so far from call to call.  fused: by
+    pam.attention, which keeps no scores and repeats no heads, instead of products and a softmax (slightly different values)."""
 
-    def __init__(self, width, heads, kv_heads, dim, *, offset=None, approx_bwd=False):
+    def __init__(self, width, heads, kv_heads, dim, *, fused=False, offset=None, approx_bwd=False):
         super().__init__()
         if heads % kv_heads:
             raise ValueError(f"Attention: {heads} heads do not share {kv_heads}")
         self.kw = dict(offset=offset, approx_bwd=approx_bwd)
-        self.heads, self.kv_heads, self.dim = heads, kv_heads, dim
+        self.heads, self.kv_heads, self.dim, self.fused = heads, kv_heads, dim, fused
         self.norm = LayerNorm(width, **self.kw)
         self.qkv = _parameter((heads + 2 * kv_heads) * dim, width, std=width ** -0.5)
         self.q_weight, self.k_weight = (torch.nn.Parameter(torch.ones(dim)) for _ in range(2))
@@ -61,6 +62,9 @@ class Attention(torch.nn.Module):
             if seen:
                 k, v = torch.cat((cache["k"], k), 1), torch.cat((cache["v"], v), 1)
             cache["k"], cache["v"] = k, v
+        if self.fused:
+            y = attention_ops.attention(q, k, v, **self.kw).reshape(batch, tokens, -1)
+            return block_ops.linear_act(y, self.out, None, None, x, **self.kw)
 
         def by_head(t):                                # [batch, tokens, heads, dim] -> [batch heads, tokens, dim]
             t = t.repeat_interleave(self.heads // t.shape[2], 2)
@@ -78,10 +82,10 @@ class Attention(torch.nn.Module):
 class DecoderBlock(torch.nn.Module):
     """Attention, then GatedFeedForward, each behind a norm and on a residual."""
 
-    def __init__(self, width, heads, kv_heads, dim, hidden, activation="silu", *, offset=None, approx_bwd=False):
+    def __init__(self, width, heads, kv_heads, dim, hidden, activation="silu", *, fused=False, offset=None, approx_bwd=False):
         super().__init__()
         kw = dict(offset=offset, approx_bwd=approx_bwd)
-        self.attention = Attention(width, heads, kv_heads, dim, **kw)
+        self.attention = Attention(width, heads, kv_heads, dim, fused=fused, **kw)
         self.feed_forward = GatedFeedForward(width, hidden, activation, **kw)
 
     def forward(self, x, cos, sin, cache=None):

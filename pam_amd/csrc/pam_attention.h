@@ -60,6 +60,7 @@ struct Args {
     const float4* records;                        // [batch][kv_heads][rows]: M (+inf: the row sees nothing), dl, largest exponent of dn, slope
     const float* qs; const float* dn;             // [batch][kv_heads][rows][dim]
     float* out0; float* out1;                     // [batch][kv_heads][chunks][lanes' rows][dim]: dq, or dk and dv
+    unsigned char* met;                           // [batch][kv_heads][chunks][tiles of 64 rows]: a tile saw something of a chunk
     int whole;                                    // ... or, of one chunk, the gradients themselves, [batch][tokens][heads][dim] and [batch][keys][kv_heads][dim]
     ApproxFlags flags;
 };

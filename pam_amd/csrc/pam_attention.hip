@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
 }
 
 // dq from the chunks' sums, through q (*) scale; or dk and dv (the second half of the launch): nothing behind the sums.
-struct SumArgs { Args a; const float* parts[2]; float* out[2]; int of_keys; };
+struct SumArgs { Args a; const float* parts[2]; float* out[2]; int of_keys; long tiles; };          // tiles: of 64 rows
 __global__ __launch_bounds__(kThreads) void attention_sum_kernel(SumArgs s)
 {
     const Args& a = s.a;
@@ -110,9 +110,10 @@ __global__ __launch_bounds__(kThreads) void attention_sum_kernel(SumArgs s)
     const float* const parts = which ? s.parts[1] : s.parts[0];
     const long at = id / quads, head = at / lanes, row = at - head * lanes, b = head / a.kv_heads, kv = head - b * a.kv_heads;
     const int d = (int)(id - at * quads) * 4;
-    v4f sum = *reinterpret_cast<const v4f*>(parts + (head * a.chunks * lanes + row) * a.dim + d);
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int c = 1; c < a.chunks; ++c) sum += *reinterpret_cast<const v4f*>(parts + ((head * a.chunks + c) * lanes + row) * a.dim + d);
+    for (int c = 0; c < a.chunks; ++c)
+        if (a.met[(head * a.chunks + c) * s.tiles + row / 64]) sum += *reinterpret_cast<const v4f*>(parts + ((head * a.chunks + c) * lanes + row) * a.dim + d);
     long to;
     if (s.of_keys) to = (b * a.keys + row) * a.kv_heads + kv;
     else {
@@ -142,7 +143,8 @@ const Variant& variant_for(const Variant* list, long dim)
 // How the streamed rows are cut.  All units of a launch run at once or in a few turns of `slots` of them, so that a last turn of a few units costs as
 // much as a full one: among the cuts that fill one, two, ... turns the one is taken whose turns times its spans are least.  (4096 causal tokens, 8 heads over 2:
 // chunks of 256 keys, two turns and a bit, 0.70 ms.)  Which spans a tile sees is what the order and the window say; prefixes and documents are on the device.
-// A chunk is at least two spans, what a unit does besides its spans counts as a fifth of one.
+// A chunk is at least two spans (documents leave a tile little of what the order does, but chunks of one span cost 307 us where three take 267: 2 x 2048
+// tokens, heads of 128), what a unit does besides its spans counts as a fifth of one.
 struct Plan { int tiles, chunks, chunk; };
 long tiles_of(int slices) { return slices >= 4 ? 1 : 4 / slices; }              // of a work-group (kTiles)
 template <class Range>                            // range(first, last row of a tile, low, high): the streamed rows that those see
@@ -248,7 +250,7 @@ Plan forward_plan(const Args& a)
 Plan dq_plan(const Args& a) { return plan_for(heads_of(a), a.rows, variant_for(kDqApprox, a.dim).slices, a.keys, 3, OfRows{a}); }
 Plan dkv_plan(const Args& a) { return plan_for(heads_of(a), a.keys, variant_for(kDkvApprox, a.dim).slices, a.rows, 2, OfKeys{a}); }
 
-struct BackwardSpace { size_t records, qs, dn, dq, dk, dv, bytes; };
+struct BackwardSpace { size_t records, qs, dn, dq, dk, dv, met_q, met_kv, bytes; };
 BackwardSpace backward_space(const Args& a, bool want_q, bool want_kv)
 {
     BackwardSpace s{};
@@ -257,9 +259,10 @@ BackwardSpace backward_space(const Args& a, bool want_q, bool want_kv)
     const auto take = [&](size_t n) { const size_t from = at; at += align256(n); return from; };
     s.records = take(rows * sizeof(float4)); s.qs = take(rows * row); s.dn = take(rows * row);
     // (a pass of one chunk writes its gradients itself)
-    const int of_q = want_q ? dq_plan(a).chunks : 1, of_kv = want_kv ? dkv_plan(a).chunks : 1;
-    if (of_q > 1) s.dq = take(rows * row * of_q);
-    if (of_kv > 1) { s.dk = take(keys * row * of_kv); s.dv = take(keys * row * of_kv); }
+    const Plan of_q = want_q ? dq_plan(a) : Plan{0, 1, 0}, of_kv = want_kv ? dkv_plan(a) : Plan{0, 1, 0};
+    const auto flags = [&](const Plan& p) { return (size_t)heads_of(a) * p.chunks * p.tiles * tiles_of(variant_for(kDqApprox, a.dim).slices); };
+    if (of_q.chunks > 1) { s.dq = take(rows * row * of_q.chunks); s.met_q = take(flags(of_q)); }
+    if (of_kv.chunks > 1) { s.dk = take(keys * row * of_kv.chunks); s.dv = take(keys * row * of_kv.chunks); s.met_kv = take(flags(of_kv)); }
     s.bytes = at;
     return s;
 }
@@ -339,18 +342,18 @@ int pam_hip_attention_bwd(const pam_hip_attention_shape* shape, const pam_hip_to
         hipLaunchKernelGGL(attention_rows_kernel, dim3(groups), dim3(kThreads), 0, st, r);
         if ((rc = pamhost::check_launch("attention_bwd"))) return rc;
     }
-    const auto pass = [&](const Variant* list, const Plan& p, float* part0, float* part1, float* out0, float* out1, int of_keys, unsigned sum_groups) {
+    const auto pass = [&](const Variant* list, const Plan& p, float* part0, float* part1, float* out0, float* out1, size_t met, int of_keys, unsigned sum_groups) {
         Args d = a;
-        d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.whole = p.chunks == 1;
+        d.tiles = p.tiles; d.chunks = p.chunks; d.chunk = p.chunk; d.whole = p.chunks == 1; d.met = (unsigned char*)ws + met;
         d.out0 = d.whole ? out0 : part0; d.out1 = d.whole ? out1 : part1;
         const int failed = launch("attention_bwd", variant_for(list, a.dim), d, st);
         if (failed || d.whole) return failed;
-        hipLaunchKernelGGL(attention_sum_kernel, dim3(sum_groups), dim3(kThreads), 0, st, SumArgs{d, {part0, part1}, {out0, out1}, of_keys});
+        hipLaunchKernelGGL(attention_sum_kernel, dim3(sum_groups), dim3(kThreads), 0, st, SumArgs{d, {part0, part1}, {out0, out1}, of_keys, (long)p.tiles * tiles_of(variant_for(list, a.dim).slices)});
         return pamhost::check_launch("attention_bwd");
     };
-    if (dq && a.rows && (rc = pass(approximate ? kDqApprox : kDqExact, dq_plan(a), (float*)(ws + space.dq), nullptr, dq, nullptr, 0, row_groups))) return rc;
+    if (dq && a.rows && (rc = pass(approximate ? kDqApprox : kDqExact, dq_plan(a), (float*)(ws + space.dq), nullptr, dq, nullptr, space.met_q, 0, row_groups))) return rc;
     if (want_kv && a.keys
-        && (rc = pass(approximate ? kDkvApprox : kDkvExact, dkv_plan(a), (float*)(ws + space.dk), (float*)(ws + space.dv), dk, dv, 1, key_groups))) return rc;
+        && (rc = pass(approximate ? kDkvApprox : kDkvExact, dkv_plan(a), (float*)(ws + space.dk), (float*)(ws + space.dv), dk, dv, space.met_kv, 1, key_groups))) return rc;
     return PAM_HIP_OK;
 }
 

@@ -70,11 +70,12 @@ template <int W4, class F> __device__ __forceinline__ void each_of_row(const v4f
     });
 }
 
-// All blocks of a chunk of streamed rows, sums joined in memory after kLink of them; false: one block did not want to.
+// All blocks of a chunk of streamed rows, sums joined in memory after kLink of them; false: one block did not want to.  met: a row of the team saw one.
 template <int NS, int W4, int SUMS, class Start, class Block>
-__device__ __forceinline__ bool all_blocks(const Sight& sight, int begin, int end, float* const (&to)[SUMS], int first, int dim, bool exists, float (&out)[SUMS][4 * W4], Start&& start,
-                                           Block&& block)
+__device__ __forceinline__ bool all_blocks(const Sight& sight, int begin, int end, float* const (&to)[SUMS], int first, int dim, bool exists, float (&out)[SUMS][4 * W4], bool& met,
+                                           Start&& start, Block&& block)
 {
+    met = false;
     bool folded = false;
     int terms = 0;
 #pragma unroll
@@ -93,6 +94,7 @@ __device__ __forceinline__ bool all_blocks(const Sight& sight, int begin, int en
     for (int j0 = begin; j0 < end; j0 += kSpan) {
         const uint64_t see = sight.span(j0);
         if (!in_team<NS>(see != 0ull)) continue;
+        met = true;
         const bool all = __ballot(see != ~0ull) == 0ull;
         if (terms >= kLink) {
             with_memory([&](float& in_memory, float& sum) __attribute__((always_inline)) { in_memory = (folded ? in_memory : 0.0f) + sum; sum = 0.0f; });
@@ -106,6 +108,14 @@ __device__ __forceinline__ bool all_blocks(const Sight& sight, int begin, int en
     }
     if (folded) with_memory([&](float& in_memory, float& sum) __attribute__((always_inline)) { sum += in_memory; });
     return true;
+}
+
+// Whether a tile saw anything of its chunk is kept for those who put the chunks together: a tile that did not writes nothing, and is not read.
+template <int NS> __device__ __forceinline__ bool met_anything(const Args& a, const Unit& u, int wave, bool met)
+{
+    if (threadIdx.x % 64 == 0 && wave % NS == 0)
+        a.met[((long)u.head * a.chunks + u.chunk) * a.tiles * kTiles<NS> + u.tile * kTiles<NS> + wave / NS] = met;
+    return met;
 }
 
 template <int NS, int W4, bool WHOLE, bool APPROXIMATE>
@@ -155,6 +165,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
         return counts;
     };
     bool gave_up = false;                         // (what all of a tile's slices find behind the sums goes with the next ones)
+    bool met = false;
     const auto skip = [&](float (&s)[kBlock], float (&de)[kBlock]) __attribute__((always_inline)) {      // (no row of the tile sees the block: its barriers)
         const bool wild = slices_s.add_up(turn, wave, s, gave_up);
         if (wild) { turn ^= 1; return false; }
@@ -173,7 +184,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     if (!careful) {
         Pipe<W4, WHOLE> pipe;
         Look<W4, WHOLE> look_k, look_v;
-        careful = !all_blocks<NS, W4, 1>(sight, begin, end, to, first, a.dim, exists, out,
+        careful = !all_blocks<NS, W4, 1>(sight, begin, end, to, first, a.dim, exists, out, met,
             [&](int j0) __attribute__((always_inline)) { pipe.request(keys, j0); look_k.load(keys, j0); look_v.load(values, j0); },
             [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
                 float s[kBlock], de[kBlock], e[kBlock];
@@ -227,7 +238,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     }
     gave_up = false;
     if (__builtin_expect(careful, 0))
-        all_blocks<NS, W4, 1>(sight, begin, end, to, first, a.dim, exists, out, [](int) {}, [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
+        all_blocks<NS, W4, 1>(sight, begin, end, to, first, a.dim, exists, out, met, [](int) {}, [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
             float s[kBlock], de[kBlock], e[kBlock];
             if (!all && __ballot(sees != 0u) == 0ull) { skip(s, de); return true; }
             bool wrong = false;
@@ -266,6 +277,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
             }
             return true;
         });
+    if (!a.whole && !met_anything<NS>(a, u, wave, met)) return;
     const float back = 1.0f / unit;
 #pragma unroll
     for (int d = 0; d < W; ++d) out[0][d] *= back;
@@ -350,6 +362,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
         return counts;
     };
     bool gave_up = false;                         // (what all of a tile's slices find behind the sums goes with the next ones)
+    bool met = false;
     const auto skip = [&](float (&s)[kBlock], float (&de)[kBlock]) __attribute__((always_inline)) {      // (no row of the tile sees the block: its barriers)
         const bool wild = slices_s.add_up(turn, wave, s, gave_up);
         if (wild) { turn ^= 1; return false; }
@@ -369,7 +382,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     if (!careful) {
         Pipe<W4, WHOLE> pipe;
         Look<W4, WHOLE> look_q, look_n;
-        careful = !all_blocks<NS, W4, 2>(sight, begin, end, to, first, a.dim, exists, out,
+        careful = !all_blocks<NS, W4, 2>(sight, begin, end, to, first, a.dim, exists, out, met,
             [&](int r0) __attribute__((always_inline)) { pipe.request(queries, r0); look_q.load(queries, r0); look_n.load(grads, r0); },
             [&](int r1, uint32_t sees, bool all) __attribute__((always_inline)) {
                 float s[kBlock], de[kBlock], e[kBlock];
@@ -433,7 +446,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     }
     gave_up = false;
     if (__builtin_expect(careful, 0))
-        all_blocks<NS, W4, 2>(sight, begin, end, to, first, a.dim, exists, out, [](int) {}, [&](int r1, uint32_t sees, bool all) __attribute__((always_inline)) {
+        all_blocks<NS, W4, 2>(sight, begin, end, to, first, a.dim, exists, out, met, [](int) {}, [&](int r1, uint32_t sees, bool all) __attribute__((always_inline)) {
             float s[kBlock], de[kBlock], e[kBlock];
             if (!all && __ballot(sees != 0u) == 0ull) { skip(s, de); return true; }
             bool wrong = false;
@@ -479,6 +492,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
             }
             return true;
         });
+    if (!a.whole && !met_anything<NS>(a, u, wave, met)) return;
     const float back = 1.0f / unit;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {

@@ -53,7 +53,7 @@ def _compare(shape, masks, seed=0, approx=True, train=True, spread=1.0, change=N
 
 SHAPES = [  # batch, tokens, keys, heads, kv heads, dim
     (1, 1, 1, 1, 1, 4), (2, 3, 3, 2, 1, 18), (1, 70, 70, 3, 3, 64), (2, 33, 65, 4, 2, 16), (1, 129, 200, 2, 2, 100), (1, 5, 130, 6, 2, 80), (1, 64, 64, 2, 1, 128),
-    (1, 40, 40, 1, 1, 96), (1, 67, 67, 2, 2, 256), (1, 50, 50, 2, 1, 130), (1, 17, 17, 1, 1, 1), (1, 33, 70, 3, 1, 48), (1, 20, 9, 2, 2, 32),
+    (1, 4, 4, 2, 2, 256), (1, 3, 5, 2, 1, 130), (1, 5, 5, 2, 2, 192), (1, 70, 300, 1, 1, 112), (3, 300, 300, 4, 1, 20), (1, 40, 40, 1, 1, 96), (1, 67, 67, 2, 2, 256), (1, 50, 50, 2, 1, 130), (1, 17, 17, 1, 1, 1), (1, 33, 70, 3, 1, 48), (1, 20, 9, 2, 2, 32),
 ]
 
 
