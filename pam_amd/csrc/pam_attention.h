@@ -8,13 +8,17 @@
 // M has been on the way.  (The softmax of the primitives subtracts the largest of all rows' scores, which is no whole number, and moves the
 // result with it.)
 //
-// A wavefront's lanes own 64 rows (queries; in the pass for dk and dv, keys), a slice of at most 32 of a row's values in a lane's registers, and the
-// other side streams by in scalar registers, that all lanes read: a product takes two instructions on 64 lanes, an integer addition and
-// a float addition, and nothing else.  One piece of a streamed row (at most 20 values) is used while the next one is on its way, wherever that
-// is: in this row, the next or the next phase's.  Longer rows are cut into slices with a wavefront each, which add up their parts of a score
-// through LDS: wider slices would do less twice, but leave room for two wavefronts on a SIMD, which did not cover the scalar loads.
+// A wavefront's lanes own 64 rows (queries; in the pass for dk and dv, keys), a slice of at most 64 of a row's values (32 in the gradients' passes, which hold
+// three or four of them) in a lane's registers, and the other side streams by in scalar registers, that all lanes read: a product takes two
+// instructions on 64 lanes, an integer addition and a float addition, and nothing else.  One piece of a streamed row (at most 20 values) is used
+// while the next one is on its way, wherever that is: in this row, the next or the next phase's; pieces of 32 took scalar registers from
+// everything else (forward 0.94, gradients 0.87 times as fast).  Longer rows are cut into slices with a wavefront each, which add up their parts of
+// a score through LDS.  A work-group's wavefronts stream the same rows, so that the scalar cache has them.
 // Rates of the inner loop alone, two wavefronts per SIMD: 28 T products/s; with the streamed values read from another lane inside the integer
 // addition (a data-parallel primitive: everything around it issues half as fast) 18.6; copied out of one once for four rows 20.5; by lane reads 12.
+// Whole passes: forward 18.7 T products/s where every row sees 4096 keys, 13.2 where the order is causal (the last turn of units is not full),
+// gradients 14.5 and 11: a sixth to a third of the instructions are the weights', which slices make twice, and two or three wavefronts on a SIMD do not
+// cover all waits for the scalar cache.
 //
 // The integer addition is the product while no exponent leaves the normal range.  Streamed values have to be in 2^[-40, 40), a lane's in 2^[-86, 80); a
 // lane's zero stands as 2^-86, which adds less to a sum than its rounding.  Streamed rows with zeros take a loop that leaves those out by a factor.
@@ -306,6 +310,26 @@ template <int N> __device__ __forceinline__ void add_lane_power_piece(const Piec
     if constexpr (N % 8 != 0)
         asm(PAM_EACH4(PAM_OF_LANE) PAM_EACH4(PAM_POWER) PAM_EACH4(PAM_ADD_BY_ROW) : PAM_O4(N - 4), PAM_T4 : PAM_S4(N - 4), PAM_M4(N - 4), [w] "v"(w), [mask] "v"(mask));
 }
+
+#undef PAM_ADD_BY_ROW
+#undef PAM_ADD
+#undef PAM_SUM_BY_ROW
+#undef PAM_SUM_BY_LANE
+#undef PAM_SUM
+#undef PAM_POWER
+#undef PAM_OF_LANE
+#undef PAM_OF_WEIGHT
+#undef PAM_OF_ROW
+#undef PAM_EACH8
+#undef PAM_EACH4
+#undef PAM_O8
+#undef PAM_O4
+#undef PAM_M8
+#undef PAM_M4
+#undef PAM_S8
+#undef PAM_S4
+#undef PAM_T4
+#undef PAM_T8
 
 // A row's block as one lane in eight sees it: every value of the slice in one lane.
 template <int W4, bool WHOLE> struct Look {
