@@ -554,6 +554,17 @@ struct Sight {
     }
 };
 
+// Whether a row of the team sees one of the rows begin ... end - 1: looked at before anything else is loaded, since half of the units of a causal pass
+// see none.
+template <int NS> __device__ __forceinline__ bool any_seen(const Sight& sight, int begin, int end)
+{
+    if (!sight.with_documents) return begin < end;
+#pragma unroll 1
+    for (int j0 = begin; j0 < end; j0 += kSpan)
+        if (in_team<NS>(sight.span(j0) != 0ull)) return true;
+    return false;
+}
+
 // ---------------------------------------------------------------- from a score to its exponent
 
 // x (*) a positive constant, whose bits less the bias (offset counted) are `add`.  Underflow is zero; NaN and infinities are not numbers afterwards.

@@ -129,6 +129,10 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     const int wave = wave_of(), slice = wave % NS, row0 = (u.tile * kTiles<NS> + wave / NS) * 64, mine = row0 + (int)threadIdx.x % 64, row = min(mine, a.rows - 1), first = slice * W;
     const bool exists = mine < a.rows;
     const int pos = a.first + row / a.group;
+    Sight sight = sight_of_row(a, u.b, row);
+    sight.close_team<NS>();
+    const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
+    if (!a.whole && !any_seen<NS>(sight, begin, end)) { met_anything<NS>(a, u, wave, false); return; }
     const Scoring scoring(a);
     const PairGrad<APPROXIMATE> pair{scoring, a.flags};
     const uint32_t dn_add = APPROXIMATE ? scoring.mul_add : 0u;
@@ -143,14 +147,11 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     // (all slopes, and no offset: what the usual way of the other kernel has)
     const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
     bool careful = in_team<NS>(odd && M != u2f(kExpo)) || unusual;
-    Sight sight = sight_of_row(a, u.b, row);
-    sight.close_team<NS>();
     const Stream<WHOLE> keys(a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.keys, slice * W4, a.dim / 4);
     const Stream<WHOLE> values(a.v.p + (long)u.b * a.v.sb + (long)u.kv * a.v.sh, a.v.st, a.keys, slice * W4, a.dim / 4);
     float out[1][W];
     const int head = u.kv * a.group + row % a.group;
     float* const to[1] = {a.out0 + (a.whole ? ((long)u.b * a.tokens + row / a.group) * a.heads + head : ((long)u.head * a.chunks + u.chunk) * a.rows + row) * a.dim};
-    const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
     int turn = 0;
     // weights from scores, and which ones count (what is no number does)
     const auto weigh = [&](const float (&s)[kBlock], float (&e)[kBlock], uint32_t sees, bool all, int j1, bool& wrong) __attribute__((always_inline)) {
@@ -320,12 +321,16 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     u.tile = a.tiles - 1 - u.tile;                // (the first keys have most queries where the order is causal)
     const int wave = wave_of(), slice = wave % NS, lane = (int)threadIdx.x % 64, key0 = (u.tile * kTiles<NS> + wave / NS) * 64, mine = key0 + lane, key = min(mine, a.keys - 1), first = slice * W;
     const bool exists = mine < a.keys;
+    const int chunk_begin = u.chunk * a.chunk, chunk_end = min(a.rows, chunk_begin + a.chunk);
+    Sight sight = sight_of_key(a, u.b, key);
+    sight.close_team<NS>();
+    const int begin = max(sight.first / kSpan * kSpan, chunk_begin), end = min(min(sight.last, a.rows), chunk_begin + a.chunk);
+    if (!a.whole && !any_seen<NS>(sight, begin, end)) { met_anything<NS>(a, u, wave, false); return; }
     const Scoring scoring(a);
     const PairGrad<APPROXIMATE> pair{scoring, a.flags};
     typedef const __attribute__((address_space(4))) float4* Records;
     const float4* const all_records = a.records + (long)u.head * a.rows;
     const auto record = [&](int r) __attribute__((always_inline)) { const Records from = (Records)(all_records + min(r, a.rows - 1)); return make_float4(from->x, from->y, from->z, from->w); };
-    const int chunk_begin = u.chunk * a.chunk, chunk_end = min(a.rows, chunk_begin + a.chunk);
     // the largest |dn| of the chunk's rows is scaled to [1, 2)
     int most = -86;
     for (int r = chunk_begin + lane; r < chunk_end; r += 64) most = max(most, (int)all_records[r].z);
@@ -340,14 +345,11 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     odd = !load_lane<W4>(a.v.p + (long)u.b * a.v.sb + (long)key * a.v.st + (long)u.kv * a.v.sh, first, a.dim, a.values, 0u, scoring.mul_add + shift, v) || odd;
     const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
     bool careful = in_team<NS>(odd) || unusual;
-    Sight sight = sight_of_key(a, u.b, key);
-    sight.close_team<NS>();
     const Stream<WHOLE> queries(a.qs + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);
     const Stream<WHOLE> grads(a.dn + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);
     float out[2][W];                              // dk, dv
     const long at = (a.whole ? ((long)u.b * a.keys + key) * a.kv_heads + u.kv : ((long)u.head * a.chunks + u.chunk) * a.keys + key) * a.dim;
     float* const to[2] = {a.out0 + at, a.out1 + at};
-    const int begin = max(sight.first / kSpan * kSpan, chunk_begin), end = min(min(sight.last, a.rows), chunk_begin + a.chunk);
     int turn = 0;
     const auto weigh = [&](const float (&s)[kBlock], float (&e)[kBlock], uint32_t sees, bool all, int r1, bool& wrong) __attribute__((always_inline)) {
         uint32_t counts = 0u;

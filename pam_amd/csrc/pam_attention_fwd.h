@@ -89,6 +89,15 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
     const int wave = wave_of(), slice = wave % NS, row0 = (u.tile * kTiles<NS> + wave / NS) * 64, mine = row0 + (int)threadIdx.x % 64, row = min(mine, a.rows - 1), first = slice * W;
     const bool exists = mine < a.rows;
     const int token = row / a.group, head = u.kv * a.group + row % a.group, pos = a.first + token;
+    Sight sight = sight_of_row(a, u.b, row);
+    sight.close_team<NS>();
+    const long stat = ((long)u.head * a.chunks + u.chunk) * a.rows + row;
+    float* const to = a.partial ? a.partial + stat * a.dim : a.y + (((long)u.b * a.tokens + token) * a.heads + head) * a.dim;
+    const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
+    if (a.partial && !any_seen<NS>(sight, begin, end)) {
+        if (exists && slice == 0) a.partial_stats[stat] = make_float2(0.0f, kNothing);
+        return;
+    }
     const Scoring scoring(a);
     const Full full{a.off, a.off != 1.0f, 0u - scoring.mul_add};
     uint32_t q[W];
@@ -108,14 +117,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
     }
     float slope = 0.0f, wrong = 0.0f;             // wrong: becomes NaN with the first number that is none
     if (scoring.slopes) { slope = held_slope(a.slopes[head]); wrong = finite(a.slopes[head]) ? 0.0f : u2f(kQNaN); }
-    Sight sight = sight_of_row(a, u.b, row);
-    sight.close_team<NS>();
     const Stream<WHOLE> keys(a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.keys, slice * W4, a.dim / 4);
     const Stream<WHOLE> values(a.v.p + (long)u.b * a.v.sb + (long)u.kv * a.v.sh, a.v.st, a.keys, slice * W4, a.dim / 4);
-    const long stat = ((long)u.head * a.chunks + u.chunk) * a.rows + row;
-    float* const to = a.partial ? a.partial + stat * a.dim : a.y + (((long)u.b * a.tokens + token) * a.heads + head) * a.dim;
-    const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
-
     float out[W], l, l_before, M, M_folded;
     bool some, folded;
     int terms, turn = 0;
