@@ -286,7 +286,7 @@ int pam_hip_attention_fwd(const pam_hip_attention_shape* shape, const pam_hip_to
 {
     Args a{};
     int rc = check("attention_fwd", shape, a);
-    if (rc != PAM_HIP_OK || a.batch == 0 || a.rows == 0) return rc;
+    if (rc != PAM_HIP_OK || a.batch == 0 || a.kv_heads == 0 || a.rows == 0) return rc;
     if (!q || !k || !v || !q->p || !y || (a.keys && (!k->p || !v->p))) return pamhost::fail(PAM_HIP_ERR_ARGUMENT, "attention_fwd: null pointer");
     const size_t need = pam_hip_attention_workspace_bytes(shape);
     if (need && (!workspace || workspace_bytes < need)) return pamhost::fail(PAM_HIP_ERR_WORKSPACE, "attention_fwd: workspace of %zu bytes needed", need);

@@ -4,6 +4,10 @@ Bounds: half a step of a float32 is EPS = 2^-24.  A piecewise-affine product or 
 in an operand, 2^t by at most 2^t per unit of t, and a sum of n terms in any order by n EPS times the sum of their magnitudes.
 Below 2^-126 a float32's step is 2^-149 whatever its size (STEP): each of the dim terms of dl, dl's own sum and de are off by up to one more,
 and so is each result.
+
+An exact gradient's slopes are powers of two that step where a factor passes from one piece into the next.  Where a factor is closer to such a border than
+it may be off, 32 bits may have the slope of either side: the step's size, what the slope changes by between the factor less and plus its bound, times
+what it weighs, is added to the bound (`moved`) where a test asks for it (`borders`); most inputs have no such pair.  One pair in some ten thousand is that close (2^t with t within 1e-6 of a whole number).
 """
 import numpy as np
 
@@ -42,6 +46,16 @@ def slope(other, own):
     return np.where(other == 0, 0.0, np.sign(other) * np.ldexp(1.0, (eo - 1 + carry).astype(int)))
 
 
+def moved(f, x, off):
+    """What a step function changes by within x - off ... x + off."""
+    here = f(x)
+    return np.maximum(np.abs(f(x + off) - here), np.abs(f(np.maximum(x - off, np.where(x > 0, 0.5 * x, -np.inf))) - here))
+
+
+def power(x):
+    return np.ldexp(1.0, np.where(x == 0, -300, floor_log2(np.where(x == 0, 1.0, x))).astype(int))
+
+
 class Head:
     """One batch entry's query head: q [tokens, dim], k and v [keys, dim], see [tokens, keys], far the distances."""
 
@@ -66,7 +80,7 @@ class Head:
             far = np.abs(np.arange(keys - tokens, keys)[:, None] - np.arange(keys)[None]).astype(float)
             bias = mul(float(np.float32(slope)), far)
             x, x_off = x - bias, x_off + 2.0 * EPS * (np.abs(x) + np.abs(bias))
-        self.x = x
+        self.x, self.x_off = x, x_off
         t = mul(x, LOG2E)
         t_off = 2.0 * x_off + 2.0 * EPS * np.abs(t)
         self.some = see.any(1, keepdims=True)
@@ -77,11 +91,11 @@ class Head:
         self.l = np.where(self.some, self.e.sum(1, keepdims=True), 1.0)
         self.l_off = self.e_off.sum(1, keepdims=True) + keys * EPS * self.l
         self.n, size = product(self.e, v)
-        n_off = 2.0 * product(self.e_off, np.abs(v))[0] + (keys + 2) * EPS * size
+        self.n_off = n_off = 2.0 * product(self.e_off, np.abs(v))[0] + (keys + 2) * EPS * size
         self.y = div(self.n, self.l)
         self.y_off = 2.0 * (n_off / self.l + np.abs(self.y) * (self.l_off / self.l + EPS))
 
-    def grads(self, dy, approx=True):
+    def grads(self, dy, approx=True, borders=False):
         """dq, dk, dv and how far each may be off."""
         dy = np.asarray(dy, float)
         keys, dim = self.k.shape
@@ -93,20 +107,31 @@ class Head:
             dn = dy * slope(div(1.0, self.l), self.n)
             part = dy * np.ldexp(np.sign(self.y), (floor_log2(self.y) - floor_log2(self.l)).astype(int))
         dn_off = np.abs(dn) * (4.0 * rel_l + 4.0 * EPS)
+        borders = borders and not approx
+        if borders:
+            inverse = div(1.0, self.l)
+            dn_off = dn_off + np.abs(dy) * (moved(lambda n: slope(inverse, n), self.n, self.n_off) + moved(lambda i: slope(i, self.n), inverse, 2.0 * inverse * (rel_l + EPS)))
         dl = -part.sum(1, keepdims=True)
         dl_off = (np.abs(part) * (6.0 * rel_l + (dim + 4) * EPS)).sum(1, keepdims=True) + 4.0 * (self.y_off / self.l * np.abs(dy)).sum(1, keepdims=True) + (dim + 1) * STEP
+        if borders:
+            quotient = moved(power, np.abs(self.y), self.y_off) / power(self.l) + power(self.y) * moved(lambda l: 1.0 / power(l), self.l, self.l_off)
+            dl_off = dl_off + 2.0 * (np.abs(dy) * quotient).sum(1, keepdims=True)
         if approx:
             p, size = product(dn, self.v.T)
         else:
             terms = dn[:, None, :] * slope(self.v[None], self.e[:, :, None])
             p, size = terms.sum(2), np.abs(terms).sum(2)
+            de_moved = 0.0 if not borders else (np.abs(dn)[:, None, :] * moved(lambda e: slope(self.v[None], e), self.e[:, :, None], self.e_off[:, :, None])).sum(2)
         de = p + dl
-        de_off = 2.0 * product(dn_off, np.abs(self.v.T))[0] + (dim + 3) * EPS * size + dl_off + EPS * np.abs(de) + STEP
+        de_off = 2.0 * product(dn_off, np.abs(self.v.T))[0] + (dim + 3) * EPS * size + dl_off + EPS * np.abs(de) + STEP + (0.0 if approx else de_moved)
         if approx:
             da = mul(self.e, de)
         else:
             da = np.ldexp(1.0, np.where(self.see, floor_log2(np.where(self.see, self.e, 1.0)), -300).astype(int)) * de * slope(LOG2E, self.x)
         da_off = 2.0 * (self.e_off * np.abs(de) + self.e * de_off) * 2.0 + 2.0 * EPS * np.abs(da)
+        if borders:
+            by_score = slope(LOG2E, self.x)
+            da_off = da_off + np.abs(de) * (moved(power, self.e, self.e_off) * by_score + power(self.e) * moved(lambda x: slope(LOG2E, x), self.x, self.x_off)) * 2.0
         if self.cap:
             m = 1.0 + self.w
             if approx:
@@ -141,11 +166,12 @@ class Head:
         else:
             terms = dn[None] * slope(self.e.T[:, :, None], self.v[:, None, :])
             dv, size = terms.sum(1), np.abs(terms).sum(1)
-        dv_off = 2.0 * (product(self.e_off.T, np.abs(dn))[0] + product(self.e.T, dn_off)[0]) + (self.e.shape[0] + 2) * EPS * size
+            dv_moved = 0.0 if not borders else (np.abs(dn)[None] * moved(lambda e: slope(e, self.v[:, None, :]), self.e.T[:, :, None], self.e_off.T[:, :, None])).sum(1)
+        dv_off = 2.0 * (product(self.e_off.T, np.abs(dn))[0] + product(self.e.T, dn_off)[0]) + (self.e.shape[0] + 2) * EPS * size + (0.0 if approx else dv_moved)
         return (dq, dk, dv), (dq_off + STEP, dk_off + STEP, dv_off + STEP)
 
 
-def attention(q, k, v, dy=None, approx=True, causal=True, window=None, prefix=None, documents=None, slopes=None, cap=None, scale=None):
+def attention(q, k, v, dy=None, approx=True, causal=True, window=None, prefix=None, documents=None, slopes=None, cap=None, scale=None, borders=False):
     """[batch, tokens, heads, dim]: y and its bound, with dy also the gradients for q, k, v and theirs."""
     batch, tokens, heads, dim = q.shape
     keys, group = k.shape[1], heads // k.shape[2]
@@ -158,7 +184,7 @@ def attention(q, k, v, dy=None, approx=True, causal=True, window=None, prefix=No
             head = Head(q[b, :, h], k[b, :, h // group], v[b, :, h // group], see, None if slopes is None else slopes[h], cap, scale)
             y[b, :, h], y_off[b, :, h] = head.y, head.y_off
             if dy is not None:
-                parts, off = head.grads(dy[b, :, h], approx)
+                parts, off = head.grads(dy[b, :, h], approx, borders)
                 grads[0][b, :, h], offs[0][b, :, h] = parts[0], off[0]
                 for i in (1, 2):
                     grads[i][b, :, h // group] += parts[i]

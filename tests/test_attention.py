@@ -39,12 +39,12 @@ def _run(q, k, v, dy, masks, approx=True):
     return (y, torch.autograd.grad(y, leaves, _cuda(dy))) if dy is not None else (y, None)
 
 
-def _compare(shape, masks, seed=0, approx=True, train=True, spread=1.0, change=None):
+def _compare(shape, masks, seed=0, approx=True, train=True, spread=1.0, change=None, borders=False):
     q, k, v, dy = _inputs(seed, *shape, spread=spread)
     if change:
         change(q, k, v, dy)
     y, grads = _run(q, k, v, dy if train else None, masks, approx)
-    want = ref.attention(q, k, v, dy if train else None, approx, **masks)
+    want = ref.attention(q, k, v, dy if train else None, approx, borders=borders, **masks)
     _check(y, want[0], want[1], "y")
     for name, got, w, off in zip("qkv", grads or (), *(want[2:] if train else ((), ()))):
         _check(got, w, off, "d" + name)
@@ -147,6 +147,65 @@ def test_values_out_of_the_ordinary(what):
         else:
             q.reshape(-1)[100] = 0; k.reshape(-1)[200] = 0; v.reshape(-1)[300] = 0; dy.reshape(-1)[400] = 0
     _compare((1, 70, 70, 2, 1, 64), {}, seed=3, change=change)
+
+
+def _odd(what):
+    def change(q, k, v, dy):
+        rng = np.random.RandomState(8)
+        if what == "zeros_in_keys":
+            k[rng.random_sample(k.shape) < 0.05] = 0
+        elif what == "zeros_in_values":
+            v[rng.random_sample(v.shape) < 0.3] = 0
+        elif what == "zeros_everywhere":
+            for x in (q, k, v, dy):
+                x[rng.random_sample(x.shape) < 0.1] = 0
+        elif what == "zero_queries_large_keys":                       # (a zero times anything is zero)
+            q[..., : q.shape[3] // 2] = 0; k[..., : k.shape[3] // 2] *= np.float32(2.0 ** 100)
+        elif what == "no_gradient_for_some":
+            dy[:, ::3] = 0
+        elif what == "powers":                                        # (2^-86 stands for zero in a lane)
+            q[:] = np.float32(2.0 ** -86) * np.sign(q); k[:] = np.float32(2.0 ** 85) * np.sign(k)
+    return change
+
+
+@gpu
+@pytest.mark.parametrize("approx", [True, False])
+@pytest.mark.parametrize("what", ["zeros_in_keys", "zeros_in_values", "zeros_everywhere", "zero_queries_large_keys", "no_gradient_for_some", "powers"])
+@pytest.mark.parametrize("dim", [16, 64, 100])
+def test_zeros_and_powers_in_either_side(dim, what, approx):
+    _compare((1, 45, 70, 2, 1, dim), {}, seed=dim, approx=approx, change=_odd(what), borders=True, train=what not in ("zero_queries_large_keys", "powers"))
+
+
+@gpu
+def test_sizes_of_nothing():
+    pam = _host()
+    def t(*shape):
+        return torch.randn(*shape, device="cuda")
+    assert pam.attention(t(0, 3, 2, 8), t(0, 3, 1, 8), t(0, 3, 1, 8)).shape == (0, 3, 2, 8)
+    assert pam.attention(t(2, 0, 2, 8), t(2, 3, 1, 8), t(2, 3, 1, 8)).shape == (2, 0, 2, 8)
+    assert (pam.attention(t(2, 3, 2, 8), t(2, 0, 1, 8), t(2, 0, 1, 8)) == 0).all()
+    assert pam.attention(t(2, 3, 0, 8), t(2, 3, 0, 8), t(2, 3, 0, 8)).shape == (2, 3, 0, 8)
+    for q, k in (((2, 3, 2, 8), (2, 0, 1, 8)), ((2, 0, 2, 8), (2, 3, 1, 8)), ((0, 3, 2, 8), (0, 3, 1, 8))):
+        leaves = [t(*s).requires_grad_() for s in (q, k, k)]
+        y = pam.attention(*leaves, approx_bwd=True)
+        for g, leaf in zip(torch.autograd.grad(y, leaves, torch.ones_like(y)), leaves):
+            assert g.shape == leaf.shape and (g == 0).all()
+
+
+@gpu
+def test_shared_and_broadcast_inputs():
+    """One tensor as keys and values, one batch entry for all, and odd numbers of heads that share a key's."""
+    pam = _host()
+    q, k = torch.randn(3, 20, 7, 36, device="cuda", requires_grad=True), torch.randn(1, 20, 1, 36, device="cuda", requires_grad=True)
+    dy = torch.randn(3, 20, 7, 36, device="cuda")
+    kb = k.expand(3, -1, -1, -1)
+    got = torch.autograd.grad(pam.attention(q, kb, kb, approx_bwd=True), (q, k), dy)
+    kc, vc = (k.detach().repeat(3, 1, 1, 1).requires_grad_() for _ in range(2))
+    want = torch.autograd.grad(pam.attention(q, kc, vc, approx_bwd=True), (q, kc, vc), dy)
+    assert torch.equal(got[0], want[0]) and got[1].shape == k.shape
+    sum_of = (want[1].double() + want[2].double()).sum(0, keepdim=True)
+    size = (want[1].abs() + want[2].abs()).sum(0, keepdim=True).double()
+    assert ((got[1] - sum_of).abs() <= 6 * 2.0 ** -24 * size).all()       # (a sum of six)
 
 
 @gpu

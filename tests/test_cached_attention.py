@@ -113,6 +113,22 @@ def test_values_out_of_the_ordinary(what):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [(1, 1), (2, 4), (3, 4), (6, 4)])
+@pytest.mark.parametrize("what", ["values", "keys", "queries", "all", "wild"])
+def test_zeros_and_wild_values(rows, what):
+    def change(q, k, v):
+        rng = np.random.RandomState(5)
+        for name, x in (("queries", q), ("keys", k), ("values", v)):
+            if what in (name, "all"):
+                x[rng.random_sample(x.shape) < 0.1] = 0
+        if what == "wild":
+            v[:, 2] *= np.float32(2.0 ** 60); k[1::3, 1] *= np.float32(2.0 ** -100); q[:, 0, 0] *= np.float32(2.0 ** -70)
+    tokens, heads = rows
+    _compare(2, tokens, heads, 1, 64, 16, [150, 300], seed=7, change=change)
+    _compare(1, tokens, heads, 1, 20, 16, [150], seed=7, change=change)
+
+
+@gpu
 @pytest.mark.parametrize("window", [1, 64, 65, 700])
 def test_windows_over_parts(window):
     _compare(5, 2, 8, 2, 32, 16, [1400, 90, 0, 777, 64], [2, 2, 1, 2, 0], seed=9, window=window)
