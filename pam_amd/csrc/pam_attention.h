@@ -300,6 +300,23 @@ template <int N> __device__ __forceinline__ void add_power_piece(const Piece& x,
     if constexpr (N % 8 != 0)
         asm(PAM_EACH4(PAM_OF_ROW) PAM_EACH4(PAM_POWER) PAM_EACH4(PAM_ADD) : PAM_O4(N - 4), PAM_T4 : PAM_S4(N - 4), PAM_M4(N - 4), [f] "v"(f), [mask] "v"(mask));
 }
+// ... of a row with zeros, whose slopes are none
+template <int N> __device__ __forceinline__ void dot_power_piece_with_zeros(const Piece& x, uint32_t w, uint32_t mask, const uint32_t* m, float& sum)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool none = (f2u(at(x, i)) << 1) == 0u;
+        sum = __builtin_fmaf(u2f(((none ? kBias : f2u(at(x, i))) + w) & (none ? 0u : mask)), u2f(m[i]), sum);
+    }
+}
+template <int N> __device__ __forceinline__ void add_power_piece_with_zeros(const Piece& x, float f, uint32_t mask, const uint32_t* m, float* o)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool none = (f2u(at(x, i)) << 1) == 0u;
+        o[i] = __builtin_fmaf(u2f(((none ? kBias : f2u(at(x, i))) + m[i]) & (none ? 0u : mask)), f, o[i]);
+    }
+}
 // out_d += row's d * power(weight (*) lane's d)
 template <int N> __device__ __forceinline__ void add_lane_power_piece(const Piece& x, uint32_t w, uint32_t mask, const uint32_t* m, float* o)
 {
@@ -457,6 +474,26 @@ __device__ __forceinline__ void block_add(Pipe<W4, WHOLE>& pipe, const Stream<WH
     pipe.block(s, j1, next, j2, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
         const bool in = (counts >> j) & 1u;
         add_piece<N>(x, in ? f2u(weight[j]) + add : 0u, in ? 1.0f : 0.0f, out + d);
+    });
+}
+
+// The same by slopes: out += the block's weights times the powers of its rows' products with `mine`.
+template <int W4, bool WHOLE>
+__device__ __forceinline__ void block_add_power(Pipe<W4, WHOLE>& pipe, const Stream<WHOLE>& s, int j1, const Stream<WHOLE>& next, int j2, bool zeros, uint32_t power,
+                                                float (&weight)[kBlock], uint32_t counts, const uint32_t (&mine)[4 * W4], float (&out)[4 * W4])
+{
+    constexpr int N = 4 * Pipe<W4, WHOLE>::kQuads;
+    if (__builtin_expect(zeros, 0)) {
+        pipe.rolled(s, j1, next, j2, [&](int h, int d, const Piece& x) __attribute__((always_inline)) {
+            const bool in = counts & 1u;
+            add_power_piece_with_zeros<N>(x, in ? weight[0] : 0.0f, in ? power : 0u, mine + d, out + d);
+            if (h == Pipe<W4, WHOLE>::kPieces - 1) { turned(weight); counts >>= 1; }
+        });
+        return;
+    }
+    pipe.block(s, j1, next, j2, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+        const bool in = counts >> j & 1u;
+        add_power_piece<N>(x, in ? weight[j] : 0.0f, in ? power : 0u, mine + d, out + d);
     });
 }
 

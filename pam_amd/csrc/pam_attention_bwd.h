@@ -199,17 +199,24 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
                 look_k.load(keys, j1 + kBlock);
                 look_v.load(values, j1 + kBlock);
                 bool wrong = false;
-                block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, APPROXIMATE && kv.zeros, q, s);
-                bool wild = slices_s.add_up(turn, wave, s, gave_up || kv.wild || vv.wild || (!APPROXIMATE && (kv.zeros || vv.zeros)));
+                block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, kv.zeros, q, s);
+                bool wild = slices_s.add_up(turn, wave, s, gave_up || kv.wild || vv.wild);
                 if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
                 uint32_t counts = weigh(s, e, sees, all, j1, wrong);
                 if constexpr (APPROXIMATE) block_dots<W4, WHOLE>(pipe, values, j1, keys, j1, vv.zeros, dn, de);
                 else {
 #pragma unroll
                     for (int j = 0; j < kBlock; ++j) de[j] = 0.0f;
-                    pipe.block(values, j1, keys, j1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
-                        dot_power_piece<N>(x, f2u(e[j]) + scoring.mul_add, counts >> j & 1u ? kPower : 0u, dn + d, de[j]);
-                    });
+                    uint32_t left = counts;
+                    if (__builtin_expect(vv.zeros, 0))
+                        pipe.rolled(values, j1, keys, j1, [&](int h, int d, const Piece& x) __attribute__((always_inline)) {
+                            dot_power_piece_with_zeros<N>(x, f2u(e[0]) + scoring.mul_add, left & 1u ? kPower : 0u, dn + d, de[0]);
+                            if (h == Pipe<W4, WHOLE>::kPieces - 1) { turned(e); turned(de); left >>= 1; }
+                        });
+                    else
+                        pipe.block(values, j1, keys, j1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+                            dot_power_piece<N>(x, f2u(e[j]) + scoring.mul_add, counts >> j & 1u ? kPower : 0u, dn + d, de[j]);
+                        });
 #pragma unroll
                     for (int j = 0; j < kBlock; ++j) de[j] = over_power(de[j], f2u(e[j]));
                 }
@@ -227,11 +234,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
                 gave_up = gave_up || __ballot(wrong) != 0ull;
                 if (NS == 1 && __builtin_expect(gave_up, 0)) return false;
                 if constexpr (APPROXIMATE) block_add<W4, WHOLE>(pipe, keys, j1, keys, j1 + kBlock, kv.zeros, de, scoring.mul_add, counts, out[0]);
-                else
-                    pipe.block(keys, j1, keys, j1 + kBlock, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
-                        const bool in = counts >> j & 1u;
-                        add_power_piece<N>(x, in ? de[j] : 0.0f, in ? kPower : 0u, q + d, out[0] + d);
-                    });
+                else block_add_power<W4, WHOLE>(pipe, keys, j1, keys, j1 + kBlock, kv.zeros, kPower, de, counts, q, out[0]);
                 return true;
             });
         careful = careful || in_team<NS>(gave_up);
@@ -401,8 +404,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
                 look_q.load(queries, r1 + kBlock);
                 look_n.load(grads, r1 + kBlock);
                 bool wrong = false;
-                block_dots<W4, WHOLE>(pipe, queries, r1, grads, r1, APPROXIMATE && qv.zeros, k, s);
-                const bool wild = slices_s.add_up(turn, wave, s, gave_up || qv.wild || nv.wild || (!APPROXIMATE && qv.zeros));
+                block_dots<W4, WHOLE>(pipe, queries, r1, grads, r1, qv.zeros, k, s);
+                const bool wild = slices_s.add_up(turn, wave, s, gave_up || qv.wild || nv.wild);
                 if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
                 uint32_t counts = weigh(s, e, sees, all, r1, wrong);
                 if constexpr (APPROXIMATE) block_dots<W4, WHOLE>(pipe, grads, r1, grads, r1, nv.zeros, v, de);
@@ -436,10 +439,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
                     pipe.block(grads, r1, queries, r1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
                         add_lane_power_piece<N>(x, f2u(e[j]), counts_e >> j & 1u ? kPower : 0u, v + d, out[1] + d);
                     });
-                    pipe.block(queries, r1, queries, r1 + kBlock, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
-                        const bool in = counts >> j & 1u;
-                        add_power_piece<N>(x, in ? de[j] : 0.0f, in ? kPower : 0u, k + d, out[0] + d);
-                    });
+                    block_add_power<W4, WHOLE>(pipe, queries, r1, queries, r1 + kBlock, qv.zeros, kPower, de, counts, k, out[0]);
                 }
                 return true;
             });
