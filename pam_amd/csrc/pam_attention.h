@@ -16,7 +16,7 @@
 // a score through LDS.  A work-group's wavefronts stream the same rows, so that the scalar cache has them.
 // Rates of the inner loop alone, two wavefronts per SIMD: 28 T products/s; with the streamed values read from another lane inside the integer
 // addition (a data-parallel primitive: everything around it issues half as fast) 18.6; copied out of one once for four rows 20.5; by lane reads 12.
-// Whole passes: forward 18.7 T products/s where every row sees 4096 keys, 13.2 where the order is causal (the last turn of units is not full),
+// Whole passes: forward 18.7 T products/s where every row sees 4096 keys, 15.6 where the order is causal (the last turn of units is not full),
 // gradients 14.5 and 11: a sixth to a third of the instructions are the weights', which slices make twice, and two or three wavefronts on a SIMD do not
 // cover all waits for the scalar cache.
 //

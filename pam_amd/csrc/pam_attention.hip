@@ -142,9 +142,9 @@ const Variant& variant_for(const Variant* list, long dim)
 
 // How the streamed rows are cut.  All units of a launch run at once or in a few turns of `slots` of them, so that a last turn of a few units costs as
 // much as a full one: among the cuts that fill one, two, ... turns the one is taken whose turns times its spans are least.  (4096 causal tokens, 8 heads over 2:
-// chunks of 256 keys, two turns and a bit, 0.70 ms.)  Which spans a tile sees is what the order and the window say; prefixes and documents are on the device.
-// A chunk is at least two spans (documents leave a tile little of what the order does, but chunks of one span cost 307 us where three take 267: 2 x 2048
-// tokens, heads of 128), what a unit does besides its spans counts as a fifth of one.
+// chunks of 256 keys, two turns and a bit, 0.70 ms; the cut taken 0.55.)  Which spans a tile sees is what the order and the window say; prefixes and documents are on the device.
+// A chunk is at least two spans (documents leave a tile little of what the order does, but chunks of one span cost 307 us where three took 267, 210 since units
+// that see nothing end early: 2 x 2048 tokens, heads of 128), what a unit does besides its spans counts as a fifth of one.
 struct Plan { int tiles, chunks, chunk; };
 long tiles_of(int slices) { return slices >= 4 ? 1 : 4 / slices; }              // of a work-group (kTiles)
 template <class Range>                            // range(first, last row of a tile, low, high): the streamed rows that those see

@@ -6,7 +6,7 @@
 // for approximate gradients; an exact one weighs the gradient by the slope of the other factor's piece instead.  Two kernels: in the first lanes own
 // queries and keys stream by (a, de and dq: three products), in the second lanes own keys and queries stream by (a, de, dk and dv: four).
 // Scores and weights are computed again in both; kept, they would be 8 bytes a pair, as long to read as two of the products of 64 values.
-// 4096 causal tokens, 8 heads of 64 over 2: 1.05 ms for dq (12 T products/s), 1.67 for dk and dv (10); three wavefronts on a SIMD are 6 % better than two for the
+// 4096 causal tokens, 8 heads of 64 over 2: 1.07 ms for dq (12 T products/s), 1.65 for dk and dv (10), exact 1.6 and 2.1; three wavefronts on a SIMD are 6 % better than two for the
 // first, and 30 % worse for the second, whose four slices of 32 then do not fit the registers.
 // All that is linear in dy is scaled by a power of two: in the first kernel a query's largest |dn| to [1, 2), in the second the largest of a chunk's.
 #pragma once
