@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kThreads, 4) void cached_attention_kernel(CacheArgs
     Args scoring_args{};
     scoring_args.cap = a.cap; scoring_args.off = a.off; scoring_args.slopes = a.slopes;
     const Scoring scoring(scoring_args);
-    const Full full{a.off, has_off, 0u - mul_add};
+    const Full full{a.off, has_off, 0u};
 
     Lane here;
     here.first = lane % L * 4; here.values = a.values;
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(kThreads, 4) void cached_attention_kernel(CacheArgs
             const uint32_t scaled = (f2u(v) << 1) == 0u ? kStandIn : f2u(v) + (f2u(a.scale) - kBias + off_add);
             const bool out = there && (scaled << 1) - kLaneBase >= kLaneSpan;
             odd = odd || out;
-            q[r][d] = there ? (out ? f2u(pam_mul_off(v, a.scale, a.off, has_off)) : scaled) + mul_add : lane_pad(0u);
+            q[r][d] = there ? scaled + mul_add : lane_pad(0u);
             acc[r][d] = 0.0f;
         }
         l[r] = 0.0f; M[r] = kNothing;
@@ -330,17 +330,18 @@ __global__ __launch_bounds__(kThreads, 4) void cached_attention_kernel(CacheArgs
                 if (__builtin_expect(careful, 0)) {
 #pragma unroll 1
                     for (int n = 0; n < kTwo * ROWS; ++n) {
-                        // (the row's and the key's values by selects: the arrays stay in registers)
+                        // (the query from memory again, as it is: q has something else in a zero's place; the key's values by selects, so that the array stays in registers)
+                        const RowPlace place_of_row = place_of(a, kv, row0 + min(n % ROWS, here_rows - 1));
+                        const float* const from = a.q.p + (long)b * a.q.sb + (long)place_of_row.token * a.q.st + (long)place_of_row.head * a.q.sh;
                         float sum = 0.0f;
 #pragma unroll
                         for (int d = 0; d < 4; ++d) {
-                            uint32_t mine = q[0][d], theirs = f2u(rows[i0][d]);
-#pragma unroll
-                            for (int r = 1; r < ROWS; ++r) mine = n % ROWS == r ? q[r][d] : mine;
+                            const bool there = here.streams && here.first + d < a.values;
+                            uint32_t theirs = f2u(rows[i0][d]);
 #pragma unroll
                             for (int i = 1; i < kTwo; ++i) theirs = n / ROWS == i ? f2u(rows[i0 + i][d]) : theirs;
-                            mine = (uint32_t)anew((int)mine);
-                            sum += full_product(full, mine == lane_pad(0u) ? 0u : mine + full.raw, theirs);
+                            const float mine = pam_mul_off(from[there ? here.first + d : 0], a.scale, a.off, has_off);
+                            sum += full_product(full, there ? f2u(mine) : 0u, theirs);
                             __builtin_amdgcn_sched_barrier(0);
                         }
                         s[0] = sum;

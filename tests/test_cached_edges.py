@@ -1,0 +1,66 @@
+"""pam.cached_attention at the ends of its windows, for heads of whole quads and others, and with an offset."""
+import numpy as np
+import pytest
+import torch
+
+import _attention_general as general
+from _attention_ref import visible
+from test_cached_attention import _cache, _compare, _cuda, _sequence
+
+gpu = pytest.mark.gpu
+DIMS = pytest.mark.parametrize("dim", [18, 66, 64, 20])
+
+
+@gpu
+@DIMS
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_zero_queries_beside_large_keys(dim, tokens):
+    """A zero times anything is zero, also where a key is out of the usual range."""
+    def change(q, k, v):
+        q[..., : dim // 2] = 0; k[..., : dim // 2] *= np.float32(2.0 ** 100)
+    _compare(2, tokens, 4, 2, dim, 16, [150, 37], seed=dim, change=change)
+
+
+@gpu
+@DIMS
+@pytest.mark.parametrize("large", [2.0 ** 85, 2.0 ** 39])
+def test_the_power_of_two_that_zeros_stand_as(dim, large):
+    def queries(q, k, v):
+        q[:] = np.float32(2.0 ** -86) * np.sign(q); k[:] = np.float32(large) * np.sign(k)
+
+    def keys(q, k, v):
+        k[:] = np.float32(2.0 ** -86) * np.sign(k); q[:] = np.float32(large) * np.sign(q)
+    for change in (queries, keys):
+        _compare(1, 2, 4, 2, dim, 16, [150], seed=dim, change=change, scale=1.0)
+
+
+@gpu
+@pytest.mark.parametrize("tokens,heads", [(1, 1), (1, 4), (6, 4)])
+@pytest.mark.parametrize("what", ["values", "keys", "queries", "all", "wild", "small", "far", "large_query", "zero_rows"])
+@pytest.mark.parametrize("dim", [18, 66])
+def test_values_out_of_the_ordinary_in_heads_of_any_size(dim, what, tokens, heads):
+    def change(q, k, v):
+        rng = np.random.RandomState(5)
+        for name, x in (("queries", q), ("keys", k), ("values", v)):
+            if what in (name, "all"):
+                x[rng.random_sample(x.shape) < 0.1] = 0
+        if what == "wild":
+            v[:, 2] *= np.float32(2.0 ** 60); k[1::3, 1] *= np.float32(2.0 ** -100); q[:, 0, 0] *= np.float32(2.0 ** -70)
+        elif what == "small":
+            v *= np.float32(1e-30); k[:, 1] *= np.float32(1e-20)
+        elif what == "far":
+            q[:] = np.abs(q); k[:] = np.abs(k) * np.linspace(-30, 30, k.shape[0], dtype=np.float32)[:, None, None, None]
+        elif what == "large_query":
+            q[:, :, 0] *= np.float32(1e26); k *= np.float32(1e-26)
+        elif what == "zero_rows":
+            k[:, 3] = 0; v[:, 5] = 0; q[:, 0, 0] = 0
+    _compare(2, tokens, heads, 1, dim, 16, [150, 300], seed=7, change=change)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [18, 66])
+@pytest.mark.parametrize("scoring", [dict(window=1), dict(window=50), dict(window=1000), dict(cap=5.0), dict(slopes=np.array([0.5, 0.01, 0.0, 1.0], np.float32)), dict(scale=0.07),
+                                     dict(cap=20.0, slopes=np.array([0.1, 0.2, 0.3, 0.4], np.float32), window=70)], ids=lambda s: "_".join(s))
+def test_scores_and_windows_in_heads_of_any_size(dim, scoring):
+    _compare(2, 3, 4, 2, dim, 16, [200, 31], seed=3, **scoring)
+    _compare(2, 1, 4, 1, dim, 16, [200, 31], seed=4, **scoring)
