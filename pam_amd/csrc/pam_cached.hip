@@ -468,7 +468,7 @@ __global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_ke
     scoring_args.cap = a.cap; scoring_args.off = a.off; scoring_args.slopes = a.slopes;
     const Scoring scoring(scoring_args);
     const Full full{a.off, has_off, 0u};
-    const uint32_t scale_add = f2u(a.scale) - kBias + scoring.off_add, key_add = scale_add + scoring.mul_add, mul_add = scoring.mul_add;
+    const uint32_t scale_add = f2u(a.scale) - kBias + scoring.off_add, key_add = scale_add + scoring.mul_add, mul_add = scoring.mul_add, none = kStandIn + mul_add;
     const Queries queries(a, me);
     const int* const table = a.table + (long)me.b * a.per_sequence;
     const float* const k = a.k + (long)me.kv * a.c_sh;
@@ -526,6 +526,7 @@ __global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_ke
         };
         // scores
         float s[ROWS];
+        bool left_out = false;                    // a key that a row does not see, or one whose weight is none
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) s[r] = 0.0f;
         const int slices = (quads + kSlice - 1) / kSlice;
@@ -618,11 +619,13 @@ __global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_ke
             const bool in = power >= kLeast;
             const float e = power_of_two(fmaxf(power, kLeast));
             l[r] += in ? e : power * 0.0f;        // (what is no number makes none of the sum)
-            // (one that does not count stands as 2^-86: nothing beside the largest, which is at least 2^-8)
+            // (one that does not count stands as 2^-86, which no weight is; a factor leaves its products out, since a value that is not seen may be of any size)
             weights[wave][lane][r] = u2f((in ? f2u(e) : kStandIn) + mul_add);
+            left_out = left_out || !in;
             __builtin_amdgcn_sched_barrier(0);    // (row by row: all of them side by side take the registers of the loops around)
         }
         wave_fence();
+        const bool factors = __ballot(left_out) != 0ull;
         // values
 #pragma unroll 1
         for (int step = 0; step < L; step += kAhead) {
@@ -651,7 +654,7 @@ __global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_ke
 #pragma unroll
                         for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-                            for (int d = 0; d < 4; ++d) acc[r][d] = __builtin_fmaf(u2f(f2u(x[d]) + f2u(of[r])), f[d], acc[r][d]);
+                            for (int d = 0; d < 4; ++d) acc[r][d] = __builtin_fmaf(u2f(f2u(x[d]) + f2u(of[r])), f2u(of[r]) == none ? 0.0f : f[d], acc[r][d]);
                     } else {
 #pragma unroll 1
                         for (int r = 0; r < ROWS; ++r) {
@@ -666,6 +669,17 @@ __global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_ke
                         }
                     }
                     turned(rows);
+                }
+            } else if (factors) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const float* const of = weights[wave][(step + i) * keys_a_step + lane / L];
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+                        const float one = f2u(of[r]) == none ? 0.0f : 1.0f;
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) acc[r][d] = __builtin_fmaf(u2f(f2u(rows[i][d]) + f2u(of[r])), one, acc[r][d]);
+                    }
                 }
             } else {
 #pragma unroll

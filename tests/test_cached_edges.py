@@ -64,3 +64,23 @@ def test_values_out_of_the_ordinary_in_heads_of_any_size(dim, what, tokens, head
 def test_scores_and_windows_in_heads_of_any_size(dim, scoring):
     _compare(2, 3, 4, 2, dim, 16, [200, 31], seed=3, **scoring)
     _compare(2, 1, 4, 1, dim, 16, [200, 31], seed=4, **scoring)
+
+
+@gpu
+@DIMS
+@pytest.mark.parametrize("seen", [1e-12, 0.0])
+@pytest.mark.parametrize("tokens,heads", [(1, 1), (1, 4), (3, 4)])
+def test_masked_values_are_in_no_result(tokens, heads, seen, dim):
+    """Large values outside the window, and those of later tokens, beside small ones within it."""
+    pam = __import__("pam_amd")
+    rng = np.random.RandomState(0)
+    k, v, table = _cache(rng, 1, 16, 14, 1, dim)
+    length = 150
+    v[:] = np.float32(1e12)
+    places = [(table[0, j // 16], j % 16) for j in range(length + tokens)]
+    for t in range(tokens):
+        v[places[length + t]] = np.float32(seen) * (1.0 + rng.random_sample(dim))
+    q = rng.standard_normal((1, tokens, heads, dim)).astype(np.float32)
+    got = pam.cached_attention(_cuda(q), _cuda(k), _cuda(v), _cuda(table), _cuda(np.array([length])), window=1)
+    want = torch.stack([_cuda(v[places[length + t]][0]) for t in range(tokens)])[None, :, None].expand(-1, -1, heads, -1)
+    assert torch.equal(got, want)
