@@ -604,11 +604,13 @@ template <int NS> __device__ __forceinline__ bool any_seen(const Sight& sight, i
 
 // ---------------------------------------------------------------- from a score to its exponent
 
-// x (*) a positive constant, whose bits less the bias (offset counted) are `add`.  Underflow is zero; NaN and infinities are not numbers afterwards.
+// x (*) a positive constant below 2, whose bits less the bias (offset counted) are `add`, below zero for one below 1.  Underflow is zero; NaN, infinities and what is
+// 2^127 or more are no number afterwards, whatever `add` is.
 __device__ __forceinline__ float times(float x, uint32_t add)
 {
-    const int m = (int)(min(f2u(x) & ~kSign, kExpo + 1u) + add);
-    return u2f((uint32_t)max(m, 0) | (f2u(x) & kSign));
+    const uint32_t size = f2u(x) & ~kSign;
+    const int m = max((int)(size + add), 0);
+    return u2f(size >= 0x7f000000u ? kQNaN : (uint32_t)m | (f2u(x) & kSign));
 }
 // a (*) b of any finite numbers whose product is below 2^128; an underflow (a zero's, too) is zero or next to nothing
 __device__ __forceinline__ float times_any(float a, float b, uint32_t off_add)

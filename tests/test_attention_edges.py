@@ -1,0 +1,86 @@
+"""pam.attention where its usual loops' windows end: gradients of very different sizes in a row, exact zeros beside tiny and large values, weights and gradients
+far below the largest, scores near the end of the range, numbers that are none beside an offset, and the scratch of long windows."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import _attention_general as general
+from test_attention import _check, _cuda, _inputs, _run
+
+gpu = pytest.mark.gpu
+APPROX = pytest.mark.parametrize("approx", [True, False], ids=["approximate", "exact"])
+
+
+def _compare(shape, masks, seed=0, approx=True, train=True, change=None, offset=None, tight=0.0):
+    """approx: as approx_bwd, a pair of it for first and second operands counts as set for the exponential.  tight: what part of the gradients' values the bounds hold to 5 % at least."""
+    pam = __import__("pam_amd")
+    q, k, v, dy = _inputs(seed, *shape)
+    if change:
+        change(q, k, v, dy)
+    flags = (*approx, True) if isinstance(approx, tuple) else (approx,) * 3
+    want, off, grads, offs = general.attention(q, k, v, dy if train else None, flags=flags, offset=offset, **masks)
+    leaves = [_cuda(x).requires_grad_(train) for x in (q, k, v)]
+    on = {n: _cuda(x) if isinstance(x, np.ndarray) else x for n, x in masks.items()}
+    y = pam.attention(*leaves, **on, approx_bwd=approx, offset=offset)
+    _check(y, want, off, "y")
+    if not train:
+        return
+    assert np.concatenate([(o < 0.05 * np.abs(w))[w != 0] for w, o in zip(grads, offs)]).mean() >= tight
+    for name, got, w, o in zip("qkv", torch.autograd.grad(y, leaves, _cuda(dy)), grads, offs):
+        _check(got, w, o, "d" + name)
+
+
+# ---------------------------------------------------------------- gradients that span more than an integer addition may
+
+
+# ---------------------------------------------------------------- a number that stands for zero
+
+
+# ---------------------------------------------------------------- weights and gradients far below the largest
+
+
+# ---------------------------------------------------------------- the ends of the range
+
+
+@gpu
+@pytest.mark.parametrize("offset", [0.7501, 0.76, 0.78, 1.0552, 1.45])
+@pytest.mark.parametrize("value", [float("nan"), -float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_no_numbers_beside_an_offset(where, value, offset):
+    pam = __import__("pam_amd")
+    q, k, v, dy = (_cuda(x) for x in _inputs(1, 1, 40, 40, 2, 1, 32))
+    clean = pam.attention(q, k, v, offset=offset)
+    (q if where == "q" else k)[0, 20, 0, 3] = np.float32(value).item()
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    y = pam.attention(*leaves, offset=offset, approx_bwd=True)
+    bad = y[0, 20, 0] if where == "q" else y[0, 20:]
+    assert bad.isnan().all() and torch.equal(y[0, :20], clean[0, :20])
+    dq = torch.autograd.grad(y, leaves, dy)[0]
+    assert (dq[0, 20, 0] if where == "q" else dq[0, 20:]).isnan().all() and torch.isfinite(dq[0, :20]).all()
+
+
+# ---------------------------------------------------------------- offsets, slopes of each kind, masks over several spans
+
+MASKS = {
+    "causal": {}, "all": dict(causal=False), "window": dict(window=70), "window_both_ways": dict(window=30, causal=False), "prefix": dict(prefix=np.array([100, 3])),
+    "documents": dict(documents=np.repeat(np.array([[0, 1, 2, -1], [5, 1 << 40, 5, 5]]), 36, axis=1)), "slopes": dict(slopes=np.array([0.5, 0.03], np.float32)),
+    "cap": dict(cap=3.0), "cap_and_window": dict(cap=10.0, window=65),
+}
+
+
+# ---------------------------------------------------------------- scratch
+
+class _Shape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_long) for n in ("batch", "tokens", "keys", "heads", "kv_heads", "dim", "values")] + [(n, ctypes.c_float) for n in ("scale", "cap", "offset")] + [
+        ("causal", ctypes.c_int), ("window", ctypes.c_long), ("prefix", ctypes.c_void_p), ("documents", ctypes.c_void_p), ("slopes", ctypes.c_void_p)]
+
+
+def _scratch(tokens, heads, kv_heads, dim, window, batch=1, keys=None, causal=True):
+    from pam_amd import _abi
+    lib = ctypes.CDLL(str(_abi.library_path()))
+    forward, backward = lib.pam_hip_attention_workspace_bytes, lib.pam_hip_attention_bwd_workspace_bytes
+    forward.restype = backward.restype = ctypes.c_size_t
+    s = _Shape(batch, tokens, keys or tokens, heads, kv_heads, dim, dim, 0.125, 0.0, 1.0, causal, window, None, None, None)
+    return forward(ctypes.byref(s)), backward(ctypes.byref(s), 1, 1)

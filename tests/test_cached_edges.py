@@ -84,3 +84,30 @@ def test_masked_values_are_in_no_result(tokens, heads, seen, dim):
     got = pam.cached_attention(_cuda(q), _cuda(k), _cuda(v), _cuda(table), _cuda(np.array([length])), window=1)
     want = torch.stack([_cuda(v[places[length + t]][0]) for t in range(tokens)])[None, :, None].expand(-1, -1, heads, -1)
     assert torch.equal(got, want)
+
+
+@gpu
+@DIMS
+@pytest.mark.parametrize("offset", [0.7501, 0.76, 0.78, 1.0552, 1.45])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_no_numbers_beside_an_offset(value, offset, dim):
+    pam = __import__("pam_amd")
+    rng = np.random.RandomState(1)
+    k, v, table = _cache(rng, 3, 8, 6, 2, dim)
+    q = _cuda(rng.standard_normal((3, 2, 4, dim)).astype(np.float32))
+    k, v, table, lengths = _cuda(k), _cuda(v), _cuda(table), _cuda(np.array([30, 30, 30]))
+    clean = pam.cached_attention(q, k, v, table, lengths, offset=offset)
+    assert torch.isfinite(clean).all()
+    hidden = k.clone()
+    hidden[table[0, 4]] = value
+    hidden[table[1, 3], 7, 1, 5] = value                                    # place 31: the second token's own
+    y = pam.cached_attention(q, hidden, v, table, lengths, offset=offset)
+    assert torch.equal(y[0], clean[0]) and y[1, 1, 2:].isnan().all() and torch.equal(y[1, 0], clean[1, 0]) and torch.equal(y[1, 1, :2], clean[1, 1, :2])
+    asked = q.clone()
+    asked[2, 0, 1, 3] = value
+    y = pam.cached_attention(asked, k, v, table, lengths, offset=offset)
+    assert y[2, 0, 1].isnan().all() and torch.equal(y[2, 1], clean[2, 1]) and torch.equal(y[:2], clean[:2])
+    broken = table.clone()
+    broken[1, 1] = -1
+    y = pam.cached_attention(q, k, v, broken, lengths, offset=offset)
+    assert y[1].isnan().all() and torch.equal(y[0], clean[0])
