@@ -669,6 +669,6 @@ __device__ __forceinline__ float power_of_two(float u) { return u2f((uint32_t)((
 // 2^(from - to), not below 2^-126 (that times a sum is nothing); from - to at most 127
 __device__ __forceinline__ float scale_between(float from, float to) { return u2f((uint32_t)((int)fmaxf(from - to, -126.0f) + 127) << 23); }
 
-constexpr float kNothing = -3.0e38f;              // M of a row that has seen nothing yet
+constexpr float kNothing = -0x1.fffffep127f;      // M of a row that has seen nothing yet: below every exponent of 2 that a score below 2^127 has
 
 }  // namespace pamatt

@@ -144,9 +144,9 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < kBlock; ++j) {
-            float power = t[j] - M;
-            if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
-            wrong = __builtin_fmaf(power, 0.0f, wrong);
+            float power = t[j] - M, number = t[j];        // (scores near both ends of the range: their difference may be an infinity, and counts for nothing)
+            if (!all) { power = (sees >> j) & 1u ? power : 2.0f * kLeast; number = (sees >> j) & 1u ? number : 0.0f; }
+            wrong = __builtin_fmaf(number, 0.0f, wrong);
             const bool in = power >= kLeast;
             t[j] = power_of_two(fmaxf(power, kLeast));
             sum += in ? t[j] : 0.0f;

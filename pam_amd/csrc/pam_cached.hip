@@ -381,7 +381,7 @@ __global__ __launch_bounds__(kThreads, 4) void cached_attention_kernel(CacheArgs
             saw |= sees ? 1u << r : 0u;
             const bool in = power >= kLeast;
             const float e = power_of_two(fmaxf(power, kLeast));
-            l[r] += in ? e : power * 0.0f;        // (what is no number makes none of the sum)
+            l[r] += in ? e : sees ? t * 0.0f : 0.0f;      // (what is no number makes none of the sum)
             scores[wave][lane][r] = in ? e : 0.0f;
             __builtin_amdgcn_sched_barrier(0);    // (row by row: all of them side by side take the registers of the loops around)
         }
@@ -618,7 +618,7 @@ __global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_ke
             saw |= sees ? 1u << r : 0u;
             const bool in = power >= kLeast;
             const float e = power_of_two(fmaxf(power, kLeast));
-            l[r] += in ? e : power * 0.0f;        // (what is no number makes none of the sum)
+            l[r] += in ? e : sees ? t * 0.0f : 0.0f;      // (what is no number makes none of the sum)
             // (one that does not count stands as 2^-86, which no weight is; a factor leaves its products out, since a value that is not seen may be of any size)
             weights[wave][lane][r] = u2f((in ? f2u(e) : kStandIn) + mul_add);
             left_out = left_out || !in;

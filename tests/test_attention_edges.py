@@ -43,6 +43,27 @@ def _compare(shape, masks, seed=0, approx=True, train=True, change=None, offset=
 
 # ---------------------------------------------------------------- the ends of the range
 
+@gpu
+@pytest.mark.parametrize("offset", [None, 1.45])
+@pytest.mark.parametrize("keys", [3, 200])
+def test_scores_at_both_ends(keys, offset):
+    """Scores of 2^126 and more beside others as far below zero: all of the weight is the largest one's.  From 2^127 on they are no numbers."""
+    pam = __import__("pam_amd")
+    q = torch.zeros(1, 1, 1, 4, device="cuda")
+    q[..., 0] = 2.0 ** 63
+    top = 2.0 ** (63 if offset is None else 62)
+    k = torch.zeros(1, keys, 1, 4, device="cuda")
+    k[..., 0] = -1.4 * top
+    k[:, keys // 2, :, 0] = 1.2 * top
+    v = torch.randn(1, keys, 1, 4, device="cuda")
+    y = pam.attention(q, k, v, scale=1.0, causal=False, offset=offset)
+    assert torch.equal(y[0, 0, 0], v[0, keys // 2, 0])
+    k[:, keys // 2, :, 0] = -1.39 * top            # (none is above zero)
+    assert torch.equal(pam.attention(q, k, v, scale=1.0, causal=False, offset=offset)[0, 0, 0], v[0, keys // 2, 0])
+    for sign in (1.0, -1.0):
+        k[:, keys // 2, :, 0] = sign * 2.5 * top
+        assert pam.attention(q, k, v, scale=1.0, causal=False, offset=offset).isnan().all()
+
 
 @gpu
 @pytest.mark.parametrize("offset", [0.7501, 0.76, 0.78, 1.0552, 1.45])

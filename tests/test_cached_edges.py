@@ -111,3 +111,23 @@ def test_no_numbers_beside_an_offset(value, offset, dim):
     broken[1, 1] = -1
     y = pam.cached_attention(q, k, v, broken, lengths, offset=offset)
     assert y[1].isnan().all() and torch.equal(y[0], clean[0])
+
+
+@gpu
+@DIMS
+@pytest.mark.parametrize("offset", [None, 1.45])
+def test_scores_at_both_ends(dim, offset):
+    pam = __import__("pam_amd")
+    q = torch.zeros(1, 1, 1, dim, device="cuda")
+    q[..., 0] = 2.0 ** 63
+    top = 2.0 ** (63 if offset is None else 62)
+    k, v = torch.zeros(30, 16, 1, dim, device="cuda"), torch.randn(30, 16, 1, dim, device="cuda")
+    table, lengths = torch.arange(30, dtype=torch.int32, device="cuda")[None], torch.tensor([470], device="cuda")
+    k[..., 0] = -1.4 * top
+    for most in (1.2 * top, -1.39 * top):
+        k[11, 3, 0, 0] = most
+        y = pam.cached_attention(q, k, v, table, lengths, scale=1.0, offset=offset)
+        assert torch.equal(y[0, 0, 0], v[11, 3, 0])
+    for sign in (1.0, -1.0):
+        k[11, 3, 0, 0] = sign * 2.5 * top
+        assert pam.cached_attention(q, k, v, table, lengths, scale=1.0, offset=offset).isnan().all()
