@@ -20,9 +20,9 @@
 // gradients 14.5 and 11: a sixth to a third of the instructions are the weights', which slices make twice, and two or three wavefronts on a SIMD do not
 // cover all waits for the scalar cache.
 //
-// The integer addition is the product while no exponent leaves the normal range.  Streamed values have to be in 2^[-40, 40), a lane's in 2^[-86, 80); a
+// The integer addition is the product while no exponent leaves the normal range.  Streamed values have to be in 2^[-40, 40), a lane's in 2^(-86, 80); a
 // lane's zero stands as 2^-86, which adds less to a sum than its rounding.  Streamed rows with zeros take a loop that leaves those out by a factor.
-// With anything else in a streamed row, or in a lane's, a unit begins again with the full definition (`careful`), a row at a time: kept apart
+// With anything else in a streamed row, or in a lane's, a unit begins again with the full definition (`careful`), its lanes' rows read again as they are: kept apart
 // from the usual loops, because side by side with them it took their registers.
 // Every value of a block is looked at for that by one lane, with vector loads of its own.
 #pragma once
@@ -82,7 +82,7 @@ template <int N, int END, class F> __device__ __forceinline__ void each(F&& f)
 }
 
 constexpr uint32_t kStreamBase = (uint32_t)(127 - 40) << 24, kStreamSpan = 80u << 24;      // 2^[-40, 40) of bits << 1
-constexpr uint32_t kLaneBase = (uint32_t)(127 - 86) << 24, kLaneSpan = 166u << 24;         // 2^[-86, 80)
+constexpr uint32_t kLaneBase = (uint32_t)(127 - 86) << 24, kLaneSpan = 166u << 24;         // 2^(-86, 80), ends left out: [-86, 80) where nothing stands in
 constexpr uint32_t kStandIn = (uint32_t)(127 - 86) << 23;
 
 // (comparisons with it are made where they are used, instead of kept from the beginning of a kernel to its end)
@@ -98,8 +98,8 @@ template <int N, class T> __device__ __forceinline__ void turned(T (&v)[N])     
     v[N - 1] = first;
 }
 
-// A lane's part of a row: bits(value) + scale + add, zeros and what lies behind the row's values stood in for (unscaled; 2^-86 itself counts as the next
-// number).  scale: of a factor in 2^[-41, 41].  Returns false if a value, scaled, is out of the window.
+// A lane's part of a row: bits(value) + scale + add, zeros and what lies behind the row's values stood in for (unscaled, by 2^-86, which is out of the
+// window).  scale: of a factor in 2^[-41, 41].  Returns false if a value, scaled, is out of the window.
 template <int W4>
 __device__ __forceinline__ bool load_lane(const float* row, int first, int dim, int values, uint32_t scale, uint32_t add, uint32_t (&out)[4 * W4])
 {
@@ -110,14 +110,23 @@ __device__ __forceinline__ bool load_lane(const float* row, int first, int dim, 
         const v4f x = *reinterpret_cast<const v4f_any*>(row + min(first + 4 * n, dim - 4));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t b = f2u(x[i]) + scale;
-            b = (b & ~kSign) == kStandIn ? b + 1u : b;
-            b = (f2u(x[i]) << 1) == 0u || first + 4 * n + i >= values ? kStandIn : b;
-            most = max(most, (b << 1) - kLaneBase);
-            out[4 * n + i] = b + add;
+            const bool none = (f2u(x[i]) << 1) == 0u || first + 4 * n + i >= values;
+            const uint32_t b = f2u(x[i]) + scale;
+            most = max(most, none ? 0u : (b << 1) - (kLaneBase + 2u));
+            out[4 * n + i] = (none ? kStandIn : b) + add;
         }
     }
-    return most < kLaneSpan;
+    return most < kLaneSpan - 2u;
+}
+// ... as the full definition takes it: the values themselves, zeros behind the row's
+template <int W4, class Value>
+__device__ __forceinline__ void load_plain(int first, int values, uint32_t (&out)[4 * W4], Value&& value)
+{
+#pragma unroll 1
+    for (int d = 0; d < 4 * W4; ++d) {
+        out[0] = first + d < values ? f2u(value(first + d)) : 0u;
+        turned(out);
+    }
 }
 
 // ---------------------------------------------------------------- streamed rows
@@ -405,25 +414,22 @@ template <int W4, bool WHOLE> __device__ __forceinline__ bool all_finite(Look<W4
     return __ballot(most >= kExpo << 1) == 0ull;
 }
 
-// The same products by the full definition, for a row that lanes hold a quad each of.  raw: what turns `mine` back into a value's bits.
-struct Full { float off; bool has_off; uint32_t raw; };
+// The same products by the full definition, for a row that lanes hold a quad each of and a lane's values as they are (load_plain).
+struct Full { float off; bool has_off; };
 __device__ __forceinline__ float full_product(const Full& f, uint32_t a, uint32_t b)
 {
     const float c = pam_general(a, b);
     return f.has_off ? pam_general(f2u(c), f2u(f.off)) : c;
 }
-__device__ __forceinline__ uint32_t real_bits(const Full& f, uint32_t mine)
-{
-    const uint32_t m = (uint32_t)anew((int)mine) + f.raw;      // (taken apart here and not, for all rows, before the loop)
-    return m == kStandIn ? 0u : m;
-}
+// (taken apart where it is used and not, for all rows, before the loop)
+__device__ __forceinline__ uint32_t plain(uint32_t mine) { return (uint32_t)anew((int)mine); }
 template <int W4> __device__ __forceinline__ float careful_dot(const Full& f, const v4f& row, const uint32_t (&mine)[4 * W4])
 {
     float sum = 0.0f;
     each<0, W4>([&](auto n) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            sum += full_product(f, real_bits(f, mine[4 * n.value + i]), from_lane<decltype(n)::value>(row[i]));
+            sum += full_product(f, plain(mine[4 * n.value + i]), from_lane<decltype(n)::value>(row[i]));
             __builtin_amdgcn_sched_barrier(0);    // (rare code: side by side the products took registers from the usual loops)
         }
     });

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     const Scoring scoring(a);
     const PairGrad<APPROXIMATE> pair{scoring, a.flags};
     const uint32_t dn_add = APPROXIMATE ? scoring.mul_add : 0u;
-    const Full full{a.off, a.off != 1.0f, 0u - scoring.mul_add}, full_dn{a.off, a.off != 1.0f, 0u - dn_add};
+    const Full full{a.off, a.off != 1.0f};
     const float4 record = a.records[(long)u.head * a.rows + row];
     const float M = record.x, unit = u2f((uint32_t)(127 - (int)record.z) << 23), dl = record.y * unit, slope = record.w;
     uint32_t q[W], dn[W];
@@ -240,10 +240,15 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
         careful = careful || in_team<NS>(gave_up);
         if (!APPROXIMATE)
 #pragma unroll
-            for (int d = 0; d < W; ++d) out[0][d] = over_power(out[0][d], q[d] + full.raw);
+            for (int d = 0; d < W; ++d) out[0][d] = over_power(out[0][d], q[d] - scoring.mul_add);
     }
     gave_up = false;
-    if (__builtin_expect(careful, 0))
+    if (__builtin_expect(careful, 0)) {
+        const Args g = arguments_again();
+        const Unit w = unit_of(g);
+        const long from = ((long)w.head * g.rows + row_of_lane<NS>(w, g.rows)) * g.dim;
+        load_plain<W4>(first, g.values, q, [&](int d) __attribute__((always_inline)) { return g.qs[from + d]; });
+        load_plain<W4>(first, g.values, dn, [&](int d) __attribute__((always_inline)) { return g.dn[from + d] * unit; });
         all_blocks<NS, W4, 1>(sight, begin, end, to, first, a.dim, exists, out, met, [](int) {}, [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
             float s[kBlock], de[kBlock], e[kBlock];
             if (!all && __ballot(sees != 0u) == 0ull) { skip(s, de); return true; }
@@ -258,10 +263,10 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
 #pragma unroll 1
             for (int j = 0; j < kBlock; ++j) {
                 const v4f row = values.template across<W4>(j1 + j);
-                if (APPROXIMATE || a.flags.a) de[0] = careful_dot<W4>(full_dn, row, dn);
+                if (APPROXIMATE || a.flags.a) de[0] = careful_dot<W4>(full, row, dn);
                 else {
                     de[0] = 0.0f;
-                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) { de[0] += exact_term(full, e[0], x, u2f(real_bits(full_dn, dn[d]))); });
+                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) { de[0] += exact_term(full, e[0], x, u2f(plain(dn[d]))); });
                 }
                 turned(de); turned(e);
             }
@@ -276,13 +281,14 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
                 if (APPROXIMATE || a.flags.a) careful_add_row<W4>(full, row, de[0], in, 1.0f, out[0]);
                 else
                     each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) {
-                        const float term = exact_term(full, u2f(real_bits(full, q[d])), x, de[0]);
+                        const float term = exact_term(full, u2f(plain(q[d])), x, de[0]);
                         out[0][d] += in ? term : 0.0f;
                     });
                 turned(de);
             }
             return true;
         });
+    }
     if (!a.whole && !met_anything<NS>(a, u, wave, met)) return;
     const float back = 1.0f / unit;
 #pragma unroll
@@ -314,14 +320,25 @@ __device__ __forceinline__ Sight sight_of_key(const Args& a, int b, int key)
     return s;
 }
 
+// A unit's keys: the first ones have most queries where the order is causal.
+__device__ __forceinline__ Unit unit_of_keys(const Args& a)
+{
+    Unit u = unit_of(a);
+    u.tile = a.tiles - 1 - u.tile;
+    return u;
+}
+template <int NS> __device__ __forceinline__ const float* key_of_lane(const Args& a, const Tokens& t)
+{
+    const Unit u = unit_of_keys(a);
+    return t.p + (long)u.b * t.sb + (long)row_of_lane<NS>(u, a.keys) * t.st + (long)u.kv * t.sh;
+}
 
 template <int NS, int W4, bool WHOLE, bool APPROXIMATE>
 __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(Args a)
 {
     constexpr int W = 4 * W4, N = 4 * Pipe<W4, WHOLE>::kQuads;
     __shared__ Slices<NS, kBlock> slices_s, slices_de;
-    Unit u = unit_of(a);
-    u.tile = a.tiles - 1 - u.tile;                // (the first keys have most queries where the order is causal)
+    const Unit u = unit_of_keys(a);
     const int wave = wave_of(), slice = wave % NS, lane = (int)threadIdx.x % 64, key0 = (u.tile * kTiles<NS> + wave / NS) * 64, mine = key0 + lane, key = min(mine, a.keys - 1), first = slice * W;
     const bool exists = mine < a.keys;
     const int chunk_begin = u.chunk * a.chunk, chunk_end = min(a.rows, chunk_begin + a.chunk);
@@ -342,10 +359,10 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     most = APPROXIMATE ? __builtin_amdgcn_readfirstlane(most) : 0;
     const uint32_t shift = 0u - ((uint32_t)most << 23);
     const float unit = u2f((uint32_t)(127 - most) << 23);
-    const Full full_q{a.off, a.off != 1.0f, 0u - scoring.mul_add}, full_n{a.off, a.off != 1.0f, 0u - scoring.mul_add - shift};
+    const Full full{a.off, a.off != 1.0f};
     uint32_t k[W], v[W];
-    bool odd = !load_lane<W4>(a.k.p + (long)u.b * a.k.sb + (long)key * a.k.st + (long)u.kv * a.k.sh, first, a.dim, a.values, 0u, scoring.mul_add, k);
-    odd = !load_lane<W4>(a.v.p + (long)u.b * a.v.sb + (long)key * a.v.st + (long)u.kv * a.v.sh, first, a.dim, a.values, 0u, scoring.mul_add + shift, v) || odd;
+    bool odd = !load_lane<W4>(key_of_lane<NS>(a, a.k), first, a.dim, a.values, 0u, scoring.mul_add, k);
+    odd = !load_lane<W4>(key_of_lane<NS>(a, a.v), first, a.dim, a.values, 0u, scoring.mul_add + shift, v) || odd;
     const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
     bool careful = in_team<NS>(odd) || unusual;
     const Stream<WHOLE> queries(a.qs + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);
@@ -446,17 +463,21 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
         careful = careful || in_team<NS>(gave_up);
         if (!APPROXIMATE)
 #pragma unroll
-            for (int d = 0; d < W; ++d) { out[0][d] = over_power(out[0][d], k[d] + full_q.raw); out[1][d] = over_power(out[1][d], v[d] + full_n.raw); }
+            for (int d = 0; d < W; ++d) { out[0][d] = over_power(out[0][d], k[d] - scoring.mul_add); out[1][d] = over_power(out[1][d], v[d] - scoring.mul_add - shift); }
     }
     gave_up = false;
-    if (__builtin_expect(careful, 0))
+    if (__builtin_expect(careful, 0)) {
+        const Args g = arguments_again();
+        const float* const of_k = key_of_lane<NS>(g, g.k); const float* const of_v = key_of_lane<NS>(g, g.v);
+        load_plain<W4>(first, g.values, k, [&](int d) __attribute__((always_inline)) { return of_k[d]; });
+        load_plain<W4>(first, g.values, v, [&](int d) __attribute__((always_inline)) { return of_v[d]; });
         all_blocks<NS, W4, 2>(sight, begin, end, to, first, a.dim, exists, out, met, [](int) {}, [&](int r1, uint32_t sees, bool all) __attribute__((always_inline)) {
             float s[kBlock], de[kBlock], e[kBlock];
             if (!all && __ballot(sees != 0u) == 0ull) { skip(s, de); return true; }
             bool wrong = false;
 #pragma unroll 1
             for (int j = 0; j < kBlock; ++j) {
-                s[0] = careful_dot<W4>(full_q, queries.template across<W4>(r1 + j), k);
+                s[0] = careful_dot<W4>(full, queries.template across<W4>(r1 + j), k);
                 turned(s);
             }
             slices_s.add_up(turn, wave, s, false);
@@ -465,15 +486,15 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
             for (int j = 0; j < kBlock; ++j) {
                 const v4f row = grads.template across<W4>(r1 + j);
                 const bool in = (counts >> j) & 1u;
-                if (APPROXIMATE || a.flags.a) de[0] = careful_dot<W4>(full_n, row, v) * unit;
+                if (APPROXIMATE || a.flags.a) de[0] = careful_dot<W4>(full, row, v) * unit;
                 else {
                     de[0] = 0.0f;
-                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) { de[0] += exact_term(full_n, e[0], u2f(real_bits(full_n, v[d])), x * unit); });
+                    each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) { de[0] += exact_term(full, e[0], u2f(plain(v[d])), x * unit); });
                 }
-                if (APPROXIMATE || a.flags.b) careful_add_row<W4>(full_n, row, e[0], in, unit, out[1]);
+                if (APPROXIMATE || a.flags.b) careful_add_row<W4>(full, row, e[0], in, unit, out[1]);
                 else
                     each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) {
-                        const float term = exact_term(full_n, u2f(real_bits(full_n, v[d])), e[0], x * unit);
+                        const float term = exact_term(full, u2f(plain(v[d])), e[0], x * unit);
                         out[1][d] += in ? term : 0.0f;
                     });
                 turned(de); turned(e);
@@ -486,16 +507,17 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
             for (int j = 0; j < kBlock; ++j) {
                 const v4f row = queries.template across<W4>(r1 + j);
                 const bool in = (counts >> j) & 1u;
-                if (APPROXIMATE || a.flags.b) careful_add_row<W4>(full_q, row, de[0], in, 1.0f, out[0]);
+                if (APPROXIMATE || a.flags.b) careful_add_row<W4>(full, row, de[0], in, 1.0f, out[0]);
                 else
                     each_of_row<W4>(row, [&](int d, float x) __attribute__((always_inline)) {
-                        const float term = exact_term(full_q, u2f(real_bits(full_q, k[d])), x, de[0]);
+                        const float term = exact_term(full, u2f(plain(k[d])), x, de[0]);
                         out[0][d] += in ? term : 0.0f;
                     });
                 turned(de);
             }
             return true;
         });
+    }
     if (!a.whole && !met_anything<NS>(a, u, wave, met)) return;
     const float back = 1.0f / unit;
 #pragma unroll

@@ -65,6 +65,21 @@ __device__ __forceinline__ Unit unit_of(const Args& a)
 }
 __device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
 
+// The launch's arguments as from memory: what the careful loops need is found again there, instead of in registers since the beginning.
+__device__ __forceinline__ Args arguments_again()
+{
+    auto at = (const __attribute__((address_space(4))) Args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const Args*)at;
+}
+template <int NS> __device__ __forceinline__ int row_of_lane(const Unit& u, int rows) { return min((u.tile * kTiles<NS> + wave_of() / NS) * 64 + (int)threadIdx.x % 64, rows - 1); }
+template <int NS> __device__ __forceinline__ const float* query_of_lane(const Args& a)
+{
+    const Unit u = unit_of(a);
+    const int row = row_of_lane<NS>(u, a.rows);
+    return a.q.p + (long)u.b * a.q.sb + (long)(row / a.group) * a.q.st + (long)(u.kv * a.group + row % a.group) * a.q.sh;
+}
+
 // What a query's row sees: its keys.
 __device__ __forceinline__ Sight sight_of_row(const Args& a, int b, int row)
 {
@@ -99,22 +114,9 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
         return;
     }
     const Scoring scoring(a);
-    const Full full{a.off, a.off != 1.0f, 0u - scoring.mul_add};
+    const Full full{a.off, a.off != 1.0f};
     uint32_t q[W];
-    bool careful;
-    {
-        // (q (*) scale first, by the full definition where it takes that)
-        const float* from = a.q.p + (long)u.b * a.q.sb + (long)token * a.q.st + (long)head * a.q.sh;
-        const uint32_t scale_add = f2u(a.scale) - kBias + scoring.off_add;
-        careful = in_team<NS>(!load_lane<W4>(from, first, a.dim, a.values, scale_add, scoring.mul_add, q));
-        if (careful) {
-#pragma unroll 1
-            for (int d = 0; d < W; ++d) {
-                if (first + d < a.values) q[0] = f2u(pam_mul_off(from[first + d], a.scale, a.off, full.has_off)) + scoring.mul_add;
-                turned(q);
-            }
-        }
-    }
+    bool careful = in_team<NS>(!load_lane<W4>(query_of_lane<NS>(a), first, a.dim, a.values, f2u(a.scale) - kBias + scoring.off_add, scoring.mul_add, q));       // (of q (*) scale)
     float slope = 0.0f, wrong = 0.0f;             // wrong: becomes NaN with the first number that is none
     if (scoring.slopes) { slope = held_slope(a.slopes[head]); wrong = finite(a.slopes[head]) ? 0.0f : u2f(kQNaN); }
     const Stream<WHOLE> keys(a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.keys, slice * W4, a.dim / 4);
@@ -210,7 +212,10 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
                 return true;
             });
     }
-    if (__builtin_expect(careful, 0))
+    if (__builtin_expect(careful, 0)) {
+        const Args g = arguments_again();
+        const float* const from = query_of_lane<NS>(g);
+        load_plain<W4>(first, g.values, q, [&](int d) __attribute__((always_inline)) { return pam_mul_off(from[d], g.scale, g.off, g.off != 1.0f); });
         run([](int) {}, [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
             float t[kBlock];
             if (!all && __ballot(sees != 0u) == 0ull) {
@@ -233,6 +238,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
             }
             return true;
         });
+    }
     if (folded) {
         const float f = scale_between(M_folded, M);
         row_in_memory<W4>(to, first, a.dim, exists, [&](int n, v4f& x) __attribute__((always_inline)) {

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kThreads, 4) void cached_attention_kernel(CacheArgs
     Args scoring_args{};
     scoring_args.cap = a.cap; scoring_args.off = a.off; scoring_args.slopes = a.slopes;
     const Scoring scoring(scoring_args);
-    const Full full{a.off, has_off, 0u};
+    const Full full{a.off, has_off};
 
     Lane here;
     here.first = lane % L * 4; here.values = a.values;
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_ke
     Args scoring_args{};
     scoring_args.cap = a.cap; scoring_args.off = a.off; scoring_args.slopes = a.slopes;
     const Scoring scoring(scoring_args);
-    const Full full{a.off, has_off, 0u};
+    const Full full{a.off, has_off};
     const uint32_t scale_add = f2u(a.scale) - kBias + scoring.off_add, key_add = scale_add + scoring.mul_add, mul_add = scoring.mul_add, none = kStandIn + mul_add;
     const Queries queries(a, me);
     const int* const table = a.table + (long)me.b * a.per_sequence;

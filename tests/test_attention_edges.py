@@ -37,6 +37,30 @@ def _compare(shape, masks, seed=0, approx=True, train=True, change=None, offset=
 
 # ---------------------------------------------------------------- a number that stands for zero
 
+@gpu
+@pytest.mark.parametrize("dim", [16, 64, 100])
+@pytest.mark.parametrize("large", [2.0 ** 85, 2.0 ** 39, 1.0])
+def test_the_power_of_two_that_zeros_stand_as(dim, large):
+    """Scaled queries, and keys, of just 2^-86 of either sign are numbers."""
+    def queries(q, k, v, dy):
+        q[:] = np.float32(2.0 ** -86) * np.sign(q); k[:] = np.float32(large) * np.sign(k)
+        q[:, 7, :, 1] = 2.0 ** -100                       # (a value out of the range sends the whole unit through the full definition)
+
+    def keys(q, k, v, dy):
+        k[:] = np.float32(2.0 ** -86) * np.sign(k); q[:] = np.float32(large) * np.sign(q)
+    for change in (queries, keys):
+        _compare((1, 45, 70, 2, 1, dim), dict(scale=1.0), seed=dim, change=change, train=False)
+
+
+@gpu
+@APPROX
+@pytest.mark.parametrize("dim", [16, 64, 100])
+def test_values_that_are_that_power(dim, approx):
+    def change(q, k, v, dy):
+        v[:, ::3] = np.float32(2.0 ** -86) * np.sign(v[:, ::3])
+        v[:, 1::3] *= np.float32(2.0 ** -80)
+    _compare((1, 45, 45, 2, 1, dim), {}, seed=dim + 1, approx=approx, change=change)
+
 
 # ---------------------------------------------------------------- weights and gradients far below the largest
 
