@@ -99,9 +99,10 @@ template <int N, class T> __device__ __forceinline__ void turned(T (&v)[N])     
 }
 
 // A lane's part of a row: bits(value) + scale + add, zeros and what lies behind the row's values stood in for (unscaled, by 2^-86, which is out of the
-// window).  scale: of a factor in 2^[-41, 41].  Returns false if a value, scaled, is out of the window.
+// window).  scale: of a factor in 2^[-41, 41]; factor: a power of two of any size, multiplied (an addition to the bits would take what is far below it through the
+// sign).  Returns false if a value, scaled, is out of the window.
 template <int W4>
-__device__ __forceinline__ bool load_lane(const float* row, int first, int dim, int values, uint32_t scale, uint32_t add, uint32_t (&out)[4 * W4])
+__device__ __forceinline__ bool load_lane(const float* row, int first, int dim, int values, uint32_t scale, uint32_t add, uint32_t (&out)[4 * W4], float factor = 1.0f)
 {
     uint32_t most = 0u;
     first = anew(first);
@@ -111,7 +112,7 @@ __device__ __forceinline__ bool load_lane(const float* row, int first, int dim, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool none = (f2u(x[i]) << 1) == 0u || first + 4 * n + i >= values;
-            const uint32_t b = f2u(x[i]) + scale;
+            const uint32_t b = f2u(x[i] * factor) + scale;
             most = max(most, none ? 0u : (b << 1) - (kLaneBase + 2u));
             out[4 * n + i] = (none ? kStandIn : b) + add;
         }
@@ -618,11 +619,11 @@ __device__ __forceinline__ float times(float x, uint32_t add)
     const int m = max((int)(size + add), 0);
     return u2f(size >= 0x7f000000u ? kQNaN : (uint32_t)m | (f2u(x) & kSign));
 }
-// a (*) b of any finite numbers whose product is below 2^128; an underflow (a zero's, too) is zero or next to nothing
+// a (*) b of any finite numbers; an underflow (a zero's, too) is zero or next to nothing, an overflow an infinity
 __device__ __forceinline__ float times_any(float a, float b, uint32_t off_add)
 {
-    const int m = (int)((f2u(a) & ~kSign) - kBias + (f2u(b) & ~kSign) + off_add);
-    return u2f((uint32_t)max(m, 0) | ((f2u(a) ^ f2u(b)) & kSign));
+    const uint32_t m = __builtin_elementwise_sub_sat((f2u(a) & ~kSign) + (f2u(b) & ~kSign), kBias - off_add);
+    return u2f(min(m, kExpo) | ((f2u(a) ^ f2u(b)) & kSign));
 }
 
 struct Scoring {

@@ -8,7 +8,8 @@
 // Scores and weights are computed again in both; kept, they would be 8 bytes a pair, as long to read as two of the products of 64 values.
 // 4096 causal tokens, 8 heads of 64 over 2: 1.07 ms for dq (12 T products/s), 1.65 for dk and dv (10), exact 1.6 and 2.1; three wavefronts on a SIMD are 6 % better than two for the
 // first, and 30 % worse for the second, whose four slices of 32 then do not fit the registers.
-// All that is linear in dy is scaled by a power of two: in the first kernel a query's largest |dn| to [1, 2), in the second the largest of a chunk's.
+// All that is linear in dy is scaled by a power of two: in the first kernel a query's largest |dn| to [1, 2), in the second the largest of a chunk's.  The full definition
+// scales up only, so that nothing is lost beside a large value.
 #pragma once
 #include "pam_attention_fwd.h"
 
@@ -25,11 +26,11 @@ struct PairGrad {
     // own (*) other, for own; other positive
     __device__ __forceinline__ float of_mul(float own, float other, float d) const
     { return a_approx() ? times_any(d, other, s.off_add) : d * slope(f2u(other) + s.off_add, own); }
-    // (integer additions know no NaN; gradients of 2^110 beside a row's largest |dn| count as one)
+    // (integer additions know no NaN; through a cap a gradient of 2^90 counts as one, whose products on the way are below 2^127)
     __device__ __forceinline__ float checked(float a, float score, float e, float de) const
     {
         const float d = (*this)(a, score, e, de);
-        return fabsf(de) < 0x1p110f && e == e ? d : u2f(kQNaN);
+        return fabsf(de) < (s.cap == 0.0f ? u2f(kExpo) : 0x1p90f) && e == e ? d : u2f(kQNaN);
     }
     __device__ __forceinline__ float operator()(float a, float score, float e, float de) const
     {
@@ -138,11 +139,12 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     const uint32_t dn_add = APPROXIMATE ? scoring.mul_add : 0u;
     const Full full{a.off, a.off != 1.0f};
     const float4 record = a.records[(long)u.head * a.rows + row];
-    const float M = record.x, unit = u2f((uint32_t)(127 - (int)record.z) << 23), dl = record.y * unit, slope = record.w;
+    const float M = record.x, slope = record.w;
+    float unit = u2f((uint32_t)(127 - (int)record.z) << 23), dl = record.y * unit;
     uint32_t q[W], dn[W];
     const long at = ((long)u.head * a.rows + row) * a.dim;
     bool odd = !load_lane<W4>(a.qs + at, first, a.dim, a.values, 0u, scoring.mul_add, q);
-    odd = !load_lane<W4>(a.dn + at, first, a.dim, a.values, 0u - ((uint32_t)(int)record.z << 23), dn_add, dn) || odd;
+    odd = !load_lane<W4>(a.dn + at, first, a.dim, a.values, 0u, dn_add, dn, unit) || odd;
     odd = odd || !finite(dl);
     // (all slopes, and no offset: what the usual way of the other kernel has)
     const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
@@ -246,7 +248,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     if (__builtin_expect(careful, 0)) {
         const Args g = arguments_again();
         const Unit w = unit_of(g);
-        const long from = ((long)w.head * g.rows + row_of_lane<NS>(w, g.rows)) * g.dim;
+        const long of = (long)w.head * g.rows + row_of_lane<NS>(w, g.rows), from = of * g.dim;
+        unit = fmaxf(unit, 1.0f); dl = g.records[of].y * unit;
         load_plain<W4>(first, g.values, q, [&](int d) __attribute__((always_inline)) { return g.qs[from + d]; });
         load_plain<W4>(first, g.values, dn, [&](int d) __attribute__((always_inline)) { return g.dn[from + d] * unit; });
         all_blocks<NS, W4, 1>(sight, begin, end, to, first, a.dim, exists, out, met, [](int) {}, [&](int j1, uint32_t sees, bool all) __attribute__((always_inline)) {
@@ -358,7 +361,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     for (int s = 1; s < 64; s *= 2) most = max(most, __shfl_xor(most, s, 64));
     most = APPROXIMATE ? __builtin_amdgcn_readfirstlane(most) : 0;
     const uint32_t shift = 0u - ((uint32_t)most << 23);
-    const float unit = u2f((uint32_t)(127 - most) << 23);
+    float unit = u2f((uint32_t)(127 - most) << 23);
     const Full full{a.off, a.off != 1.0f};
     uint32_t k[W], v[W];
     bool odd = !load_lane<W4>(key_of_lane<NS>(a, a.k), first, a.dim, a.values, 0u, scoring.mul_add, k);
@@ -468,6 +471,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     gave_up = false;
     if (__builtin_expect(careful, 0)) {
         const Args g = arguments_again();
+        unit = fmaxf(unit, 1.0f);
         const float* const of_k = key_of_lane<NS>(g, g.k); const float* const of_v = key_of_lane<NS>(g, g.v);
         load_plain<W4>(first, g.values, k, [&](int d) __attribute__((always_inline)) { return of_k[d]; });
         load_plain<W4>(first, g.values, v, [&](int d) __attribute__((always_inline)) { return of_v[d]; });

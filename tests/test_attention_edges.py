@@ -34,6 +34,33 @@ def _compare(shape, masks, seed=0, approx=True, train=True, change=None, offset=
 
 # ---------------------------------------------------------------- gradients that span more than an integer addition may
 
+@gpu
+@APPROX
+@pytest.mark.parametrize("large,small", [(2.0 ** 12, 1e-40), (2.0 ** 9, 1e-39), (2.0 ** 60, 2.0 ** -118), (2.0 ** 40, 2.0 ** -100), (1e-20, 1e-41)])
+@pytest.mark.parametrize("dim", [16, 64, 130])
+def test_a_gradient_of_very_different_sizes(dim, large, small, approx):
+    """A query's gradient is scaled by its largest value: what is far below that may neither wrap nor be read for another number."""
+    def change(q, k, v, dy):
+        dy[:, 11] = np.float32(small) * np.sign(dy[:, 11])
+        dy[:, 11, :, 0] = large
+        dy[:, 30, :, 5] = large
+        dy[:, 30, :, 7] = small
+    _compare((1, 45, 45, 2, 1, dim), {}, seed=dim, approx=approx, change=change)
+
+
+@gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@APPROX
+def test_a_gradient_that_is_no_number(value, approx):
+    """It reaches its query's gradient, and those of the keys that the query sees, whatever else is in the row."""
+    q, k, v, dy = _inputs(4, 1, 40, 40, 2, 1, 32)
+    v[..., 7] = 0                                        # (y is zero there, too)
+    dy[0, 20, 0, 7] = value
+    y, (dq, dk, dv) = _run(q, k, v, dy, {}, approx)
+    assert torch.isfinite(y).all()
+    assert dq[0, 20, 0].isnan().all() and torch.isfinite(dq[0, :20]).all() and torch.isfinite(dq[0, 21:]).all() and torch.isfinite(dq[0, 20, 1]).all()
+    assert dk[0, :21].isnan().all() and torch.isfinite(dk[0, 21:]).all()
+
 
 # ---------------------------------------------------------------- a number that stands for zero
 
