@@ -82,7 +82,7 @@ template <int N, int END, class F> __device__ __forceinline__ void each(F&& f)
 }
 
 constexpr uint32_t kStreamBase = (uint32_t)(127 - 40) << 24, kStreamSpan = 80u << 24;      // 2^[-40, 40) of bits << 1
-constexpr uint32_t kLaneBase = (uint32_t)(127 - 86) << 24, kLaneSpan = 166u << 24;         // 2^(-86, 80), ends left out: [-86, 80) where nothing stands in
+constexpr uint32_t kLaneBase = (uint32_t)(127 - 86) << 24, kLaneSpan = 166u << 24;         // 2^[-86, 80)
 constexpr uint32_t kStandIn = (uint32_t)(127 - 86) << 23;
 
 // (comparisons with it are made where they are used, instead of kept from the beginning of a kernel to its end)
@@ -98,10 +98,10 @@ template <int N, class T> __device__ __forceinline__ void turned(T (&v)[N])     
     v[N - 1] = first;
 }
 
-// A lane's part of a row: bits(value) + scale + add, zeros and what lies behind the row's values stood in for (unscaled, by 2^-86, which is out of the
-// window).  scale: of a factor in 2^[-41, 41]; factor: a power of two of any size, multiplied (an addition to the bits would take what is far below it through the
+// A lane's part of a row: bits(value) + scale + add, zeros and what lies behind the row's values stood in for (unscaled, by 2^LOW, which is out of the
+// window, 2^(LOW, 80)).  scale: of a factor in 2^[-41, 41]; factor: a power of two of any size, multiplied (an addition to the bits would take what is far below it through the
 // sign).  Returns false if a value, scaled, is out of the window.
-template <int W4>
+template <int W4, int LOW = -86>
 __device__ __forceinline__ bool load_lane(const float* row, int first, int dim, int values, uint32_t scale, uint32_t add, uint32_t (&out)[4 * W4], float factor = 1.0f)
 {
     uint32_t most = 0u;
@@ -113,11 +113,11 @@ __device__ __forceinline__ bool load_lane(const float* row, int first, int dim, 
         for (int i = 0; i < 4; ++i) {
             const bool none = (f2u(x[i]) << 1) == 0u || first + 4 * n + i >= values;
             const uint32_t b = f2u(x[i] * factor) + scale;
-            most = max(most, none ? 0u : (b << 1) - (kLaneBase + 2u));
-            out[4 * n + i] = (none ? kStandIn : b) + add;
+            most = max(most, none ? 0u : (b << 1) - (((uint32_t)(127 + LOW) << 24) + 2u));
+            out[4 * n + i] = (none ? (uint32_t)(127 + LOW) << 23 : b) + add;
         }
     }
-    return most < kLaneSpan - 2u;
+    return most < ((uint32_t)(80 - LOW) << 24) - 2u;
 }
 // ... as the full definition takes it: the values themselves, zeros behind the row's
 template <int W4, class Value>

@@ -365,7 +365,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     const Full full{a.off, a.off != 1.0f};
     uint32_t k[W], v[W];
     bool odd = !load_lane<W4>(key_of_lane<NS>(a, a.k), first, a.dim, a.values, 0u, scoring.mul_add, k);
-    odd = !load_lane<W4>(key_of_lane<NS>(a, a.v), first, a.dim, a.values, 0u, scoring.mul_add + shift, v) || odd;
+    // (exact slopes of e (*) v are taken with v in the lane: weights of 2^-62 leave it 2^-64)
+    odd = !load_lane<W4, APPROXIMATE ? -86 : -64>(key_of_lane<NS>(a, a.v), first, a.dim, a.values, 0u, scoring.mul_add + shift, v) || odd;
     const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
     bool careful = in_team<NS>(odd) || unusual;
     const Stream<WHOLE> queries(a.qs + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import _attention_general as general
+import test_attention
 from test_attention import _check, _cuda, _inputs, _run
 
 gpu = pytest.mark.gpu
@@ -91,6 +92,18 @@ def test_values_that_are_that_power(dim, approx):
 
 # ---------------------------------------------------------------- weights and gradients far below the largest
 
+@gpu
+@APPROX
+@pytest.mark.parametrize("dim", [16, 32, 100])
+def test_zeros_and_tiny_values_of_small_weight(dim, approx):
+    """Weights down to 2^-60 with values that are zero, or small: their products are far below one."""
+    def change(q, k, v, dy):
+        rng = np.random.RandomState(dim)
+        q[:] = np.abs(q); k[:] = np.abs(k) * np.linspace(-4.0, 4.0, k.shape[1], dtype=np.float32)[None, :, None, None] * np.float32(16.0 / dim ** 0.5)
+        v[rng.random_sample(v.shape) < 0.2] = 0
+        v[:, ::5] *= np.float32(2.0 ** -70)
+    _compare((1, 60, 130, 1, 1, dim), dict(causal=False), seed=4, approx=approx, change=change)
+
 
 # ---------------------------------------------------------------- the ends of the range
 
@@ -136,10 +149,32 @@ def test_no_numbers_beside_an_offset(where, value, offset):
 # ---------------------------------------------------------------- offsets, slopes of each kind, masks over several spans
 
 MASKS = {
-    "causal": {}, "all": dict(causal=False), "window": dict(window=70), "window_both_ways": dict(window=30, causal=False), "prefix": dict(prefix=np.array([100, 3])),
-    "documents": dict(documents=np.repeat(np.array([[0, 1, 2, -1], [5, 1 << 40, 5, 5]]), 36, axis=1)), "slopes": dict(slopes=np.array([0.5, 0.03], np.float32)),
+    "causal": {}, "all": dict(causal=False), "window": dict(window=70), "window_both_ways": dict(window=30, causal=False), "prefix": dict(prefix=np.array([100])),
+    "documents": dict(documents=np.repeat(np.array([[0, 1 << 40, 0, -1, 2]]), 29, axis=1)[:, :144]), "slopes": dict(slopes=np.array([0.5, 0.03], np.float32)),
     "cap": dict(cap=3.0), "cap_and_window": dict(cap=10.0, window=65),
 }
+
+
+@gpu
+@pytest.mark.parametrize("name", MASKS)
+@pytest.mark.parametrize("dim", [16, 24])
+def test_exact_gradients_over_several_spans(dim, name):
+    _compare((1, 144, 144, 2, 1, dim), MASKS[name], 31, False, tight=0.0 if "cap" in name else 0.2)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [130, 256])
+def test_exact_gradients_of_wide_heads(dim):
+    _compare((1, 70, 70, 1, 1, dim), {}, 32, False, tight=0.1)
+
+
+@gpu
+@pytest.mark.parametrize("approx", [True, False, (True, False), (False, True), (False, False)], ids=str)
+@pytest.mark.parametrize("offset", [None, 0.77, 1.0552, 1.4])
+@pytest.mark.parametrize("more", [{}, dict(cap=4.0), dict(slopes=np.array([0.25, 0.5], np.float32))], ids=["plain", "cap", "slopes"])
+def test_gradients_of_either_kind_and_offset(more, offset, approx):
+    _compare((1, 7, 9, 2, 1, 8), more, 34, approx, offset=offset, tight=0.25)
+    _compare((1, 30, 75, 2, 1, 24), more, 35, approx, offset=offset)
 
 
 # ---------------------------------------------------------------- scratch
@@ -156,3 +191,12 @@ def _scratch(tokens, heads, kv_heads, dim, window, batch=1, keys=None, causal=Tr
     forward.restype = backward.restype = ctypes.c_size_t
     s = _Shape(batch, tokens, keys or tokens, heads, kv_heads, dim, dim, 0.125, 0.0, 1.0, causal, window, None, None, None)
     return forward(ctypes.byref(s)), backward(ctypes.byref(s), 1, 1)
+
+
+@gpu
+@pytest.mark.parametrize("shape,masks", [((1, 700, 700, 2, 1, 16), dict(window=100)), ((1, 1100, 1100, 1, 1, 16), dict(window=65)), ((2, 300, 1000, 2, 2, 20), dict(window=333)),
+                                         ((1, 900, 900, 1, 1, 20), dict(window=90, causal=False)), ((1, 500, 700, 1, 1, 16), dict(window=80, prefix=np.array([130]))),
+                                         ((1, 64, 2000, 1, 1, 16), dict(window=1500)), ((1, 40, 20, 1, 1, 16), dict(window=5)), ((1, 300, 200, 2, 1, 16), dict(window=90, causal=False))],
+                         ids=lambda x: "x".join(map(str, x)) if isinstance(x, tuple) else "_".join(x))
+def test_windows_of_many_tiles(shape, masks):
+    test_attention._compare(shape, masks, seed=sum(shape))
