@@ -20,8 +20,10 @@
 // gradients 14.5 and 11: a sixth to a third of the instructions are the weights', which slices make twice, and two or three wavefronts on a SIMD do not
 // cover all waits for the scalar cache.
 //
-// The integer addition is the product while no exponent leaves the normal range.  Streamed values have to be in 2^[-40, 40), a lane's in 2^(-86, 80); a
-// lane's zero stands as 2^-86, which adds less to a sum than its rounding.  Streamed rows with zeros take a loop that leaves those out by a factor.
+// The integer addition is the product while no exponent leaves the normal range.  Streamed values have to be in 2^[-40, 40), a lane's in 2^(-86, 80).  A
+// lane's zero stands as 2^-86, and so does what lies behind a head's values: next to nothing in a score, and beside products that the sum has besides.  Where it may
+// have none such: sums of approximate gradients that are that small make their unit begin again (below); exact slopes, which take the fraction of a score, have a lane with zeros
+// in the loop that streamed rows with zeros take, which leaves those out by a factor.  Values in front of the places behind a head's are at least 2^28 times what stands there.
 // With anything else in a streamed row, or in a lane's, a unit begins again with the full definition (`careful`), its lanes' rows read again as they are: kept apart
 // from the usual loops, because side by side with them it took their registers.
 // Every value of a block is looked at for that by one lane, with vector loads of its own.
@@ -87,6 +89,8 @@ constexpr uint32_t kStandIn = (uint32_t)(127 - 86) << 23;
 
 // (comparisons with it are made where they are used, instead of kept from the beginning of a kernel to its end)
 __device__ __forceinline__ int anew(int v) { asm volatile("" : "+v"(v)); return v; }
+// (a lane's value, taken apart where it is used and not, for all rows, before the loop)
+__device__ __forceinline__ uint32_t plain(uint32_t mine) { return (uint32_t)anew((int)mine); }
 
 __device__ __forceinline__ uint32_t lane_pad(uint32_t shift) { return shift - kBias; }
 
@@ -98,26 +102,37 @@ template <int N, class T> __device__ __forceinline__ void turned(T (&v)[N])     
     v[N - 1] = first;
 }
 
-// A lane's part of a row: bits(value) + scale + add, zeros and what lies behind the row's values stood in for (unscaled, by 2^LOW, which is out of the
-// window, 2^(LOW, 80)).  scale: of a factor in 2^[-41, 41]; factor: a power of two of any size, multiplied (an addition to the bits would take what is far below it through the
-// sign).  Returns false if a value, scaled, is out of the window.
-template <int W4, int LOW = -86>
-__device__ __forceinline__ bool load_lane(const float* row, int first, int dim, int values, uint32_t scale, uint32_t add, uint32_t (&out)[4 * W4], float factor = 1.0f)
+// How a lane's values are held: they have to be in 2^(least, top); a zero and what lies behind the row's values have bits that no such value has.
+constexpr uint32_t bits_of_power(int e) { return (uint32_t)(127 + e) << 23; }
+struct Form {
+    int least, top; uint32_t zero, behind;
+    static __device__ __forceinline__ Form plain() { return Form{-86, 80, kStandIn, kStandIn}; }
+};
+// What a lane found in its part of a row: a value out of the window, a zero, anything but zeros.
+struct Held { bool odd, zeros, numbers; };
+// A lane's part of a row: bits(value) + scale + add, zeros and what lies behind the row's values stood in for (unscaled).  scale: of a factor in 2^[-41, 41];
+// factor: a power of two of any size, multiplied (an addition to the bits would take what is far below it through the sign).
+template <int W4>
+__device__ __forceinline__ Held load_lane(const float* row, int first, int dim, int values, uint32_t scale, uint32_t add, uint32_t (&out)[4 * W4], const Form& form, float factor = 1.0f)
 {
     uint32_t most = 0u;
+    bool zeros = false, numbers = false;
     first = anew(first);
+    const uint32_t base = ((uint32_t)(127 + form.least) << 24) + 2u;
 #pragma unroll
     for (int n = 0; n < W4; ++n) {
         const v4f x = *reinterpret_cast<const v4f_any*>(row + min(first + 4 * n, dim - 4));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool none = (f2u(x[i]) << 1) == 0u || first + 4 * n + i >= values;
+            const bool behind = first + 4 * n + i >= values, zero = (f2u(x[i]) << 1) == 0u;
             const uint32_t b = f2u(x[i] * factor) + scale;
-            most = max(most, none ? 0u : (b << 1) - (((uint32_t)(127 + LOW) << 24) + 2u));
-            out[4 * n + i] = (none ? (uint32_t)(127 + LOW) << 23 : b) + add;
+            most = max(most, zero || behind ? 0u : (b << 1) - base);
+            zeros = zeros || (zero && !behind);
+            numbers = numbers || !(zero || behind);
+            out[4 * n + i] = (behind ? form.behind : zero ? form.zero : b) + add;
         }
     }
-    return most < ((uint32_t)(80 - LOW) << 24) - 2u;
+    return Held{most >= ((uint32_t)(form.top - form.least) << 24) - 2u, zeros, numbers};
 }
 // ... as the full definition takes it: the values themselves, zeros behind the row's
 template <int W4, class Value>
@@ -260,13 +275,31 @@ template <int N> __device__ __forceinline__ void add_piece(const Piece& x, uint3
     if constexpr (N % 8 != 0) asm(PAM_EACH4(PAM_OF_WEIGHT) PAM_EACH4(PAM_ADD) : PAM_O4(N - 4), PAM_T4 : PAM_S4(N - 4), [w] "v"(w), [f] "v"(f));
 }
 
-// ... of a row with zeros, whose products count for nothing
-template <int N> __device__ __forceinline__ void dot_piece_with_zeros(const Piece& x, const uint32_t* m, float& sum)
+// ... of a row with zeros, whose products count for nothing; so do a lane's, of which `lane` has what stands for them (with `add`)
+struct Zeros { uint32_t zero, behind; };
+// Lanes whose zeros stand as 2^ZERO and what lies behind as 2^BEHIND: whether there are zeros, and `add`.
+template <int ZERO, int BEHIND> struct LaneZeros {
+    static constexpr bool kLanes = true;
+    int any; uint32_t add;
+    __device__ __forceinline__ Zeros codes() const
+    {
+        uint32_t from = add;
+        asm volatile("" : "+s"(from));            // (made where they are used: all the time they would take scalar registers from the usual loops)
+        return Zeros{bits_of_power(ZERO) + from, bits_of_power(BEHIND) + from};
+    }
+};
+struct NoLaneZeros {
+    static constexpr bool kLanes = false;
+    static constexpr int any = 0;
+    __device__ __forceinline__ Zeros codes() const { return Zeros{}; }
+};
+template <int N, bool LANES> __device__ __forceinline__ void dot_piece_with_zeros(const Piece& x, const uint32_t* m, const Zeros& lane, float& sum)
 {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const bool none = (f2u(at(x, i)) << 1) == 0u;
-        sum = __builtin_fmaf(u2f((none ? kBias : f2u(at(x, i))) + m[i]), none ? 0.0f : 1.0f, sum);
+        const uint32_t mine = LANES ? plain(m[i]) : m[i];
+        const bool streamed = (f2u(at(x, i)) << 1) == 0u, none = streamed || (LANES && (mine == lane.zero || mine == lane.behind));
+        sum = __builtin_fmaf(u2f((streamed ? kBias : f2u(at(x, i))) + mine), none ? 0.0f : 1.0f, sum);
     }
 }
 template <int N> __device__ __forceinline__ void add_piece_with_zeros(const Piece& x, uint32_t w, float f, float* o)
@@ -299,6 +332,15 @@ template <int N> __device__ __forceinline__ void dot_lane_power_piece(const Piec
         asm(PAM_EACH8(PAM_OF_LANE) PAM_EACH8(PAM_POWER) PAM_EACH8(PAM_SUM_BY_ROW) : [sum] "+v"(sum), PAM_T8 : PAM_S8(n), PAM_M8(n), [w] "v"(w), [mask] "v"(mask));
     if constexpr (N % 8 != 0)
         asm(PAM_EACH4(PAM_OF_LANE) PAM_EACH4(PAM_POWER) PAM_EACH4(PAM_SUM_BY_ROW) : [sum] "+v"(sum), PAM_T4 : PAM_S4(N - 4), PAM_M4(N - 4), [w] "v"(w), [mask] "v"(mask));
+}
+// ... with zeros in the lane
+template <int N> __device__ __forceinline__ void dot_lane_power_piece_with_zeros(const Piece& x, uint32_t w, uint32_t mask, const uint32_t* m, const Zeros& lane, float& sum)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t mine = plain(m[i]);
+        sum = __builtin_fmaf(at(x, i), u2f((w + mine) & (mine == lane.zero || mine == lane.behind ? 0u : mask)), sum);
+    }
 }
 // out_d += f * power(row's d (*) lane's d)
 template <int N> __device__ __forceinline__ void add_power_piece(const Piece& x, float f, uint32_t mask, const uint32_t* m, float* o)
@@ -403,6 +445,19 @@ template <int W4, bool WHOLE> __device__ __forceinline__ Verdict judge(Look<W4, 
     return v;
 }
 
+// The power of two above a block's values.
+template <int W4, bool WHOLE> __device__ __forceinline__ float above_all(const Look<W4, WHOLE>& look)
+{
+    uint32_t most = 0u;
+#pragma unroll
+    for (int i = 0; i < Look<W4, WHOLE>::kParts; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) most = max(most, f2u(look.r[i][c]) & ~kSign);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, s, 64));
+    return u2f((most & kExpo) + (1u << 23));
+}
+
 // ... where values are only factors of a float product: zeros and small ones are as good as any
 template <int W4, bool WHOLE> __device__ __forceinline__ bool all_finite(Look<W4, WHOLE>& look, const Stream<WHOLE>& s, int values)
 {
@@ -422,8 +477,6 @@ __device__ __forceinline__ float full_product(const Full& f, uint32_t a, uint32_
     const float c = pam_general(a, b);
     return f.has_off ? pam_general(f2u(c), f2u(f.off)) : c;
 }
-// (taken apart where it is used and not, for all rows, before the loop)
-__device__ __forceinline__ uint32_t plain(uint32_t mine) { return (uint32_t)anew((int)mine); }
 template <int W4> __device__ __forceinline__ float careful_dot(const Full& f, const v4f& row, const uint32_t (&mine)[4 * W4])
 {
     float sum = 0.0f;
@@ -448,16 +501,19 @@ template <int W4> __device__ __forceinline__ void careful_add_row(const Full& f,
     });
 }
 
-// A block's sums of products with the rows of s; then comes row j2 of `next`.
-template <int W4, bool WHOLE>
-__device__ __forceinline__ void block_dots(Pipe<W4, WHOLE>& pipe, const Stream<WHOLE>& s, int j1, const Stream<WHOLE>& next, int j2, bool zeros, const uint32_t (&mine)[4 * W4], float (&sum)[kBlock])
+// A block's sums of products with the rows of s; then comes row j2 of `next`.  With LaneZeros a lane's zeros have products of zero to the bit, else of next to nothing,
+// which is as good for a score alone.
+template <int W4, bool WHOLE, class Lane>
+__device__ __forceinline__ void block_dots(Pipe<W4, WHOLE>& pipe, const Stream<WHOLE>& s, int j1, const Stream<WHOLE>& next, int j2, bool zeros, const Lane& lane, const uint32_t (&mine)[4 * W4],
+                                           float (&sum)[kBlock])
 {
     constexpr int N = 4 * Pipe<W4, WHOLE>::kQuads;
 #pragma unroll
     for (int j = 0; j < kBlock; ++j) sum[j] = 0.0f;
-    if (__builtin_expect(zeros, 0)) {
+    if (__builtin_expect(zeros || lane.any != 0, 0)) {
+        const Zeros codes = lane.codes();
         pipe.rolled(s, j1, next, j2, [&](int h, int d, const Piece& x) __attribute__((always_inline)) {
-            dot_piece_with_zeros<N>(x, mine + d, sum[0]);
+            dot_piece_with_zeros<N, Lane::kLanes>(x, mine + d, codes, sum[0]);
             if (h == Pipe<W4, WHOLE>::kPieces - 1) turned(sum);
         });
         return;

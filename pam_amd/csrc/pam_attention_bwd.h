@@ -121,6 +121,31 @@ template <int NS> __device__ __forceinline__ bool met_anything(const Args& a, co
     return met;
 }
 
+// How lanes hold what they own.  behind: the slices have places behind a head's values.  Exact slopes are taken with the lane's value, whose zero has to be a power of
+// two that keeps the product where sums have all their bits: the window's end.  (Those of e (*) v with v in the lane: weights of 2^-62 leave it 2^-64.)
+constexpr int kZero = -86, kZeroOfSlopes = 30, kBehindWeights = -64;
+__device__ __forceinline__ Form form_of(bool approximate, bool behind)
+{ return Form{behind ? kZero + 28 : kZero, approximate ? 80 : kZeroOfSlopes, bits_of_power(approximate ? kZero : kZeroOfSlopes), bits_of_power(kZero)}; }
+__device__ __forceinline__ Form form_of_weighted(bool behind) { return Form{behind ? kBehindWeights + 28 : kBehindWeights, kZeroOfSlopes, bits_of_power(kZeroOfSlopes), bits_of_power(kBehindWeights)}; }
+
+// Sums of up to 256 products of which a lane's zeros have made some 2^-86 times a streamed value below `above`: as good as rounded if they are at least this, and zero where the
+// lane has nothing else.
+constexpr float kLeastSum = 0x1p-54f;             // 2^8 2^-86 2^24
+__device__ __forceinline__ void without_zeros(bool zeros, bool numbers, float (&sum)[kBlock])
+{
+    if (__builtin_expect(zeros, 0))
+#pragma unroll
+        for (int j = 0; j < kBlock; ++j) sum[j] = numbers ? sum[j] : 0.0f;
+}
+__device__ __forceinline__ bool too_small(bool zeros, const float (&sum)[kBlock], uint32_t counts, float above)
+{
+    bool found = false;
+    if (__builtin_expect(zeros, 0))
+#pragma unroll
+        for (int j = 0; j < kBlock; ++j) found = found || ((counts >> j) & 1u && sum[j] != 0.0f && fabsf(sum[j]) < kLeastSum * above);
+    return found;
+}
+
 template <int NS, int W4, bool WHOLE, bool APPROXIMATE>
 __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Args a)
 {
@@ -143,12 +168,19 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     float unit = u2f((uint32_t)(127 - (int)record.z) << 23), dl = record.y * unit;
     uint32_t q[W], dn[W];
     const long at = ((long)u.head * a.rows + row) * a.dim;
-    bool odd = !load_lane<W4>(a.qs + at, first, a.dim, a.values, 0u, scoring.mul_add, q);
-    odd = !load_lane<W4>(a.dn + at, first, a.dim, a.values, 0u, dn_add, dn, unit) || odd;
+    // (what the exact slopes of e (*) v weigh is a factor, and may be zero)
+    const bool behind = a.values < NS * W;
+    const Form q_form = form_of(APPROXIMATE, behind), dn_form = APPROXIMATE ? form_of(true, behind) : Form{-86, 80, 0u, 0u};
+    const Held of_q = load_lane<W4>(a.qs + at, first, a.dim, a.values, 0u, scoring.mul_add, q, q_form);
+    const Held of_dn = load_lane<W4>(a.dn + at, first, a.dim, a.values, 0u, dn_add, dn, dn_form, unit);
+    const bool counts_at_all = M != u2f(kExpo);
+    bool odd = of_q.odd || of_dn.odd;
+    const bool zeros = in_team<NS>((APPROXIMATE ? of_dn.zeros : of_q.zeros) && counts_at_all);
+    const LaneZeros<kZeroOfSlopes, kZero> q_zeros{zeros, scoring.mul_add};
     odd = odd || !finite(dl);
     // (all slopes, and no offset: what the usual way of the other kernel has)
     const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
-    bool careful = in_team<NS>(odd && M != u2f(kExpo)) || unusual;
+    bool careful = in_team<NS>(odd && counts_at_all) || unusual;
     const Stream<WHOLE> keys(a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.keys, slice * W4, a.dim / 4);
     const Stream<WHOLE> values(a.v.p + (long)u.b * a.v.sb + (long)u.kv * a.v.sh, a.v.st, a.keys, slice * W4, a.dim / 4);
     float out[1][W];
@@ -156,6 +188,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     float* const to[1] = {a.out0 + (a.whole ? ((long)u.b * a.tokens + row / a.group) * a.heads + head : ((long)u.head * a.chunks + u.chunk) * a.rows + row) * a.dim};
     int turn = 0;
     // weights from scores, and which ones count (what is no number does)
+    const bool ones_behind = !APPROXIMATE && a.values != a.dim;                  // (a key's row has ones behind its values: beside them a tiny score has no fraction left)
     const auto weigh = [&](const float (&s)[kBlock], float (&e)[kBlock], uint32_t sees, bool all, int j1, bool& wrong) __attribute__((always_inline)) {
         uint32_t counts = 0u;
 #pragma unroll
@@ -163,6 +196,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
             float power = scoring.exponent(s[j], slope, pos - (j1 + j)) - M;
             if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
             wrong = wrong || power != power;
+            if (!APPROXIMATE) wrong = wrong || (ones_behind && power >= kLeast && s[j] != 0.0f && fabsf(s[j]) < 0x1p-50f);
             counts |= power < kLeast ? 0u : 1u << j;
             e[j] = power_of_two(fminf(fmaxf(power, kLeast), 60.0f));
             e[j] = power != power ? power : e[j];
@@ -198,15 +232,20 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
                     return skip(s, de);
                 }
                 const Verdict kv = judge(look_k, keys, a.values, 0u), vv = judge(look_v, values, a.values, 0u);
+                float above = 0.0f;
+                if (APPROXIMATE && zeros) above = above_all(look_v);
                 look_k.load(keys, j1 + kBlock);
                 look_v.load(values, j1 + kBlock);
                 bool wrong = false;
-                block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, kv.zeros, q, s);
+                if constexpr (APPROXIMATE) block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, kv.zeros, NoLaneZeros{}, q, s);
+                else block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, kv.zeros, q_zeros, q, s);
                 bool wild = slices_s.add_up(turn, wave, s, gave_up || kv.wild || vv.wild);
                 if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
                 uint32_t counts = weigh(s, e, sees, all, j1, wrong);
-                if constexpr (APPROXIMATE) block_dots<W4, WHOLE>(pipe, values, j1, keys, j1, vv.zeros, dn, de);
-                else {
+                if constexpr (APPROXIMATE) {
+                    block_dots<W4, WHOLE>(pipe, values, j1, keys, j1, vv.zeros, NoLaneZeros{}, dn, de);
+                    without_zeros(zeros, of_dn.numbers, de);
+                } else {
 #pragma unroll
                     for (int j = 0; j < kBlock; ++j) de[j] = 0.0f;
                     uint32_t left = counts;
@@ -224,6 +263,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
                 }
                 slices_de.add_up(turn, wave, de, false);
                 turn ^= 1;
+                if (APPROXIMATE) wrong = wrong || too_small(zeros, de, counts, above);
 #pragma unroll
                 for (int j = 0; j < kBlock; ++j) {
                     de[j] = score_gradient(s[j], e[j], de[j], pos - (j1 + j));
@@ -364,9 +404,13 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     float unit = u2f((uint32_t)(127 - most) << 23);
     const Full full{a.off, a.off != 1.0f};
     uint32_t k[W], v[W];
-    bool odd = !load_lane<W4>(key_of_lane<NS>(a, a.k), first, a.dim, a.values, 0u, scoring.mul_add, k);
-    // (exact slopes of e (*) v are taken with v in the lane: weights of 2^-62 leave it 2^-64)
-    odd = !load_lane<W4, APPROXIMATE ? -86 : -64>(key_of_lane<NS>(a, a.v), first, a.dim, a.values, 0u, scoring.mul_add + shift, v) || odd;
+    const bool behind = a.values < NS * W;
+    const Form k_form = form_of(APPROXIMATE, behind), v_form = APPROXIMATE ? k_form : form_of_weighted(behind);
+    const Held of_k = load_lane<W4>(key_of_lane<NS>(a, a.k), first, a.dim, a.values, 0u, scoring.mul_add, k, k_form);
+    const Held of_v = load_lane<W4>(key_of_lane<NS>(a, a.v), first, a.dim, a.values, 0u, scoring.mul_add + shift, v, v_form);
+    const bool zeros = in_team<NS>(of_v.zeros), odd = of_k.odd || of_v.odd || (APPROXIMATE && zeros && most >= 60);      // (else streamed values are below 2)
+    const LaneZeros<kZeroOfSlopes, kZero> k_zeros{APPROXIMATE ? 0 : in_team<NS>(of_k.zeros), scoring.mul_add};
+    const LaneZeros<kZeroOfSlopes, kBehindWeights> v_zeros{zeros, scoring.mul_add};
     const bool unusual = !APPROXIMATE && (a.flags.a || a.flags.b || a.flags.e || a.off != 1.0f);
     bool careful = in_team<NS>(odd) || unusual;
     const Stream<WHOLE> queries(a.qs + (long)u.head * a.rows * a.dim, a.dim, a.rows, slice * W4, a.dim / 4);
@@ -425,22 +469,34 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
                 look_q.load(queries, r1 + kBlock);
                 look_n.load(grads, r1 + kBlock);
                 bool wrong = false;
-                block_dots<W4, WHOLE>(pipe, queries, r1, grads, r1, qv.zeros, k, s);
+                if constexpr (APPROXIMATE) block_dots<W4, WHOLE>(pipe, queries, r1, grads, r1, qv.zeros, NoLaneZeros{}, k, s);
+                else block_dots<W4, WHOLE>(pipe, queries, r1, grads, r1, qv.zeros, k_zeros, k, s);
                 const bool wild = slices_s.add_up(turn, wave, s, gave_up || qv.wild || nv.wild);
                 if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
                 uint32_t counts = weigh(s, e, sees, all, r1, wrong);
-                if constexpr (APPROXIMATE) block_dots<W4, WHOLE>(pipe, grads, r1, grads, r1, nv.zeros, v, de);
-                else {
+                if constexpr (APPROXIMATE) {
+                    block_dots<W4, WHOLE>(pipe, grads, r1, grads, r1, nv.zeros, NoLaneZeros{}, v, de);
+                    without_zeros(zeros, of_v.numbers, de);
+                } else {
 #pragma unroll
                     for (int j = 0; j < kBlock; ++j) de[j] = 0.0f;
-                    pipe.block(grads, r1, grads, r1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
-                        dot_lane_power_piece<N>(x, f2u(e[j]), counts >> j & 1u ? kPower : 0u, v + d, de[j]);
-                    });
+                    uint32_t left = counts;
+                    if (__builtin_expect(v_zeros.any, 0)) {
+                        const Zeros codes = v_zeros.codes();
+                        pipe.rolled(grads, r1, grads, r1, [&](int h, int d, const Piece& x) __attribute__((always_inline)) {
+                            dot_lane_power_piece_with_zeros<N>(x, f2u(e[0]), left & 1u ? kPower : 0u, v + d, codes, de[0]);
+                            if (h == Pipe<W4, WHOLE>::kPieces - 1) { turned(e); turned(de); left >>= 1; }
+                        });
+                    } else
+                        pipe.block(grads, r1, grads, r1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
+                            dot_lane_power_piece<N>(x, f2u(e[j]), counts >> j & 1u ? kPower : 0u, v + d, de[j]);
+                        });
 #pragma unroll
                     for (int j = 0; j < kBlock; ++j) de[j] = over_power(de[j], f2u(e[j]));
                 }
                 slices_de.add_up(turn, wave, de, false);
                 turn ^= 1;
+                if (APPROXIMATE) wrong = wrong || too_small(zeros, de, counts, 2.0f);
                 const uint32_t counts_e = counts;
 #pragma unroll
                 for (int j = 0; j < kBlock; ++j) {

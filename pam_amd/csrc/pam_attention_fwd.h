@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
     const Scoring scoring(a);
     const Full full{a.off, a.off != 1.0f};
     uint32_t q[W];
-    bool careful = in_team<NS>(!load_lane<W4>(query_of_lane<NS>(a), first, a.dim, a.values, f2u(a.scale) - kBias + scoring.off_add, scoring.mul_add, q));       // (of q (*) scale)
+    bool careful = in_team<NS>(load_lane<W4>(query_of_lane<NS>(a), first, a.dim, a.values, f2u(a.scale) - kBias + scoring.off_add, scoring.mul_add, q, Form::plain()).odd);       // (of q (*) scale)
     float slope = 0.0f, wrong = 0.0f;             // wrong: becomes NaN with the first number that is none
     if (scoring.slopes) { slope = held_slope(a.slopes[head]); wrong = finite(a.slopes[head]) ? 0.0f : u2f(kQNaN); }
     const Stream<WHOLE> keys(a.k.p + (long)u.b * a.k.sb + (long)u.kv * a.k.sh, a.k.st, a.keys, slice * W4, a.dim / 4);
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
                 const Verdict kv = judge(look_k, keys, a.values, 0u), vv = judge(look_v, values, a.values, 0u);
                 look_k.load(keys, j1 + kBlock);      // (the next block's; past the end the last key again)
                 look_v.load(values, j1 + kBlock);
-                block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, kv.zeros, q, t);
+                block_dots<W4, WHOLE>(pipe, keys, j1, values, j1, kv.zeros, NoLaneZeros{}, q, t);
                 const bool wild = slices.add_up(turn, wave, t, kv.wild || vv.wild);
                 turn ^= 1;
                 if (__builtin_expect(wild, 0)) return false;

@@ -567,9 +567,9 @@ __global__ __launch_bounds__(kThreads, groups_at_once(ROWS)) void cached_rows_ke
             } else {
 #pragma unroll 1
                 for (int r = 0; r < ROWS; ++r) {
-                    dot_piece_with_zeros<16>(now, mine, s[0]);
+                    dot_piece_with_zeros<16, false>(now, mine, Zeros{}, s[0]);
                     now = piece_of<4, WHOLE>(layout, (const float*)row, 4);
-                    dot_piece_with_zeros<16>(now, mine + 16, s[0]);
+                    dot_piece_with_zeros<16, false>(now, mine + 16, Zeros{}, s[0]);
                     row = queries.after(row, head, r);
                     now = piece_of<4, WHOLE>(layout, (const float*)row, 0);
                     turned(s);

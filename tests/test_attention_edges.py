@@ -90,6 +90,33 @@ def test_values_that_are_that_power(dim, approx):
     _compare((1, 45, 45, 2, 1, dim), {}, seed=dim + 1, approx=approx, change=change)
 
 
+@gpu
+@APPROX
+@pytest.mark.parametrize("what", ["gradients"])
+@pytest.mark.parametrize("dim", [16, 64, 100])
+def test_zeros_beside_tiny_and_large_values(dim, what, approx):
+    """A zero's product is zero, not a small number that others are smaller than."""
+    def change(q, k, v, dy):
+        if what == "values":
+            v *= np.float32(2.0 ** -80); v[..., : dim // 2] = 0; dy[..., : dim // 2] = np.abs(dy[..., : dim // 2]) * np.float32(32.0)
+        else:
+            dy[..., :-1] = 0; v[..., :-1] = np.float32(2.0 ** 39) * (1.0 + np.abs(v[..., :-1]) % 0.9)
+            v[..., -1] = np.float32(2.0 ** -39) * (1.0 + np.abs(v[..., -1]) % 0.5) * np.sign(v[..., -1])
+    for tokens, keys in ((7, 9), (45, 70)):
+        _compare((1, tokens, keys, 2, 1, dim), {}, seed=dim, approx=approx, change=change)
+
+
+@gpu
+@APPROX
+@pytest.mark.parametrize("more", [{}, dict(cap=4.0), dict(slopes=np.array([0.25, 0.5], np.float32))], ids=["plain", "cap", "slopes"])
+@pytest.mark.parametrize("dim", [16, 64, 100])
+def test_rows_of_zeros(dim, more, approx):
+    """Queries and keys that are all zeros, as a layer's are that begins with them, or padding's: every score is zero, and so is its fraction."""
+    def change(q, k, v, dy):
+        q[:, 20:30] = 0; k[:, 5:12] = 0; q[:, 40, :, 1:] = 0; q[:, 40, :, 0] = np.float32(2.0 ** -60)
+    _compare((1, 45, 70, 2, 1, dim), more, seed=dim, approx=approx, change=change)
+
+
 # ---------------------------------------------------------------- weights and gradients far below the largest
 
 @gpu
