@@ -520,17 +520,20 @@ __device__ __forceinline__ void block_dots(Pipe<W4, WHOLE>& pipe, const Stream<W
     }
     pipe.block(s, j1, next, j2, [&](int j, int d, const Piece& x) __attribute__((always_inline)) { dot_piece<N>(x, mine + d, sum[j]); });
 }
-// out += the block's weights times its rows; a weight that does not count is anything.  add: as in load_lane.
+// out += the block's weights times its rows; a weight that does not count is anything.  add: as in load_lane.  small, if there are some: weights below 2^-86, whose products with small
+// values would leave the exponents' range: they come 2^kLift times as large, and the block takes the loop with factors, which scale their products back.
+constexpr int kLift = 30;
 template <int W4, bool WHOLE>
 __device__ __forceinline__ void block_add(Pipe<W4, WHOLE>& pipe, const Stream<WHOLE>& s, int j1, const Stream<WHOLE>& next, int j2, bool zeros, float (&weight)[kBlock], uint32_t add, uint32_t counts,
-                                          float (&out)[4 * W4])
+                                          float (&out)[4 * W4], bool some_small = false, uint32_t small = 0u)
 {
     constexpr int N = 4 * Pipe<W4, WHOLE>::kQuads;
-    if (__builtin_expect(zeros, 0)) {
+    if (__builtin_expect(zeros || some_small, 0)) {
         pipe.rolled(s, j1, next, j2, [&](int h, int d, const Piece& x) __attribute__((always_inline)) {
             const bool in = counts & 1u;
-            add_piece_with_zeros<N>(x, in ? f2u(weight[0]) + add : 0u, in ? 1.0f : 0.0f, out + d);
-            if (h == Pipe<W4, WHOLE>::kPieces - 1) { turned(weight); counts >>= 1; }
+            const float one = small & 1u ? 1.0f / (float)(1 << kLift) : 1.0f;
+            add_piece_with_zeros<N>(x, in ? f2u(weight[0]) + add : 0u, in ? one : 0.0f, out + d);
+            if (h == Pipe<W4, WHOLE>::kPieces - 1) { turned(weight); counts >>= 1; small >>= 1; }
         });
         return;
     }

@@ -146,6 +146,20 @@ __device__ __forceinline__ bool too_small(bool zeros, const float (&sum)[kBlock]
     return found;
 }
 
+// Pairs' gradients below 2^-86 (|dn| is 1, streamed values are at least 2^-40): those of at least 2^-116 are lifted to where products are in range, the others are none.
+__device__ __forceinline__ bool lift(float (&da)[kBlock], uint32_t& counts, uint32_t& small)
+{
+    small &= counts;
+    if (__builtin_expect(__ballot(small != 0u) == 0ull, 1)) return false;
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j) {
+        const bool lifted = (small >> j) & 1u;
+        da[j] = lifted ? da[j] * (float)(1 << kLift) : da[j];
+        if (lifted && fabsf(da[j]) < 0x1p-86f) { counts &= ~(1u << j); small &= ~(1u << j); }
+    }
+    return __ballot(small != 0u) != 0ull;
+}
+
 template <int NS, int W4, bool WHOLE, bool APPROXIMATE>
 __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Args a)
 {
@@ -264,18 +278,21 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
                 slices_de.add_up(turn, wave, de, false);
                 turn ^= 1;
                 if (APPROXIMATE) wrong = wrong || too_small(zeros, de, counts, above);
+                uint32_t small = 0u;
 #pragma unroll
                 for (int j = 0; j < kBlock; ++j) {
                     de[j] = score_gradient(s[j], e[j], de[j], pos - (j1 + j));
                     if (APPROXIMATE) {
-                        // (less than 2^-86 is nothing beside |dn| of 1 and values of at least 2^-40)
                         wrong = wrong || ((counts >> j) & 1u && !(fabsf(de[j]) < 0x1p80f));
-                        counts &= fabsf(de[j]) < 0x1p-86f ? ~(1u << j) : ~0u;
+                        small |= fabsf(de[j]) < 0x1p-86f ? 1u << j : 0u;
                     }
                 }
                 gave_up = gave_up || __ballot(wrong) != 0ull;
                 if (NS == 1 && __builtin_expect(gave_up, 0)) return false;
-                if constexpr (APPROXIMATE) block_add<W4, WHOLE>(pipe, keys, j1, keys, j1 + kBlock, kv.zeros, de, scoring.mul_add, counts, out[0]);
+                if constexpr (APPROXIMATE) {
+                    const bool some_small = lift(de, counts, small);
+                    block_add<W4, WHOLE>(pipe, keys, j1, keys, j1 + kBlock, kv.zeros, de, scoring.mul_add, counts, out[0], some_small, small);
+                }
                 else block_add_power<W4, WHOLE>(pipe, keys, j1, keys, j1 + kBlock, kv.zeros, kPower, de, counts, q, out[0]);
                 return true;
             });
@@ -498,12 +515,13 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
                 turn ^= 1;
                 if (APPROXIMATE) wrong = wrong || too_small(zeros, de, counts, 2.0f);
                 const uint32_t counts_e = counts;
+                uint32_t small = 0u;
 #pragma unroll
                 for (int j = 0; j < kBlock; ++j) {
                     de[j] = score_gradient(s[j], e[j], de[j], r1 + j);
                     if (APPROXIMATE) {
                         wrong = wrong || ((counts >> j) & 1u && !(fabsf(de[j]) < 0x1p80f));
-                        counts &= fabsf(de[j]) < 0x1p-86f ? ~(1u << j) : ~0u;
+                        small |= fabsf(de[j]) < 0x1p-86f ? 1u << j : 0u;
                     }
                 }
                 gave_up = gave_up || __ballot(wrong) != 0ull;
@@ -511,7 +529,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
                 // dv: e (*) dn, dk: da (*) qs
                 if constexpr (APPROXIMATE) {
                     block_add<W4, WHOLE>(pipe, grads, r1, queries, r1, nv.zeros, e, scoring.mul_add + shift, counts_e, out[1]);
-                    block_add<W4, WHOLE>(pipe, queries, r1, queries, r1 + kBlock, qv.zeros, de, scoring.mul_add, counts, out[0]);
+                    const bool some_small = lift(de, counts, small);
+                    block_add<W4, WHOLE>(pipe, queries, r1, queries, r1 + kBlock, qv.zeros, de, scoring.mul_add, counts, out[0], some_small, small);
                 } else {
                     pipe.block(grads, r1, queries, r1, [&](int j, int d, const Piece& x) __attribute__((always_inline)) {
                         add_lane_power_piece<N>(x, f2u(e[j]), counts_e >> j & 1u ? kPower : 0u, v + d, out[1] + d);

@@ -92,7 +92,7 @@ def test_values_that_are_that_power(dim, approx):
 
 @gpu
 @APPROX
-@pytest.mark.parametrize("what", ["gradients"])
+@pytest.mark.parametrize("what", ["values", "gradients"])
 @pytest.mark.parametrize("dim", [16, 64, 100])
 def test_zeros_beside_tiny_and_large_values(dim, what, approx):
     """A zero's product is zero, not a small number that others are smaller than."""
@@ -130,6 +130,20 @@ def test_zeros_and_tiny_values_of_small_weight(dim, approx):
         v[rng.random_sample(v.shape) < 0.2] = 0
         v[:, ::5] *= np.float32(2.0 ** -70)
     _compare((1, 60, 130, 1, 1, dim), dict(causal=False), seed=4, approx=approx, change=change)
+
+
+@gpu
+@APPROX
+@pytest.mark.parametrize("dim", [16, 64, 100])
+def test_a_small_gradient_at_a_small_weight(dim, approx):
+    """The last key is seen by the last query alone, at a weight of 2^-50, and that query's gradient is 2^-34 of the others'."""
+    def change(q, k, v, dy):
+        for x in (v, dy):
+            x[:] = (1.0 + np.abs(x) % 1.0) * np.sign(x)
+        v *= np.float32(2.0 ** -10)
+        k[:, -1] = -q[:, -1, :1] * np.float32(50.0 * np.log(2.0) * dim ** 0.5 / np.square(q[0, -1, 0]).sum())
+        dy[:, -1] *= np.float32(2.0 ** -32)
+    _compare((1, 70, 70, 1, 1, dim), {}, seed=dim, approx=approx, change=change, tight=0.2)
 
 
 # ---------------------------------------------------------------- the ends of the range
