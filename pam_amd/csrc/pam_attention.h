@@ -58,6 +58,7 @@ struct Args {
     const float* slopes;
     float scale, cap, off;                        // cap: 0 none
     int tiles, chunks, chunk;                     // a unit is a tile of lanes' rows and a chunk (a multiple of kSpan) of the streamed ones
+    int windows;                                  // chunks begin where the window of a tile's first row does (in whole spans), else at row 0
     // forward
     float* y;                                     // [batch][tokens][heads][dim]
     float2* stats;                                // l and M, [batch][kv_heads][rows], or null

@@ -141,24 +141,29 @@ const Variant& variant_for(const Variant* list, long dim)
 }
 
 // How the streamed rows are cut.  All units of a launch run at once or in a few turns of `slots` of them, so that a last turn of a few units costs as
-// much as a full one: among the cuts that fill one, two, ... turns the one is taken whose turns times its spans are least.  (4096 causal tokens, 8 heads over 2:
+// much as a full one: among the cuts that fill one, two, ... turns the one is taken whose turns times the spans that a unit works on are least.  (4096 causal tokens, 8 heads over 2:
 // chunks of 256 keys, two turns and a bit, 0.70 ms; the cut taken 0.55.)  Which spans a tile sees is what the order and the window say; prefixes and documents are on the device.
 // A chunk is at least two spans (documents leave a tile little of what the order does, but chunks of one span cost 307 us where three took 267, 210 since units
 // that see nothing end early: 2 x 2048 tokens, heads of 128), what a unit does besides its spans counts as a fifth of one.
+// Of a window the chunks are counted from where a tile's begins, so that there are as many as one window has and no more scratch than that, however long the rows are.
 struct Plan { int tiles, chunks, chunk; };
 long tiles_of(int slices) { return slices >= 4 ? 1 : 4 / slices; }              // of a work-group (kTiles)
-template <class Range>                            // range(first, last row of a tile, low, high): the streamed rows that those see
-Plan plan_for(long heads, long lanes, int slices, long streamed, int waves_per_simd, Range range)
+template <class Range>                            // range(first, last row of a tile, low, high): the streamed rows that those see; range.reach(rows of a tile): of any tile at most
+Plan plan_for(long heads, long lanes, int slices, long streamed, int waves_per_simd, const Range& range)
 {
-    const long per_tile = 64 * tiles_of(slices), tiles = (lanes + per_tile - 1) / per_tile, spans = std::max(1L, (streamed + kSpan - 1) / kSpan);
-    const long slots = 256L * 4 * waves_per_simd / (slices * tiles_of(slices)), samples = std::min(tiles, 32L);
-    long low[32], high[32], total = 0;            // of tiles evenly spread, in spans
+    const long per_tile = 64 * tiles_of(slices), tiles = (lanes + per_tile - 1) / per_tile, samples = std::min(tiles, 32L);
+    const bool windows = range.a.windows;
+    long spans = std::max(1L, (streamed + kSpan - 1) / kSpan);
+    if (windows) spans = std::min(spans, (range.reach(per_tile) + kSpan - 2) / kSpan + 1);
+    const long slots = 256L * 4 * waves_per_simd / (slices * tiles_of(slices));
+    long low[32], high[32], total = 0, longest = 0;      // of tiles evenly spread, in spans
     for (long n = 0; n < samples; ++n) {
         const long tile = (2 * n + 1) * tiles / (2 * samples);
         long from = 0, to = streamed;
         range(tile * per_tile, std::min(lanes, (tile + 1) * per_tile) - 1, from, to);
         low[n] = std::max(0L, from) / kSpan; high[n] = std::max(low[n], (std::min(to, streamed) + kSpan - 1) / kSpan);
-        total += high[n] - low[n];
+        if (windows) { high[n] -= low[n]; low[n] = 0; }
+        total += high[n] - low[n]; longest = std::max(longest, high[n] - low[n]);
     }
     const double each = samples ? (double)heads * tiles / samples : 0.0;
     double best = 0.0;
@@ -167,13 +172,14 @@ Plan plan_for(long heads, long lanes, int slices, long streamed, int waves_per_s
         long size = std::max(2L, (long)(each * total / (turns * slots)));
         double units = 0.0;
         for (int tries = 0; tries < 12; ++tries, size += 1 + size / 16) {
+            size = std::min(size, std::max(2L, spans));
             units = 0.0;
             for (long n = 0; n < samples; ++n) units += high[n] == low[n] ? 0.0 : (double)((high[n] - 1) / size - low[n] / size + 1);
             units *= each;
             if (units <= turns * slots || size >= spans) break;
         }
         size = std::min(size, spans);
-        const double cost = std::ceil(units / slots) * (size + 0.2);
+        const double cost = std::ceil(units / slots) * (std::min(size, windows ? longest : spans) + 0.2);
         if (turns == 1 || cost < best * 0.97) { best = cost; chosen = size; }
         if (size <= 2) break;
     }
@@ -200,6 +206,7 @@ int check(const char* what, const pam_hip_attention_shape* s, Args& a)
     a.group = s->kv_heads ? (int)(s->heads / s->kv_heads) : 1; a.dim = (int)s->dim; a.values = (int)s->values;
     a.rows = a.tokens * a.group; a.first = a.keys - a.tokens; a.causal = s->causal != 0; a.window = (int)std::min(s->window, 1L << 29);
     a.prefix = s->prefix; a.documents = s->documents; a.slopes = s->slopes; a.scale = s->scale; a.cap = s->cap; a.off = s->offset;
+    a.windows = a.window != 0 && !a.prefix;
     return PAM_HIP_OK;
 }
 Tokens tokens_of(const pam_hip_tokens* t) { return Tokens{t->p, t->sb, t->st, t->sh}; }
@@ -227,10 +234,11 @@ struct OfRows {
     void operator()(long from, long to, long& low, long& high) const
     {
         const long first = a.first + from / a.group, last = a.first + to / a.group;
-        if (a.window && !a.prefix) low = first - a.window + 1;
+        if (a.windows) low = first - a.window + 1;
         if (a.causal) high = last + 1;
         else if (a.window) high = last + a.window;
     }
+    long reach(long rows) const { return (rows + a.group - 2) / a.group + (a.causal ? 1L : 2L) * a.window; }
 };
 struct OfKeys {
     const Args& a;
@@ -241,6 +249,7 @@ struct OfKeys {
         else if (a.window) low = (from - a.window + 1 - a.first) * a.group;
         if (a.window) high = (to + a.window - a.first) * a.group;
     }
+    long reach(long keys) const { return (keys - 1 + (a.causal ? 1L : 2L) * a.window) * a.group; }
 };
 Plan forward_plan(const Args& a)
 {

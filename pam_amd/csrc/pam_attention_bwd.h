@@ -171,7 +171,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     const int pos = a.first + row / a.group;
     Sight sight = sight_of_row(a, u.b, row);
     sight.close_team<NS>();
-    const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
+    const Chunk chunk = chunk_of_keys(a, u, u.tile * kTiles<NS> * 64);
+    const int begin = max(sight.first / kSpan * kSpan, chunk.begin), end = min(sight.last, chunk.end);
     if (!a.whole && !any_seen<NS>(sight, begin, end)) { met_anything<NS>(a, u, wave, false); return; }
     const Scoring scoring(a);
     const PairGrad<APPROXIMATE> pair{scoring, a.flags};
@@ -365,13 +366,17 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
 }
 
 // What a key's lane sees: the rows of its head's queries.
+__device__ __forceinline__ int row_of_token(const Args& a, long token) { return (int)max(0l, min(token * a.group, (long)a.rows)); }
+__device__ __forceinline__ int first_row_of_key(const Args& a, int key)
+{
+    const long at = (long)key - a.first;
+    return a.causal ? row_of_token(a, at) : a.window ? row_of_token(a, at - a.window + 1) : 0;
+}
 __device__ __forceinline__ Sight sight_of_key(const Args& a, int b, int key)
 {
-    const long at = (long)key - a.first, g = a.group, rows = a.rows;
-    const auto held = [&](long tokens) { return (int)max(0l, min(tokens * g, rows)); };
     Sight s;
-    s.low = a.causal ? held(at) : a.window ? held(at - a.window + 1) : 0;
-    s.high = a.window ? held(at + a.window) : a.rows;
+    s.low = first_row_of_key(a, key);
+    s.high = a.window ? row_of_token(a, (long)key - a.first + a.window) : a.rows;
     s.before = a.prefix && key < a.prefix[b] ? a.rows : 0;
     s.with_documents = a.documents != nullptr;
     s.of_streamed = a.documents ? a.documents + (long)b * a.keys + a.first : nullptr; s.per = a.group;
@@ -401,10 +406,10 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     const Unit u = unit_of_keys(a);
     const int wave = wave_of(), slice = wave % NS, lane = (int)threadIdx.x % 64, key0 = (u.tile * kTiles<NS> + wave / NS) * 64, mine = key0 + lane, key = min(mine, a.keys - 1), first = slice * W;
     const bool exists = mine < a.keys;
-    const int chunk_begin = u.chunk * a.chunk, chunk_end = min(a.rows, chunk_begin + a.chunk);
+    const Chunk chunk = chunk_of(a, u, first_row_of_key(a, u.tile * kTiles<NS> * 64), a.rows);
     Sight sight = sight_of_key(a, u.b, key);
     sight.close_team<NS>();
-    const int begin = max(sight.first / kSpan * kSpan, chunk_begin), end = min(min(sight.last, a.rows), chunk_begin + a.chunk);
+    const int begin = max(sight.first / kSpan * kSpan, chunk.begin), end = min(sight.last, chunk.end);
     if (!a.whole && !any_seen<NS>(sight, begin, end)) { met_anything<NS>(a, u, wave, false); return; }
     const Scoring scoring(a);
     const PairGrad<APPROXIMATE> pair{scoring, a.flags};
@@ -413,7 +418,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
     const auto record = [&](int r) __attribute__((always_inline)) { const Records from = (Records)(all_records + min(r, a.rows - 1)); return make_float4(from->x, from->y, from->z, from->w); };
     // the largest |dn| of the chunk's rows is scaled to [1, 2)
     int most = -86;
-    for (int r = chunk_begin + lane; r < chunk_end; r += 64) most = max(most, (int)all_records[r].z);
+    for (int r = chunk.begin + lane; r < chunk.end; r += 64) most = max(most, (int)all_records[r].z);
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) most = max(most, __shfl_xor(most, s, 64));
     most = APPROXIMATE ? __builtin_amdgcn_readfirstlane(most) : 0;

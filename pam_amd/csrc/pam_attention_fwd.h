@@ -65,6 +65,16 @@ __device__ __forceinline__ Unit unit_of(const Args& a)
 }
 __device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
 
+// The streamed rows of a unit's chunk: from row `origin` or its span on.
+struct Chunk { int begin, end; };
+__device__ __forceinline__ Chunk chunk_of(const Args& a, const Unit& u, int origin, int streamed)
+{
+    const long from = (a.windows ? origin / kSpan * kSpan : 0) + (long)u.chunk * a.chunk;
+    return Chunk{(int)min(from, (long)streamed), (int)min(from + a.chunk, (long)streamed)};
+}
+// ... of the keys, where the tiles of queries begin with row row0
+__device__ __forceinline__ Chunk chunk_of_keys(const Args& a, const Unit& u, int row0) { return chunk_of(a, u, max(0, a.first + row0 / a.group - a.window + 1), a.keys); }
+
 // The launch's arguments as from memory: what the careful loops need is found again there, instead of in registers since the beginning.
 __device__ __forceinline__ Args arguments_again()
 {
@@ -108,7 +118,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
     sight.close_team<NS>();
     const long stat = ((long)u.head * a.chunks + u.chunk) * a.rows + row;
     float* const to = a.partial ? a.partial + stat * a.dim : a.y + (((long)u.b * a.tokens + token) * a.heads + head) * a.dim;
-    const int begin = max(sight.first / kSpan * kSpan, u.chunk * a.chunk), end = min(min(sight.last, a.keys), (u.chunk + 1) * a.chunk);
+    const Chunk chunk = chunk_of_keys(a, u, u.tile * kTiles<NS> * 64);
+    const int begin = max(sight.first / kSpan * kSpan, chunk.begin), end = min(sight.last, chunk.end);
     if (a.partial && !any_seen<NS>(sight, begin, end)) {
         if (exists && slice == 0) a.partial_stats[stat] = make_float2(0.0f, kNothing);
         return;

@@ -234,6 +234,29 @@ def _scratch(tokens, heads, kv_heads, dim, window, batch=1, keys=None, causal=Tr
     return forward(ctypes.byref(s)), backward(ctypes.byref(s), 1, 1)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [1, 64, 256, 1000, 5000])
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim", [(2048, 8, 2, 64), (32768, 32, 8, 128), (131072, 32, 8, 128), (524288, 8, 2, 64), (8192, 1, 1, 16), (100001, 3, 3, 256)])
+def test_scratch_of_a_window_is_what_its_tiles_see(tokens, heads, kv_heads, dim, window, causal):
+    """A tile of at most 256 rows of one head sees a window's worth of keys: cut into two spans of 64 at least, that many parts of every row; and no more
+    than some turns of the chip's units, whatever the length."""
+    forward, backward = _scratch(tokens, heads, kv_heads, dim, window, causal=causal)
+    rows = tokens * heads * dim * 4
+    parts = (256 + (1 if causal else 2) * window) // 128 + 2
+    assert forward <= rows * parts + (rows // dim * parts * 2 + 4096)
+    seen_rows = (256 + (1 if causal else 2) * window) * (heads // kv_heads) // 128 + 2
+    records = 2 * rows + 4 * rows // dim + 4096
+    keys = 2 * tokens * kv_heads * dim * 4 * seen_rows
+    assert backward <= records + rows * parts + keys + (1 << 24)
+    assert max(forward, backward - records) <= max(4 * rows, 3 << 29)
+
+
+@pytest.mark.parametrize("tokens,keys", [(1, 1 << 20), (64, 1 << 20), (4096, 4096), (32768, 32768), (300, 100000)])
+def test_scratch_of_long_rows_is_bounded(tokens, keys):
+    forward, backward = _scratch(tokens, 8, 2, 64, 0, keys=keys)
+    assert max(forward, backward - 2 * tokens * 8 * 65 * 4) <= 3 << 29
+
+
 @gpu
 @pytest.mark.parametrize("shape,masks", [((1, 700, 700, 2, 1, 16), dict(window=100)), ((1, 1100, 1100, 1, 1, 16), dict(window=65)), ((2, 300, 1000, 2, 2, 20), dict(window=333)),
                                          ((1, 900, 900, 1, 1, 20), dict(window=90, causal=False)), ((1, 500, 700, 1, 1, 16), dict(window=80, prefix=np.array([130]))),
