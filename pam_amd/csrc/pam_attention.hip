@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kThreads) void attention_rows_kernel(RowArgs r)
     const float* const dy = r.dy.p + b * r.dy.sb + t * r.dy.st + (long)head * r.dy.sh;
     const float* const y = r.y + id * a.dim;
     const bool sees = stats.y != kNothing;
-    const float l = sees ? stats.x : 1.0f, inverse = pad_div_off(1.0f, l, off, has_off);
+    const float l = sees ? stats.x : 1.0f;
     const bool whole = fabsf(l) < u2f(kExpo);
     float dl = 0.0f;
     uint32_t most = 0u;

@@ -131,3 +131,25 @@ def test_scores_at_both_ends(dim, offset):
     for sign in (1.0, -1.0):
         k[11, 3, 0, 0] = sign * 2.5 * top
         assert pam.cached_attention(q, k, v, table, lengths, scale=1.0, offset=offset).isnan().all()
+
+
+@gpu
+@DIMS
+@pytest.mark.parametrize("offset", [0.77, 1.0552, 1.4])
+@pytest.mark.parametrize("more", [{}, dict(cap=4.0), dict(window=60, slopes=np.array([0.25, 0.5, 0.01, 1.0], np.float32))], ids=lambda s: "_".join(s) or "plain")
+def test_offset_moves_every_product(more, offset, dim):
+    pam = __import__("pam_amd")
+    rng = np.random.RandomState(dim)
+    batch, tokens, heads, kv_heads, page = 2, 3, 4, 2, 16
+    k, v, table = _cache(rng, batch, page, 12, kv_heads, dim)
+    q = rng.standard_normal((batch, tokens, heads, dim)).astype(np.float32)
+    lengths = np.array([150, 9])
+    on = {n: _cuda(x) if isinstance(x, np.ndarray) else x for n, x in more.items()}
+    got = pam.cached_attention(_cuda(q), _cuda(k), _cuda(v), _cuda(table), _cuda(lengths), offset=offset, **on).cpu().double().numpy()
+    scoring = {n: x for n, x in more.items() if n == "cap"}
+    for b in range(batch):
+        end = lengths[b] + tokens
+        keys, values, see = _sequence(k, table, b, end), _sequence(v, table, b, end), visible(tokens, end, True, more.get("window"))
+        for h in range(heads):
+            head = general.Head(q[b, :, h], keys[:, h // 2], values[:, h // 2], see, more["slopes"][h] if "slopes" in more else None, offset=offset, **scoring)
+            assert (np.abs(got[b, :, h] - head.y.v) <= head.y.o).all()
