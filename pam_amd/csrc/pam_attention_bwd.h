@@ -258,7 +258,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
                 if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
                 uint32_t counts = weigh(s, e, sees, all, j1, wrong);
                 if constexpr (APPROXIMATE) {
-                    block_dots<W4, WHOLE>(pipe, values, j1, keys, j1, vv.zeros, NoLaneZeros{}, dn, de);
+                    // (where the streamed values are zeros, nothing but what stands for the lane's zeros and behind its values may be left)
+                    block_dots<W4, WHOLE>(pipe, values, j1, keys, j1, vv.zeros, LaneZeros<kZero, kZero>{0, scoring.mul_add}, dn, de);
                     without_zeros(zeros, of_dn.numbers, de);
                 } else {
 #pragma unroll
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
             slices_de.add_up(turn, wave, de, false);
             turn ^= 1;
 #pragma unroll
-            for (int j = 0; j < kBlock; ++j) de[j] = score_gradient(s[j], e[j], de[j], pos - (j1 + j));
+            for (int j = 0; j < kBlock; ++j) de[j] = de[j] + dl == 0.0f ? 0.0f : score_gradient(s[j], e[j], de[j], pos - (j1 + j));      // (the usual loop leaves out what a zero makes)
 #pragma unroll 1
             for (int j = 0; j < kBlock; ++j) {
                 const v4f row = keys.template across<W4>(j1 + j);
@@ -497,7 +498,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
                 if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
                 uint32_t counts = weigh(s, e, sees, all, r1, wrong);
                 if constexpr (APPROXIMATE) {
-                    block_dots<W4, WHOLE>(pipe, grads, r1, grads, r1, nv.zeros, NoLaneZeros{}, v, de);
+                    block_dots<W4, WHOLE>(pipe, grads, r1, grads, r1, nv.zeros, LaneZeros<kZero, kZero>{0, scoring.mul_add + shift}, v, de);
                     without_zeros(zeros, of_v.numbers, de);
                 } else {
 #pragma unroll
@@ -587,7 +588,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
             slices_de.add_up(turn, wave, de, false);
             turn ^= 1;
 #pragma unroll
-            for (int j = 0; j < kBlock; ++j) de[j] = score_gradient(s[j], e[j], de[j], r1 + j);
+            for (int j = 0; j < kBlock; ++j) de[j] = de[j] + record(r1 + j).y * unit == 0.0f ? 0.0f : score_gradient(s[j], e[j], de[j], r1 + j);
 #pragma unroll 1
             for (int j = 0; j < kBlock; ++j) {
                 const v4f row = queries.template across<W4>(r1 + j);

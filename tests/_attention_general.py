@@ -72,9 +72,10 @@ class Arithmetic:
         factor = block.mul(other.v, self.offset) if with_offset else other.v
         off = 2.0 * other.o
         here = step_of(factor, own.v)
-        by_own = np.maximum(*(np.abs(step_of(factor, own.v + s * own.o) - here) for s in (1, -1)))
-        by_other = np.maximum(*(np.abs(step_of(factor + s * off, own.v) - here) for s in (1, -1)))
-        return Known(here, by_own + by_other)
+        corners = [np.abs(step_of(factor + i * off, own.v + j * own.o) - here) for i in (1, 0, -1) for j in (1, 0, -1)]         # (together they may pass where neither does alone)
+        # (what is known to less than a piece's width may be anywhere in one)
+        anywhere = np.where(own.o > 0.2 * np.abs(own.v), np.abs(here), 0.0) + np.where(off > 0.2 * np.abs(factor), np.abs(here) + 2.0 * np.abs(step_of(np.abs(factor) + off, own.v)), 0.0)
+        return Known(here, np.maximum.reduce(corners + [anywhere]))
 
     def of_mul(self, own, other, d, approx):
         return self.mul(d, other) if approx else d.times(self.slope(other, own))
@@ -121,7 +122,8 @@ class Head:
         most = np.where(self.some, np.floor(np.where(see, t.v, -np.inf).max(1, keepdims=True, initial=-np.inf)), 0.0)
         lower = np.where(see, t.v - most, -100.0)
         e = np.where(see, block.exp2(lower), 0.0)
-        rounded = np.where((t.o == 0) & (t.v == np.rint(t.v)), 0.0, t.o + 2.0 * EPS * (2.0 + np.abs(lower)))          # (a whole t is a power of two to the bit)
+        # (a whole t is a power of two to the bit; the whole number taken off it is up to 8 below the largest's, so that the difference is rounded at up to that much more)
+        rounded = np.where((t.o == 0) & (t.v == np.rint(t.v)), 0.0, t.o + 2.0 * EPS * (6.0 + np.abs(lower)))
         self.e = Known(e, np.where(see, e * rounded + np.where(e < 2.0 ** -58, 2.0 ** -60, 0.0), 0.0))
         l = total(self.e, 1, True)
         self.l = Known(np.where(self.some, l.v, 1.0), np.where(self.some, l.o, 0.0))

@@ -218,6 +218,24 @@ def test_gradients_of_either_kind_and_offset(more, offset, approx):
     _compare((1, 30, 75, 2, 1, 24), more, 35, approx, offset=offset)
 
 
+@gpu
+@pytest.mark.parametrize("approx", [True, False, (True, False), (False, True)], ids=str)
+@pytest.mark.parametrize("offset", [None, 1.05, 1.4])
+def test_pairs_without_a_gradient_give_none(offset, approx):
+    """Values that are all zeros, and queries of a single key: zeros to the bit, in the full definition (offsets, mixed slopes, values out of the usual range) too."""
+    pam = __import__("pam_amd")
+    for dim in (1, 18, 64, 130):
+        q, k, v, dy = _inputs(dim, 1, 70, 70, 4, 2, dim)
+        dy[:, 50] *= np.float32(1e14)
+        for values, window in ((np.zeros_like(v), None), (v, 1)):
+            if window and (isinstance(approx, tuple) or approx and offset):              # (the quotient's slopes are of two kinds, or have the offset another number of times, and do not cancel)
+                continue
+            leaves = [_cuda(x).requires_grad_() for x in (q, k, values)]
+            y = pam.attention(*leaves, window=window, offset=offset, approx_bwd=approx)
+            dq, dk, dv = torch.autograd.grad(y, leaves, _cuda(dy))
+            assert (dq == 0).all() and (dk == 0).all() and torch.isfinite(dv).all() and (dv != 0).any()
+
+
 # ---------------------------------------------------------------- scratch
 
 class _Shape(ctypes.Structure):
