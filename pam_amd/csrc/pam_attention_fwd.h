@@ -140,12 +140,14 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
         float most = kNothing;
 #pragma unroll
         for (int j = 0; j < kBlock; ++j) t[j] = scoring.exponent(t[j], slope, pos - (j1 + j));
+        // (not from its distance to M: of scores near both ends of the range that may be an infinity, and counts for nothing)
+        const auto met = [&](float exponent) __attribute__((always_inline)) { most = fmaxf(most, exponent); wrong = __builtin_fmaf(exponent, 0.0f, wrong); };
         if (all)
 #pragma unroll
-            for (int j = 0; j < kBlock; ++j) most = fmaxf(most, t[j]);
+            for (int j = 0; j < kBlock; ++j) met(t[j]);
         else
 #pragma unroll
-            for (int j = 0; j < kBlock; ++j) most = fmaxf(most, (sees >> j) & 1u ? t[j] : kNothing);
+            for (int j = 0; j < kBlock; ++j) met((sees >> j) & 1u ? t[j] : kNothing);
         if (__ballot(most > M + kLag) != 0ull) {
             const float raised = most > M + kLag ? floorf(most) : M, f = scale_between(M, raised);
             l *= f; l_before *= f;
@@ -157,9 +159,8 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, W4 > 8 ? 2 : 3) void attention
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < kBlock; ++j) {
-            float power = t[j] - M, number = t[j];        // (scores near both ends of the range: their difference may be an infinity, and counts for nothing)
-            if (!all) { power = (sees >> j) & 1u ? power : 2.0f * kLeast; number = (sees >> j) & 1u ? number : 0.0f; }
-            wrong = __builtin_fmaf(number, 0.0f, wrong);
+            float power = t[j] - M;
+            if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
             const bool in = power >= kLeast;
             t[j] = power_of_two(fmaxf(power, kLeast));
             sum += in ? t[j] : 0.0f;
