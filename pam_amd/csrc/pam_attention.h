@@ -103,10 +103,11 @@ template <int N, class T> __device__ __forceinline__ void turned(T (&v)[N])     
     v[N - 1] = first;
 }
 
-// How a lane's values are held: they have to be in 2^(least, top); a zero and what lies behind the row's values have bits that no such value has.
+// How a lane's values are held: they have to be in 2^(least, top); a zero and what lies behind the row's values have bits that no such value has.  ones: from that value of
+// a quad on, what streams by behind the values is ones (keys and values of heads that are no whole quads); the products with those are zeros to the bit.
 constexpr uint32_t bits_of_power(int e) { return (uint32_t)(127 + e) << 23; }
 struct Form {
-    int least, top; uint32_t zero, behind;
+    int least, top; uint32_t zero, behind; int ones = 4;
     static __device__ __forceinline__ Form plain() { return Form{-86, 80, kStandIn, kStandIn}; }
 };
 // What a lane found in its part of a row: a value out of the window, a zero, anything but zeros.
@@ -130,7 +131,7 @@ __device__ __forceinline__ Held load_lane(const float* row, int first, int dim, 
             most = max(most, zero || behind ? 0u : (b << 1) - base);
             zeros = zeros || (zero && !behind);
             numbers = numbers || !(zero || behind);
-            out[4 * n + i] = (behind ? form.behind : zero ? form.zero : b) + add;
+            out[4 * n + i] = behind && i >= form.ones ? lane_pad(0u) : (behind ? form.behind : zero ? form.zero : b) + add;
         }
     }
     return Held{most >= ((uint32_t)(form.top - form.least) << 24) - 2u, zeros, numbers};

@@ -185,7 +185,9 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     const long at = ((long)u.head * a.rows + row) * a.dim;
     // (what the exact slopes of e (*) v weigh is a factor, and may be zero)
     const bool behind = a.values < NS * W;
-    const Form q_form = form_of(APPROXIMATE, behind), dn_form = APPROXIMATE ? form_of(true, behind) : Form{-86, 80, 0u, 0u};
+    Form q_form = form_of(APPROXIMATE, behind);
+    if (a.values % 4 != 0) q_form.ones = a.values % 4;
+    const Form dn_form = APPROXIMATE ? q_form : Form{-86, 80, 0u, 0u};
     const Held of_q = load_lane<W4>(a.qs + at, first, a.dim, a.values, 0u, scoring.mul_add, q, q_form);
     const Held of_dn = load_lane<W4>(a.dn + at, first, a.dim, a.values, 0u, dn_add, dn, dn_form, unit);
     const bool counts_at_all = M != u2f(kExpo);
@@ -203,7 +205,6 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
     float* const to[1] = {a.out0 + (a.whole ? ((long)u.b * a.tokens + row / a.group) * a.heads + head : ((long)u.head * a.chunks + u.chunk) * a.rows + row) * a.dim};
     int turn = 0;
     // weights from scores, and which ones count (what is no number does)
-    const bool ones_behind = !APPROXIMATE && a.values != a.dim;                  // (a key's row has ones behind its values: beside them a tiny score has no fraction left)
     const auto weigh = [&](const float (&s)[kBlock], float (&e)[kBlock], uint32_t sees, bool all, int j1, bool& wrong) __attribute__((always_inline)) {
         uint32_t counts = 0u;
 #pragma unroll
@@ -211,7 +212,6 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
             float power = scoring.exponent(s[j], slope, pos - (j1 + j)) - M;
             if (!all) power = (sees >> j) & 1u ? power : 2.0f * kLeast;
             wrong = wrong || power != power;
-            if (!APPROXIMATE) wrong = wrong || (ones_behind && power >= kLeast && s[j] != 0.0f && fabsf(s[j]) < 0x1p-50f);
             counts |= power < kLeast ? 0u : 1u << j;
             e[j] = power_of_two(fminf(fmaxf(power, kLeast), 60.0f));
             e[j] = power != power ? power : e[j];
@@ -258,8 +258,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 3) void attention_dq_kernel(Ar
                 if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
                 uint32_t counts = weigh(s, e, sees, all, j1, wrong);
                 if constexpr (APPROXIMATE) {
-                    // (where the streamed values are zeros, nothing but what stands for the lane's zeros and behind its values may be left)
-                    block_dots<W4, WHOLE>(pipe, values, j1, keys, j1, vv.zeros, LaneZeros<kZero, kZero>{0, scoring.mul_add}, dn, de);
+                    block_dots<W4, WHOLE>(pipe, values, j1, keys, j1, vv.zeros, NoLaneZeros{}, dn, de);
                     without_zeros(zeros, of_dn.numbers, de);
                 } else {
 #pragma unroll
@@ -498,7 +497,7 @@ __global__ __launch_bounds__(64 * kWaveCount<NS>, 2) void attention_dkv_kernel(A
                 if (__builtin_expect(wild, 0)) { turn ^= 1; return false; }      // (others may be reading that buffer)
                 uint32_t counts = weigh(s, e, sees, all, r1, wrong);
                 if constexpr (APPROXIMATE) {
-                    block_dots<W4, WHOLE>(pipe, grads, r1, grads, r1, nv.zeros, LaneZeros<kZero, kZero>{0, scoring.mul_add + shift}, v, de);
+                    block_dots<W4, WHOLE>(pipe, grads, r1, grads, r1, nv.zeros, NoLaneZeros{}, v, de);
                     without_zeros(zeros, of_v.numbers, de);
                 } else {
 #pragma unroll
