@@ -53,6 +53,12 @@ def step_of(x, y):
     return np.where(x == 0, 0.0, np.sign(x) * np.ldexp(1.0, (ex - 1 + carry).astype(int)))
 
 
+def ends(v, o):
+    """What is o off: as it is, at both ends, and right below a power of two that lies between."""
+    border = below(np.abs(v) + o) * (1.0 - 2.0 ** -40)
+    return v, v + o, v - o, np.where(border > np.abs(v) - o, np.sign(v) * border, v)
+
+
 class Arithmetic:
     def __init__(self, offset, first, second, exponent):
         self.offset = float(np.float32(1.0 if offset is None else offset))
@@ -72,7 +78,8 @@ class Arithmetic:
         factor = block.mul(other.v, self.offset) if with_offset else other.v
         off = 2.0 * other.o
         here = step_of(factor, own.v)
-        corners = [np.abs(step_of(factor + i * off, own.v + j * own.o) - here) for i in (1, 0, -1) for j in (1, 0, -1)]         # (together they may pass where neither does alone)
+        # (together they may pass where neither does alone, and a piece may begin and end in between: right below a power of two)
+        corners = [np.abs(step_of(f, o) - here) for f in ends(factor, off) for o in ends(own.v, own.o)]
         # (what is known to less than a piece's width may be anywhere in one)
         anywhere = np.where(own.o > 0.2 * np.abs(own.v), np.abs(here), 0.0) + np.where(off > 0.2 * np.abs(factor), np.abs(here) + 2.0 * np.abs(step_of(np.abs(factor) + off, own.v)), 0.0)
         return Known(here, np.maximum.reduce(corners + [anywhere]))
