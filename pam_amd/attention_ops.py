@@ -33,7 +33,8 @@ def attention(q, k, v, *, scale=None, causal=True, window=None, prefix=None, doc
       window      |i - j| < window
       prefix      int64 [batch]: the first keys of a batch entry, which every query sees besides
       documents   int64 [batch, keys]: only keys of the query's own document; a negative number is padding's
-    A query that sees no key has the result zero, and no gradient.  The quotient is taken after the sum, and a power of two moves no result, so
+    A query that sees no key has the result zero, and no gradient.  Weights below 2 ** -62 of the largest that came before them are none, and scores of 2 ** 127
+    and more are no numbers.  The quotient is taken after the sum, and a power of two moves no result, so
     that softmax and bmm (which divide before it and subtract the largest score of all rows) give slightly different values."""
     _require_kernel(q, use_kernel)
     dim = q.shape[-1] if q.dim() else 0
@@ -59,7 +60,8 @@ def rotary_append(q, k, v, cos, sin, cache_k, cache_v, pages, lengths, counts=No
 def cached_attention(q, cache_k, cache_v, pages, lengths, counts=None, *, scale=None, window=None, slopes=None, cap=None, offset=None, use_kernel=True):
     """`attention` of the next tokens of every sequence, q [batch, tokens, heads, dim], over a paged cache that has their keys and values already
     (see rotary_append, whose pages, lengths and counts these are): token t sees the places 0 ... lengths + t, or with a window the last of them.
-    Made for one or a few tokens, and tables of up to 2 ** 30 places: the cache is read again for every twelve of tokens x heads / kv_heads.  Padding's results are zeros.  A place that
+    Made for one or a few tokens, and tables of up to 2 ** 30 places: the cache is read again for every
+    twelve of tokens x heads / kv_heads (every four in heads that are no whole quads).  Weights below 2 ** -62 of the largest that came before them are none.  Padding's results are zeros.  A place that
     the table of pages does not have, or on a page that is not there, makes the results that see it NaN.  There are no gradients."""
     _require_kernel(q, use_kernel)
     scale, window, cap = _scoring("cached_attention", q.shape[-1] if q.dim() else 0, scale, window, cap)

@@ -16,8 +16,8 @@
 // a score through LDS.  A work-group's wavefronts stream the same rows, so that the scalar cache has them.
 // Rates of the inner loop alone, two wavefronts per SIMD: 28 T products/s; with the streamed values read from another lane inside the integer
 // addition (a data-parallel primitive: everything around it issues half as fast) 18.6; copied out of one once for four rows 20.5; by lane reads 12.
-// Whole passes: forward 18.7 T products/s where every row sees 4096 keys, 15.6 where the order is causal (the last turn of units is not full),
-// gradients 14.5 and 11: a sixth to a third of the instructions are the weights', which slices make twice, and two or three wavefronts on a SIMD do not
+// Whole passes: forward 18.7 T products/s where every row sees 4096 keys, 15.8 where the order is causal (the last turn of units is not full),
+// gradients 13.8 and 10: a sixth to a third of the instructions are the weights', which slices make twice, and two or three wavefronts on a SIMD do not
 // cover all waits for the scalar cache.
 //
 // The integer addition is the product while no exponent leaves the normal range.  Streamed values have to be in 2^[-40, 40), a lane's in 2^(-86, 80).  A
@@ -61,7 +61,7 @@ struct Args {
     int windows;                                  // chunks begin where the window of a tile's first row does (in whole spans), else at row 0
     // forward
     float* y;                                     // [batch][tokens][heads][dim]
-    float2* stats;                                // l and M, [batch][kv_heads][rows], or null
+    float2* stats;                                // l and M, [batch][tokens][heads], or null
     float* partial; float2* partial_stats;        // [batch][kv_heads][chunks][rows][dim], [...][rows]; or null: chunks is 1
     // backward
     const float4* records;                        // [batch][kv_heads][rows]: M (+inf: the row sees nothing), dl, largest exponent of dn, slope

@@ -3,10 +3,11 @@
 // of a kernel before (attention_rows_kernel),
 //   de_ij = sum_d dn_id (*) v_jd + dl_i,   dx_ij = e_ij (*) de_ij,   da_ij through the cap,
 //   dqs_id = sum_j da_ij (*) k_jd,   dk_jd = sum_i da_ij (*) qs_id,   dv_jd = sum_i e_ij (*) dn_id
-// for approximate gradients; an exact one weighs the gradient by the slope of the other factor's piece instead.  Two kernels: in the first lanes own
+// for approximate gradients; an exact one weighs the gradient by the slope of the other factor's piece instead.  (All slopes exact and no offset, or all
+// approximate, have usual loops; mixed slopes and exact ones with an offset take the full definition throughout: 31 and 44 ms where 4.4 are below.)  Two kernels: in the first lanes own
 // queries and keys stream by (a, de and dq: three products), in the second lanes own keys and queries stream by (a, de, dk and dv: four).
 // Scores and weights are computed again in both; kept, they would be 8 bytes a pair, as long to read as two of the products of 64 values.
-// 4096 causal tokens, 8 heads of 64 over 2: 1.07 ms for dq (12 T products/s), 1.65 for dk and dv (10), exact 1.6 and 2.1; three wavefronts on a SIMD are 6 % better than two for the
+// 4096 causal tokens, 8 heads of 64 over 2: 0.93 ms for dq (13.8 T products/s), 1.70 for dk and dv (10), exact 1.7 and 2.1; three wavefronts on a SIMD are 6 % better than two for the
 // first, and 30 % worse for the second, whose four slices of 32 then do not fit the registers.
 // All that is linear in dy is scaled by a power of two: in the first kernel a query's largest |dn| to [1, 2), in the second the largest of a chunk's.  The full definition
 // scales up only, so that nothing is lost beside a large value.

@@ -8,7 +8,8 @@
 // together through LDS, and the parts' by a second kernel.  Scaling by powers of two is exact, so that none of this moves a result beyond the
 // order of its sums.
 // 16 sequences of up to 4000 tokens, 16 heads of 128 over 4: 42 us for 134 MB (3.2 TB/s; 2040 spans are one for every wavefront, whose waits for memory follow
-// each other), the join 6; one sequence of 100000, five tokens, 8 heads over 2: 159 us for two sets of rows, 20 G products at 13 T/s.
+// each other), the join 6; one sequence of 100000, five tokens, 8 heads over 2: 170 us for 1.02 G products, 6 T/s: two sets of twelve rows for twenty, a
+// query's piece used for one key of every lane, and with a bias by distance most spans' weights are none, which takes a factor for every product (159 us without).
 // Heads that are no whole quads take a kernel in which groups of lanes own keys for the scores, too.
 #include <algorithm>
 
