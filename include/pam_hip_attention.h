@@ -45,7 +45,8 @@ int pam_hip_attention_fwd(const pam_hip_attention_shape *shape, const pam_hip_to
                           float *y, float *stats, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Gradients for q, k and v (contiguous; dq, or dk and dv, may be NULL) from that of y: the chain of the primitives' gradients, with the
- * sums of heads that share a key.  y (contiguous) and stats are the forward pass's.  The approx flags are those of pam_hip_act_bwd. */
+ * sums of heads that share a key.  y (contiguous) and stats are the forward pass's.  The approx flags are those of pam_hip_act_bwd.  Of approximate gradients a
+ * pair's (that for a) is none below 2^-116 of the largest dy (*) (1 (/) l) of its query or, for dk and dv, of the queries that are worked on together. */
 size_t pam_hip_attention_bwd_workspace_bytes(const pam_hip_attention_shape *shape, int want_q, int want_kv);
 int pam_hip_attention_bwd(const pam_hip_attention_shape *shape, const pam_hip_tokens *q, const pam_hip_tokens *k, const pam_hip_tokens *v,
                           const float *y, const float *stats, const pam_hip_tokens *dy, float *dq, float *dk, float *dv,
