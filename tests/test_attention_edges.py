@@ -282,3 +282,64 @@ def test_scratch_of_long_rows_is_bounded(tokens, keys):
                          ids=lambda x: "x".join(map(str, x)) if isinstance(x, tuple) else "_".join(x))
 def test_windows_of_many_tiles(shape, masks):
     test_attention._compare(shape, masks, seed=sum(shape))
+
+
+@gpu
+@pytest.mark.parametrize("dim", [40, 64, 128, 130, 256])
+@pytest.mark.parametrize("tokens,window,heads,kv_heads", [(3000, 256, 6, 2), (2500, 700, 2, 2), (5000, 65, 3, 1)])
+def test_a_long_window_by_pieces(tokens, window, heads, kv_heads, dim):
+    """A window over many tiles against the same by some hundred queries at a time, each over the keys that they see."""
+    pam = __import__("pam_amd")
+    torch.manual_seed(dim)
+    q, k, v = (torch.randn(1, tokens, n, dim, device="cuda") for n in (heads, kv_heads, kv_heads))
+    dy = torch.randn_like(q)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    y = pam.attention(*leaves, window=window, approx_bwd=True)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    want = [torch.zeros_like(x, dtype=torch.float64) for x in (q, q, k, v)]
+    for begin in range(0, tokens, 500):
+        end, first = min(tokens, begin + 500), max(0, begin - window + 1)
+        rows, seen = slice(begin, end), slice(first, end)
+        piece = [x[:, at].clone().requires_grad_() for x, at in ((q, rows), (k, seen), (v, seen))]
+        part = pam.attention(*piece, window=window, approx_bwd=True)
+        for total, at, add in zip(want, (rows, rows, seen, seen), (part.detach(), *torch.autograd.grad(part, piece, dy[:, rows]))):
+            total[:, at] += add
+    # (sums of dim and of window x heads terms in other orders, the steps between at most twice as sensitive each)
+    for name, a, b in zip(("y", "dq", "dk", "dv"), got, want):
+        assert (a - b).norm() <= 4 * 2.0 ** -24 * (dim + window * (heads // kv_heads)) * b.norm(), name
+
+
+@gpu
+@pytest.mark.parametrize("approx", [True, False, (True, False)], ids=str)
+def test_the_full_definition_in_a_graph(approx):
+    """Units that begin again, and zeros' loops, recorded and replayed on other values."""
+    pam = __import__("pam_amd")
+    sets = [[_cuda(x) for x in _inputs(seed, 1, 150, 150, 4, 2, 40)] for seed in (1, 2)]
+    for q, k, v, dy in sets:
+        v[:, 33] *= 1e14; k[:, 70, :, 3] = 0; q[:, 5] = 0; dy[:, 20, 0, 0] = 1e30
+    eager = []
+    for q, k, v, dy in sets:
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        y = pam.attention(*leaves, window=100, approx_bwd=approx)
+        eager.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    del leaves, y
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    static = [x.clone() for x in sets[0]]
+    with torch.cuda.stream(side):
+        leaves = [x.requires_grad_() for x in static[:3]]
+        torch.autograd.grad(pam.attention(*leaves, window=100, approx_bwd=approx), leaves, static[3])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = pam.attention(*leaves, window=100, approx_bwd=approx)
+        grads = torch.autograd.grad(y, leaves, static[3])
+    for turn in (1, 0, 1, 0):
+        with torch.no_grad():
+            for to, x in zip(static, sets[turn]):
+                to.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip([y, *grads], eager[turn]):
+            assert torch.equal(a, b) or torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+        torch.randn(1000, 1000, device="cuda").sum()
